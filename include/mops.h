@@ -1,6 +1,7 @@
 /* Umbrella header of the mops C ABI: 60 operation entry points plus the
  * error-text accessor (replaces mops/include/mops.h:1-22 of lab-cosmo/mops),
- * and the AMD-specific additions of mops/amd.h. */
+ * and what goes beyond it: the AMD-specific additions of mops/amd.h and the
+ * operators of mops/layers.h. */
 #ifndef MOPS_H
 #define MOPS_H
 
@@ -11,6 +12,7 @@
 #include "mops/sap.h"
 #include "mops/sasaw.h"
 #include "mops/amd.h"
+#include "mops/layers.h"
 
 #ifdef __cplusplus
 extern "C" {

@@ -7,6 +7,7 @@
 
 #include "mops/capi.hpp"
 #include "mops/hpe.hpp"
+#include "mops/layers.hpp"
 #include "mops/opsa.hpp"
 #include "mops/opsaw.hpp"
 #include "mops/sap.hpp"

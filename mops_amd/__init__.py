@@ -1,10 +1,20 @@
 """mops on AMD Instinct MI355X: the five sparse tensor operations of
 lab-cosmo/mops and their vector-Jacobian products, as hand-written HIP kernels
-for gfx950 behind mops' own C ABI, called here on PyTorch-ROCm tensors.
+for gfx950 behind mops' own C ABI, called here on PyTorch-ROCm tensors; and the
+operators of the layers around them (``mops_amd.layers``).
 
 The public names are those of the reference's Python package
 (``python/mops/src/mops/__init__.py`` of lab-cosmo/mops).
 """
+from .layers import (  # noqa: F401
+    gated_residual_norm,
+    gated_residual_norm_vjp,
+    grouped_matrix_product,
+    grouped_matrix_product_vjp,
+    order_by_group,
+    scaled_embedding,
+    scaled_embedding_vjp,
+)
 from .ops import (  # noqa: F401
     accept_unsorted_indices,
     first_occurrences,

@@ -31,9 +31,19 @@ constexpr Kind R1{false, 1}, R2{false, 2}, R3{false, 3}, I1{true, 1}, I2{true, 2
 /// The tensors among `arguments`, if all of them are what a kernel can take as it is.
 template <size_t N> struct Inputs {
     std::array<const at::Tensor*, N> tensor;
+    at::Tensor nothing;
 
-    bool take(PyObject* const* arguments, const std::array<Kind, N>& kinds) {
+    /// `layers`: the element types of the layers' operators, 16 bits among them, and an argument of type I1 or R2
+    /// that is None stays undefined where `optional` says so.
+    bool take(
+        PyObject* const* arguments, const std::array<Kind, N>& kinds, bool layers = false,
+        const std::array<bool, N>& optional = {}
+    ) {
         for (size_t i = 0; i < N; i++) {
+            if (optional[i] && arguments[i] == Py_None) {
+                tensor[i] = &nothing;
+                continue;
+            }
             if (!THPVariable_CheckExact(arguments[i])) {
                 return false;
             }
@@ -42,7 +52,8 @@ template <size_t N> struct Inputs {
                 t.dim() != kinds[i].dimensions || !t.is_contiguous()) {
                 return false;
             }
-            if (i == 0 && t.scalar_type() != at::kFloat && t.scalar_type() != at::kDouble) {
+            if (i == 0 && !(layers ? is_layer_dtype(t.scalar_type())
+                                   : t.scalar_type() == at::kFloat || t.scalar_type() == at::kDouble)) {
                 return false; // (the first tensor of every function is a floating-point one)
             }
             if (i > 0 && (t.device() != tensor[0]->device() ||
@@ -83,15 +94,23 @@ template <size_t N> PyObject* wrap(const std::array<at::Tensor, N>& tensors) {
     return tuple;
 }
 
+struct OfOperations {
+    template <typename Call> static void with(const at::Tensor& like, Call&& call) { by_dtype(like, call); }
+};
+struct OfLayers {
+    template <typename Call> static void with(const at::Tensor& like, Call&& call) { by_layer_dtype(like, call); }
+};
+
 /// outputs(), then call(zero of the element type, outputs) on the tensors' stream and without the
 /// interpreter lock; None when anything goes wrong.
-template <typename Outputs, typename Call> PyObject* run(const at::Tensor& like, Outputs&& outputs, Call&& call) {
+template <typename Types = OfOperations, typename Outputs, typename Call>
+PyObject* run(const at::Tensor& like, Outputs&& outputs, Call&& call) {
     try {
         OnTorchStream stream(like);
         auto results = outputs();
         PyThreadState* state = PyEval_SaveThread();
         try {
-            by_dtype(like, [&](auto zero) { call(zero, results); });
+            Types::with(like, [&](auto zero) { call(zero, results); });
         } catch (...) {
             PyEval_RestoreThread(state);
             Py_RETURN_NONE;
@@ -371,6 +390,140 @@ PyObject* sasaw_vjp(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
     );
 }
 
+// ------------------------------------------------------- layers' operators ----
+/// A number: a Python float or integer.
+bool number(PyObject* object, double& value) {
+    if (!PyFloat_CheckExact(object) && !PyLong_CheckExact(object)) {
+        return false;
+    }
+    value = PyFloat_AsDouble(object);
+    if (PyErr_Occurred() != nullptr) {
+        PyErr_Clear();
+        return false;
+    }
+    return true;
+}
+
+PyObject* scaled_embedding(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
+    Inputs<2> t; // table indices
+    double scale;
+    if (n != 3 || !t.take(arguments, {R2, I1}, true) || !number(arguments[2], scale)) {
+        Py_RETURN_NONE;
+    }
+    return run<OfLayers>(
+        t[0], [&] { return new_tensor({t[1].size(0), t[0].size(1)}, t[0]); },
+        [&](auto zero, at::Tensor& output) {
+            using T = decltype(zero);
+            mops::cuda::scaled_embedding<T>(
+                view<T, 2>(output, "output"), view<T, 2>(t[0], "table"), view<int32_t, 1>(t[1], "indices"), scale
+            );
+        }
+    );
+}
+
+PyObject* scaled_embedding_vjp(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
+    Inputs<5> t; // grad_output table indices order offsets
+    double scale;
+    if (n != 6 || !t.take(arguments, {R2, R2, I1, I1, I1}, true, {false, false, false, true, true}) ||
+        !number(arguments[5], scale)) {
+        Py_RETURN_NONE;
+    }
+    return run<OfLayers>(t[0], [&] { return new_like(t[1]); }, [&](auto zero, at::Tensor& grad_table) {
+        using T = decltype(zero);
+        mops::cuda::scaled_embedding_vjp<T>(
+            view<T, 2>(grad_table, "grad_table"), view<T, 2>(t[0], "grad_output"), view<int32_t, 1>(t[2], "indices"),
+            view<int32_t, 1>(t[3], "order"), view<int32_t, 1>(t[4], "offsets"), scale
+        );
+    });
+}
+
+PyObject* grouped_matrix_product(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
+    Inputs<4> t; // A W offsets order
+    if (n != 4 || !t.take(arguments, {R2, R3, I1, I1}, true, {false, false, false, true})) {
+        Py_RETURN_NONE;
+    }
+    return run<OfLayers>(
+        t[0], [&] { return new_tensor({t[0].size(0), t[1].size(2)}, t[0]); },
+        [&](auto zero, at::Tensor& output) {
+            using T = decltype(zero);
+            mops::cuda::grouped_matrix_product<T>(
+                view<T, 2>(output, "output"), view<T, 2>(t[0], "A"), view<T, 3>(t[1], "W"),
+                view<int32_t, 1>(t[2], "offsets"), view<int32_t, 1>(t[3], "order")
+            );
+        }
+    );
+}
+
+PyObject* grouped_matrix_product_vjp(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
+    Inputs<5> t; // grad_output A W offsets order
+    std::array<bool, 2> want;
+    if (n != 7 || !t.take(arguments, {R2, R2, R3, I1, I1}, true, {false, false, false, false, true}) ||
+        !flags(arguments + 5, want)) {
+        Py_RETURN_NONE;
+    }
+    return run<OfLayers>(
+        t[0], [&] { return std::array<at::Tensor, 2>{like_if(want[0], t[1]), like_if(want[1], t[2])}; },
+        [&](auto zero, auto& out) {
+            using T = decltype(zero);
+            mops::cuda::grouped_matrix_product_vjp<T>(
+                view<T, 2>(out[0], "grad_A"), view<T, 3>(out[1], "grad_W"), view<T, 2>(t[0], "grad_output"),
+                view<T, 2>(t[1], "A"), view<T, 3>(t[2], "W"), view<int32_t, 1>(t[3], "offsets"),
+                view<int32_t, 1>(t[4], "order")
+            );
+        }
+    );
+}
+
+PyObject* gated_residual_norm(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
+    Inputs<5> t; // residual block gate weight_block weight_next
+    double scale, epsilon;
+    if (n != 7 || !t.take(arguments, {R2, R2, R2, R1, R1}, true) || !number(arguments[5], scale) ||
+        !number(arguments[6], epsilon)) {
+        Py_RETURN_NONE;
+    }
+    return run<OfLayers>(
+        t[0], [&] { return std::array<at::Tensor, 2>{new_like(t[0]), new_like(t[0])}; },
+        [&](auto zero, auto& out) {
+            using T = decltype(zero);
+            mops::cuda::gated_residual_norm<T>(
+                view<T, 2>(out[0], "state"), view<T, 2>(out[1], "next"), view<T, 2>(t[0], "residual"),
+                view<T, 2>(t[1], "block"), view<T, 2>(t[2], "gate"), view<T, 1>(t[3], "weight_block"),
+                view<T, 1>(t[4], "weight_next"), scale, epsilon
+            );
+        }
+    );
+}
+
+PyObject* gated_residual_norm_vjp(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
+    // residual block gate weight_block weight_next grad_state grad_next (the last two may be None)
+    Inputs<7> t;
+    double scale, epsilon;
+    std::array<bool, 5> want;
+    if (n != 14 || !t.take(arguments, {R2, R2, R2, R1, R1, R2, R2}, true, {false, false, false, false, false, true, true}) ||
+        !number(arguments[7], scale) || !number(arguments[8], epsilon) || !flags(arguments + 9, want)) {
+        Py_RETURN_NONE;
+    }
+    return run<OfLayers>(
+        t[0],
+        [&] {
+            return std::array<at::Tensor, 5>{
+                like_if(want[0], t[0]), like_if(want[1], t[1]), like_if(want[2], t[2]), like_if(want[3], t[3]),
+                like_if(want[4], t[4]),
+            };
+        },
+        [&](auto zero, auto& out) {
+            using T = decltype(zero);
+            mops::cuda::gated_residual_norm_vjp<T>(
+                view<T, 2>(out[0], "grad_residual"), view<T, 2>(out[1], "grad_block"), view<T, 2>(out[2], "grad_gate"),
+                view<T, 1>(out[3], "grad_weight_block"), view<T, 1>(out[4], "grad_weight_next"),
+                view<T, 2>(t[5], "grad_state"), view<T, 2>(t[6], "grad_next"), view<T, 2>(t[0], "residual"),
+                view<T, 2>(t[1], "block"), view<T, 2>(t[2], "gate"), view<T, 1>(t[3], "weight_block"),
+                view<T, 1>(t[4], "weight_next"), scale, epsilon
+            );
+        }
+    );
+}
+
 #define MOPS_METHOD(NAME, FUNCTION)                                                                 \
     {NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(FUNCTION)), METH_FASTCALL, nullptr}
 PyMethodDef METHODS[] = {
@@ -387,6 +540,12 @@ PyMethodDef METHODS[] = {
     MOPS_METHOD("outer_product_scatter_add_with_weights_vjp", opsaw_vjp),
     MOPS_METHOD("sparse_accumulation_scatter_add_with_weights", sasaw),
     MOPS_METHOD("sparse_accumulation_scatter_add_with_weights_vjp", sasaw_vjp),
+    MOPS_METHOD("scaled_embedding", scaled_embedding),
+    MOPS_METHOD("scaled_embedding_vjp", scaled_embedding_vjp),
+    MOPS_METHOD("grouped_matrix_product", grouped_matrix_product),
+    MOPS_METHOD("grouped_matrix_product_vjp", grouped_matrix_product_vjp),
+    MOPS_METHOD("gated_residual_norm", gated_residual_norm),
+    MOPS_METHOD("gated_residual_norm_vjp", gated_residual_norm_vjp),
     {nullptr, nullptr, 0, nullptr},
 };
 

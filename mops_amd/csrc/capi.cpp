@@ -1,5 +1,5 @@
-// The C ABI: 60 operation entry points, the error-text accessor and the
-// AMD-specific additions. Every operation wrapper does the same three
+// The C ABI: 60 operation entry points, the error-text accessor, the
+// AMD-specific additions and the layers' operators. Every operation wrapper does the same three
 // things as mops/src/<op>/capi.cpp of lab-cosmo/mops: convert each int64
 // extent to size_t (rejecting negative values), call the C++ template, and
 // translate exceptions into a status code plus a per-thread message.
@@ -50,6 +50,25 @@ MOPS_DEFINE_VIEW(mops_tensor_2d_f64_t, double)
 MOPS_DEFINE_VIEW(mops_tensor_3d_f64_t, double)
 MOPS_DEFINE_VIEW(mops_tensor_1d_i32_t, int32_t)
 MOPS_DEFINE_VIEW(mops_tensor_2d_i32_t, int32_t)
+
+// 16-bit floating-point data: given by its bits
+#define MOPS_DEFINE_16_BIT_VIEW(STRUCT, ELEMENT)                                                   \
+    mops::Tensor<ELEMENT, sizeof(STRUCT::shape) / sizeof(int64_t)> view(STRUCT t) {                \
+        constexpr size_t N = sizeof(STRUCT::shape) / sizeof(int64_t);                              \
+        mops::Tensor<ELEMENT, N> result;                                                           \
+        result.data = reinterpret_cast<ELEMENT*>(t.data);                                          \
+        for (size_t d = 0; d < N; d++) {                                                           \
+            result.shape[d] = extent(t.shape[d]);                                                  \
+        }                                                                                          \
+        return result;                                                                             \
+    }
+
+MOPS_DEFINE_16_BIT_VIEW(mops_tensor_1d_bf16_t, mops::bfloat16)
+MOPS_DEFINE_16_BIT_VIEW(mops_tensor_2d_bf16_t, mops::bfloat16)
+MOPS_DEFINE_16_BIT_VIEW(mops_tensor_3d_bf16_t, mops::bfloat16)
+MOPS_DEFINE_16_BIT_VIEW(mops_tensor_1d_f16_t, mops::float16)
+MOPS_DEFINE_16_BIT_VIEW(mops_tensor_2d_f16_t, mops::float16)
+MOPS_DEFINE_16_BIT_VIEW(mops_tensor_3d_f16_t, mops::float16)
 
 // A tensor that the C ABI declares with the 2-D struct although it has three
 // dimensions: the missing last extent is taken from `last`.
@@ -166,3 +185,90 @@ extern "C" int mops_amd_sparse_accumulation_scatter_add_with_weights_vjp_no_allo
     mops::amd::sasaw_vjp_no_alloc(MOPS_SASAW_VJP_PARAMS(MOPS_FORWARD_FIRST, MOPS_FORWARD_NEXT));
     MOPS_CATCH_EXCEPTIONS_END
 }
+
+// ---- the layers' operators (mops/layers.h) --------------------------------
+
+extern "C" int mops_amd_order_by_group(
+    mops_tensor_1d_i32_t order, mops_tensor_1d_i32_t offsets, mops_tensor_1d_i32_t indices
+) {
+    MOPS_CATCH_EXCEPTIONS_BEGIN
+    mops::cuda::order_by_group(view(order), view(offsets), view(indices));
+    MOPS_CATCH_EXCEPTIONS_END
+}
+
+#define MOPS_LAYERS_DEFINE(S, T)                                                                   \
+    extern "C" int mops_amd_scaled_embedding_##S(                                                  \
+        mops_tensor_2d_##S##_t output, mops_tensor_2d_##S##_t table, mops_tensor_1d_i32_t indices, \
+        double scale                                                                               \
+    ) {                                                                                            \
+        MOPS_CATCH_EXCEPTIONS_BEGIN                                                                \
+        mops::cuda::scaled_embedding<T>(view(output), view(table), view(indices), scale);          \
+        MOPS_CATCH_EXCEPTIONS_END                                                                  \
+    }                                                                                              \
+    extern "C" int mops_amd_scaled_embedding_vjp_##S(                                              \
+        mops_tensor_2d_##S##_t grad_table, mops_tensor_2d_##S##_t grad_output,                     \
+        mops_tensor_1d_i32_t indices, mops_tensor_1d_i32_t order, mops_tensor_1d_i32_t offsets,    \
+        double scale                                                                               \
+    ) {                                                                                            \
+        MOPS_CATCH_EXCEPTIONS_BEGIN                                                                \
+        mops::cuda::scaled_embedding_vjp<T>(                                                       \
+            view(grad_table), view(grad_output), view(indices), view(order), view(offsets), scale  \
+        );                                                                                         \
+        MOPS_CATCH_EXCEPTIONS_END                                                                  \
+    }                                                                                              \
+    extern "C" int mops_amd_grouped_matrix_product_##S(                                            \
+        mops_tensor_2d_##S##_t output, mops_tensor_2d_##S##_t A, mops_tensor_3d_##S##_t W,         \
+        mops_tensor_1d_i32_t offsets, mops_tensor_1d_i32_t order                                   \
+    ) {                                                                                            \
+        MOPS_CATCH_EXCEPTIONS_BEGIN                                                                \
+        mops::cuda::grouped_matrix_product<T>(                                                     \
+            view(output), view(A), view(W), view(offsets), view(order)                             \
+        );                                                                                         \
+        MOPS_CATCH_EXCEPTIONS_END                                                                  \
+    }                                                                                              \
+    extern "C" int mops_amd_grouped_matrix_product_vjp_##S(                                        \
+        mops_tensor_2d_##S##_t grad_A, mops_tensor_3d_##S##_t grad_W,                              \
+        mops_tensor_2d_##S##_t grad_output, mops_tensor_2d_##S##_t A, mops_tensor_3d_##S##_t W,    \
+        mops_tensor_1d_i32_t offsets, mops_tensor_1d_i32_t order                                   \
+    ) {                                                                                            \
+        MOPS_CATCH_EXCEPTIONS_BEGIN                                                                \
+        mops::cuda::grouped_matrix_product_vjp<T>(                                                 \
+            view(grad_A), view(grad_W), view(grad_output), view(A), view(W), view(offsets), view(order) \
+        );                                                                                         \
+        MOPS_CATCH_EXCEPTIONS_END                                                                  \
+    }                                                                                              \
+    extern "C" int mops_amd_gated_residual_norm_##S(                                               \
+        mops_tensor_2d_##S##_t state, mops_tensor_2d_##S##_t next,                                 \
+        mops_tensor_2d_##S##_t residual, mops_tensor_2d_##S##_t block,                             \
+        mops_tensor_2d_##S##_t gate, mops_tensor_1d_##S##_t weight_block,                          \
+        mops_tensor_1d_##S##_t weight_next, double residual_scale, double epsilon                  \
+    ) {                                                                                            \
+        MOPS_CATCH_EXCEPTIONS_BEGIN                                                                \
+        mops::cuda::gated_residual_norm<T>(                                                        \
+            view(state), view(next), view(residual), view(block), view(gate), view(weight_block),  \
+            view(weight_next), residual_scale, epsilon                                             \
+        );                                                                                         \
+        MOPS_CATCH_EXCEPTIONS_END                                                                  \
+    }                                                                                              \
+    extern "C" int mops_amd_gated_residual_norm_vjp_##S(                                           \
+        mops_tensor_2d_##S##_t grad_residual, mops_tensor_2d_##S##_t grad_block,                   \
+        mops_tensor_2d_##S##_t grad_gate, mops_tensor_1d_##S##_t grad_weight_block,                \
+        mops_tensor_1d_##S##_t grad_weight_next, mops_tensor_2d_##S##_t grad_state,                \
+        mops_tensor_2d_##S##_t grad_next, mops_tensor_2d_##S##_t residual,                         \
+        mops_tensor_2d_##S##_t block, mops_tensor_2d_##S##_t gate,                                 \
+        mops_tensor_1d_##S##_t weight_block, mops_tensor_1d_##S##_t weight_next,                   \
+        double residual_scale, double epsilon                                                      \
+    ) {                                                                                            \
+        MOPS_CATCH_EXCEPTIONS_BEGIN                                                                \
+        mops::cuda::gated_residual_norm_vjp<T>(                                                    \
+            view(grad_residual), view(grad_block), view(grad_gate), view(grad_weight_block),       \
+            view(grad_weight_next), view(grad_state), view(grad_next), view(residual), view(block), \
+            view(gate), view(weight_block), view(weight_next), residual_scale, epsilon             \
+        );                                                                                         \
+        MOPS_CATCH_EXCEPTIONS_END                                                                  \
+    }
+
+MOPS_LAYERS_DEFINE(f32, float)
+MOPS_LAYERS_DEFINE(f64, double)
+MOPS_LAYERS_DEFINE(bf16, mops::bfloat16)
+MOPS_LAYERS_DEFINE(f16, mops::float16)

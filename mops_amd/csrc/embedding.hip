@@ -1,0 +1,419 @@
+// A table looked up by an index, times a constant, and its gradient:
+//
+//   output[i, :]     = scale * table[indices[i], :]
+//   grad_table[v, :] = scale * sum_{i: indices[i] = v} grad_output[i, :]
+//
+// Both only move memory. Forward: a team of lanes per row, a lane per 16 bytes
+// of it, several rows on their way at once. Gradient: the rows are put in the
+// order of their index first (order_all_by_group, or the caller's plan); then
+// every row of the table is the sum over consecutive places of that order, by
+// the one team that stores it: no atomics, and an order of summation that
+// depends on the indices only. A row of the table that very many rows name (a
+// frequent word, an abundant element) would be one team's work of thousands of
+// steps: a launch before sums up every whole chunk of places that lies inside
+// one row of the table, by workgroups that are spread over the GPU, and its
+// owner adds those sums and the places at either end.
+#include "mops/layers.hpp"
+
+#include <algorithm>
+
+#include "checks.hpp"
+#include "device_common.hpp"
+#include "numbers.hpp"
+#include "runtime.hpp"
+#include "sender_buckets.hpp"
+
+namespace mops::amd {
+namespace embedding {
+namespace {
+
+constexpr int THREADS = 256;
+constexpr int AHEAD = 8;            // rows that a team has on their way
+constexpr int32_t PLACES_EACH = 32; // of a chunk, per team
+constexpr int32_t ALONE = 64;       // places that a team sums up by itself
+
+/// How a row's pieces are shared out: `team` lanes (a power of two) hold a piece each.
+struct Teams {
+    PiecesOfRow row;
+    int32_t team, teams; // lanes per team, teams per workgroup
+    unsigned tiles;      // workgroups beside each other that hold a row
+
+    template <int N> static Teams make(int32_t columns) {
+        Teams t;
+        t.row = PiecesOfRow::make<N>(columns);
+        t.team = 1;
+        while (t.team < THREADS && t.team < t.row.pieces) {
+            t.team *= 2;
+        }
+        t.teams = THREADS / t.team;
+        t.tiles = static_cast<unsigned>(ceil_div(static_cast<size_t>(t.row.pieces), static_cast<size_t>(t.team)));
+        return t;
+    }
+};
+
+template <typename T, int N, int ROWS>
+__global__ __launch_bounds__(THREADS) void lookup_kernel(
+    T* __restrict__ output, const T* __restrict__ table, const int32_t* __restrict__ indices, int32_t n_rows,
+    int32_t table_rows, Teams teams, wide_t<T> scale
+) {
+    const int32_t piece = blockIdx.y * teams.team + (threadIdx.x & (teams.team - 1));
+    const int32_t first = (blockIdx.x * teams.teams + threadIdx.x / teams.team) * ROWS;
+    if (piece >= teams.row.pieces) {
+        return;
+    }
+    const int32_t column = teams.row.start<N>(piece);
+    const size_t columns = teams.row.columns;
+    int32_t index[ROWS];
+    Piece<T, N> value[ROWS];
+#pragma unroll
+    for (int u = 0; u < ROWS; u++) {
+        index[u] = indices[min(first + u, n_rows - 1)];
+    }
+#pragma unroll
+    for (int u = 0; u < ROWS; u++) {
+        value[u] = Piece<T, N>::load(table + (in_bounds(index[u], table_rows) ? index[u] : 0) * columns + column);
+    }
+#pragma unroll
+    for (int u = 0; u < ROWS; u++) {
+        if (first + u >= n_rows) {
+            break;
+        }
+        const bool inside = in_bounds(index[u], table_rows);
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            value[u].set(j, inside ? scale * value[u].get(j) : wide_t<T>(0));
+        }
+        value[u].store(output + static_cast<size_t>(first + u) * columns + column);
+    }
+}
+
+/// sum[j] += rows order[begin], order[begin + step], ... before `end`, at `column`.
+template <typename T, int N>
+__device__ __forceinline__ void add_rows(
+    wide_t<T> (&sum)[N], const T* __restrict__ rows, const int32_t* __restrict__ order, int32_t n_rows, int32_t begin,
+    int32_t end, int32_t step, size_t columns, int32_t column
+) {
+    for (int32_t p = begin; p < end; p += AHEAD * step) {
+        int32_t row[AHEAD];
+        Piece<T, N> value[AHEAD];
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            row[u] = p + u * step < end ? order[p + u * step] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            value[u] = Piece<T, N>::load(rows + (in_bounds(row[u], n_rows) ? row[u] : 0) * columns + column);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; u++) {
+            if (in_bounds(row[u], n_rows)) {
+#pragma unroll
+                for (int j = 0; j < N; j++) {
+                    sum[j] += value[u].get(j);
+                }
+            }
+        }
+    }
+}
+
+/// sum[j] of all teams, in the registers of team 0. All threads.
+template <typename W, int N> __device__ __forceinline__ void join_teams(W (&sum)[N], W* joined, const Teams& teams) {
+    if (teams.teams == 1) {
+        return;
+    }
+#pragma unroll
+    for (int j = 0; j < N; j++) {
+        joined[j * THREADS + threadIdx.x] = sum[j];
+    }
+    __syncthreads();
+    if (static_cast<int32_t>(threadIdx.x) < teams.team) {
+        for (int32_t t = 1; t < teams.teams; t++) {
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                sum[j] += joined[j * THREADS + t * teams.team + threadIdx.x];
+            }
+        }
+    }
+    __syncthreads();
+}
+
+/// partial[chunk, :] := the sum over the places of a chunk that lies inside one row of the table.
+template <typename T, int N>
+__global__ __launch_bounds__(THREADS) void chunk_kernel(
+    wide_t<T>* __restrict__ partial, const T* __restrict__ grad_output, const int32_t* __restrict__ indices,
+    const int32_t* __restrict__ order, int32_t n_rows, int32_t table_rows, Teams teams, int32_t chunk
+) {
+    __shared__ wide_t<T> joined[N * THREADS];
+    const int32_t begin = blockIdx.x * chunk, end = begin + chunk;
+    const int32_t first = order[begin], last = order[end - 1];
+    const int32_t index = in_bounds(first, n_rows) ? indices[first] : -1;
+    if (!in_bounds(index, table_rows) || !in_bounds(last, n_rows) || indices[last] != index) {
+        return; // (uniform)
+    }
+    const int32_t piece = min(
+        static_cast<int32_t>(blockIdx.y * teams.team + (threadIdx.x & (teams.team - 1))), teams.row.pieces - 1
+    );
+    const int32_t column = teams.row.start<N>(piece);
+    wide_t<T> sum[N] = {};
+    add_rows<T, N>(
+        sum, grad_output, order, n_rows, begin + threadIdx.x / teams.team, end, teams.teams, teams.row.columns, column
+    );
+    join_teams<wide_t<T>, N>(sum, joined, teams);
+    if (static_cast<int32_t>(threadIdx.x) < teams.team) {
+        wide_t<T>* to = partial + static_cast<size_t>(blockIdx.x) * teams.row.columns + column;
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            to[j] = sum[j];
+        }
+    }
+}
+
+/// grad_table[v, :]: a team per row of the table where few rows name it, the workgroup together where many do.
+template <typename T, int N>
+__global__ __launch_bounds__(THREADS) void gradient_kernel(
+    T* __restrict__ grad_table, const T* __restrict__ grad_output, const wide_t<T>* __restrict__ partial,
+    const int32_t* __restrict__ order, const int32_t* __restrict__ offsets, int32_t n_rows, int32_t table_rows,
+    Teams teams, int32_t chunk, wide_t<T> scale
+) {
+    __shared__ wide_t<T> joined[N * THREADS];
+    const int32_t piece = blockIdx.y * teams.team + (threadIdx.x & (teams.team - 1));
+    const bool holds = piece < teams.row.pieces;
+    const int32_t column = teams.row.start<N>(min(piece, teams.row.pieces - 1));
+    const int32_t mine = threadIdx.x / teams.team;
+    const int32_t row0 = blockIdx.x * teams.teams;
+    auto store = [&](int32_t row, const wide_t<T>(&sum)[N]) {
+        Piece<T, N> value;
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            value.set(j, scale * sum[j]);
+        }
+        value.store(grad_table + static_cast<size_t>(row) * teams.row.columns + column);
+    };
+    {
+        const int32_t row = row0 + mine;
+        if (row < table_rows && holds) {
+            const int32_t begin = max(offsets[row], 0), end = min(offsets[row + 1], n_rows);
+            if (end - begin <= ALONE) {
+                wide_t<T> sum[N] = {};
+                add_rows<T, N>(sum, grad_output, order, n_rows, begin, end, 1, teams.row.columns, column);
+                store(row, sum);
+            }
+        }
+    }
+    for (int32_t t = 0; t < teams.teams; t++) {
+        const int32_t row = row0 + t;
+        if (row >= table_rows) {
+            break;
+        }
+        const int32_t begin = max(offsets[row], 0), end = min(offsets[row + 1], n_rows);
+        if (end - begin <= ALONE) { // (uniform)
+            continue;
+        }
+        wide_t<T> sum[N] = {};
+        const int32_t first_chunk = (begin + chunk - 1) / chunk, past_chunk = end / chunk;
+        const bool chunks = partial != nullptr && first_chunk < past_chunk;
+        add_rows<T, N>(
+            sum, grad_output, order, n_rows, begin + mine, chunks ? first_chunk * chunk : end, teams.teams,
+            teams.row.columns, column
+        );
+        if (chunks) {
+            for (int32_t c = first_chunk + mine; c < past_chunk; c += AHEAD * teams.teams) {
+                wide_t<T> value[AHEAD][N];
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++) {
+                    const size_t from = min(c + u * teams.teams, past_chunk - 1);
+#pragma unroll
+                    for (int j = 0; j < N; j++) {
+                        value[u][j] = partial[from * teams.row.columns + column + j];
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < AHEAD; u++) {
+                    if (c + u * teams.teams < past_chunk) {
+#pragma unroll
+                        for (int j = 0; j < N; j++) {
+                            sum[j] += value[u][j];
+                        }
+                    }
+                }
+            }
+            add_rows<T, N>(
+                sum, grad_output, order, n_rows, past_chunk * chunk + mine, end, teams.teams, teams.row.columns, column
+            );
+        }
+        join_teams<wide_t<T>, N>(sum, joined, teams);
+        if (mine == 0 && holds) {
+            store(row, sum);
+        }
+    }
+}
+
+/// body(number of columns in a piece): 16 bytes, or single numbers for rows shorter than that.
+template <typename T, typename Body> void by_width(int32_t columns, Body&& body) {
+    if (columns >= PIECE<T>) {
+        body(std::integral_constant<int, PIECE<T>>{});
+    } else {
+        body(std::integral_constant<int, 1>{});
+    }
+}
+
+template <typename T>
+void lookup(T* output, const T* table, const int32_t* indices, int32_t n_rows, int32_t table_rows, int32_t columns,
+            double scale, hipStream_t stream) {
+    by_width<T>(columns, [&](auto width) {
+        constexpr int N = decltype(width)::value;
+        const Teams teams = Teams::make<N>(columns);
+        auto launch = [&](auto rows) {
+            constexpr int ROWS = decltype(rows)::value;
+            const size_t blocks = ceil_div(static_cast<size_t>(n_rows), static_cast<size_t>(teams.teams) * ROWS);
+            lookup_kernel<T, N, ROWS><<<dim3(static_cast<unsigned>(blocks), teams.tiles), THREADS, 0, stream>>>(
+                output, table, indices, n_rows, table_rows, teams, static_cast<wide_t<T>>(scale)
+            );
+        };
+        // several rows per lane once there are enough of them for every compute unit
+        if (static_cast<size_t>(n_rows) * teams.row.pieces >= static_cast<size_t>(compute_units()) * THREADS * 16) {
+            launch(std::integral_constant<int, 4>{});
+        } else {
+            launch(std::integral_constant<int, 1>{});
+        }
+    });
+    MOPS_HIP_CHECK(hipGetLastError());
+}
+
+template <typename T>
+void gradient(
+    T* grad_table, const T* grad_output, const int32_t* indices, const int32_t* order, const int32_t* offsets,
+    int32_t n_rows, int32_t table_rows, int32_t columns, double scale, hipStream_t stream
+) {
+    by_width<T>(columns, [&](auto width) {
+        constexpr int N = decltype(width)::value;
+        const Teams teams = Teams::make<N>(columns);
+        const int32_t chunk = PLACES_EACH * teams.teams;
+        const int32_t chunks = n_rows / chunk;
+        const size_t partial_bytes =
+            n_rows > ALONE ? align256(static_cast<size_t>(chunks) * columns * sizeof(wide_t<T>)) : 0;
+        const size_t order_bytes = order == nullptr ? align256(static_cast<size_t>(n_rows) * 4) : 0;
+        const size_t offsets_bytes = order == nullptr ? align256((static_cast<size_t>(table_rows) + 1) * 4) : 0;
+        const size_t sort_bytes = order == nullptr ? order_all_by_group_bytes(table_rows, n_rows) : 0;
+        char* workspace = nullptr;
+        if (partial_bytes + order_bytes + offsets_bytes + sort_bytes > 0) {
+            workspace = static_cast<char*>(scratch(partial_bytes + order_bytes + offsets_bytes + sort_bytes));
+        }
+        wide_t<T>* partial = partial_bytes > 0 ? reinterpret_cast<wide_t<T>*>(workspace) : nullptr;
+        if (order == nullptr) {
+            int32_t* places = reinterpret_cast<int32_t*>(workspace + partial_bytes);
+            int32_t* begins = reinterpret_cast<int32_t*>(workspace + partial_bytes + order_bytes);
+            order_all_by_group(
+                places, begins, indices, n_rows, table_rows, workspace + partial_bytes + order_bytes + offsets_bytes,
+                stream
+            );
+            order = places;
+            offsets = begins;
+        }
+        if (partial != nullptr) {
+            chunk_kernel<T, N><<<dim3(static_cast<unsigned>(chunks), teams.tiles), THREADS, 0, stream>>>(
+                partial, grad_output, indices, order, n_rows, table_rows, teams, chunk
+            );
+        }
+        const size_t blocks = ceil_div(static_cast<size_t>(table_rows), static_cast<size_t>(teams.teams));
+        gradient_kernel<T, N><<<dim3(static_cast<unsigned>(blocks), teams.tiles), THREADS, 0, stream>>>(
+            grad_table, grad_output, partial, order, offsets, n_rows, table_rows, teams, chunk,
+            static_cast<wide_t<T>>(scale)
+        );
+    });
+    MOPS_HIP_CHECK(hipGetLastError());
+}
+
+} // namespace
+} // namespace embedding
+} // namespace mops::amd
+
+namespace mops::cuda {
+
+using namespace mops::amd;
+
+void order_by_group(Tensor<int32_t, 1> order, Tensor<int32_t, 1> offsets, Tensor<int32_t, 1> indices) {
+    const checks::Validator check("order_by_group");
+    check.same_extent(checks::axis_of(order, "order", 0), checks::axis_of(indices, "indices", 0));
+    if (offsets.shape[0] < 1) {
+        throw std::runtime_error("offsets must have at least one element in order_by_group");
+    }
+    const int32_t n_rows = count_i32(indices.shape[0], "number of rows");
+    const int32_t groups = count_i32(offsets.shape[0], "number of groups + 1") - 1;
+    void* workspace = n_rows > 0 ? scratch(order_all_by_group_bytes(groups, n_rows)) : nullptr;
+    order_all_by_group(order.data, offsets.data, indices.data, n_rows, groups, workspace, current_stream());
+    finish_call("order_by_group");
+}
+
+template <typename scalar_t>
+void scaled_embedding(
+    Tensor<scalar_t, 2> output, Tensor<scalar_t, 2> table, Tensor<int32_t, 1> indices, double scale
+) {
+    const checks::Validator check("scaled_embedding");
+    check.same_extent(checks::axis_of(output, "output", 0), checks::axis_of(indices, "indices", 0));
+    check.same_extent(checks::axis_of(output, "output", 1), checks::axis_of(table, "table", 1));
+    const int32_t n_rows = count_i32(indices.shape[0], "number of rows");
+    const int32_t table_rows = count_i32(table.shape[0], "number of table rows");
+    const int32_t columns = count_i32(table.shape[1], "number of columns");
+    if (n_rows > 0 && columns > 0) {
+        typedef device_t<scalar_t> T;
+        T* to = data_of(output);
+        if (table_rows > 0) {
+            embedding::lookup<T>(
+                to, data_of(table), indices.data, n_rows, table_rows, columns, scale,
+                current_stream()
+            );
+        } else { // (no row to look anything up in: every index is outside; `to` is never read as a table)
+            embedding::lookup<T>(to, to, indices.data, n_rows, 0, columns, scale, current_stream());
+        }
+    }
+    finish_call("scaled_embedding");
+}
+
+template <typename scalar_t>
+void scaled_embedding_vjp(
+    Tensor<scalar_t, 2> grad_table, Tensor<scalar_t, 2> grad_output, Tensor<int32_t, 1> indices,
+    Tensor<int32_t, 1> order, Tensor<int32_t, 1> offsets, double scale
+) {
+    if (grad_table.data == nullptr) {
+        return;
+    }
+    const checks::Validator check("scaled_embedding_vjp");
+    check.same_extent(checks::axis_of(grad_output, "grad_output", 0), checks::axis_of(indices, "indices", 0));
+    check.same_extent(checks::axis_of(grad_output, "grad_output", 1), checks::axis_of(grad_table, "grad_table", 1));
+    const int32_t n_rows = count_i32(indices.shape[0], "number of rows");
+    const int32_t table_rows = count_i32(grad_table.shape[0], "number of table rows");
+    const int32_t columns = count_i32(grad_table.shape[1], "number of columns");
+    if ((order.data == nullptr) != (offsets.data == nullptr) && n_rows > 0) {
+        throw std::runtime_error("order and offsets must be given together in scaled_embedding_vjp");
+    }
+    if (order.data != nullptr) {
+        check.same_extent(checks::axis_of(order, "order", 0), checks::axis_of(indices, "indices", 0));
+        if (offsets.shape[0] != grad_table.shape[0] + 1) {
+            throw std::runtime_error(
+                "offsets must have " + std::to_string(grad_table.shape[0] + 1) + " elements (the rows of the table "
+                "and one more) in scaled_embedding_vjp, got " + std::to_string(offsets.shape[0])
+            );
+        }
+    }
+    if (table_rows > 0 && columns > 0) {
+        typedef device_t<scalar_t> T;
+        embedding::gradient<T>(
+            data_of(grad_table), data_of(grad_output), indices.data,
+            order.data, offsets.data, n_rows, table_rows, columns, scale, current_stream()
+        );
+    }
+    finish_call("scaled_embedding_vjp");
+}
+
+#define MOPS_EMBEDDING_INSTANTIATE(T)                                                              \
+    template void scaled_embedding<T>(Tensor<T, 2>, Tensor<T, 2>, Tensor<int32_t, 1>, double);     \
+    template void scaled_embedding_vjp<T>(                                                         \
+        Tensor<T, 2>, Tensor<T, 2>, Tensor<int32_t, 1>, Tensor<int32_t, 1>, Tensor<int32_t, 1>, double \
+    );
+MOPS_EMBEDDING_INSTANTIATE(float)
+MOPS_EMBEDDING_INSTANTIATE(double)
+MOPS_EMBEDDING_INSTANTIATE(bfloat16)
+MOPS_EMBEDDING_INSTANTIATE(float16)
+
+} // namespace mops::cuda

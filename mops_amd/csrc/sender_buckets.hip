@@ -29,10 +29,16 @@ constexpr int32_t SENDERS_AT_A_TIME = 4096;  // of the second level: counters in
 constexpr int HELD = 4;                      // positions a lane keeps from counting to placing
 constexpr int32_t STAGED = 5120;             // edges of a bucket that are put in order in LDS
 
+/// What an edge is sorted by: its sender; an edge whose sender is none of the `known` ones goes to a last sender
+/// of their own where there is one (n_nodes = known + 1), or is not listed (-1).
+__device__ __forceinline__ int32_t listed_under(int32_t sender, int32_t known, int32_t n_nodes) {
+    return in_bounds(sender, known) ? sender : known < n_nodes ? known : -1;
+}
+
 /// counts[workgroup][pitch]: how many in every bucket of the workgroup's share of the edges.
 __global__ __launch_bounds__(SORT_THREADS) void count_buckets_kernel(
-    int32_t* __restrict__ counts, const int32_t* __restrict__ senders, int32_t n_edges, int32_t n_nodes, int shift,
-    int32_t pitch, int32_t share
+    int32_t* __restrict__ counts, const int32_t* __restrict__ senders, int32_t n_edges, int32_t n_nodes,
+    int32_t known, int shift, int32_t pitch, int32_t share
 ) {
     __shared__ int32_t histogram[MOST_BUCKETS];
     for (int32_t b = threadIdx.x; b < pitch; b += SORT_THREADS) {
@@ -49,8 +55,9 @@ __global__ __launch_bounds__(SORT_THREADS) void count_buckets_kernel(
         }
 #pragma unroll
         for (int u = 0; u < AHEAD; u++) {
-            if (e + u * SORT_THREADS < end && in_bounds(sender[u], n_nodes)) {
-                atomicAdd(&histogram[sender[u] >> shift], 1);
+            const int32_t under = listed_under(sender[u], known, n_nodes);
+            if (e + u * SORT_THREADS < end && under >= 0) {
+                atomicAdd(&histogram[under >> shift], 1);
             }
         }
     }
@@ -61,13 +68,14 @@ __global__ __launch_bounds__(SORT_THREADS) void count_buckets_kernel(
 }
 
 /// The edges into their buckets, in ascending order. With one sender per bucket this is the result;
-/// `offsets`: where every bucket begins, and where the last one ends. `pitch`: the buckets, rounded
-/// up to a multiple of four.
+/// `offsets`: where every bucket begins, and where the last one ends (as many of these as there are places in it,
+/// n_offsets). `pitch`: the buckets, rounded up to a multiple of four.
 /// LDS: counters[wavefronts][pitch], before[pitch], total[pitch], of_wave[wavefronts].
 __global__ __launch_bounds__(SORT_THREADS) void fill_buckets_kernel(
     int32_t* __restrict__ sender_of_place, int32_t* __restrict__ edge_of_place, int32_t* __restrict__ offsets,
-    const int32_t* __restrict__ counts, const int32_t* __restrict__ senders, int32_t n_edges, int32_t n_nodes, int shift,
-    int32_t buckets, int32_t pitch, int bits, int32_t share, int packed_above
+    const int32_t* __restrict__ counts, const int32_t* __restrict__ senders, int32_t n_edges, int32_t n_nodes,
+    int32_t known, int shift, int32_t buckets, int32_t pitch, int bits, int32_t share, int packed_above,
+    int32_t n_offsets
 ) {
     constexpr int WAVES = SORT_THREADS / WAVE;
     extern __shared__ int32_t shared[];
@@ -79,8 +87,8 @@ __global__ __launch_bounds__(SORT_THREADS) void fill_buckets_kernel(
     const int32_t first = blockIdx.x * share, last = first + min(share, n_edges - first);
     const WaveShare mine(first, last, wave, WAVES);
     auto item_at = [&](int32_t e) {
-        const int32_t sender = senders[e];
-        return Item{in_bounds(sender, n_nodes) ? sender >> shift : -1, e, sender};
+        const int32_t sender = listed_under(senders[e], known, n_nodes);
+        return Item{sender >> shift, e, sender}; // (-1 stays -1)
     };
     for (int32_t b = threadIdx.x; b < pitch; b += SORT_THREADS) {
         before[b] = 0;
@@ -124,10 +132,10 @@ __global__ __launch_bounds__(SORT_THREADS) void fill_buckets_kernel(
     __syncthreads();
     const int32_t listed = scan_in_place<WAVES>(total, buckets, 0, of_wave);
     if (blockIdx.x == 0) {
-        for (int32_t bucket = threadIdx.x; bucket < buckets; bucket += SORT_THREADS) {
+        for (int32_t bucket = threadIdx.x; bucket < min(buckets, n_offsets); bucket += SORT_THREADS) {
             offsets[bucket] = total[bucket];
         }
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0 && buckets < n_offsets) {
             offsets[buckets] = listed;
         }
     }
@@ -158,7 +166,8 @@ template <int WAVES>
 __global__ __launch_bounds__(WAVES* WAVE) void sort_buckets_kernel(
     int32_t* __restrict__ sender_of_place, int32_t* __restrict__ edge_of_place, int32_t* __restrict__ offsets,
     const int32_t* __restrict__ bucket_offsets, const int32_t* __restrict__ senders, const int32_t* __restrict__ edges,
-    int packed_above, int32_t n_edges, int32_t n_nodes, int shift, int32_t at_a_time, int bits, int32_t staged_room
+    int packed_above, int32_t n_edges, int32_t n_nodes, int shift, int32_t at_a_time, int bits, int32_t staged_room,
+    int32_t n_offsets
 ) {
     extern __shared__ int32_t shared[];
     const int lane = threadIdx.x & (WAVE - 1), wave = threadIdx.x / WAVE;
@@ -196,7 +205,9 @@ __global__ __launch_bounds__(WAVES* WAVE) void sort_buckets_kernel(
         __syncthreads();
         place0 = scan_in_place<WAVES>(start, keys, place0, of_wave);
         for (int32_t key = threadIdx.x; key < keys; key += blockDim.x) {
-            offsets[node0 + base + key] = start[key];
+            if (node0 + base + key < n_offsets) {
+                offsets[node0 + base + key] = start[key];
+            }
         }
         starts_of_waves<WAVES>(counters, keys, [&](int32_t key) { return start[key]; });
         place_keys<4>(held, counters, keys, bits, mine, wave, lane, item_at, [&](int32_t place, const Item& item) {
@@ -221,7 +232,7 @@ __global__ __launch_bounds__(WAVES* WAVE) void sort_buckets_kernel(
         }
     }
     if (blockIdx.x == gridDim.x - 1) {
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0 && n_nodes < n_offsets) {
             offsets[n_nodes] = end;
         }
         for (int32_t place = end + static_cast<int32_t>(threadIdx.x); place < n_edges; place += blockDim.x) {
@@ -415,6 +426,59 @@ size_t edges_by_sender_bytes(int32_t n_nodes, int32_t n_edges, bool with_senders
            (2 + with_senders + senders_in_buckets) * align256(static_cast<size_t>(n_edges) * 4);
 }
 
+namespace {
+
+/// The launches of the sort. `offsets` has n_offsets places, edge (and sender, unless null) n_edges.
+/// `workspace`: what edges_by_sender_bytes counts behind the offsets.
+void sort_by_sender(
+    int32_t* offsets, int32_t n_offsets, int32_t* edge, int32_t* sender, int32_t* bucket_offsets,
+    int32_t* edge_in_buckets, int32_t* sender_in_buckets, const int32_t* senders, int32_t n_edges, int32_t n_nodes,
+    int32_t known, const SortPlan& plan, hipStream_t stream
+) {
+    const bool two_levels = plan.shift > 0;
+    // The counts of several shares lie where nothing is written by the launch that reads them. They
+    // fit: a share is 1024 edges or more, and there are 512 buckets at most.
+    int32_t* counts = two_levels ? edge : edge_in_buckets;
+    if (plan.shares > 1) {
+        count_buckets_kernel<<<plan.shares, SORT_THREADS, 0, stream>>>(
+            counts, senders, n_edges, n_nodes, known, plan.shift, plan.pitch, plan.share
+        );
+    }
+    constexpr int WAVES = SORT_THREADS / WAVE;
+    const size_t lds = (static_cast<size_t>(WAVES + 2) * plan.pitch + WAVES) * sizeof(int32_t);
+    fill_buckets_kernel<<<plan.shares, SORT_THREADS, lds, stream>>>(
+        two_levels ? sender_in_buckets : sender, two_levels ? edge_in_buckets : edge,
+        two_levels ? bucket_offsets : offsets, counts, senders, n_edges, n_nodes, known, plan.shift, plan.buckets,
+        plan.pitch, bits_for(plan.buckets), plan.share, plan.packed_above, two_levels ? plan.buckets + 1 : n_offsets
+    );
+    if (two_levels) {
+        const int32_t at_a_time = std::min(int32_t(1) << plan.shift, SENDERS_AT_A_TIME);
+        // (the counters of all wavefronts within 64 KB)
+        auto sort = [&](auto with_waves) {
+            constexpr int WAVES = decltype(with_waves)::value;
+            const int32_t room = WAVES >= 4 ? STAGED : 0;
+            const size_t sort_lds = (static_cast<size_t>(WAVES + 1) * at_a_time + WAVES + room) * sizeof(int32_t);
+            sort_buckets_kernel<WAVES><<<plan.buckets, WAVES * WAVE, sort_lds, stream>>>(
+                sender, edge, offsets, bucket_offsets, sender_in_buckets, edge_in_buckets,
+                plan.packed_above, n_edges, n_nodes, plan.shift, at_a_time, bits_for(at_a_time), room, n_offsets
+            );
+        };
+        // (within 64 KB: the counters of all wavefronts, and the edges of a bucket where there is room)
+        if (at_a_time <= 512) {
+            sort(std::integral_constant<int, 16>{});
+        } else if (at_a_time <= 1024) {
+            sort(std::integral_constant<int, 8>{});
+        } else if (at_a_time <= 2048) {
+            sort(std::integral_constant<int, 4>{});
+        } else {
+            sort(std::integral_constant<int, 2>{});
+        }
+    }
+    MOPS_HIP_CHECK(hipGetLastError());
+}
+
+} // namespace
+
 EdgesBySender order_edges_by_sender(
     const int32_t* senders, int32_t n_edges, int32_t n_nodes, bool with_senders, void* workspace, hipStream_t stream
 ) {
@@ -437,48 +501,40 @@ EdgesBySender order_edges_by_sender(
         return EdgesBySender{sender, edge, offsets};
     }
     const SortPlan plan = sort_plan(n_nodes, n_edges);
-    const bool two_levels = plan.shift > 0;
     int32_t* sender_in_buckets = plan.packed_above == 32 ? take(static_cast<size_t>(n_edges)) : nullptr;
-    // The counts of several shares lie where nothing is written by the launch that reads them. They
-    // fit: a share is 1024 edges or more, and there are 512 buckets at most.
-    int32_t* counts = two_levels ? edge : edge_in_buckets;
-    if (plan.shares > 1) {
-        count_buckets_kernel<<<plan.shares, SORT_THREADS, 0, stream>>>(
-            counts, senders, n_edges, n_nodes, plan.shift, plan.pitch, plan.share
-        );
-    }
-    constexpr int WAVES = SORT_THREADS / WAVE;
-    const size_t lds = (static_cast<size_t>(WAVES + 2) * plan.pitch + WAVES) * sizeof(int32_t);
-    fill_buckets_kernel<<<plan.shares, SORT_THREADS, lds, stream>>>(
-        two_levels ? sender_in_buckets : sender, two_levels ? edge_in_buckets : edge,
-        two_levels ? bucket_offsets : offsets, counts, senders, n_edges, n_nodes, plan.shift, plan.buckets,
-        plan.pitch, bits_for(plan.buckets), plan.share, plan.packed_above
+    sort_by_sender(
+        offsets, n_nodes + 1, edge, sender, bucket_offsets, edge_in_buckets, sender_in_buckets, senders, n_edges,
+        n_nodes, n_nodes, plan, stream
     );
-    if (two_levels) {
-        const int32_t at_a_time = std::min(int32_t(1) << plan.shift, SENDERS_AT_A_TIME);
-        // (the counters of all wavefronts within 64 KB)
-        auto sort = [&](auto with_waves) {
-            constexpr int WAVES = decltype(with_waves)::value;
-            const int32_t room = WAVES >= 4 ? STAGED : 0;
-            const size_t sort_lds = (static_cast<size_t>(WAVES + 1) * at_a_time + WAVES + room) * sizeof(int32_t);
-            sort_buckets_kernel<WAVES><<<plan.buckets, WAVES * WAVE, sort_lds, stream>>>(
-                sender, edge, offsets, bucket_offsets, sender_in_buckets, edge_in_buckets,
-                plan.packed_above, n_edges, n_nodes, plan.shift, at_a_time, bits_for(at_a_time), room
-            );
-        };
-        // (within 64 KB: the counters of all wavefronts, and the edges of a bucket where there is room)
-        if (at_a_time <= 512) {
-            sort(std::integral_constant<int, 16>{});
-        } else if (at_a_time <= 1024) {
-            sort(std::integral_constant<int, 8>{});
-        } else if (at_a_time <= 2048) {
-            sort(std::integral_constant<int, 4>{});
-        } else {
-            sort(std::integral_constant<int, 2>{});
-        }
-    }
-    MOPS_HIP_CHECK(hipGetLastError());
     return EdgesBySender{sender, edge, offsets};
+}
+
+size_t order_all_by_group_bytes(int32_t groups, int32_t n_rows) {
+    return edges_by_sender_bytes(groups + 1, n_rows, false);
+}
+
+void order_all_by_group(
+    int32_t* order, int32_t* offsets, const int32_t* indices, int32_t n_rows, int32_t groups, void* workspace,
+    hipStream_t stream
+) {
+    if (n_rows < 1) {
+        clear_counters(offsets, static_cast<size_t>(groups) + 1, stream);
+        return;
+    }
+    char* at = static_cast<char*>(workspace);
+    auto take = [&](size_t integers) {
+        int32_t* p = reinterpret_cast<int32_t*>(at);
+        at += align256(integers * 4);
+        return p;
+    };
+    int32_t* bucket_offsets = take(MOST_BUCKETS + 1);
+    int32_t* row_in_buckets = take(static_cast<size_t>(n_rows));
+    const SortPlan plan = sort_plan(groups + 1, n_rows);
+    int32_t* group_in_buckets = plan.packed_above == 32 ? take(static_cast<size_t>(n_rows)) : nullptr;
+    sort_by_sender(
+        offsets, groups + 1, order, nullptr, bucket_offsets, row_in_buckets, group_in_buckets, indices, n_rows,
+        groups + 1, groups, plan, stream
+    );
 }
 
 } // namespace mops::amd

@@ -45,6 +45,15 @@ EdgesBySender order_edges_by_sender(
     const int32_t* senders, int32_t n_edges, int32_t n_nodes, bool with_senders, void* workspace, hipStream_t stream
 );
 
+/// The same sort with nothing left out, into arrays of the caller: order [n_rows] is a permutation of the rows,
+/// those whose index is outside [0, groups) behind all others; offsets [groups + 1]. groups below the largest
+/// integer; `workspace`: order_all_by_group_bytes() bytes.
+size_t order_all_by_group_bytes(int32_t groups, int32_t n_rows);
+void order_all_by_group(
+    int32_t* order, int32_t* offsets, const int32_t* indices, int32_t n_rows, int32_t groups, void* workspace,
+    hipStream_t stream
+);
+
 /// Sparse graphs (a few dozen edges per sender): every sender owns
 /// SLOT_CAPACITY places, so no offsets have to be known before the lists are
 /// written and ONE launch does it, without counters shared between workgroups

@@ -12,6 +12,7 @@
 #include <torch/types.h>
 
 #include "mops/amd.h"
+#include "mops/layers.hpp"
 #include "mops/tensor.hpp"
 
 namespace mops::amd::torch_tensors {
@@ -29,7 +30,11 @@ template <typename T, size_t N> mops::Tensor<T, N> view(const at::Tensor& tensor
             std::string(name) + " must have " + std::to_string(N) + " dimensions, got " + std::to_string(tensor.dim())
         );
     }
-    result.data = tensor.data_ptr<T>();
+    if constexpr (sizeof(T) == 2) { // (the bits; by_layer_dtype has looked at the type)
+        result.data = static_cast<T*>(tensor.data_ptr());
+    } else {
+        result.data = tensor.data_ptr<T>();
+    }
     for (size_t d = 0; d < N; d++) {
         result.shape[d] = static_cast<size_t>(tensor.size(static_cast<int64_t>(d)));
     }
@@ -52,6 +57,20 @@ template <typename Body> void by_dtype(const at::Tensor& like, Body&& body) {
         body(float{});
     } else {
         body(double{});
+    }
+}
+
+/// The element types of the layers' operators (mops/layers.h).
+inline bool is_layer_dtype(at::ScalarType type) {
+    return type == at::kFloat || type == at::kDouble || type == at::kBFloat16 || type == at::kHalf;
+}
+template <typename Body> void by_layer_dtype(const at::Tensor& like, Body&& body) {
+    if (like.scalar_type() == at::kBFloat16) {
+        body(mops::bfloat16{});
+    } else if (like.scalar_type() == at::kHalf) {
+        body(mops::float16{});
+    } else {
+        by_dtype(like, body);
     }
 }
 
