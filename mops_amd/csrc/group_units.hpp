@@ -40,19 +40,31 @@ struct GroupUnit {
     int32_t index, of_group; // which unit of its group this is, and how many the group has
 };
 
+/// What becomes of a group without rows, and of the rows without a group.
+enum class Units {
+    OF_ROWS,  // no unit for an empty group; units of the rows of no group behind all others
+    OF_GROUPS // a unit (of no places) for an empty group; none for the rows of no group
+};
+
 /// Units there are at most.
 inline size_t most_units(int32_t n_rows, int32_t n_groups, int32_t step) {
     return (static_cast<size_t>(n_rows) + step - 1) / step + static_cast<size_t>(n_groups) + 1;
 }
 
+/// The units of a group with `count` places.
+template <Units WHICH> __device__ __forceinline__ int32_t units_of(int32_t count, int32_t step) {
+    return max((count + step - 1) / step, WHICH == Units::OF_GROUPS ? 1 : 0);
+}
+
 /// Unit number `unit`, by every wavefront for itself (64 groups per step). All lanes.
-__device__ __forceinline__ GroupUnit find_unit(const RowGroups& groups, int32_t step, int32_t unit, bool with_rest) {
+template <Units WHICH>
+__device__ __forceinline__ GroupUnit find_unit(const RowGroups& groups, int32_t step, int32_t unit) {
     const int lane = threadIdx.x & (WAVE - 1);
     for (int32_t base = 0; base < groups.n_groups; base += WAVE) {
         const int32_t group = min(base + lane, groups.n_groups - 1);
         const int32_t begin = groups.begin_of(group);
-        const int32_t count = base + lane < groups.n_groups ? groups.end_of(group, begin) - begin : 0;
-        const int32_t units = (count + step - 1) / step;
+        const int32_t count = groups.end_of(group, begin) - begin;
+        const int32_t units = base + lane < groups.n_groups ? units_of<WHICH>(count, step) : 0;
         int32_t upto = units;
 #pragma unroll
         for (int s = 1; s < WAVE; s <<= 1) {
@@ -70,7 +82,7 @@ __device__ __forceinline__ GroupUnit find_unit(const RowGroups& groups, int32_t 
         }
         unit -= __builtin_amdgcn_readlane(upto, WAVE - 1);
     }
-    if (with_rest) {
+    if (WHICH == Units::OF_ROWS) {
         const int32_t first = groups.begin_of(0), listed = groups.end_of(groups.n_groups - 1, first) - first;
         const int32_t rest = groups.n_rows - listed, units = (rest + step - 1) / step;
         if (unit < units) {
@@ -78,6 +90,26 @@ __device__ __forceinline__ GroupUnit find_unit(const RowGroups& groups, int32_t 
         }
     }
     return GroupUnit{-1, 0, 0, 0, 0};
+}
+
+/// How many units there are. All lanes of a wavefront.
+template <Units WHICH> __device__ __forceinline__ int32_t count_units(const RowGroups& groups, int32_t step) {
+    const int lane = threadIdx.x & (WAVE - 1);
+    int32_t total = 0;
+    for (int32_t group = lane; group < groups.n_groups; group += WAVE) {
+        const int32_t begin = groups.begin_of(group);
+        total += units_of<WHICH>(groups.end_of(group, begin) - begin, step);
+    }
+#pragma unroll
+    for (int s = 1; s < WAVE; s <<= 1) {
+        total += __shfl_xor(total, s);
+    }
+    if (WHICH == Units::OF_ROWS) {
+        const int32_t first = groups.begin_of(0);
+        const int32_t rest = groups.n_rows - (groups.end_of(groups.n_groups - 1, first) - first);
+        total += (rest + step - 1) / step;
+    }
+    return total;
 }
 
 /// The place of number `i` of the rows that belong to no group: before the first group's places, or behind the last's.

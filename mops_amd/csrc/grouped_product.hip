@@ -14,6 +14,7 @@
 #include "checks.hpp"
 #include "device_common.hpp"
 #include "group_units.hpp"
+#include "grouped_tiles.hpp"
 #include "numbers.hpp"
 #include "runtime.hpp"
 
@@ -21,126 +22,74 @@ namespace mops::amd {
 namespace grouped_product {
 namespace {
 
-/// out[r, n] = sum_k x[r, k] w(g, k, n), with w(g, k, n) at g * k_size * n_size + k * step_k + n * step_n.
-template <typename T> struct RowsTimes {
-    T* out;
-    const T *x, *w;
-    RowGroups groups;
-    int32_t k_size, n_size;
-    int32_t step_k, step_n;
-};
+unsigned tiles(int32_t size, int tile) { return static_cast<unsigned>(ceil_div(static_cast<size_t>(size), tile)); }
 
-/// out[g, m, n] = sum over the rows r of group g of a[r, m] b[r, n].
-template <typename T> struct SumOfRows {
-    T* out;
-    const T *a, *b;
-    RowGroups groups;
-    int32_t m_size, n_size;
-};
-
-// Tiles of 64 x 64 numbers, 16 of them per lane, through LDS in steps of 16.
-constexpr int TILE = 64, STEP = 16, THREADS = 256;
-
-/// sum[4][4] += the product of two tiles in LDS, [STEP][TILE] each.
-template <typename W>
-__device__ __forceinline__ void multiply_tiles(W (&sum)[4][4], const W (*a)[TILE + 1], const W (*b)[TILE + 1]) {
-    const int m = threadIdx.x / 16, n = threadIdx.x % 16;
-#pragma unroll
-    for (int k = 0; k < STEP; k++) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                sum[i][j] += a[k][m + 16 * i] * b[k][n + 16 * j];
-            }
-        }
+template <typename T, Form FORM, int BM, int BN, int WM, int WN> void launch(Product<T> g, hipStream_t stream) {
+    constexpr bool SUMS = FORM == Form::GRAD_SUMS;
+    g.m_tiles = SUMS ? static_cast<int32_t>(tiles(g.m_size, BM)) : 1;
+    g.n_tiles = static_cast<int32_t>(tiles(g.n_size, BN));
+    if (!SUMS) {
+        g.step = BM;
     }
+    g.most_units = narrow_i32(most_units(g.groups.n_rows, g.groups.n_groups, g.step), "number of units of rows");
+    const size_t workgroups = ceil_div(static_cast<size_t>(g.most_units) * g.m_tiles * g.n_tiles, 8) * 8;
+    tiles_kernel<T, FORM, BM, BN, WM, WN>
+        <<<static_cast<unsigned>(narrow_i32(workgroups, "number of tiles")), WM * WN * WAVE, 0, stream>>>(g);
 }
 
-template <typename T> __global__ __launch_bounds__(THREADS) void rows_kernel(RowsTimes<T> p) {
-    typedef wide_t<T> W;
-    __shared__ W x[STEP][TILE + 1], w[STEP][TILE + 1];
-    __shared__ int32_t rows[TILE];
-    const GroupUnit unit = find_unit(p.groups, TILE, blockIdx.x, true);
-    if (unit.group < 0) {
-        return; // (uniform)
-    }
-    const bool rest = unit.group == p.groups.n_groups;
-    const int32_t n0 = blockIdx.y * TILE;
-    if (threadIdx.x < TILE) {
-        const int32_t i = min(static_cast<int32_t>(threadIdx.x), unit.count - 1);
-        rows[threadIdx.x] =
-            p.groups.row_at(rest ? place_of_rest(p.groups, unit.begin + i) : unit.begin + i);
-    }
-    __syncthreads();
-    W sum[4][4] = {};
-    if (!rest) {
-        const T* of_group = p.w + static_cast<size_t>(unit.group) * p.k_size * p.n_size;
-        for (int32_t k0 = 0; k0 < p.k_size; k0 += STEP) {
-            for (int i = threadIdx.x; i < STEP * TILE; i += THREADS) {
-                const int k = i % STEP, m = i / STEP;
-                x[k][m] = k0 + k < p.k_size ? static_cast<W>(p.x[static_cast<size_t>(rows[m]) * p.k_size + k0 + k]) : W(0);
-            }
-            for (int i = threadIdx.x; i < STEP * TILE; i += THREADS) {
-                const int k = p.step_k == 1 ? i % STEP : i / TILE, n = p.step_k == 1 ? i / STEP : i % TILE;
-                w[k][n] = k0 + k < p.k_size && n0 + n < p.n_size
-                              ? static_cast<W>(of_group[static_cast<size_t>(k0 + k) * p.step_k + static_cast<size_t>(n0 + n) * p.step_n])
-                              : W(0);
-            }
-            __syncthreads();
-            multiply_tiles<W>(sum, x, w);
-            __syncthreads();
+template <typename T, Form FORM> void rows_times(const Product<T>& g, hipStream_t stream) {
+    const size_t rows = static_cast<size_t>(g.groups.n_rows);
+    const size_t big = ceil_div(rows, 256) * tiles(g.n_size, 256), middle = ceil_div(rows, 128) * tiles(g.n_size, 128);
+    const size_t units = static_cast<size_t>(compute_units());
+    if (sizeof(T) == 2 && big >= units && rows >= 128 * static_cast<size_t>(g.groups.n_groups)) {
+        if constexpr (sizeof(T) == 2) {
+            launch<T, FORM, 256, 256, 2, 4>(g, stream);
         }
+    } else if (middle >= units && rows >= 64 * static_cast<size_t>(g.groups.n_groups)) {
+        launch<T, FORM, 128, 128, 2, 2>(g, stream);
+    } else {
+        launch<T, FORM, 64, 64, 2, 2>(g, stream);
     }
-    const int m = threadIdx.x / 16, n = threadIdx.x % 16;
-    for (int i = 0; i < 4; i++) {
-        for (int j = 0; j < 4; j++) {
-            if (m + 16 * i < unit.count && n0 + n + 16 * j < p.n_size) {
-                p.out[static_cast<size_t>(rows[m + 16 * i]) * p.n_size + n0 + n + 16 * j] = static_cast<T>(sum[i][j]);
-            }
-        }
-    }
-}
-
-template <typename T> __global__ __launch_bounds__(THREADS) void sums_kernel(SumOfRows<T> p) {
-    typedef wide_t<T> W;
-    __shared__ W a[STEP][TILE + 1], b[STEP][TILE + 1];
-    const int32_t m0 = blockIdx.x * TILE, n0 = blockIdx.y * TILE;
-    const int32_t begin = p.groups.begin_of(blockIdx.z), end = p.groups.end_of(blockIdx.z, begin);
-    W sum[4][4] = {};
-    for (int32_t place0 = begin; place0 < end; place0 += STEP) {
-        for (int i = threadIdx.x; i < STEP * TILE; i += THREADS) {
-            const int k = i / TILE, at = i % TILE;
-            const bool inside = place0 + k < end;
-            const size_t row = inside ? p.groups.row_at(place0 + k) : 0;
-            a[k][at] = inside && m0 + at < p.m_size ? static_cast<W>(p.a[row * p.m_size + m0 + at]) : W(0);
-            b[k][at] = inside && n0 + at < p.n_size ? static_cast<W>(p.b[row * p.n_size + n0 + at]) : W(0);
-        }
-        __syncthreads();
-        multiply_tiles<W>(sum, a, b);
-        __syncthreads();
-    }
-    const int m = threadIdx.x / 16, n = threadIdx.x % 16;
-    T* out = p.out + static_cast<size_t>(blockIdx.z) * p.m_size * p.n_size;
-    for (int i = 0; i < 4; i++) {
-        for (int j = 0; j < 4; j++) {
-            if (m0 + m + 16 * i < p.m_size && n0 + n + 16 * j < p.n_size) {
-                out[static_cast<size_t>(m0 + m + 16 * i) * p.n_size + n0 + n + 16 * j] = static_cast<T>(sum[i][j]);
-            }
-        }
-    }
-}
-
-unsigned tiles(int32_t size) { return static_cast<unsigned>(ceil_div(static_cast<size_t>(size), TILE)); }
-
-template <typename T> void rows_times(const RowsTimes<T>& p, hipStream_t stream) {
-    const size_t units = most_units(p.groups.n_rows, p.groups.n_groups, TILE);
-    rows_kernel<T><<<dim3(static_cast<unsigned>(units), tiles(p.n_size)), THREADS, 0, stream>>>(p);
     MOPS_HIP_CHECK(hipGetLastError());
 }
 
-template <typename T> void sum_of_rows(const SumOfRows<T>& p, hipStream_t stream) {
-    sums_kernel<T><<<dim3(tiles(p.m_size), tiles(p.n_size), static_cast<unsigned>(p.groups.n_groups)), THREADS, 0, stream>>>(p);
+template <typename T> void sum_of_rows(Product<T> g, hipStream_t stream) {
+    const size_t units = static_cast<size_t>(compute_units()), groups = static_cast<size_t>(g.groups.n_groups);
+    const size_t rows = static_cast<size_t>(std::max(g.groups.n_rows, 1));
+    const size_t big = static_cast<size_t>(tiles(g.m_size, 256)) * tiles(g.n_size, 256);
+    const size_t middle = static_cast<size_t>(tiles(g.m_size, 128)) * tiles(g.n_size, 128);
+    const bool use_big = sizeof(T) == 2 && big * groups >= units;
+    const bool use_middle = g.m_size > 64 && g.n_size > 64;
+    const size_t tiles_of_unit =
+        use_big ? big : use_middle ? middle : static_cast<size_t>(tiles(g.m_size, 64)) * tiles(g.n_size, 64);
+    size_t step = rows;
+    if (tiles_of_unit * groups >= units) {
+        step = std::max<size_t>(4 * rows / groups, 4096);
+    } else {
+        step = std::max<size_t>(ceil_div(rows, ceil_div(2 * units, tiles_of_unit)), 256);
+    }
+    step = std::min(ceil_div(step, 64) * 64, ceil_div(rows, 64) * 64);
+    g.step = static_cast<int32_t>(step);
+    const bool splits = step < rows;
+    const size_t most = most_units(g.groups.n_rows, g.groups.n_groups, g.step);
+    const size_t size = static_cast<size_t>(g.m_size) * g.n_size;
+    if (splits) {
+        g.partial = static_cast<wide_t<T>*>(scratch(most * size * sizeof(wide_t<T>)));
+    }
+    if (use_big) {
+        if constexpr (sizeof(T) == 2) {
+            launch<T, Form::GRAD_SUMS, 256, 256, 2, 4>(g, stream);
+        }
+    } else if (use_middle) {
+        launch<T, Form::GRAD_SUMS, 128, 128, 2, 2>(g, stream);
+    } else {
+        launch<T, Form::GRAD_SUMS, 64, 64, 2, 2>(g, stream);
+    }
+    if (splits) {
+        const unsigned blocks = static_cast<unsigned>(std::min<size_t>(ceil_div(size, JOIN_THREADS), 4 * units));
+        g.most_units = narrow_i32(most, "number of units of rows");
+        join_units_kernel<T><<<dim3(static_cast<unsigned>(most), blocks), JOIN_THREADS, 0, stream>>>(g);
+    }
     MOPS_HIP_CHECK(hipGetLastError());
 }
 
@@ -189,10 +138,14 @@ void grouped_matrix_product(
     const int32_t K = count_i32(W.shape[1], "W.shape[1]"), L = count_i32(W.shape[2], "W.shape[2]");
     if (groups.n_rows > 0 && L > 0) {
         typedef device_t<scalar_t> T;
-        grouped_product::rows_times(
-            grouped_product::RowsTimes<T>{data_of(output), data_of(A), data_of(W), groups, K, L, L, 1},
-            current_stream()
-        );
+        grouped_product::Product<T> g{};
+        g.out = data_of(output);
+        g.q = data_of(A);
+        g.p = data_of(W);
+        g.groups = groups;
+        g.n_size = L;
+        g.k_size = K;
+        grouped_product::rows_times<T, grouped_product::Form::FORWARD>(g, current_stream());
     }
     finish_call("grouped_matrix_product");
 }
@@ -219,16 +172,24 @@ void grouped_matrix_product_vjp(
     const int32_t K = count_i32(W.shape[1], "W.shape[1]"), L = count_i32(W.shape[2], "W.shape[2]");
     typedef device_t<scalar_t> T;
     if (grad_A.data != nullptr && groups.n_rows > 0 && K > 0) {
-        grouped_product::rows_times(
-            grouped_product::RowsTimes<T>{data_of(grad_A), data_of(grad_output), data_of(W), groups, L, K, 1, L},
-            current_stream()
-        );
+        grouped_product::Product<T> g{};
+        g.out = data_of(grad_A);
+        g.q = data_of(grad_output);
+        g.p = data_of(W);
+        g.groups = groups;
+        g.n_size = K;
+        g.k_size = L;
+        grouped_product::rows_times<T, grouped_product::Form::GRAD_ROWS>(g, current_stream());
     }
     if (grad_W.data != nullptr && groups.n_groups > 0 && K > 0 && L > 0) {
-        grouped_product::sum_of_rows(
-            grouped_product::SumOfRows<T>{data_of(grad_W), data_of(A), data_of(grad_output), groups, K, L},
-            current_stream()
-        );
+        grouped_product::Product<T> g{};
+        g.out = data_of(grad_W);
+        g.q = data_of(A);
+        g.p = data_of(grad_output);
+        g.groups = groups;
+        g.m_size = K;
+        g.n_size = L;
+        grouped_product::sum_of_rows(g, current_stream());
     }
     finish_call("grouped_matrix_product_vjp");
 }
