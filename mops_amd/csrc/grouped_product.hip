@@ -24,6 +24,17 @@ namespace {
 
 unsigned tiles(int32_t size, int tile) { return static_cast<unsigned>(ceil_div(static_cast<size_t>(size), tile)); }
 
+/// Rows of `width` numbers that all begin on 16-byte boundaries.
+template <typename T> bool aligned(const T* data, int32_t width) {
+    return reinterpret_cast<uintptr_t>(data) % 16 == 0 && static_cast<size_t>(width) * sizeof(T) % 16 == 0;
+}
+template <typename T, Form FORM> int32_t q_width(const Product<T>& g) {
+    return FORM == Form::GRAD_SUMS ? g.m_size : g.k_size;
+}
+template <typename T, Form FORM> int32_t p_width(const Product<T>& g) {
+    return FORM == Form::GRAD_ROWS ? g.k_size : g.n_size;
+}
+
 template <typename T, Form FORM, int BM, int BN, int WM, int WN> void launch(Product<T> g, hipStream_t stream) {
     constexpr bool SUMS = FORM == Form::GRAD_SUMS;
     g.m_tiles = SUMS ? static_cast<int32_t>(tiles(g.m_size, BM)) : 1;
@@ -33,8 +44,12 @@ template <typename T, Form FORM, int BM, int BN, int WM, int WN> void launch(Pro
     }
     g.most_units = narrow_i32(most_units(g.groups.n_rows, g.groups.n_groups, g.step), "number of units of rows");
     const size_t workgroups = ceil_div(static_cast<size_t>(g.most_units) * g.m_tiles * g.n_tiles, 8) * 8;
-    tiles_kernel<T, FORM, BM, BN, WM, WN>
-        <<<static_cast<unsigned>(narrow_i32(workgroups, "number of tiles")), WM * WN * WAVE, 0, stream>>>(g);
+    const unsigned blocks = static_cast<unsigned>(narrow_i32(workgroups, "number of tiles"));
+    if (aligned(g.q, q_width<T, FORM>(g)) && aligned(g.p, p_width<T, FORM>(g))) {
+        tiles_kernel<T, FORM, BM, BN, WM, WN, true><<<blocks, WM * WN * WAVE, 0, stream>>>(g);
+    } else {
+        tiles_kernel<T, FORM, BM, BN, WM, WN, false><<<blocks, WM * WN * WAVE, 0, stream>>>(g);
+    }
 }
 
 template <typename T, Form FORM> void rows_times(const Product<T>& g, hipStream_t stream) {

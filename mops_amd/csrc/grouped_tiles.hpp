@@ -13,17 +13,25 @@
 //             the rows of the group
 //
 // A side goes through LDS in steps of 128 bytes of k (64 numbers of 16 bits, 32
-// of 32, 16 of 64), double-buffered: while a step is multiplied, the next one is
-// on its way to registers, and goes to the other buffer when it has arrived; one
-// barrier per step. A side whose k is contiguous in memory ("straight") lies in
-// LDS as it is read by the matrix instructions, [outer][k], in pieces of 16
-// bytes that are permuted within a row so that the rows of a block fall into
-// different banks. A side whose k is the row of memory ("turned") lies in LDS as
-// [k][outer]; 16-bit numbers are turned by the LDS's transposing reads, wider
-// ones are read one by one. Pieces of memory are loaded at any alignment; what
-// lies outside a side in the direction of k is zero in LDS (never a value from
-// somewhere else: 0 x infinity is not 0), what lies outside in the other
+// of 32, 16 of 64), double-buffered. A side whose k is contiguous in memory
+// ("straight") lies in LDS as it is read by the matrix instructions,
+// [outer][k], in pieces of 16 bytes that are permuted within a row so that the
+// rows of a block fall into different banks. A side whose k is the row of memory
+// ("turned") lies in LDS as [k][outer]; 16-bit numbers are turned by the LDS's
+// transposing reads, wider ones are read one by one. Either way piece i of a
+// buffer is the business of thread i (i + THREADS, ..), so that a piece can go
+// from memory to LDS without a register (ALIGNED: rows that begin on 16-byte
+// boundaries, in which a piece is inside a row or outside as a whole), or
+// through registers (rows of any length, pieces at any alignment). What lies
+// outside a side in the direction of k is zero in LDS (never a value from
+// somewhere else: 0 x infinity is not 0); what lies outside in the other
 // direction is not stored.
+//
+// The numbers of a multiplication are read from LDS while the one before runs.
+// In front of the last multiplication of a step, whose numbers are in registers
+// by then, the workgroup meets: the step's buffer is free for the step after
+// the next, the next step's has arrived. So there is one barrier per step, and
+// nothing waits for LDS or memory behind it.
 #ifndef MOPS_AMD_GROUPED_TILES_HPP
 #define MOPS_AMD_GROUPED_TILES_HPP
 
@@ -111,11 +119,11 @@ constexpr int PIECES_OF_STEP = 8; // pieces of 16 bytes of k in LDS
 
 template <typename T> using Numbers = typename Matrix<T>::Numbers;
 
-/// The first `count` of a piece's numbers, zeros behind them (count may be negative, or beyond the piece).
-template <typename T> __device__ __forceinline__ Numbers<T> load_numbers(const T* from, int32_t count) {
+/// The first `count` of a piece's numbers, zeros behind them (count may be negative, or beyond the piece). WHOLE: all.
+template <typename T, bool WHOLE> __device__ __forceinline__ Numbers<T> load_numbers(const T* from, int32_t count) {
     constexpr int COUNT = Matrix<T>::COUNT;
     Numbers<T> v;
-    if (count >= COUNT) {
+    if (WHOLE || count >= COUNT) {
         typedef T Anywhere __attribute__((ext_vector_type(COUNT), aligned(sizeof(T))));
         const Anywhere a = *reinterpret_cast<const Anywhere*>(from);
 #pragma unroll
@@ -136,6 +144,8 @@ template <typename T, int OUTER> struct Straight {
     static __device__ __forceinline__ int place(int row, int piece) {
         return (row * PIECES_OF_STEP + (piece ^ (row >> 1 & 7))) * 16;
     }
+    /// which piece of its row lies at place i
+    static __device__ __forceinline__ int piece(int i) { return i % PIECES_OF_STEP ^ (i / PIECES_OF_STEP >> 1 & 7); }
     /// Numbers `step` of the k of a block that begins at row `outer0`.
     static __device__ __forceinline__ Numbers<T> read(const char* lds, int outer0, int step, int lane) {
         constexpr int BLOCK = Matrix<T>::BLOCK;
@@ -148,15 +158,18 @@ template <typename T, int OUTER> struct Straight {
 /// a transposing read look at fall into different banks.
 template <typename T, int OUTER> struct Turned {
     static constexpr int PIECES = OUTER / Matrix<T>::COUNT; // of a row of k
-    static __device__ __forceinline__ int place(int k, int piece) {
-        int at = piece;
+    static __device__ __forceinline__ int permuted(int k, int piece) {
         if constexpr (sizeof(T) == 2 && PIECES >= 16) {
-            at = piece ^ (k & 3) << 2;
+            return piece ^ (k & 3) << 2;
         } else if constexpr (sizeof(T) == 2 && PIECES == 8) {
-            at = piece ^ (k >> 1 & 1) << 2;
+            return piece ^ (k >> 1 & 1) << 2;
+        } else {
+            return piece;
         }
-        return (k * PIECES + at) * 16;
     }
+    static __device__ __forceinline__ int place(int k, int piece) { return (k * PIECES + permuted(k, piece)) * 16; }
+    /// which piece of its row lies at place i
+    static __device__ __forceinline__ int piece(int i) { return permuted(i / PIECES, i % PIECES); }
     static __device__ __forceinline__ Numbers<T> read(const char* lds, int outer0, int step, int lane) {
         constexpr int BLOCK = Matrix<T>::BLOCK, COUNT = Matrix<T>::COUNT;
         const int k0 = (step * (WAVE / BLOCK) + lane / BLOCK) * COUNT;
@@ -188,18 +201,55 @@ template <typename T, int OUTER> struct Turned {
     }
 };
 
-/// A straight side on its way to LDS: THREADS threads, OUTER rows.
-template <typename T, int OUTER, int THREADS> struct StraightLoader {
-    typedef Straight<T, OUTER> Layout;
+__device__ __constant__ const uint4 zeros_in_memory = {0, 0, 0, 0};
+
+/// 16 bytes from memory to LDS, at `lds` (the same for all lanes) + 16 * lane, without a register. Arrived when the
+/// wavefront's vmcnt says so, which `meet` waits for. (Not the builtin: behind it the compiler waits for vmcnt at the
+/// next read of LDS, of whichever buffer. There is no register here that it could lose track of.)
+__device__ __forceinline__ void fetch(const void* from, char* lds) {
+    const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "m0");
+}
+
+/// A side of the product on its way to LDS: piece i = threadIdx.x + j * THREADS, j < EACH.
+template <typename T, int OUTER, int THREADS, bool ALIGNED> struct Pieces {
     static constexpr int EACH = OUTER * PIECES_OF_STEP / THREADS, COUNT = Matrix<T>::COUNT;
+    Numbers<T> piece[ALIGNED ? 1 : EACH];
+
+    /// piece j: numbers `from` .. of a row, of which `left` are in the row (at most 0: none). WHOLE: all of them are,
+    /// or the side's row does not matter.
+    template <bool WHOLE> __device__ __forceinline__ void take(int j, const T* from, int32_t left, char* lds, int wave) {
+        if constexpr (ALIGNED) {
+            const void* at = WHOLE || left > 0 ? static_cast<const void*>(from) : &zeros_in_memory;
+            fetch(at, lds + (wave * WAVE + j * THREADS) * 16);
+        } else {
+            piece[j] = load_numbers<T, WHOLE>(from, left);
+        }
+    }
+    /// the pieces that came through registers
+    __device__ __forceinline__ void store(char* lds) const {
+        if constexpr (!ALIGNED) {
+#pragma unroll
+            for (int j = 0; j < EACH; j++) {
+                *reinterpret_cast<Numbers<T>*>(lds + (threadIdx.x + j * THREADS) * 16) = piece[j];
+            }
+        }
+    }
+};
+
+template <typename T, int OUTER, int THREADS, bool ALIGNED>
+struct StraightLoader : public Pieces<T, OUTER, THREADS, ALIGNED> {
+    typedef Pieces<T, OUTER, THREADS, ALIGNED> Base;
+    typedef Straight<T, OUTER> Layout;
+    using Base::COUNT;
+    using Base::EACH;
     const T* from[EACH];
-    Numbers<T> piece[EACH];
     int32_t k_size;
 
     static __device__ __forceinline__ int row(int j) { return (threadIdx.x + j * THREADS) / PIECES_OF_STEP; }
-    static __device__ __forceinline__ int of_row(int j) { return (threadIdx.x + j * THREADS) % PIECES_OF_STEP; }
+    static __device__ __forceinline__ int of_row(int j) { return Layout::piece((threadIdx.x + j * THREADS)); }
 
-    /// row_at(i): pointer to the row of memory behind row i of the side
+    /// row_at(i): pointer to the row of memory behind row i of the side (any one for a row that does not matter)
     template <typename RowAt> __device__ __forceinline__ void begin(int32_t k, RowAt&& row_at) {
         k_size = k;
 #pragma unroll
@@ -207,56 +257,70 @@ template <typename T, int OUTER, int THREADS> struct StraightLoader {
             from[j] = row_at(row(j)) + of_row(j) * COUNT;
         }
     }
-    __device__ __forceinline__ void load(int32_t k0) {
+    /// The next step, which begins at k0 (they are asked for in order).
+    template <bool WHOLE> __device__ __forceinline__ void load(int32_t k0, char* lds, int wave) {
 #pragma unroll
         for (int j = 0; j < EACH; j++) {
-            piece[j] = load_numbers<T>(from[j] + k0, k_size - k0 - of_row(j) * COUNT);
-        }
-    }
-    __device__ __forceinline__ void store(char* lds) const {
-#pragma unroll
-        for (int j = 0; j < EACH; j++) {
-            *reinterpret_cast<Numbers<T>*>(lds + Layout::place(row(j), of_row(j))) = piece[j];
+            this->template take<WHOLE>(j, from[j], k_size - k0 - of_row(j) * COUNT, lds, wave);
+            from[j] += PIECES_OF_STEP * COUNT;
         }
     }
 };
 
-/// A turned side: rows of `width` numbers, of which those from outer0 on are used.
-template <typename T, int OUTER, int THREADS> struct TurnedLoader {
+/// Rows of `width` numbers, of which those from outer0 on are used.
+template <typename T, int OUTER, int THREADS, bool ALIGNED>
+struct TurnedLoader : public Pieces<T, OUTER, THREADS, ALIGNED> {
+    typedef Pieces<T, OUTER, THREADS, ALIGNED> Base;
     typedef Turned<T, OUTER> Layout;
-    static constexpr int EACH = OUTER * PIECES_OF_STEP / THREADS, COUNT = Matrix<T>::COUNT;
-    Numbers<T> piece[EACH];
-    const T* from;
-    int32_t width, outer0;
+    using Base::COUNT;
+    using Base::EACH;
+    static constexpr int K_EACH = THREADS / Layout::PIECES; // rows of k between a thread's pieces
+    const T* from; // the thread's column of row 0 of the matrix; of the next step's first piece (load)
+    size_t next;   // numbers from a step to the next
+    size_t between; // numbers between a thread's pieces
+    int32_t left;   // numbers in the row from the thread's column on
 
-    static __device__ __forceinline__ int k(int j) { return (threadIdx.x + j * THREADS) / Layout::PIECES; }
-    static __device__ __forceinline__ int of_row(int j) { return (threadIdx.x + j * THREADS) % Layout::PIECES; }
+    static __device__ __forceinline__ int k(int j) { return threadIdx.x / Layout::PIECES + j * K_EACH; }
+    /// (the same for all pieces of a thread: their rows differ by multiples of four)
+    static __device__ __forceinline__ int of_row() { return Layout::piece(threadIdx.x); }
 
     __device__ __forceinline__ void begin(const T* memory, int32_t row_width, int32_t first) {
-        from = memory;
-        width = row_width;
-        outer0 = first;
+        static_assert(K_EACH % 4 == 0 && EACH * THREADS == OUTER * PIECES_OF_STEP, "");
+        const int32_t outer = first + of_row() * COUNT;
+        left = row_width - outer;
+        // (a piece that is outside of the rows: any piece that is not)
+        from = memory + (left > 0 ? outer : 0);
+        next = static_cast<size_t>(PIECES_OF_STEP * COUNT) * row_width;
+        between = static_cast<size_t>(K_EACH) * row_width;
     }
-    /// row_at(k): the row of memory, negative: none
-    template <typename RowAt> __device__ __forceinline__ void load(RowAt&& row_at) {
+    /// Every piece of the step inside of its row, or outside as a whole.
+    __device__ __forceinline__ bool whole() const { return ALIGNED || left >= COUNT || left <= 0; }
+
+    /// The next step of consecutive rows (after begin_rows), of which the matrix has rows_left.
+    __device__ __forceinline__ void begin_rows() { from += static_cast<size_t>(k(0)) * (between / K_EACH); }
+    template <bool WHOLE> __device__ __forceinline__ void load(int32_t rows_left, char* lds, int wave) {
 #pragma unroll
         for (int j = 0; j < EACH; j++) {
-            const int32_t row = row_at(k(j));
-            const int32_t outer = outer0 + of_row(j) * COUNT;
-            const size_t at = static_cast<size_t>(max(row, 0)) * width + outer;
-            piece[j] = load_numbers<T>(from + at, row < 0 ? 0 : width - outer);
+            const int32_t inside = k(j) < rows_left ? left : 0;
+            this->template take<WHOLE>(j, from + j * between, inside, lds, wave);
         }
+        from += next;
     }
-    __device__ __forceinline__ void store(char* lds) const {
+    /// The step whose rows are row[j] (negative: none; not with WHOLE).
+    template <bool WHOLE> __device__ __forceinline__ void load(const int32_t (&row)[EACH], char* lds, int wave) {
 #pragma unroll
         for (int j = 0; j < EACH; j++) {
-            *reinterpret_cast<Numbers<T>*>(lds + Layout::place(k(j), of_row(j))) = piece[j];
+            const size_t at = static_cast<size_t>(WHOLE ? row[j] : max(row[j], 0)) * (between / K_EACH);
+            this->template take<WHOLE>(j, from + at, row[j] >= 0 ? left : 0, lds, wave);
         }
     }
 };
 
+/// Everything this wavefront has asked of memory and LDS has arrived, then the workgroup meets.
+__device__ __forceinline__ void meet() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 /// WM x WN wavefronts; every one of them makes BM / WM x BN / WN numbers.
-template <typename T, Form FORM, int BM, int BN, int WM, int WN>
+template <typename T, Form FORM, int BM, int BN, int WM, int WN, bool ALIGNED>
 __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
     typedef Matrix<T> M;
     constexpr int THREADS = WM * WN * WAVE, COUNT = M::COUNT, BLOCK = M::BLOCK;
@@ -264,10 +328,12 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
     constexpr int MB = BM / WM / BLOCK, NB = BN / WN / BLOCK; // blocks of a wavefront
     constexpr bool SUMS = FORM == Form::GRAD_SUMS, Q_TURNED = SUMS, P_TURNED = FORM != Form::GRAD_ROWS;
     constexpr Units UNITS = SUMS ? Units::OF_GROUPS : Units::OF_ROWS;
-    using QLoader = std::conditional_t<Q_TURNED, TurnedLoader<T, BM, THREADS>, StraightLoader<T, BM, THREADS>>;
-    using PLoader = std::conditional_t<P_TURNED, TurnedLoader<T, BN, THREADS>, StraightLoader<T, BN, THREADS>>;
-    constexpr int BYTES = (BM + BN) * PIECES_OF_STEP * 16;
-    __shared__ __attribute__((aligned(16))) char lds[2 * BYTES];
+    using QLoader =
+        std::conditional_t<Q_TURNED, TurnedLoader<T, BM, THREADS, ALIGNED>, StraightLoader<T, BM, THREADS, ALIGNED>>;
+    using PLoader =
+        std::conditional_t<P_TURNED, TurnedLoader<T, BN, THREADS, ALIGNED>, StraightLoader<T, BN, THREADS, ALIGNED>>;
+    constexpr int P_AT = BM * PIECES_OF_STEP * 16, BYTES = P_AT + BN * PIECES_OF_STEP * 16;
+    __shared__ __attribute__((aligned(16))) char even[BYTES], odd[BYTES];
     __shared__ int32_t rows[SUMS ? 1 : BM];
 
     // Workgroups b, b + 8, .. run on the same XCD: each XCD gets consecutive tiles, so that its L2 holds what they share.
@@ -306,7 +372,7 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
         __syncthreads();
     }
 
-    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+    const int lane = threadIdx.x % WAVE, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / WAVE);
     const int wave_m = wave / WN * (BM / WM), wave_n = wave % WN * (BN / WN);
     typename M::Sums sums[MB][NB];
 #pragma unroll
@@ -320,7 +386,7 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
         }
     }
 
-    const int32_t k_size = rest ? 0 : SUMS ? unit.count : g.k_size;
+    const int32_t k_size = __builtin_amdgcn_readfirstlane(rest ? 0 : SUMS ? unit.count : g.k_size);
     if (k_size > 0) {
         QLoader q;
         PLoader p;
@@ -334,64 +400,132 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
             p.begin(g.p, g.n_size, n0);
         } else if constexpr (P_TURNED) {
             p.begin(g.p + of_group, g.n_size, n0);
+            p.begin_rows();
         } else {
             p.begin(k_size, [&](int i) { return g.p + of_group + static_cast<size_t>(min(n0 + i, g.n_size - 1)) * g.k_size; });
         }
-        auto load = [&](int32_t k0) {
+        // no step but the last one needs to look where the matrices end
+        bool whole = true;
+        if constexpr (Q_TURNED) {
+            whole = whole && q.whole();
+        }
+        if constexpr (P_TURNED) {
+            whole = whole && p.whole();
+        }
+        whole = ALIGNED || __all(whole);
+        // (through registers: from memory here, to LDS in store)
+        auto load_step = [&](auto is_whole, int32_t k0, char* buffer) {
+            constexpr bool WHOLE = decltype(is_whole)::value;
             if constexpr (SUMS) {
-                auto row_at = [&](int k) { return k0 + k < k_size ? g.groups.row_at(unit.begin + k0 + k) : -1; };
-                q.load(row_at);
-                p.load(row_at);
+                int32_t of_q[QLoader::EACH], of_p[PLoader::EACH];
+                auto row_at = [&](int k) { return WHOLE || k0 + k < k_size ? g.groups.row_at(unit.begin + k0 + k) : -1; };
+#pragma unroll
+                for (int j = 0; j < QLoader::EACH; j++) {
+                    of_q[j] = row_at(q.k(j));
+                }
+#pragma unroll
+                for (int j = 0; j < PLoader::EACH; j++) {
+                    of_p[j] = row_at(p.k(j));
+                }
+                q.template load<WHOLE>(of_q, buffer, wave);
+                p.template load<WHOLE>(of_p, buffer + P_AT, wave);
             } else {
-                q.load(k0);
+                q.template load<WHOLE>(k0, buffer, wave);
                 if constexpr (P_TURNED) {
-                    p.load([&](int k) { return k0 + k < k_size ? k0 + k : -1; });
+                    p.template load<WHOLE>(k_size - k0, buffer + P_AT, wave);
                 } else {
-                    p.load(k0);
+                    p.template load<WHOLE>(k0, buffer + P_AT, wave);
                 }
             }
         };
-        load(0);
-        char* buffer = lds;
-        q.store(buffer);
-        p.store(buffer + BM * PIECES_OF_STEP * 16);
-        __syncthreads();
-        for (int32_t k0 = 0; k0 < k_size; k0 += STEP) {
-            const bool more = k0 + STEP < k_size; // (uniform)
-            if (more) {
-                load(k0 + STEP);
+        auto load = [&](int32_t k0, char* buffer) {
+            if (whole && k0 + STEP <= k_size) { // (uniform)
+                load_step(std::true_type(), k0, buffer);
+            } else {
+                load_step(std::false_type(), k0, buffer);
+            }
+        };
+        auto store = [&](char* buffer) {
+            q.store(buffer);
+            p.store(buffer + P_AT);
+        };
+        Numbers<T> of_q[2][MB], of_p[2][NB];
+        auto read = [&](const char* buffer, int step) {
+#pragma unroll
+            for (int i = 0; i < MB; i++) {
+                of_q[step % 2][i] = QLoader::Layout::read(buffer, wave_m + i * BLOCK, step, lane);
             }
 #pragma unroll
-            for (int step = 0; step < STEPS; step++) {
-                Numbers<T> of_q[MB], of_p[NB];
+            for (int j = 0; j < NB; j++) {
+                of_p[step % 2][j] = PLoader::Layout::read(buffer + P_AT, wave_n + j * BLOCK, step, lane);
+            }
+        };
+        auto multiply = [&](int step) {
 #pragma unroll
-                for (int i = 0; i < MB; i++) {
-                    of_q[i] = QLoader::Layout::read(buffer, wave_m + i * BLOCK, step, lane);
-                }
+            for (int i = 0; i < MB; i++) {
 #pragma unroll
                 for (int j = 0; j < NB; j++) {
-                    of_p[j] = PLoader::Layout::read(buffer + BM * PIECES_OF_STEP * 16, wave_n + j * BLOCK, step, lane);
-                }
-#pragma unroll
-                for (int i = 0; i < MB; i++) {
-#pragma unroll
-                    for (int j = 0; j < NB; j++) {
-                        sums[i][j] = M::multiply(of_p[j], of_q[i], sums[i][j]);
-                    }
+                    sums[i][j] = M::multiply(of_p[step % 2][j], of_q[step % 2][i], sums[i][j]);
                 }
             }
-            if (more) {
-                buffer = lds + (buffer == lds ? BYTES : 0);
-                q.store(buffer);
-                p.store(buffer + BM * PIECES_OF_STEP * 16);
-                __syncthreads();
+        };
+        // A read between two matrix instructions: left to itself the compiler puts all reads of a multiplication in
+        // front of it, where they are waited for.
+        auto interleave = [&] {
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int i = 0; i < MB * NB; i++) {
+                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // matrix instruction
+                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); // read of LDS
+                }
+            }
+        };
+        // wavefronts whose rows are all behind the unit's only carry pieces (a unit's last tile)
+        const bool works = SUMS || wave_m < unit.count;
+        static_assert(STEPS % 2 == 0, "the numbers of step 0 come to the place of the last step but one");
+        load(0, even);
+        store(even);
+        meet();
+        if (STEP < k_size) {
+            load(STEP, odd);
+        }
+        if (works) {
+            read(even, 0);
+        }
+        auto step_at = [&](int32_t k0, char* buffer, char* other) {
+#pragma unroll
+            for (int step = 0; step < STEPS - 1; step++) {
+                if (works) {
+                    read(buffer, step + 1);
+                    multiply(step);
+                    interleave();
+                }
+            }
+            if (k0 + STEP < k_size) { // (uniform)
+                store(other);
+                meet();
+                if (k0 + 2 * STEP < k_size) {
+                    load(k0 + 2 * STEP, buffer);
+                }
+                if (works) {
+                    read(other, 0);
+                }
+            }
+            if (works) {
+                multiply(STEPS - 1);
+            }
+        };
+        for (int32_t k0 = 0; k0 < k_size; k0 += 2 * STEP) {
+            step_at(k0, even, odd);
+            if (k0 + STEP < k_size) {
+                step_at(k0 + STEP, odd, even);
             }
         }
     }
 
     // lane l has column wave_m + i * BLOCK + l % BLOCK of the tile's transpose, RUN consecutive numbers at a time
     constexpr int RUN = M::RUN;
-    auto store = [&](auto* row, int j, int i, auto zero) {
+    auto put = [&](auto* row, int j, int i, auto zero) {
         typedef decltype(zero) To;
         typedef To Run __attribute__((ext_vector_type(RUN), aligned(sizeof(To))));
 #pragma unroll
@@ -424,16 +558,16 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
 #pragma unroll
                 for (int j = 0; j < NB; j++) {
                     if (unit.of_group > 1) {
-                        store(g.partial + unit_index * size + of_unit, j, i, wide_t<T>());
+                        put(g.partial + unit_index * size + of_unit, j, i, wide_t<T>());
                     } else {
-                        store(g.out + unit.group * size + of_unit, j, i, T());
+                        put(g.out + unit.group * size + of_unit, j, i, T());
                     }
                 }
             }
         } else if (m < unit.count) {
 #pragma unroll
             for (int j = 0; j < NB; j++) {
-                store(g.out + static_cast<size_t>(rows[m]) * g.n_size, j, i, T());
+                put(g.out + static_cast<size_t>(rows[m]) * g.n_size, j, i, T());
             }
         }
     }
