@@ -56,6 +56,15 @@ template <Units WHICH> __device__ __forceinline__ int32_t units_of(int32_t count
     return max((count + step - 1) / step, WHICH == Units::OF_GROUPS ? 1 : 0);
 }
 
+/// (the same in all lanes, and known to be)
+__device__ __forceinline__ GroupUnit uniform(const GroupUnit& unit) {
+    return GroupUnit{
+        __builtin_amdgcn_readfirstlane(unit.group), __builtin_amdgcn_readfirstlane(unit.begin),
+        __builtin_amdgcn_readfirstlane(unit.count), __builtin_amdgcn_readfirstlane(unit.index),
+        __builtin_amdgcn_readfirstlane(unit.of_group),
+    };
+}
+
 /// Unit number `unit`, by every wavefront for itself (64 groups per step). All lanes.
 template <Units WHICH>
 __device__ __forceinline__ GroupUnit find_unit(const RowGroups& groups, int32_t step, int32_t unit) {
@@ -78,7 +87,7 @@ __device__ __forceinline__ GroupUnit find_unit(const RowGroups& groups, int32_t 
             const int32_t index = unit - (__builtin_amdgcn_readlane(upto, at) - of_group);
             const int32_t first = __builtin_amdgcn_readlane(begin, at) + index * step;
             const int32_t left = __builtin_amdgcn_readlane(count, at) - index * step;
-            return GroupUnit{base + at, first, min(left, step), index, of_group};
+            return uniform(GroupUnit{base + at, first, min(left, step), index, of_group});
         }
         unit -= __builtin_amdgcn_readlane(upto, WAVE - 1);
     }
@@ -86,7 +95,7 @@ __device__ __forceinline__ GroupUnit find_unit(const RowGroups& groups, int32_t 
         const int32_t first = groups.begin_of(0), listed = groups.end_of(groups.n_groups - 1, first) - first;
         const int32_t rest = groups.n_rows - listed, units = (rest + step - 1) / step;
         if (unit < units) {
-            return GroupUnit{groups.n_groups, unit * step, min(rest - unit * step, step), unit, units};
+            return uniform(GroupUnit{groups.n_groups, unit * step, min(rest - unit * step, step), unit, units});
         }
     }
     return GroupUnit{-1, 0, 0, 0, 0};
@@ -109,7 +118,7 @@ template <Units WHICH> __device__ __forceinline__ int32_t count_units(const RowG
         const int32_t rest = groups.n_rows - (groups.end_of(groups.n_groups - 1, first) - first);
         total += (rest + step - 1) / step;
     }
-    return total;
+    return __builtin_amdgcn_readfirstlane(total);
 }
 
 /// The place of number `i` of the rows that belong to no group: before the first group's places, or behind the last's.

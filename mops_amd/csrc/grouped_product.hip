@@ -35,7 +35,7 @@ template <typename T, Form FORM> int32_t p_width(const Product<T>& g) {
     return FORM == Form::GRAD_ROWS ? g.k_size : g.n_size;
 }
 
-template <typename T, Form FORM, int BM, int BN, int WM, int WN> void launch(Product<T> g, hipStream_t stream) {
+template <typename T, Form FORM, int BM, int BN, int WM, int WN, int DEEP = 8, int STAGES = 2> void launch(Product<T> g, hipStream_t stream) {
     constexpr bool SUMS = FORM == Form::GRAD_SUMS;
     g.m_tiles = SUMS ? static_cast<int32_t>(tiles(g.m_size, BM)) : 1;
     g.n_tiles = static_cast<int32_t>(tiles(g.n_size, BN));
@@ -46,9 +46,9 @@ template <typename T, Form FORM, int BM, int BN, int WM, int WN> void launch(Pro
     const size_t workgroups = ceil_div(static_cast<size_t>(g.most_units) * g.m_tiles * g.n_tiles, 8) * 8;
     const unsigned blocks = static_cast<unsigned>(narrow_i32(workgroups, "number of tiles"));
     if (aligned(g.q, q_width<T, FORM>(g)) && aligned(g.p, p_width<T, FORM>(g))) {
-        tiles_kernel<T, FORM, BM, BN, WM, WN, true><<<blocks, WM * WN * WAVE, 0, stream>>>(g);
+        tiles_kernel<T, FORM, BM, BN, WM, WN, DEEP, STAGES, true><<<blocks, WM * WN * WAVE, 0, stream>>>(g);
     } else {
-        tiles_kernel<T, FORM, BM, BN, WM, WN, false><<<blocks, WM * WN * WAVE, 0, stream>>>(g);
+        tiles_kernel<T, FORM, BM, BN, WM, WN, 8, 2, false><<<blocks, WM * WN * WAVE, 0, stream>>>(g);
     }
 }
 
@@ -58,7 +58,7 @@ template <typename T, Form FORM> void rows_times(const Product<T>& g, hipStream_
     const size_t units = static_cast<size_t>(compute_units());
     if (sizeof(T) == 2 && big >= units && rows >= 128 * static_cast<size_t>(g.groups.n_groups)) {
         if constexpr (sizeof(T) == 2) {
-            launch<T, FORM, 256, 256, 2, 4>(g, stream);
+            launch<T, FORM, 256, 256, 2, 4, 8, 2>(g, stream);
         }
     } else if (middle >= units && rows >= 64 * static_cast<size_t>(g.groups.n_groups)) {
         launch<T, FORM, 128, 128, 2, 2>(g, stream);
@@ -93,7 +93,7 @@ template <typename T> void sum_of_rows(Product<T> g, hipStream_t stream) {
     }
     if (use_big) {
         if constexpr (sizeof(T) == 2) {
-            launch<T, Form::GRAD_SUMS, 256, 256, 2, 4>(g, stream);
+            launch<T, Form::GRAD_SUMS, 256, 256, 2, 4, 8, 2>(g, stream);
         }
     } else if (use_middle) {
         launch<T, Form::GRAD_SUMS, 128, 128, 2, 2>(g, stream);

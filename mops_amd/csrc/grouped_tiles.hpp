@@ -115,8 +115,6 @@ template <> struct Matrix<double> {
     static constexpr int RUN = 1;
 };
 
-constexpr int PIECES_OF_STEP = 8; // pieces of 16 bytes of k in LDS
-
 template <typename T> using Numbers = typename Matrix<T>::Numbers;
 
 /// The first `count` of a piece's numbers, zeros behind them (count may be negative, or beyond the piece). WHOLE: all.
@@ -139,13 +137,15 @@ template <typename T, bool WHOLE> __device__ __forceinline__ Numbers<T> load_num
     return v;
 }
 
-/// LDS of a straight side of OUTER rows: [OUTER][8 pieces].
-template <typename T, int OUTER> struct Straight {
-    static __device__ __forceinline__ int place(int row, int piece) {
-        return (row * PIECES_OF_STEP + (piece ^ (row >> 1 & 7))) * 16;
+/// LDS of a straight side of OUTER rows: [OUTER][DEEP pieces], DEEP 4 or 8, permuted so that 16 lanes that read the same
+/// piece of 16 rows reach all banks.
+template <typename T, int OUTER, int DEEP> struct Straight {
+    static __device__ __forceinline__ int permuted(int row, int piece) {
+        return DEEP == 8 ? piece ^ (row >> 1 & 7) : piece ^ (row >> 2 & 3);
     }
+    static __device__ __forceinline__ int place(int row, int piece) { return (row * DEEP + permuted(row, piece)) * 16; }
     /// which piece of its row lies at place i
-    static __device__ __forceinline__ int piece(int i) { return i % PIECES_OF_STEP ^ (i / PIECES_OF_STEP >> 1 & 7); }
+    static __device__ __forceinline__ int piece(int i) { return permuted(i / DEEP, i % DEEP); }
     /// Numbers `step` of the k of a block that begins at row `outer0`.
     static __device__ __forceinline__ Numbers<T> read(const char* lds, int outer0, int step, int lane) {
         constexpr int BLOCK = Matrix<T>::BLOCK;
@@ -156,7 +156,7 @@ template <typename T, int OUTER> struct Straight {
 
 /// LDS of a turned side: [k][OUTER numbers], 16-byte pieces of a row permuted so that the four rows that the lanes of
 /// a transposing read look at fall into different banks.
-template <typename T, int OUTER> struct Turned {
+template <typename T, int OUTER, int DEEP> struct Turned {
     static constexpr int PIECES = OUTER / Matrix<T>::COUNT; // of a row of k
     static __device__ __forceinline__ int permuted(int k, int piece) {
         if constexpr (sizeof(T) == 2 && PIECES >= 16) {
@@ -212,8 +212,8 @@ __device__ __forceinline__ void fetch(const void* from, char* lds) {
 }
 
 /// A side of the product on its way to LDS: piece i = threadIdx.x + j * THREADS, j < EACH.
-template <typename T, int OUTER, int THREADS, bool ALIGNED> struct Pieces {
-    static constexpr int EACH = OUTER * PIECES_OF_STEP / THREADS, COUNT = Matrix<T>::COUNT;
+template <typename T, int OUTER, int DEEP, int THREADS, bool ALIGNED> struct Pieces {
+    static constexpr int EACH = OUTER * DEEP / THREADS, COUNT = Matrix<T>::COUNT;
     Numbers<T> piece[ALIGNED ? 1 : EACH];
 
     /// piece j: numbers `from` .. of a row, of which `left` are in the row (at most 0: none). WHOLE: all of them are,
@@ -237,16 +237,16 @@ template <typename T, int OUTER, int THREADS, bool ALIGNED> struct Pieces {
     }
 };
 
-template <typename T, int OUTER, int THREADS, bool ALIGNED>
-struct StraightLoader : public Pieces<T, OUTER, THREADS, ALIGNED> {
-    typedef Pieces<T, OUTER, THREADS, ALIGNED> Base;
-    typedef Straight<T, OUTER> Layout;
+template <typename T, int OUTER, int DEEP, int THREADS, bool ALIGNED>
+struct StraightLoader : public Pieces<T, OUTER, DEEP, THREADS, ALIGNED> {
+    typedef Pieces<T, OUTER, DEEP, THREADS, ALIGNED> Base;
+    typedef Straight<T, OUTER, DEEP> Layout;
     using Base::COUNT;
     using Base::EACH;
     const T* from[EACH];
     int32_t k_size;
 
-    static __device__ __forceinline__ int row(int j) { return (threadIdx.x + j * THREADS) / PIECES_OF_STEP; }
+    static __device__ __forceinline__ int row(int j) { return (threadIdx.x + j * THREADS) / DEEP; }
     static __device__ __forceinline__ int of_row(int j) { return Layout::piece((threadIdx.x + j * THREADS)); }
 
     /// row_at(i): pointer to the row of memory behind row i of the side (any one for a row that does not matter)
@@ -257,21 +257,18 @@ struct StraightLoader : public Pieces<T, OUTER, THREADS, ALIGNED> {
             from[j] = row_at(row(j)) + of_row(j) * COUNT;
         }
     }
-    /// The next step, which begins at k0 (they are asked for in order).
-    template <bool WHOLE> __device__ __forceinline__ void load(int32_t k0, char* lds, int wave) {
-#pragma unroll
-        for (int j = 0; j < EACH; j++) {
-            this->template take<WHOLE>(j, from[j], k_size - k0 - of_row(j) * COUNT, lds, wave);
-            from[j] += PIECES_OF_STEP * COUNT;
-        }
+    /// Piece j of the next step, which begins at k0 (steps are asked for in order).
+    template <bool WHOLE> __device__ __forceinline__ void load(int j, int32_t k0, char* lds, int wave) {
+        this->template take<WHOLE>(j, from[j], k_size - k0 - of_row(j) * COUNT, lds, wave);
+        from[j] += DEEP * COUNT;
     }
 };
 
 /// Rows of `width` numbers, of which those from outer0 on are used.
-template <typename T, int OUTER, int THREADS, bool ALIGNED>
-struct TurnedLoader : public Pieces<T, OUTER, THREADS, ALIGNED> {
-    typedef Pieces<T, OUTER, THREADS, ALIGNED> Base;
-    typedef Turned<T, OUTER> Layout;
+template <typename T, int OUTER, int DEEP, int THREADS, bool ALIGNED>
+struct TurnedLoader : public Pieces<T, OUTER, DEEP, THREADS, ALIGNED> {
+    typedef Pieces<T, OUTER, DEEP, THREADS, ALIGNED> Base;
+    typedef Turned<T, OUTER, DEEP> Layout;
     using Base::COUNT;
     using Base::EACH;
     static constexpr int K_EACH = THREADS / Layout::PIECES; // rows of k between a thread's pieces
@@ -285,55 +282,53 @@ struct TurnedLoader : public Pieces<T, OUTER, THREADS, ALIGNED> {
     static __device__ __forceinline__ int of_row() { return Layout::piece(threadIdx.x); }
 
     __device__ __forceinline__ void begin(const T* memory, int32_t row_width, int32_t first) {
-        static_assert(K_EACH % 4 == 0 && EACH * THREADS == OUTER * PIECES_OF_STEP, "");
+        static_assert(K_EACH % 4 == 0 && EACH * THREADS == OUTER * DEEP, "");
         const int32_t outer = first + of_row() * COUNT;
         left = row_width - outer;
         // (a piece that is outside of the rows: any piece that is not)
         from = memory + (left > 0 ? outer : 0);
-        next = static_cast<size_t>(PIECES_OF_STEP * COUNT) * row_width;
+        next = static_cast<size_t>(DEEP * COUNT) * row_width;
         between = static_cast<size_t>(K_EACH) * row_width;
     }
     /// Every piece of the step inside of its row, or outside as a whole.
     __device__ __forceinline__ bool whole() const { return ALIGNED || left >= COUNT || left <= 0; }
 
-    /// The next step of consecutive rows (after begin_rows), of which the matrix has rows_left.
+    /// Piece j of the next step of consecutive rows (after begin_rows), of which the matrix has rows_left.
     __device__ __forceinline__ void begin_rows() { from += static_cast<size_t>(k(0)) * (between / K_EACH); }
-    template <bool WHOLE> __device__ __forceinline__ void load(int32_t rows_left, char* lds, int wave) {
-#pragma unroll
-        for (int j = 0; j < EACH; j++) {
-            const int32_t inside = k(j) < rows_left ? left : 0;
-            this->template take<WHOLE>(j, from + j * between, inside, lds, wave);
-        }
-        from += next;
+    template <bool WHOLE> __device__ __forceinline__ void load(int j, int32_t rows_left, char* lds, int wave) {
+        this->template take<WHOLE>(j, from + j * between, k(j) < rows_left ? left : 0, lds, wave);
+        from += j == EACH - 1 ? next : 0;
     }
-    /// The step whose rows are row[j] (negative: none; not with WHOLE).
-    template <bool WHOLE> __device__ __forceinline__ void load(const int32_t (&row)[EACH], char* lds, int wave) {
-#pragma unroll
-        for (int j = 0; j < EACH; j++) {
-            const size_t at = static_cast<size_t>(WHOLE ? row[j] : max(row[j], 0)) * (between / K_EACH);
-            this->template take<WHOLE>(j, from + at, row[j] >= 0 ? left : 0, lds, wave);
-        }
+    /// Piece j of a step whose row is `row` there (negative: none; not with WHOLE).
+    template <bool WHOLE> __device__ __forceinline__ void load_row(int j, int32_t row, char* lds, int wave) {
+        const size_t at = static_cast<size_t>(WHOLE ? row : max(row, 0)) * (between / K_EACH);
+        this->template take<WHOLE>(j, from + at, row >= 0 ? left : 0, lds, wave);
     }
 };
 
-/// Everything this wavefront has asked of memory and LDS has arrived, then the workgroup meets.
-__device__ __forceinline__ void meet() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+/// Everything this wavefront has asked of LDS has arrived, and of memory all but the last LATER pieces; then the
+/// workgroup meets.
+template <int LATER> __device__ __forceinline__ void meet() {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
+}
 
-/// WM x WN wavefronts; every one of them makes BM / WM x BN / WN numbers.
-template <typename T, Form FORM, int BM, int BN, int WM, int WN, bool ALIGNED>
+/// WM x WN wavefronts; every one of them makes BM / WM x BN / WN numbers, in steps of DEEP pieces of k of which STAGES
+/// are in LDS or on their way there.
+template <typename T, Form FORM, int BM, int BN, int WM, int WN, int DEEP, int STAGES, bool ALIGNED>
 __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
     typedef Matrix<T> M;
     constexpr int THREADS = WM * WN * WAVE, COUNT = M::COUNT, BLOCK = M::BLOCK;
-    constexpr int STEP = PIECES_OF_STEP * COUNT, STEPS = PIECES_OF_STEP * BLOCK / WAVE;
+    constexpr int STEP = DEEP * COUNT, STEPS = DEEP * BLOCK / WAVE;
     constexpr int MB = BM / WM / BLOCK, NB = BN / WN / BLOCK; // blocks of a wavefront
     constexpr bool SUMS = FORM == Form::GRAD_SUMS, Q_TURNED = SUMS, P_TURNED = FORM != Form::GRAD_ROWS;
     constexpr Units UNITS = SUMS ? Units::OF_GROUPS : Units::OF_ROWS;
-    using QLoader =
-        std::conditional_t<Q_TURNED, TurnedLoader<T, BM, THREADS, ALIGNED>, StraightLoader<T, BM, THREADS, ALIGNED>>;
-    using PLoader =
-        std::conditional_t<P_TURNED, TurnedLoader<T, BN, THREADS, ALIGNED>, StraightLoader<T, BN, THREADS, ALIGNED>>;
-    constexpr int P_AT = BM * PIECES_OF_STEP * 16, BYTES = P_AT + BN * PIECES_OF_STEP * 16;
-    __shared__ __attribute__((aligned(16))) char even[BYTES], odd[BYTES];
+    using QLoader = std::conditional_t<
+        Q_TURNED, TurnedLoader<T, BM, DEEP, THREADS, ALIGNED>, StraightLoader<T, BM, DEEP, THREADS, ALIGNED>>;
+    using PLoader = std::conditional_t<
+        P_TURNED, TurnedLoader<T, BN, DEEP, THREADS, ALIGNED>, StraightLoader<T, BN, DEEP, THREADS, ALIGNED>>;
+    constexpr int P_AT = BM * DEEP * 16, BYTES = P_AT + BN * DEEP * 16;
+    static_assert(ALIGNED || STAGES == 2, "through registers: one step on its way, one in LDS beside the present one");
+    __shared__ __attribute__((aligned(16))) char stages[STAGES * BYTES];
     __shared__ int32_t rows[SUMS ? 1 : BM];
 
     // Workgroups b, b + 8, .. run on the same XCD: each XCD gets consecutive tiles, so that its L2 holds what they share.
@@ -359,7 +354,7 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
         m0 = 0;
         n0 = in_band / height * BN;
     }
-    const GroupUnit unit = find_unit<UNITS>(g.groups, g.step, unit_index);
+    const GroupUnit unit = uniform(find_unit<UNITS>(g.groups, g.step, unit_index));
     if (unit.group < 0) {
         return; // (uniform; offsets that are none)
     }
@@ -404,45 +399,57 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
         } else {
             p.begin(k_size, [&](int i) { return g.p + of_group + static_cast<size_t>(min(n0 + i, g.n_size - 1)) * g.k_size; });
         }
-        // no step but the last one needs to look where the matrices end
-        bool whole = true;
-        if constexpr (Q_TURNED) {
-            whole = whole && q.whole();
-        }
-        if constexpr (P_TURNED) {
-            whole = whole && p.whole();
-        }
-        whole = ALIGNED || __all(whole);
-        // (through registers: from memory here, to LDS in store)
-        auto load_step = [&](auto is_whole, int32_t k0, char* buffer) {
-            constexpr bool WHOLE = decltype(is_whole)::value;
+        constexpr int Q_EACH = QLoader::EACH, P_EACH = PLoader::EACH, EACH = Q_EACH + P_EACH;
+        // GRAD_SUMS: the rows behind the pieces of a step
+        [[maybe_unused]] int32_t row_of_piece[SUMS ? EACH : 1];
+        auto find_rows = [&](int32_t k0) {
             if constexpr (SUMS) {
-                int32_t of_q[QLoader::EACH], of_p[PLoader::EACH];
-                auto row_at = [&](int k) { return WHOLE || k0 + k < k_size ? g.groups.row_at(unit.begin + k0 + k) : -1; };
+                auto row_at = [&](int k) { return k0 + k < k_size ? g.groups.row_at(unit.begin + k0 + k) : -1; };
 #pragma unroll
-                for (int j = 0; j < QLoader::EACH; j++) {
-                    of_q[j] = row_at(q.k(j));
-                }
-#pragma unroll
-                for (int j = 0; j < PLoader::EACH; j++) {
-                    of_p[j] = row_at(p.k(j));
-                }
-                q.template load<WHOLE>(of_q, buffer, wave);
-                p.template load<WHOLE>(of_p, buffer + P_AT, wave);
-            } else {
-                q.template load<WHOLE>(k0, buffer, wave);
-                if constexpr (P_TURNED) {
-                    p.template load<WHOLE>(k_size - k0, buffer + P_AT, wave);
-                } else {
-                    p.template load<WHOLE>(k0, buffer + P_AT, wave);
+                for (int j = 0; j < EACH; j++) {
+                    row_of_piece[j] = j >= Q_EACH && QLoader::K_EACH == PLoader::K_EACH
+                                          ? row_of_piece[j - Q_EACH]
+                                          : row_at(j < Q_EACH ? QLoader::k(j) : PLoader::k(j - Q_EACH));
                 }
             }
         };
-        auto load = [&](int32_t k0, char* buffer) {
-            if (whole && k0 + STEP <= k_size) { // (uniform)
-                load_step(std::true_type(), k0, buffer);
+        // Piece `piece` of the step that begins at k0 (find_rows of it before).
+        auto load_piece = [&](auto is_whole, int piece, int32_t k0, char* buffer) {
+            constexpr bool WHOLE = decltype(is_whole)::value;
+            if constexpr (SUMS) {
+                if (piece < Q_EACH) {
+                    q.template load_row<WHOLE>(piece, row_of_piece[piece], buffer, wave);
+                } else {
+                    p.template load_row<WHOLE>(piece - Q_EACH, row_of_piece[piece], buffer + P_AT, wave);
+                }
+            } else if (piece < Q_EACH) {
+                q.template load<WHOLE>(piece, k0, buffer, wave);
             } else {
-                load_step(std::false_type(), k0, buffer);
+                p.template load<WHOLE>(piece - Q_EACH, P_TURNED ? k_size - k0 : k0, buffer + P_AT, wave);
+            }
+        };
+        // through registers, no step but the last one needs to look where the matrices end
+        bool whole = true;
+        if constexpr (!ALIGNED) {
+            if constexpr (Q_TURNED) {
+                whole = whole && q.whole();
+            }
+            if constexpr (P_TURNED) {
+                whole = whole && p.whole();
+            }
+            whole = __all(whole);
+        }
+        auto load = [&](int32_t k0, char* buffer) {
+            if (!ALIGNED && whole && k0 + STEP <= k_size) { // (uniform)
+#pragma unroll
+                for (int piece = 0; piece < EACH; piece++) {
+                    load_piece(std::true_type(), piece, k0, buffer);
+                }
+            } else {
+#pragma unroll
+                for (int piece = 0; piece < EACH; piece++) {
+                    load_piece(std::false_type(), piece, k0, buffer);
+                }
             }
         };
         auto store = [&](char* buffer) {
@@ -450,126 +457,174 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
             p.store(buffer + P_AT);
         };
         Numbers<T> of_q[2][MB], of_p[2][NB];
-        auto read = [&](const char* buffer, int step) {
-#pragma unroll
-            for (int i = 0; i < MB; i++) {
+        // what a multiplication needs, in the order in which it needs it: q 0, p 0 .. NB - 1, q 1 .. MB - 1
+        auto read = [&](const char* buffer, int step, int which) {
+            if (which == 0 || which > NB) {
+                const int i = which == 0 ? 0 : which - NB;
                 of_q[step % 2][i] = QLoader::Layout::read(buffer, wave_m + i * BLOCK, step, lane);
-            }
-#pragma unroll
-            for (int j = 0; j < NB; j++) {
+            } else {
+                const int j = which - 1;
                 of_p[step % 2][j] = PLoader::Layout::read(buffer + P_AT, wave_n + j * BLOCK, step, lane);
-            }
-        };
-        auto multiply = [&](int step) {
-#pragma unroll
-            for (int i = 0; i < MB; i++) {
-#pragma unroll
-                for (int j = 0; j < NB; j++) {
-                    sums[i][j] = M::multiply(of_p[step % 2][j], of_q[step % 2][i], sums[i][j]);
-                }
-            }
-        };
-        // A read between two matrix instructions: left to itself the compiler puts all reads of a multiplication in
-        // front of it, where they are waited for.
-        auto interleave = [&] {
-            if constexpr (sizeof(T) == 2) {
-#pragma unroll
-                for (int i = 0; i < MB * NB; i++) {
-                    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); // matrix instruction
-                    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); // read of LDS
-                }
             }
         };
         // wavefronts whose rows are all behind the unit's only carry pieces (a unit's last tile)
         const bool works = SUMS || wave_m < unit.count;
-        static_assert(STEPS % 2 == 0, "the numbers of step 0 come to the place of the last step but one");
-        load(0, even);
-        store(even);
-        meet();
-        if (STEP < k_size) {
-            load(STEP, odd);
-        }
-        if (works) {
-            read(even, 0);
-        }
-        auto step_at = [&](int32_t k0, char* buffer, char* other) {
+        // One multiplication of a step, and between its matrix instructions, in this order (left to itself the compiler
+        // puts all reads in front, where they are waited for, and a wavefront that asks for eight pieces in a row waits
+        // until the memory pipeline has taken them): the reads of the next one, and between(0), between(1), .., one of them
+        // for every second matrix instruction.
+        constexpr int SLOTS = MB * NB, READS = MB + NB, OF_SLOT = (READS + SLOTS - 1) / SLOTS;
+        auto multiply = [&](int step, const char* next_buffer, int next_step, bool reads, auto&& between) {
+            if (!works) {
+                between(0, EACH);
+                return;
+            }
+            int asked = 0;
 #pragma unroll
-            for (int step = 0; step < STEPS - 1; step++) {
-                if (works) {
-                    read(buffer, step + 1);
-                    multiply(step);
-                    interleave();
+            for (int slot = 0; slot < SLOTS; slot++) {
+                if (reads) {
+#pragma unroll
+                    for (int r = slot * OF_SLOT; r < (slot + 1) * OF_SLOT; r++) {
+                        if (r < READS) {
+                            read(next_buffer, next_step, r);
+                        }
+                    }
                 }
-            }
-            if (k0 + STEP < k_size) { // (uniform)
-                store(other);
-                meet();
-                if (k0 + 2 * STEP < k_size) {
-                    load(k0 + 2 * STEP, buffer);
-                }
-                if (works) {
-                    read(other, 0);
-                }
-            }
-            if (works) {
-                multiply(STEPS - 1);
+                const int upto = (slot + 1) * EACH / SLOTS;
+                between(asked, upto);
+                asked = upto;
+                const int i = slot / NB, j = slot % NB;
+                sums[i][j] = M::multiply(of_p[step % 2][j], of_q[step % 2][i], sums[i][j]);
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
-        for (int32_t k0 = 0; k0 < k_size; k0 += 2 * STEP) {
-            step_at(k0, even, odd);
-            if (k0 + STEP < k_size) {
-                step_at(k0 + STEP, odd, even);
+        auto nothing = [](int, int) {};
+        static_assert(STEPS % 2 == 0, "the numbers of step 0 come to the place of the last step but one");
+        // Step t is multiplied from stage t % STAGES. Where the workgroup meets in it, step t + 1 has arrived, and the
+        // stage is free for step t + STAGES (ALIGNED), or step t + 1 is put into its stage from registers, which are
+        // free for step t + 2. (ALIGNED: steps behind the last one are asked for like all others: zeros.)
+        constexpr int FIRST = ALIGNED ? STAGES : 1, AHEAD = ALIGNED ? STAGES : 2;
+#pragma unroll
+        for (int t = 0; t < FIRST; t++) {
+            find_rows(t * STEP);
+            load(t * STEP, stages + t * BYTES);
+        }
+        find_rows(FIRST * STEP);
+        store(stages);
+        meet<ALIGNED ? (STAGES - 1) * EACH : 0>();
+        if (!ALIGNED && STEP < k_size) {
+            load(STEP, stages);
+            find_rows(2 * STEP);
+        }
+        char* buffer = stages;
+        if (works) {
+#pragma unroll
+            for (int r = 0; r < READS; r++) {
+                read(buffer, 0, r);
             }
         }
+        for (int32_t k0 = 0; k0 < k_size; k0 += STEP) {
+#pragma unroll
+            for (int step = 0; step < STEPS - 1; step++) {
+                multiply(step, buffer, step + 1, true, nothing);
+            }
+            char* const following = buffer + BYTES < stages + STAGES * BYTES ? buffer + BYTES : stages;
+            store(following);
+            meet<ALIGNED ? (STAGES - 2) * EACH : 0>();
+            if constexpr (ALIGNED) {
+                multiply(STEPS - 1, following, 0, true, [&](int from, int upto) {
+#pragma unroll
+                    for (int piece = 0; piece < EACH; piece++) {
+                        if (piece >= from && piece < upto) {
+                            load_piece(std::false_type(), piece, k0 + AHEAD * STEP, buffer);
+                        }
+                    }
+                });
+                find_rows(k0 + (AHEAD + 1) * STEP);
+            } else {
+                if (k0 + 2 * STEP < k_size) { // (uniform)
+                    load(k0 + 2 * STEP, buffer);
+                    find_rows(k0 + 3 * STEP);
+                }
+                multiply(STEPS - 1, following, 0, true, nothing);
+            }
+            buffer = following;
+        }
+        meet<0>(); // (nothing is on its way to LDS any more)
     }
 
-    // lane l has column wave_m + i * BLOCK + l % BLOCK of the tile's transpose, RUN consecutive numbers at a time
-    constexpr int RUN = M::RUN;
-    auto put = [&](auto* row, int j, int i, auto zero) {
+    // Every wavefront turns its blocks over in LDS of its own, to store whole pieces of rows side by side (straight from
+    // the registers, 8 bytes of 32 rows per store: 32768 rows, K = 2048, L = 4096, bfloat16: 657 us instead of 446).
+    __syncthreads();
+    auto put = [&](auto zero, auto&& row_at) {
         typedef decltype(zero) To;
-        typedef To Run __attribute__((ext_vector_type(RUN), aligned(sizeof(To))));
+        constexpr int COLUMNS = BN / WN, OF_PIECE = 16 / sizeof(To), RUN = M::RUN, PIECES = COLUMNS / OF_PIECE;
+        constexpr int ROWS_ABREAST = PIECES >= 16 ? 1 : 16 / PIECES; // rows in 256 bytes, all banks
+        static_assert(BLOCK * COLUMNS * sizeof(To) * WM * WN <= sizeof(stages), "");
+        typedef To Run __attribute__((ext_vector_type(RUN)));
+        typedef To Piece __attribute__((ext_vector_type(OF_PIECE), aligned(sizeof(To))));
+        char* const mine = stages + wave * (BLOCK * COLUMNS * sizeof(To));
+        auto place = [](int row, int piece) {
+            return (row * PIECES + (piece ^ (row / ROWS_ABREAST & (PIECES - 1)))) * 16;
+        };
 #pragma unroll
-        for (int e = 0; e < M::HELD; e += RUN) {
-            const int32_t n = n0 + wave_n + j * BLOCK + M::row_of(lane, e);
-            if (n + RUN <= g.n_size) {
-                Run run;
-#pragma unroll
-                for (int r = 0; r < RUN; r++) {
-                    run[r] = static_cast<To>(sums[i][j][e + r]);
-                }
-                *reinterpret_cast<Run*>(row + n) = run;
-            } else {
-#pragma unroll
-                for (int r = 0; r < RUN; r++) {
-                    if (n + r < g.n_size) {
-                        row[n + r] = static_cast<To>(sums[i][j][e + r]);
-                    }
-                }
-            }
-        }
-    };
-#pragma unroll
-    for (int i = 0; i < MB; i++) {
-        const int32_t m = wave_m + i * BLOCK + lane % BLOCK;
-        if constexpr (SUMS) {
-            if (m0 + m < g.m_size) {
-                const size_t of_unit = static_cast<size_t>(m0 + m) * g.n_size;
-                const size_t size = static_cast<size_t>(g.m_size) * g.n_size;
-#pragma unroll
-                for (int j = 0; j < NB; j++) {
-                    if (unit.of_group > 1) {
-                        put(g.partial + unit_index * size + of_unit, j, i, wide_t<T>());
-                    } else {
-                        put(g.out + unit.group * size + of_unit, j, i, T());
-                    }
-                }
-            }
-        } else if (m < unit.count) {
+        for (int i = 0; i < MB; i++) {
 #pragma unroll
             for (int j = 0; j < NB; j++) {
-                put(g.out + static_cast<size_t>(rows[m]) * g.n_size, j, i, T());
+#pragma unroll
+                for (int e = 0; e < M::HELD; e += RUN) {
+                    const int column = j * BLOCK + M::row_of(lane, e);
+                    Run run;
+#pragma unroll
+                    for (int r = 0; r < RUN; r++) {
+                        run[r] = static_cast<To>(sums[i][j][e + r]);
+                    }
+                    *reinterpret_cast<Run*>(
+                        mine + place(lane % BLOCK, column / OF_PIECE) + column % OF_PIECE * sizeof(To)
+                    ) = run;
+                }
             }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+            for (int at = 0; at < BLOCK * PIECES; at += WAVE) {
+                const int row = (at + lane) / PIECES, piece = (at + lane) % PIECES;
+                const int32_t n = n0 + wave_n + piece * OF_PIECE;
+                To* const to = row_at(wave_m + i * BLOCK + row); // (null: no such row)
+                if (to != nullptr && n < g.n_size) {
+                    const Piece numbers = *reinterpret_cast<const Piece*>(mine + place(row, piece));
+                    if (n + OF_PIECE <= g.n_size) {
+                        *reinterpret_cast<Piece*>(to + n) = numbers;
+                    } else {
+#pragma unroll
+                        for (int r = 0; r < OF_PIECE; r++) {
+                            if (n + r < g.n_size) {
+                                to[n + r] = numbers[r];
+                            }
+                        }
+                    }
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
         }
+    };
+    if constexpr (SUMS) {
+        const size_t size = static_cast<size_t>(g.m_size) * g.n_size;
+        auto row_of = [&](auto* result) {
+            return [=, &g](int m) {
+                return m0 + m < g.m_size ? result + static_cast<size_t>(m0 + m) * g.n_size : nullptr;
+            };
+        };
+        if (unit.of_group > 1) { // (uniform)
+            put(wide_t<T>(), row_of(g.partial + unit_index * size));
+        } else {
+            put(T(), row_of(g.out + unit.group * size));
+        }
+    } else {
+        put(T(), [&](int m) { return m < unit.count ? g.out + static_cast<size_t>(rows[m]) * g.n_size : nullptr; });
     }
 }
 
