@@ -439,6 +439,14 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
             }
             whole = __all(whole);
         }
+        auto load_some = [&](int from, int upto, int32_t k0, char* buffer) {
+#pragma unroll
+            for (int piece = 0; piece < EACH; piece++) {
+                if (piece >= from && piece < upto) {
+                    load_piece(std::false_type(), piece, k0, buffer);
+                }
+            }
+        };
         auto load = [&](int32_t k0, char* buffer) {
             if (!ALIGNED && whole && k0 + STEP <= k_size) { // (uniform)
 #pragma unroll
@@ -446,10 +454,7 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
                     load_piece(std::true_type(), piece, k0, buffer);
                 }
             } else {
-#pragma unroll
-                for (int piece = 0; piece < EACH; piece++) {
-                    load_piece(std::false_type(), piece, k0, buffer);
-                }
+                load_some(0, EACH, k0, buffer);
             }
         };
         auto store = [&](char* buffer) {
@@ -469,28 +474,26 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
         };
         // wavefronts whose rows are all behind the unit's only carry pieces (a unit's last tile)
         const bool works = SUMS || wave_m < unit.count;
-        // One multiplication of a step, and between its matrix instructions, in this order (left to itself the compiler
-        // puts all reads in front, where they are waited for, and a wavefront that asks for eight pieces in a row waits
-        // until the memory pipeline has taken them): the reads of the next one, and between(0), between(1), .., one of them
-        // for every second matrix instruction.
+        // One multiplication of a step, and between its matrix instructions, in this order: the reads of the next one, and
+        // pieces [first, last) of another step, asked for by between(from, upto). (Left to itself the compiler puts all
+        // reads in front, where they are waited for, and a wavefront that asks for eight pieces in a row waits until the
+        // memory pipeline has taken them.)
         constexpr int SLOTS = MB * NB, READS = MB + NB, OF_SLOT = (READS + SLOTS - 1) / SLOTS;
-        auto multiply = [&](int step, const char* next_buffer, int next_step, bool reads, auto&& between) {
+        auto multiply = [&](int step, const char* next_buffer, int next_step, int first, int last, auto&& between) {
             if (!works) {
-                between(0, EACH);
+                between(first, last);
                 return;
             }
-            int asked = 0;
+            int asked = first;
 #pragma unroll
             for (int slot = 0; slot < SLOTS; slot++) {
-                if (reads) {
 #pragma unroll
-                    for (int r = slot * OF_SLOT; r < (slot + 1) * OF_SLOT; r++) {
-                        if (r < READS) {
-                            read(next_buffer, next_step, r);
-                        }
+                for (int r = slot * OF_SLOT; r < (slot + 1) * OF_SLOT; r++) {
+                    if (r < READS) {
+                        read(next_buffer, next_step, r);
                     }
                 }
-                const int upto = (slot + 1) * EACH / SLOTS;
+                const int upto = first + (slot + 1) * (last - first) / SLOTS;
                 between(asked, upto);
                 asked = upto;
                 const int i = slot / NB, j = slot % NB;
@@ -501,22 +504,29 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
         auto nothing = [](int, int) {};
         static_assert(STEPS % 2 == 0, "the numbers of step 0 come to the place of the last step but one");
         // Step t is multiplied from stage t % STAGES. Where the workgroup meets in it, step t + 1 has arrived, and the
-        // stage is free for step t + STAGES (ALIGNED), or step t + 1 is put into its stage from registers, which are
-        // free for step t + 2. (ALIGNED: steps behind the last one are asked for like all others: zeros.)
-        constexpr int FIRST = ALIGNED ? STAGES : 1, AHEAD = ALIGNED ? STAGES : 2;
+        // stage is free for step t + STAGES (ALIGNED: EARLY of its pieces are asked for right then, the others in the next
+        // step's first multiplication), or step t + 1 is put into its stage from registers, which are free for step t + 2.
+        // (ALIGNED: steps behind the last one are asked for like all others: zeros.)
+        constexpr int FIRST = ALIGNED ? STAGES : 1, EARLY = EACH / 2;
 #pragma unroll
         for (int t = 0; t < FIRST; t++) {
             find_rows(t * STEP);
-            load(t * STEP, stages + t * BYTES);
+            if (ALIGNED && t == FIRST - 1) {
+                load_some(0, EARLY, t * STEP, stages + t * BYTES);
+            } else {
+                load(t * STEP, stages + t * BYTES);
+            }
         }
-        find_rows(FIRST * STEP);
         store(stages);
-        meet<ALIGNED ? (STAGES - 1) * EACH : 0>();
-        if (!ALIGNED && STEP < k_size) {
-            load(STEP, stages);
+        meet<ALIGNED ? (STAGES - 2) * EACH + EARLY : 0>();
+        if (!ALIGNED) {
+            find_rows(STEP);
+            if (STEP < k_size) {
+                load(STEP, stages);
+            }
             find_rows(2 * STEP);
         }
-        char* buffer = stages;
+        char *before = stages + (STAGES - 1) * BYTES, *buffer = stages;
         if (works) {
 #pragma unroll
             for (int r = 0; r < READS; r++) {
@@ -526,28 +536,30 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
         for (int32_t k0 = 0; k0 < k_size; k0 += STEP) {
 #pragma unroll
             for (int step = 0; step < STEPS - 1; step++) {
-                multiply(step, buffer, step + 1, true, nothing);
+                if (ALIGNED && step == 0) {
+                    multiply(step, buffer, step + 1, EARLY, EACH, [&](int from, int upto) {
+                        load_some(from, upto, k0 + (STAGES - 1) * STEP, before);
+                    });
+                    find_rows(k0 + STAGES * STEP);
+                } else {
+                    multiply(step, buffer, step + 1, 0, 0, nothing);
+                }
             }
             char* const following = buffer + BYTES < stages + STAGES * BYTES ? buffer + BYTES : stages;
             store(following);
             meet<ALIGNED ? (STAGES - 2) * EACH : 0>();
             if constexpr (ALIGNED) {
-                multiply(STEPS - 1, following, 0, true, [&](int from, int upto) {
-#pragma unroll
-                    for (int piece = 0; piece < EACH; piece++) {
-                        if (piece >= from && piece < upto) {
-                            load_piece(std::false_type(), piece, k0 + AHEAD * STEP, buffer);
-                        }
-                    }
+                multiply(STEPS - 1, following, 0, 0, EARLY, [&](int from, int upto) {
+                    load_some(from, upto, k0 + STAGES * STEP, buffer);
                 });
-                find_rows(k0 + (AHEAD + 1) * STEP);
             } else {
                 if (k0 + 2 * STEP < k_size) { // (uniform)
                     load(k0 + 2 * STEP, buffer);
                     find_rows(k0 + 3 * STEP);
                 }
-                multiply(STEPS - 1, following, 0, true, nothing);
+                multiply(STEPS - 1, following, 0, 0, 0, nothing);
             }
+            before = buffer;
             buffer = following;
         }
         meet<0>(); // (nothing is on its way to LDS any more)
