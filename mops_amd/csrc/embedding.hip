@@ -31,6 +31,8 @@ constexpr int THREADS = 256;
 constexpr int AHEAD = 8;            // rows that a team has on their way
 constexpr int32_t PLACES_EACH = 32; // of a chunk, per team
 constexpr int32_t ALONE = 64;       // places that a team sums up by itself
+constexpr int32_t FEW = 16;         // rows per table row from which on a workgroup has one table row
+constexpr int32_t ROWS_PER_TEAM = 4;
 
 /// How a row's pieces are shared out: `team` lanes (a power of two) hold a piece each.
 struct Teams {
@@ -87,29 +89,36 @@ __global__ __launch_bounds__(THREADS) void lookup_kernel(
     }
 }
 
-/// sum[j] += rows order[begin], order[begin + step], ... before `end`, at `column`.
+/// sum[j] += rows order[begin], order[begin + step], ... before `end`, at `column`. A team's lanes read the order side by
+/// side and hand it round, so that a row waits for its place once per `team` rows, not each time.
 template <typename T, int N>
 __device__ __forceinline__ void add_rows(
     wide_t<T> (&sum)[N], const T* __restrict__ rows, const int32_t* __restrict__ order, int32_t n_rows, int32_t begin,
-    int32_t end, int32_t step, size_t columns, int32_t column
+    int32_t end, int32_t step, size_t columns, int32_t column, int32_t team
 ) {
-    for (int32_t p = begin; p < end; p += AHEAD * step) {
-        int32_t row[AHEAD];
-        Piece<T, N> value[AHEAD];
+    const int32_t width = min(team, WAVE), lane = threadIdx.x & (width - 1);
+    for (int32_t p = begin; p < end; p += width * step) {
+        const int32_t left = min((end - p + step - 1) / step, width); // rows of this round
+        const int32_t mine = lane < left ? order[p + lane * step] : -1;
+        for (int32_t first = 0; first < left; first += AHEAD) {
+            int32_t row[AHEAD];
+            Piece<T, N> value[AHEAD];
 #pragma unroll
-        for (int u = 0; u < AHEAD; u++) {
-            row[u] = p + u * step < end ? order[p + u * step] : -1;
-        }
+            for (int u = 0; u < AHEAD; u++) {
+                row[u] = __shfl(mine, min(first + u, width - 1), width);
+                row[u] = first + u < left && in_bounds(row[u], n_rows) ? row[u] : -1;
+            }
 #pragma unroll
-        for (int u = 0; u < AHEAD; u++) {
-            value[u] = Piece<T, N>::load(rows + (in_bounds(row[u], n_rows) ? row[u] : 0) * columns + column);
-        }
+            for (int u = 0; u < AHEAD; u++) {
+                value[u] = Piece<T, N>::load(rows + max(row[u], 0) * columns + column);
+            }
 #pragma unroll
-        for (int u = 0; u < AHEAD; u++) {
-            if (in_bounds(row[u], n_rows)) {
+            for (int u = 0; u < AHEAD; u++) {
+                if (row[u] >= 0) {
 #pragma unroll
-                for (int j = 0; j < N; j++) {
-                    sum[j] += value[u].get(j);
+                    for (int j = 0; j < N; j++) {
+                        sum[j] += value[u].get(j);
+                    }
                 }
             }
         }
@@ -156,7 +165,8 @@ __global__ __launch_bounds__(THREADS) void chunk_kernel(
     const int32_t column = teams.row.start<N>(piece);
     wide_t<T> sum[N] = {};
     add_rows<T, N>(
-        sum, grad_output, order, n_rows, begin + threadIdx.x / teams.team, end, teams.teams, teams.row.columns, column
+        sum, grad_output, order, n_rows, begin + threadIdx.x / teams.team, end, teams.teams, teams.row.columns, column,
+        teams.team
     );
     join_teams<wide_t<T>, N>(sum, joined, teams);
     if (static_cast<int32_t>(threadIdx.x) < teams.team) {
@@ -168,19 +178,20 @@ __global__ __launch_bounds__(THREADS) void chunk_kernel(
     }
 }
 
-/// grad_table[v, :]: a team per row of the table where few rows name it, the workgroup together where many do.
+/// grad_table[v, :] for `each` rows of the table per team: a team per row where few rows name it, the workgroup
+/// together where many do.
 template <typename T, int N>
 __global__ __launch_bounds__(THREADS) void gradient_kernel(
     T* __restrict__ grad_table, const T* __restrict__ grad_output, const wide_t<T>* __restrict__ partial,
     const int32_t* __restrict__ order, const int32_t* __restrict__ offsets, int32_t n_rows, int32_t table_rows,
-    Teams teams, int32_t chunk, wide_t<T> scale
+    Teams teams, int32_t chunk, int32_t each, int32_t alone, wide_t<T> scale
 ) {
     __shared__ wide_t<T> joined[N * THREADS];
     const int32_t piece = blockIdx.y * teams.team + (threadIdx.x & (teams.team - 1));
     const bool holds = piece < teams.row.pieces;
     const int32_t column = teams.row.start<N>(min(piece, teams.row.pieces - 1));
     const int32_t mine = threadIdx.x / teams.team;
-    const int32_t row0 = blockIdx.x * teams.teams;
+    const int32_t row0 = blockIdx.x * each, row_end = min(row0 + each, table_rows);
     auto store = [&](int32_t row, const wide_t<T>(&sum)[N]) {
         Piece<T, N> value;
 #pragma unroll
@@ -189,24 +200,25 @@ __global__ __launch_bounds__(THREADS) void gradient_kernel(
         }
         value.store(grad_table + static_cast<size_t>(row) * teams.row.columns + column);
     };
-    {
-        const int32_t row = row0 + mine;
-        if (row < table_rows && holds) {
-            const int32_t begin = max(offsets[row], 0), end = min(offsets[row + 1], n_rows);
-            if (end - begin <= ALONE) {
-                wide_t<T> sum[N] = {};
-                add_rows<T, N>(sum, grad_output, order, n_rows, begin, end, 1, teams.row.columns, column);
+    bool many = false;
+    for (int32_t row = row0 + mine; row < row_end; row += teams.teams) {
+        const int32_t begin = max(offsets[row], 0), end = min(offsets[row + 1], n_rows);
+        if (end - begin > alone) {
+            many = true;
+        } else {
+            wide_t<T> sum[N] = {};
+            add_rows<T, N>(sum, grad_output, order, n_rows, begin, end, 1, teams.row.columns, column, teams.team);
+            if (holds) {
                 store(row, sum);
             }
         }
     }
-    for (int32_t t = 0; t < teams.teams; t++) {
-        const int32_t row = row0 + t;
-        if (row >= table_rows) {
-            break;
-        }
+    if (!__syncthreads_or(many)) {
+        return;
+    }
+    for (int32_t row = row0; row < row_end; row++) {
         const int32_t begin = max(offsets[row], 0), end = min(offsets[row + 1], n_rows);
-        if (end - begin <= ALONE) { // (uniform)
+        if (end - begin <= alone) { // (uniform)
             continue;
         }
         wide_t<T> sum[N] = {};
@@ -214,7 +226,7 @@ __global__ __launch_bounds__(THREADS) void gradient_kernel(
         const bool chunks = partial != nullptr && first_chunk < past_chunk;
         add_rows<T, N>(
             sum, grad_output, order, n_rows, begin + mine, chunks ? first_chunk * chunk : end, teams.teams,
-            teams.row.columns, column
+            teams.row.columns, column, teams.team
         );
         if (chunks) {
             for (int32_t c = first_chunk + mine; c < past_chunk; c += AHEAD * teams.teams) {
@@ -238,7 +250,8 @@ __global__ __launch_bounds__(THREADS) void gradient_kernel(
                 }
             }
             add_rows<T, N>(
-                sum, grad_output, order, n_rows, past_chunk * chunk + mine, end, teams.teams, teams.row.columns, column
+                sum, grad_output, order, n_rows, past_chunk * chunk + mine, end, teams.teams, teams.row.columns, column,
+                teams.team
             );
         }
         join_teams<wide_t<T>, N>(sum, joined, teams);
@@ -315,10 +328,16 @@ void gradient(
                 partial, grad_output, indices, order, n_rows, table_rows, teams, chunk
             );
         }
-        const size_t blocks = ceil_div(static_cast<size_t>(table_rows), static_cast<size_t>(teams.teams));
+        // Rows of the table per workgroup: one where many rows name each on average (200 000 rows, 94 table rows, 128
+        // floats: 73 us for the whole gradient with one row per team, 4 x as long as this kernel needs otherwise), else
+        // some per team, for workgroups that have nothing but zeros to store come and go faster than they are started.
+        const bool many = static_cast<size_t>(n_rows) > static_cast<size_t>(table_rows) * FEW;
+        const size_t rows_each = many ? 1 : static_cast<size_t>(teams.teams) * ROWS_PER_TEAM;
+        const int32_t alone = many ? 0 : ALONE;
+        const size_t blocks = ceil_div(static_cast<size_t>(table_rows), rows_each);
         gradient_kernel<T, N><<<dim3(static_cast<unsigned>(blocks), teams.tiles), THREADS, 0, stream>>>(
             grad_table, grad_output, partial, order, offsets, n_rows, table_rows, teams, chunk,
-            static_cast<wide_t<T>>(scale)
+            static_cast<int32_t>(rows_each), alone, static_cast<wide_t<T>>(scale)
         );
     });
     MOPS_HIP_CHECK(hipGetLastError());
