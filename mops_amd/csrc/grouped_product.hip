@@ -101,9 +101,19 @@ template <typename T> void sum_of_rows(Product<T> g, hipStream_t stream) {
         launch<T, Form::GRAD_SUMS, 64, 64, 2, 2>(g, stream);
     }
     if (splits) {
-        const unsigned blocks = static_cast<unsigned>(std::min<size_t>(ceil_div(size, JOIN_THREADS), 4 * units));
+        // (few workgroups per unit: most units are not the first one of several, and theirs have nothing to do)
         g.most_units = narrow_i32(most, "number of units of rows");
-        join_units_kernel<T><<<dim3(static_cast<unsigned>(most), blocks), JOIN_THREADS, 0, stream>>>(g);
+        auto join = [&](auto joined) {
+            constexpr int JOINED = decltype(joined)::value;
+            const size_t wanted = ceil_div(size / JOINED, JOIN_THREADS);
+            const unsigned blocks = static_cast<unsigned>(std::min(wanted, std::max<size_t>(16, 8 * units / most)));
+            join_units_kernel<T, JOINED><<<dim3(static_cast<unsigned>(most), blocks), JOIN_THREADS, 0, stream>>>(g);
+        };
+        if (size % 4 == 0) {
+            join(std::integral_constant<int, 4>{});
+        } else {
+            join(std::integral_constant<int, 1>{});
+        }
     }
     MOPS_HIP_CHECK(hipGetLastError());
 }

@@ -331,12 +331,14 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
     __shared__ __attribute__((aligned(16))) char stages[STAGES * BYTES];
     __shared__ int32_t rows[SUMS ? 1 : BM];
 
-    // Workgroups b, b + 8, .. run on the same XCD: each XCD gets consecutive tiles, so that its L2 holds what they share.
+    // Workgroups b, b + 8, .. run on the same XCD. Tiles of rows take the same time each: an XCD gets consecutive ones, so
+    // that its L2 holds what they share. A unit of GRAD_SUMS takes as long as it has rows: its tiles go to all XCDs (24
+    // uneven groups in consecutive tiles: 122 us instead of 88).
     const int32_t tiles_of_unit = (SUMS ? g.m_tiles : 1) * g.n_tiles;
     const int32_t units = min(count_units<UNITS>(g.groups, g.step), g.most_units);
     const int64_t tiles = static_cast<int64_t>(units) * tiles_of_unit;
     const int32_t per_xcd = static_cast<int32_t>((tiles + 7) / 8);
-    const int64_t tile = static_cast<int64_t>(blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
+    const int64_t tile = SUMS ? blockIdx.x : static_cast<int64_t>(blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
     if (static_cast<int32_t>(blockIdx.x / 8) >= per_xcd || tile >= tiles) {
         return; // (uniform)
     }
@@ -640,25 +642,33 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
     }
 }
 
-/// out[g, :] := the sum of its units' partial results, for groups of more than one unit.
+/// out[g, :] := the sum of its units' partial results, for groups of more than one unit. Four numbers per lane: partial
+/// results of four numbers begin on 16-byte boundaries (JOINED), or lanes take one each.
 constexpr int JOIN_THREADS = 256;
-template <typename T> __global__ __launch_bounds__(JOIN_THREADS) void join_units_kernel(Product<T> g) {
+template <typename T, int JOINED> __global__ __launch_bounds__(JOIN_THREADS) void join_units_kernel(Product<T> g) {
+    typedef wide_t<T> Wide __attribute__((ext_vector_type(JOINED)));
+    typedef T Narrow __attribute__((ext_vector_type(JOINED), aligned(sizeof(T))));
     const int32_t first = static_cast<int32_t>(blockIdx.x);
-    const GroupUnit unit = find_unit<Units::OF_GROUPS>(g.groups, g.step, first);
+    const GroupUnit unit = uniform(find_unit<Units::OF_GROUPS>(g.groups, g.step, first));
     if (unit.group < 0 || unit.of_group < 2 || unit.index != 0) {
         return; // (uniform)
     }
     const int32_t parts = min(unit.of_group, g.most_units - first);
-    const size_t size = static_cast<size_t>(g.m_size) * g.n_size;
-    const wide_t<T>* from = g.partial + first * size;
+    const size_t size = static_cast<size_t>(g.m_size) * g.n_size / JOINED;
+    const Wide* from = reinterpret_cast<const Wide*>(g.partial) + first * size;
     for (size_t i = blockIdx.y * static_cast<size_t>(JOIN_THREADS) + threadIdx.x; i < size;
          i += static_cast<size_t>(gridDim.y) * JOIN_THREADS) {
-        wide_t<T> sum = 0;
+        Wide sum = from[i];
 #pragma unroll 8
-        for (int32_t u = 0; u < parts; u++) {
+        for (int32_t u = 1; u < parts; u++) {
             sum += from[u * size + i];
         }
-        g.out[unit.group * size + i] = static_cast<T>(sum);
+        Narrow narrow;
+#pragma unroll
+        for (int j = 0; j < JOINED; j++) {
+            narrow[j] = static_cast<T>(sum[j]);
+        }
+        *reinterpret_cast<Narrow*>(g.out + (unit.group * size + i) * JOINED) = narrow;
     }
 }
 
