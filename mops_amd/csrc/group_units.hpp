@@ -65,66 +65,93 @@ __device__ __forceinline__ GroupUnit uniform(const GroupUnit& unit) {
     };
 }
 
-/// Unit number `unit`, by every wavefront for itself (64 groups per step). All lanes.
-template <Units WHICH>
-__device__ __forceinline__ GroupUnit find_unit(const RowGroups& groups, int32_t step, int32_t unit) {
-    const int lane = threadIdx.x & (WAVE - 1);
-    for (int32_t base = 0; base < groups.n_groups; base += WAVE) {
-        const int32_t group = min(base + lane, groups.n_groups - 1);
-        const int32_t begin = groups.begin_of(group);
-        const int32_t count = groups.end_of(group, begin) - begin;
-        const int32_t units = base + lane < groups.n_groups ? units_of<WHICH>(count, step) : 0;
-        int32_t upto = units;
+/// The units of all groups, looked at by every wavefront for itself: a lane per group, 64 groups at a time; up to 64
+/// groups are read once for everything. All lanes call everything.
+template <Units WHICH> class UnitsOfGroups {
+public:
+    __device__ __forceinline__ UnitsOfGroups(const RowGroups& groups, int32_t step) : groups_(groups), step_(step) {
+        look(0);
+        listed_first_ = groups.n_groups > 0 ? __builtin_amdgcn_readlane(begin_, 0) : 0;
+    }
+
+    /// How many there are.
+    __device__ __forceinline__ int32_t total() {
+        int32_t total = __builtin_amdgcn_readlane(upto_, WAVE - 1);
+        for (int32_t base = WAVE; base < groups_.n_groups; base += WAVE) {
+            look(base);
+            total += __builtin_amdgcn_readlane(upto_, WAVE - 1);
+        }
+        if (WHICH == Units::OF_ROWS) {
+            total += (rest() + step_ - 1) / step_;
+        }
+        return total;
+    }
+
+    /// Unit number `unit`.
+    __device__ __forceinline__ GroupUnit find(int32_t unit) {
+        for (int32_t base = 0; base < groups_.n_groups; base += WAVE) {
+            if (base != base_) {
+                look(base);
+            }
+            const uint64_t past = __ballot(upto_ > unit);
+            if (past != 0) {
+                const int at = __builtin_ctzll(past);
+                const int32_t of_group = __builtin_amdgcn_readlane(units_, at);
+                const int32_t index = unit - (__builtin_amdgcn_readlane(upto_, at) - of_group);
+                const int32_t first = __builtin_amdgcn_readlane(begin_, at) + index * step_;
+                const int32_t left = __builtin_amdgcn_readlane(count_, at) - index * step_;
+                return uniform(GroupUnit{base + at, first, min(left, step_), index, of_group});
+            }
+            unit -= __builtin_amdgcn_readlane(upto_, WAVE - 1);
+        }
+        if (WHICH == Units::OF_ROWS) {
+            const int32_t rest_rows = rest(), units = (rest_rows + step_ - 1) / step_;
+            if (unit < units) {
+                return uniform(
+                    GroupUnit{groups_.n_groups, unit * step_, min(rest_rows - unit * step_, step_), unit, units}
+                );
+            }
+        }
+        return GroupUnit{-1, 0, 0, 0, 0};
+    }
+
+private:
+    /// Groups base .. base + 63: their places and units, and how many units they have up to this one.
+    __device__ __forceinline__ void look(int32_t base) {
+        const int lane = threadIdx.x & (WAVE - 1);
+        const int32_t group = max(min(base + lane, groups_.n_groups - 1), 0);
+        base_ = base;
+        begin_ = groups_.begin_of(group);
+        end_ = groups_.n_groups > 0 ? groups_.end_of(group, begin_) : begin_;
+        count_ = end_ - begin_;
+        units_ = base + lane < groups_.n_groups ? units_of<WHICH>(count_, step_) : 0;
+        upto_ = units_;
 #pragma unroll
         for (int s = 1; s < WAVE; s <<= 1) {
-            const int32_t other = __shfl_up(upto, s);
-            upto += lane >= s ? other : 0;
-        }
-        const uint64_t past = __ballot(upto > unit);
-        if (past != 0) {
-            const int at = __builtin_ctzll(past);
-            const int32_t of_group = __builtin_amdgcn_readlane(units, at);
-            const int32_t index = unit - (__builtin_amdgcn_readlane(upto, at) - of_group);
-            const int32_t first = __builtin_amdgcn_readlane(begin, at) + index * step;
-            const int32_t left = __builtin_amdgcn_readlane(count, at) - index * step;
-            return uniform(GroupUnit{base + at, first, min(left, step), index, of_group});
-        }
-        unit -= __builtin_amdgcn_readlane(upto, WAVE - 1);
-    }
-    if (WHICH == Units::OF_ROWS) {
-        const int32_t first = groups.begin_of(0), listed = groups.end_of(groups.n_groups - 1, first) - first;
-        const int32_t rest = groups.n_rows - listed, units = (rest + step - 1) / step;
-        if (unit < units) {
-            return uniform(GroupUnit{groups.n_groups, unit * step, min(rest - unit * step, step), unit, units});
+            const int32_t other = __shfl_up(upto_, s);
+            upto_ += lane >= s ? other : 0;
         }
     }
-    return GroupUnit{-1, 0, 0, 0, 0};
-}
+    /// The rows of no group (lanes behind the last group hold the last one).
+    __device__ __forceinline__ int32_t rest() {
+        const int32_t last = (groups_.n_groups - 1) / WAVE * WAVE;
+        if (groups_.n_groups > 0 && base_ != last) {
+            look(last);
+        }
+        const int32_t listed = max(__builtin_amdgcn_readlane(end_, WAVE - 1) - listed_first_, 0);
+        return groups_.n_rows - (groups_.n_groups > 0 ? listed : 0);
+    }
 
-/// How many units there are. All lanes of a wavefront.
-template <Units WHICH> __device__ __forceinline__ int32_t count_units(const RowGroups& groups, int32_t step) {
-    const int lane = threadIdx.x & (WAVE - 1);
-    int32_t total = 0;
-    for (int32_t group = lane; group < groups.n_groups; group += WAVE) {
-        const int32_t begin = groups.begin_of(group);
-        total += units_of<WHICH>(groups.end_of(group, begin) - begin, step);
-    }
-#pragma unroll
-    for (int s = 1; s < WAVE; s <<= 1) {
-        total += __shfl_xor(total, s);
-    }
-    if (WHICH == Units::OF_ROWS) {
-        const int32_t first = groups.begin_of(0);
-        const int32_t rest = groups.n_rows - (groups.end_of(groups.n_groups - 1, first) - first);
-        total += (rest + step - 1) / step;
-    }
-    return __builtin_amdgcn_readfirstlane(total);
-}
+    const RowGroups& groups_;
+    int32_t step_, base_, listed_first_;
+    int32_t begin_, end_, count_, units_, upto_; // of this lane's group
+};
 
 /// The place of number `i` of the rows that belong to no group: before the first group's places, or behind the last's.
 __device__ __forceinline__ int32_t place_of_rest(const RowGroups& groups, int32_t i) {
-    const int32_t first = groups.begin_of(0);
-    return i < first ? i : i - first + groups.end_of(groups.n_groups - 1, first);
+    const int32_t first = groups.n_groups > 0 ? groups.begin_of(0) : 0;
+    const int32_t last = groups.n_groups > 0 ? max(groups.end_of(groups.n_groups - 1, groups.begin_of(groups.n_groups - 1)), first) : 0;
+    return min(i < first ? i : i - first + last, groups.n_rows - 1);
 }
 
 } // namespace mops::amd

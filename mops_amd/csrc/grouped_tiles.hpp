@@ -63,14 +63,15 @@ template <typename T> struct Product {
 
 /// The matrix instructions of a type: blocks of BLOCK x BLOCK, and a piece of 16 bytes of k per lane and side: lane l
 /// has row l % BLOCK of the block, numbers (l / BLOCK) * COUNT + (0 .. COUNT - 1) of the k of one multiplication.
-/// Lane l, number i of the result: column l % BLOCK (of q's side), row row_of(l, i) (of p's side).
+/// PARTS instructions make up the multiplication. Lane l, number i of the result: column l % BLOCK (of q's side), row row_of(l, i) (of p's side).
 template <typename T> struct Matrix;
 
 template <> struct Matrix<__bf16> {
     static constexpr int BLOCK = 32, COUNT = 8, HELD = 16;
     typedef __bf16 Numbers __attribute__((ext_vector_type(8)));
     typedef float Sums __attribute__((ext_vector_type(16)));
-    static __device__ __forceinline__ Sums multiply(Numbers p, Numbers q, Sums sums) {
+    static constexpr int PARTS = 1;
+    static __device__ __forceinline__ Sums multiply(int, Numbers p, Numbers q, Sums sums) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(p, q, sums, 0, 0, 0);
     }
     static __device__ __forceinline__ int row_of(int lane, int i) { return 8 * (i / 4) + 4 * (lane / 32) + i % 4; }
@@ -80,7 +81,8 @@ template <> struct Matrix<_Float16> {
     static constexpr int BLOCK = 32, COUNT = 8, HELD = 16;
     typedef _Float16 Numbers __attribute__((ext_vector_type(8)));
     typedef float Sums __attribute__((ext_vector_type(16)));
-    static __device__ __forceinline__ Sums multiply(Numbers p, Numbers q, Sums sums) {
+    static constexpr int PARTS = 1;
+    static __device__ __forceinline__ Sums multiply(int, Numbers p, Numbers q, Sums sums) {
         return __builtin_amdgcn_mfma_f32_32x32x16_f16(p, q, sums, 0, 0, 0);
     }
     static __device__ __forceinline__ int row_of(int lane, int i) { return 8 * (i / 4) + 4 * (lane / 32) + i % 4; }
@@ -90,12 +92,9 @@ template <> struct Matrix<float> {
     static constexpr int BLOCK = 32, COUNT = 4, HELD = 16;
     typedef float Numbers __attribute__((ext_vector_type(4)));
     typedef float Sums __attribute__((ext_vector_type(16)));
-    static __device__ __forceinline__ Sums multiply(Numbers p, Numbers q, Sums sums) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            sums = __builtin_amdgcn_mfma_f32_32x32x2f32(p[i], q[i], sums, 0, 0, 0);
-        }
-        return sums;
+    static constexpr int PARTS = 4;
+    static __device__ __forceinline__ Sums multiply(int part, Numbers p, Numbers q, Sums sums) {
+        return __builtin_amdgcn_mfma_f32_32x32x2f32(p[part], q[part], sums, 0, 0, 0);
     }
     static __device__ __forceinline__ int row_of(int lane, int i) { return 8 * (i / 4) + 4 * (lane / 32) + i % 4; }
     static constexpr int RUN = 4;
@@ -104,12 +103,9 @@ template <> struct Matrix<double> {
     static constexpr int BLOCK = 16, COUNT = 2, HELD = 4;
     typedef double Numbers __attribute__((ext_vector_type(2)));
     typedef double Sums __attribute__((ext_vector_type(4)));
-    static __device__ __forceinline__ Sums multiply(Numbers p, Numbers q, Sums sums) {
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            sums = __builtin_amdgcn_mfma_f64_16x16x4f64(p[i], q[i], sums, 0, 0, 0);
-        }
-        return sums;
+    static constexpr int PARTS = 2;
+    static __device__ __forceinline__ Sums multiply(int part, Numbers p, Numbers q, Sums sums) {
+        return __builtin_amdgcn_mfma_f64_16x16x4f64(p[part], q[part], sums, 0, 0, 0);
     }
     static __device__ __forceinline__ int row_of(int lane, int i) { return 4 * i + lane / 16; }
     static constexpr int RUN = 1;
@@ -335,7 +331,8 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
     // that its L2 holds what they share. A unit of GRAD_SUMS takes as long as it has rows: its tiles go to all XCDs (24
     // uneven groups in consecutive tiles: 122 us instead of 88).
     const int32_t tiles_of_unit = (SUMS ? g.m_tiles : 1) * g.n_tiles;
-    const int32_t units = min(count_units<UNITS>(g.groups, g.step), g.most_units);
+    UnitsOfGroups<UNITS> of_groups(g.groups, g.step);
+    const int32_t units = min(of_groups.total(), g.most_units);
     const int64_t tiles = static_cast<int64_t>(units) * tiles_of_unit;
     const int32_t per_xcd = static_cast<int32_t>((tiles + 7) / 8);
     const int64_t tile = SUMS ? blockIdx.x : static_cast<int64_t>(blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
@@ -356,7 +353,7 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
         m0 = 0;
         n0 = in_band / height * BN;
     }
-    const GroupUnit unit = uniform(find_unit<UNITS>(g.groups, g.step, unit_index));
+    const GroupUnit unit = of_groups.find(unit_index);
     if (unit.group < 0) {
         return; // (uniform; offsets that are none)
     }
@@ -480,7 +477,7 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
         // pieces [first, last) of another step, asked for by between(from, upto). (Left to itself the compiler puts all
         // reads in front, where they are waited for, and a wavefront that asks for eight pieces in a row waits until the
         // memory pipeline has taken them.)
-        constexpr int SLOTS = MB * NB, READS = MB + NB, OF_SLOT = (READS + SLOTS - 1) / SLOTS;
+        constexpr int SLOTS = MB * NB * M::PARTS, READS = MB + NB, OF_SLOT = (READS + SLOTS - 1) / SLOTS;
         auto multiply = [&](int step, const char* next_buffer, int next_step, int first, int last, auto&& between) {
             if (!works) {
                 between(first, last);
@@ -498,8 +495,8 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
                 const int upto = first + (slot + 1) * (last - first) / SLOTS;
                 between(asked, upto);
                 asked = upto;
-                const int i = slot / NB, j = slot % NB;
-                sums[i][j] = M::multiply(of_p[step % 2][j], of_q[step % 2][i], sums[i][j]);
+                const int i = slot / (NB * M::PARTS), j = slot % NB;
+                sums[i][j] = M::multiply(slot / NB % M::PARTS, of_p[step % 2][j], of_q[step % 2][i], sums[i][j]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
@@ -649,7 +646,7 @@ template <typename T, int JOINED> __global__ __launch_bounds__(JOIN_THREADS) voi
     typedef wide_t<T> Wide __attribute__((ext_vector_type(JOINED)));
     typedef T Narrow __attribute__((ext_vector_type(JOINED), aligned(sizeof(T))));
     const int32_t first = static_cast<int32_t>(blockIdx.x);
-    const GroupUnit unit = uniform(find_unit<Units::OF_GROUPS>(g.groups, g.step, first));
+    const GroupUnit unit = UnitsOfGroups<Units::OF_GROUPS>(g.groups, g.step).find(first);
     if (unit.group < 0 || unit.of_group < 2 || unit.index != 0) {
         return; // (uniform)
     }
