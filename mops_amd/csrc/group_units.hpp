@@ -72,6 +72,9 @@ public:
     __device__ __forceinline__ UnitsOfGroups(const RowGroups& groups, int32_t step) : groups_(groups), step_(step) {
         look(0);
         listed_first_ = groups.n_groups > 0 ? __builtin_amdgcn_readlane(begin_, 0) : 0;
+        if (WHICH == Units::OF_GROUPS && groups.n_groups <= WAVE) {
+            largest_first();
+        }
     }
 
     /// How many there are.
@@ -100,7 +103,8 @@ public:
                 const int32_t index = unit - (__builtin_amdgcn_readlane(upto_, at) - of_group);
                 const int32_t first = __builtin_amdgcn_readlane(begin_, at) + index * step_;
                 const int32_t left = __builtin_amdgcn_readlane(count_, at) - index * step_;
-                return uniform(GroupUnit{base + at, first, min(left, step_), index, of_group});
+                const int32_t group = __builtin_amdgcn_readlane(group_, at);
+                return uniform(GroupUnit{group, first, min(left, step_), index, of_group});
             }
             unit -= __builtin_amdgcn_readlane(upto_, WAVE - 1);
         }
@@ -115,22 +119,61 @@ public:
         return GroupUnit{-1, 0, 0, 0, 0};
     }
 
+    /// The first unit of a group, and how many it has (in GroupUnit::index, of_group).
+    __device__ __forceinline__ GroupUnit of(int32_t group) {
+        int32_t before = 0;
+        for (int32_t base = 0; base < groups_.n_groups; base += WAVE) {
+            if (base != base_) {
+                look(base);
+            }
+            const uint64_t here = __ballot(group_ == group);
+            if (here != 0) {
+                const int at = __builtin_ctzll(here);
+                const int32_t of_group = __builtin_amdgcn_readlane(units_, at);
+                return uniform(GroupUnit{group, 0, 0, before + __builtin_amdgcn_readlane(upto_, at) - of_group, of_group});
+            }
+            before += __builtin_amdgcn_readlane(upto_, WAVE - 1);
+        }
+        return GroupUnit{-1, 0, 0, 0, 0};
+    }
+
 private:
     /// Groups base .. base + 63: their places and units, and how many units they have up to this one.
     __device__ __forceinline__ void look(int32_t base) {
         const int lane = threadIdx.x & (WAVE - 1);
         const int32_t group = max(min(base + lane, groups_.n_groups - 1), 0);
         base_ = base;
+        group_ = base + lane;
         begin_ = groups_.begin_of(group);
         end_ = groups_.n_groups > 0 ? groups_.end_of(group, begin_) : begin_;
         count_ = end_ - begin_;
         units_ = base + lane < groups_.n_groups ? units_of<WHICH>(count_, step_) : 0;
+        add_up();
+    }
+    __device__ __forceinline__ void add_up() {
+        const int lane = threadIdx.x & (WAVE - 1);
         upto_ = units_;
 #pragma unroll
         for (int s = 1; s < WAVE; s <<= 1) {
             const int32_t other = __shfl_up(upto_, s);
             upto_ += lane >= s ? other : 0;
         }
+    }
+    /// The groups in the order of their sizes: a unit of OF_GROUPS takes as long as it has rows, and the last ones to be
+    /// started should be short.
+    __device__ __forceinline__ void largest_first() {
+        const int lane = threadIdx.x & (WAVE - 1);
+        const int32_t size = lane < groups_.n_groups ? count_ : -1;
+        int32_t rank = 0;
+        for (int other = 0; other < WAVE; other++) {
+            const int32_t of_other = __builtin_amdgcn_readlane(size, other);
+            rank += of_other > size || (of_other == size && other < lane) ? 1 : 0;
+        }
+        group_ = __builtin_amdgcn_ds_permute(4 * rank, lane);
+        begin_ = __shfl(begin_, group_);
+        count_ = __shfl(count_, group_);
+        units_ = __shfl(units_, group_);
+        add_up();
     }
     /// The rows of no group (lanes behind the last group hold the last one).
     __device__ __forceinline__ int32_t rest() {
@@ -144,7 +187,7 @@ private:
 
     const RowGroups& groups_;
     int32_t step_, base_, listed_first_;
-    int32_t begin_, end_, count_, units_, upto_; // of this lane's group
+    int32_t group_, begin_, end_, count_, units_, upto_; // of this lane's group
 };
 
 /// The place of number `i` of the rows that belong to no group: before the first group's places, or behind the last's.

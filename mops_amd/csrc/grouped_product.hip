@@ -73,7 +73,9 @@ template <typename T> void sum_of_rows(Product<T> g, hipStream_t stream) {
     const size_t rows = static_cast<size_t>(std::max(g.groups.n_rows, 1));
     const size_t big = static_cast<size_t>(tiles(g.m_size, 256)) * tiles(g.n_size, 256);
     const size_t middle = static_cast<size_t>(tiles(g.m_size, 128)) * tiles(g.n_size, 128);
-    const bool use_big = sizeof(T) == 2 && big * groups >= units;
+    // (big tiles: one workgroup per compute unit, in groups that can be split if there are too few of them)
+    const bool use_big = sizeof(T) == 2 && g.m_size >= 256 && g.n_size >= 256 &&
+                         big * std::max(groups, ceil_div(rows, 2048)) >= units;
     const bool use_middle = g.m_size > 64 && g.n_size > 64;
     const size_t tiles_of_unit =
         use_big ? big : use_middle ? middle : static_cast<size_t>(tiles(g.m_size, 64)) * tiles(g.n_size, 64);
@@ -81,7 +83,7 @@ template <typename T> void sum_of_rows(Product<T> g, hipStream_t stream) {
     if (tiles_of_unit * groups >= units) {
         step = std::max<size_t>(4 * rows / groups, 4096);
     } else {
-        step = std::max<size_t>(ceil_div(rows, ceil_div(2 * units, tiles_of_unit)), 256);
+        step = std::max<size_t>(ceil_div(rows, ceil_div((use_big ? 1 : 2) * units, tiles_of_unit)), 256);
     }
     step = std::min(ceil_div(step, 64) * 64, ceil_div(rows, 64) * 64);
     g.step = static_cast<int32_t>(step);
@@ -101,13 +103,13 @@ template <typename T> void sum_of_rows(Product<T> g, hipStream_t stream) {
         launch<T, Form::GRAD_SUMS, 64, 64, 2, 2>(g, stream);
     }
     if (splits) {
-        // (few workgroups per unit: most units are not the first one of several, and theirs have nothing to do)
         g.most_units = narrow_i32(most, "number of units of rows");
         auto join = [&](auto joined) {
             constexpr int JOINED = decltype(joined)::value;
-            const size_t wanted = ceil_div(size / JOINED, JOIN_THREADS);
-            const unsigned blocks = static_cast<unsigned>(std::min(wanted, std::max<size_t>(16, 8 * units / most)));
-            join_units_kernel<T, JOINED><<<dim3(static_cast<unsigned>(most), blocks), JOIN_THREADS, 0, stream>>>(g);
+            const size_t wanted = ceil_div(size / JOINED, WAVE), room = ceil_div(4 * units, groups);
+            join_units_kernel<T, JOINED><<<
+                dim3(static_cast<unsigned>(groups), static_cast<unsigned>(std::min(wanted, room))), JOIN_WAVES * WAVE, 0,
+                stream>>>(g);
         };
         if (size % 4 == 0) {
             join(std::integral_constant<int, 4>{});

@@ -639,33 +639,48 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
     }
 }
 
-/// out[g, :] := the sum of its units' partial results, for groups of more than one unit. Four numbers per lane: partial
-/// results of four numbers begin on 16-byte boundaries (JOINED), or lanes take one each.
-constexpr int JOIN_THREADS = 256;
-template <typename T, int JOINED> __global__ __launch_bounds__(JOIN_THREADS) void join_units_kernel(Product<T> g) {
+/// out[g, :] := the sum of its units' partial results, for groups of more than one unit; blockIdx.x: the group. A lane
+/// has JOINED numbers (four where partial results of four numbers begin on 16-byte boundaries), a wavefront every
+/// fourth of the partial results.
+constexpr int JOIN_WAVES = 4;
+template <typename T, int JOINED>
+__global__ __launch_bounds__(JOIN_WAVES* WAVE) void join_units_kernel(Product<T> g) {
     typedef wide_t<T> Wide __attribute__((ext_vector_type(JOINED)));
     typedef T Narrow __attribute__((ext_vector_type(JOINED), aligned(sizeof(T))));
-    const int32_t first = static_cast<int32_t>(blockIdx.x);
-    const GroupUnit unit = UnitsOfGroups<Units::OF_GROUPS>(g.groups, g.step).find(first);
-    if (unit.group < 0 || unit.of_group < 2 || unit.index != 0) {
+    __shared__ Wide shared[JOIN_WAVES][WAVE];
+    const GroupUnit unit =
+        UnitsOfGroups<Units::OF_GROUPS>(g.groups, g.step).of(static_cast<int32_t>(blockIdx.x));
+    if (unit.group < 0 || unit.of_group < 2 || unit.index >= g.most_units) {
         return; // (uniform)
     }
-    const int32_t parts = min(unit.of_group, g.most_units - first);
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+    const int32_t parts = min(unit.of_group, g.most_units - unit.index);
     const size_t size = static_cast<size_t>(g.m_size) * g.n_size / JOINED;
-    const Wide* from = reinterpret_cast<const Wide*>(g.partial) + first * size;
-    for (size_t i = blockIdx.y * static_cast<size_t>(JOIN_THREADS) + threadIdx.x; i < size;
-         i += static_cast<size_t>(gridDim.y) * JOIN_THREADS) {
-        Wide sum = from[i];
+    const Wide* from = reinterpret_cast<const Wide*>(g.partial) + unit.index * size;
+    for (size_t first = blockIdx.y * static_cast<size_t>(WAVE); first < size; first += static_cast<size_t>(gridDim.y) * WAVE) {
+        const size_t i = first + lane;
+        Wide sum{};
+        if (i < size) {
 #pragma unroll 8
-        for (int32_t u = 1; u < parts; u++) {
-            sum += from[u * size + i];
+            for (int32_t u = wave; u < parts; u += JOIN_WAVES) {
+                sum += from[u * size + i];
+            }
         }
-        Narrow narrow;
+        shared[wave][lane] = sum;
+        __syncthreads();
+        if (wave == 0 && i < size) {
+            Narrow narrow;
 #pragma unroll
-        for (int j = 0; j < JOINED; j++) {
-            narrow[j] = static_cast<T>(sum[j]);
+            for (int w = 1; w < JOIN_WAVES; w++) {
+                sum += shared[w][lane];
+            }
+#pragma unroll
+            for (int j = 0; j < JOINED; j++) {
+                narrow[j] = static_cast<T>(sum[j]);
+            }
+            *reinterpret_cast<Narrow*>(g.out + (unit.group * size + i) * JOINED) = narrow;
         }
-        *reinterpret_cast<Narrow*>(g.out + (unit.group * size + i) * JOINED) = narrow;
+        __syncthreads();
     }
 }
 
