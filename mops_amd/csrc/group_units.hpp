@@ -119,22 +119,23 @@ public:
         return GroupUnit{-1, 0, 0, 0, 0};
     }
 
-    /// The first unit of a group, and how many it has (in GroupUnit::index, of_group).
-    __device__ __forceinline__ GroupUnit of(int32_t group) {
+    /// body(unit) for every group of more than one unit: its first one (index: its number), without its places.
+    template <typename Body> __device__ __forceinline__ void for_split_groups(Body&& body) {
         int32_t before = 0;
         for (int32_t base = 0; base < groups_.n_groups; base += WAVE) {
             if (base != base_) {
                 look(base);
             }
-            const uint64_t here = __ballot(group_ == group);
-            if (here != 0) {
-                const int at = __builtin_ctzll(here);
+            uint64_t split = __ballot(units_ > 1);
+            while (split != 0) {
+                const int at = __builtin_ctzll(split);
+                split &= split - 1;
                 const int32_t of_group = __builtin_amdgcn_readlane(units_, at);
-                return uniform(GroupUnit{group, 0, 0, before + __builtin_amdgcn_readlane(upto_, at) - of_group, of_group});
+                const int32_t first = before + __builtin_amdgcn_readlane(upto_, at) - of_group;
+                body(uniform(GroupUnit{__builtin_amdgcn_readlane(group_, at), 0, 0, first, of_group}));
             }
             before += __builtin_amdgcn_readlane(upto_, WAVE - 1);
         }
-        return GroupUnit{-1, 0, 0, 0, 0};
     }
 
 private:

@@ -45,9 +45,9 @@ template <typename T, Form FORM, int BM, int BN, int WM, int WN, int DEEP = 8, i
     g.most_units = narrow_i32(most_units(g.groups.n_rows, g.groups.n_groups, g.step), "number of units of rows");
     const size_t workgroups = ceil_div(static_cast<size_t>(g.most_units) * g.m_tiles * g.n_tiles, 8) * 8;
     const unsigned blocks = static_cast<unsigned>(narrow_i32(workgroups, "number of tiles"));
-    if (aligned(g.q, q_width<T, FORM>(g)) && aligned(g.p, p_width<T, FORM>(g))) {
+    if (BM == 256 || (aligned(g.q, q_width<T, FORM>(g)) && aligned(g.p, p_width<T, FORM>(g)))) {
         tiles_kernel<T, FORM, BM, BN, WM, WN, DEEP, STAGES, true><<<blocks, WM * WN * WAVE, 0, stream>>>(g);
-    } else {
+    } else if constexpr (BM < 256) {
         tiles_kernel<T, FORM, BM, BN, WM, WN, 8, 2, false><<<blocks, WM * WN * WAVE, 0, stream>>>(g);
     }
 }
@@ -56,7 +56,9 @@ template <typename T, Form FORM> void rows_times(const Product<T>& g, hipStream_
     const size_t rows = static_cast<size_t>(g.groups.n_rows);
     const size_t big = ceil_div(rows, 256) * tiles(g.n_size, 256), middle = ceil_div(rows, 128) * tiles(g.n_size, 128);
     const size_t units = static_cast<size_t>(compute_units());
-    if (sizeof(T) == 2 && big >= units && rows >= 128 * static_cast<size_t>(g.groups.n_groups)) {
+    // (through registers the tiles of 256 leave none for the pieces that are on their way)
+    const bool in_place = aligned(g.q, q_width<T, FORM>(g)) && aligned(g.p, p_width<T, FORM>(g));
+    if (sizeof(T) == 2 && in_place && big >= units && rows >= 128 * static_cast<size_t>(g.groups.n_groups)) {
         if constexpr (sizeof(T) == 2) {
             launch<T, FORM, 256, 256, 2, 4, 8, 2>(g, stream);
         }
@@ -74,24 +76,21 @@ template <typename T> void sum_of_rows(Product<T> g, hipStream_t stream) {
     const size_t big = static_cast<size_t>(tiles(g.m_size, 256)) * tiles(g.n_size, 256);
     const size_t middle = static_cast<size_t>(tiles(g.m_size, 128)) * tiles(g.n_size, 128);
     // (big tiles: one workgroup per compute unit, in groups that can be split if there are too few of them)
-    const bool use_big = sizeof(T) == 2 && g.m_size >= 256 && g.n_size >= 256 &&
+    const bool use_big = sizeof(T) == 2 && aligned(g.q, g.m_size) && aligned(g.p, g.n_size) && g.m_size >= 256 && g.n_size >= 256 &&
                          big * std::max(groups, ceil_div(rows, 2048)) >= units;
     const bool use_middle = g.m_size > 64 && g.n_size > 64;
     const size_t tiles_of_unit =
         use_big ? big : use_middle ? middle : static_cast<size_t>(tiles(g.m_size, 64)) * tiles(g.n_size, 64);
-    size_t step = rows;
-    if (tiles_of_unit * groups >= units) {
-        step = std::max<size_t>(4 * rows / groups, 4096);
-    } else {
-        step = std::max<size_t>(ceil_div(rows, ceil_div((use_big ? 1 : 2) * units, tiles_of_unit)), 256);
-    }
+    // Rows per unit: what every workgroup that the GPU has room for would have if the work were shared out evenly. Larger
+    // groups than that are split, smaller ones are not.
+    const size_t room = (use_big ? 1 : 2) * units;
+    size_t step = std::max<size_t>(ceil_div(rows * tiles_of_unit, room), 256);
     step = std::min(ceil_div(step, 64) * 64, ceil_div(rows, 64) * 64);
     g.step = static_cast<int32_t>(step);
     const bool splits = step < rows;
     const size_t most = most_units(g.groups.n_rows, g.groups.n_groups, g.step);
-    const size_t size = static_cast<size_t>(g.m_size) * g.n_size;
     if (splits) {
-        g.partial = static_cast<wide_t<T>*>(scratch(most * size * sizeof(wide_t<T>)));
+        g.partial = static_cast<wide_t<T>*>(scratch(most * partial_size(g.m_size, g.n_size) * sizeof(wide_t<T>)));
     }
     if (use_big) {
         if constexpr (sizeof(T) == 2) {
@@ -104,18 +103,7 @@ template <typename T> void sum_of_rows(Product<T> g, hipStream_t stream) {
     }
     if (splits) {
         g.most_units = narrow_i32(most, "number of units of rows");
-        auto join = [&](auto joined) {
-            constexpr int JOINED = decltype(joined)::value;
-            const size_t wanted = ceil_div(size / JOINED, WAVE), room = ceil_div(4 * units, groups);
-            join_units_kernel<T, JOINED><<<
-                dim3(static_cast<unsigned>(groups), static_cast<unsigned>(std::min(wanted, room))), JOIN_WAVES * WAVE, 0,
-                stream>>>(g);
-        };
-        if (size % 4 == 0) {
-            join(std::integral_constant<int, 4>{});
-        } else {
-            join(std::integral_constant<int, 1>{});
-        }
+        join_units_kernel<T><<<static_cast<unsigned>(4 * units), JOIN_WAVES * WAVE, 0, stream>>>(g);
     }
     MOPS_HIP_CHECK(hipGetLastError());
 }

@@ -52,7 +52,7 @@ enum class Form { FORWARD, GRAD_ROWS, GRAD_SUMS };
 /// [rows][m_size], p is [rows][n_size].
 template <typename T> struct Product {
     T* out;
-    wide_t<T>* partial; // GRAD_SUMS: [unit][m_size][n_size], for groups of more than one unit
+    wide_t<T>* partial; // GRAD_SUMS: [unit][partial_size(m_size, n_size)], for groups of more than one unit
     const T *q, *p;
     RowGroups groups;
     int32_t m_size, n_size, k_size;
@@ -60,6 +60,11 @@ template <typename T> struct Product {
     int32_t most_units;      // that the grid and `partial` have room for (offsets that are none could give more)
     int32_t m_tiles, n_tiles; // tiles of a unit (m_tiles: GRAD_SUMS)
 };
+
+/// Numbers from one unit's partial result to the next: whole pieces of four.
+__host__ __device__ __forceinline__ size_t partial_size(int32_t m_size, int32_t n_size) {
+    return (static_cast<size_t>(m_size) * n_size + 3) / 4 * 4;
+}
 
 /// The matrix instructions of a type: blocks of BLOCK x BLOCK, and a piece of 16 bytes of k per lane and side: lane l
 /// has row l % BLOCK of the block, numbers (l / BLOCK) * COUNT + (0 .. COUNT - 1) of the k of one multiplication.
@@ -113,24 +118,39 @@ template <> struct Matrix<double> {
 
 template <typename T> using Numbers = typename Matrix<T>::Numbers;
 
-/// The first `count` of a piece's numbers, zeros behind them (count may be negative, or beyond the piece). WHOLE: all.
-template <typename T, bool WHOLE> __device__ __forceinline__ Numbers<T> load_numbers(const T* from, int32_t count) {
+/// A piece at any alignment.
+template <typename T> __device__ __forceinline__ Numbers<T> load_numbers(const T* from) {
     constexpr int COUNT = Matrix<T>::COUNT;
+    typedef T Anywhere __attribute__((ext_vector_type(COUNT), aligned(sizeof(T))));
+    const Anywhere a = *reinterpret_cast<const Anywhere*>(from);
     Numbers<T> v;
-    if (WHOLE || count >= COUNT) {
-        typedef T Anywhere __attribute__((ext_vector_type(COUNT), aligned(sizeof(T))));
-        const Anywhere a = *reinterpret_cast<const Anywhere*>(from);
 #pragma unroll
-        for (int i = 0; i < COUNT; i++) {
-            v[i] = a[i];
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < COUNT; i++) {
-            v[i] = i < count ? from[i] : static_cast<T>(0.f);
-        }
+    for (int i = 0; i < COUNT; i++) {
+        v[i] = a[i];
     }
     return v;
+}
+/// The first `count` numbers, zeros behind them.
+template <typename T> __device__ __forceinline__ Numbers<T> load_some_numbers(const T* from, int32_t count) {
+    Numbers<T> v;
+#pragma unroll
+    for (int i = 0; i < Matrix<T>::COUNT; i++) {
+        v[i] = i < count ? from[i] : static_cast<T>(0.f);
+    }
+    return v;
+}
+/// Numbers `missing` .. of a piece, and as many zeros behind them (missing = all: zeros).
+template <typename T> __device__ __forceinline__ Numbers<T> without_first(Numbers<T> v, int32_t missing) {
+    union {
+        Numbers<T> numbers;
+        uint64_t half[2];
+    } both;
+    both.numbers = v;
+    const int bits = missing * static_cast<int>(8 * sizeof(T));
+    const uint64_t low = both.half[0], high = both.half[1];
+    both.half[0] = bits >= 128 ? 0 : bits >= 64 ? high >> (bits - 64) : bits > 0 ? low >> bits | high << (64 - bits) : low;
+    both.half[1] = bits >= 64 ? 0 : high >> bits;
+    return both.numbers;
 }
 
 /// LDS of a straight side of OUTER rows: [OUTER][DEEP pieces], DEEP 4 or 8, permuted so that 16 lanes that read the same
@@ -211,15 +231,29 @@ __device__ __forceinline__ void fetch(const void* from, char* lds) {
 template <typename T, int OUTER, int DEEP, int THREADS, bool ALIGNED> struct Pieces {
     static constexpr int EACH = OUTER * DEEP / THREADS, COUNT = Matrix<T>::COUNT;
     Numbers<T> piece[ALIGNED ? 1 : EACH];
+    int32_t missing[ALIGNED ? 1 : EACH]; // of the piece's numbers, which then hold `missing` of the row's earlier ones in front
+    bool complete;                       // no piece of the step misses any (uniform)
 
     /// piece j: numbers `from` .. of a row, of which `left` are in the row (at most 0: none). WHOLE: all of them are,
-    /// or the side's row does not matter.
-    template <bool WHOLE> __device__ __forceinline__ void take(int j, const T* from, int32_t left, char* lds, int wave) {
+    /// or the side's row does not matter. Through registers, the last piece of a row is the row's last COUNT numbers
+    /// (`short_rows`: there are fewer), of which it drops those of the piece before when it is stored.
+    template <bool WHOLE>
+    __device__ __forceinline__ void take(int j, const T* from, int32_t left, bool short_rows, char* lds, int wave) {
         if constexpr (ALIGNED) {
             const void* at = WHOLE || left > 0 ? static_cast<const void*>(from) : &zeros_in_memory;
             fetch(at, lds + (wave * WAVE + j * THREADS) * 16);
+        } else if constexpr (WHOLE) {
+            complete = true;
+            piece[j] = load_numbers<T>(from);
+        } else if (short_rows) { // (uniform)
+            complete = true;
+            piece[j] = load_some_numbers<T>(from, left);
         } else {
-            piece[j] = load_numbers<T, WHOLE>(from, left);
+            complete = false;
+            missing[j] = min(max(COUNT - left, 0), COUNT);
+            if (missing[j] < COUNT) {
+                piece[j] = load_numbers<T>(from - missing[j]);
+            }
         }
     }
     /// the pieces that came through registers
@@ -227,7 +261,8 @@ template <typename T, int OUTER, int DEEP, int THREADS, bool ALIGNED> struct Pie
         if constexpr (!ALIGNED) {
 #pragma unroll
             for (int j = 0; j < EACH; j++) {
-                *reinterpret_cast<Numbers<T>*>(lds + (threadIdx.x + j * THREADS) * 16) = piece[j];
+                *reinterpret_cast<Numbers<T>*>(lds + (threadIdx.x + j * THREADS) * 16) =
+                    complete ? piece[j] : without_first<T>(piece[j], missing[j]);
             }
         }
     }
@@ -255,7 +290,7 @@ struct StraightLoader : public Pieces<T, OUTER, DEEP, THREADS, ALIGNED> {
     }
     /// Piece j of the next step, which begins at k0 (steps are asked for in order).
     template <bool WHOLE> __device__ __forceinline__ void load(int j, int32_t k0, char* lds, int wave) {
-        this->template take<WHOLE>(j, from[j], k_size - k0 - of_row(j) * COUNT, lds, wave);
+        this->template take<WHOLE>(j, from[j], k_size - k0 - of_row(j) * COUNT, k_size < COUNT, lds, wave);
         from[j] += DEEP * COUNT;
     }
 };
@@ -272,6 +307,7 @@ struct TurnedLoader : public Pieces<T, OUTER, DEEP, THREADS, ALIGNED> {
     size_t next;   // numbers from a step to the next
     size_t between; // numbers between a thread's pieces
     int32_t left;   // numbers in the row from the thread's column on
+    bool short_rows;
 
     static __device__ __forceinline__ int k(int j) { return threadIdx.x / Layout::PIECES + j * K_EACH; }
     /// (the same for all pieces of a thread: their rows differ by multiples of four)
@@ -281,6 +317,7 @@ struct TurnedLoader : public Pieces<T, OUTER, DEEP, THREADS, ALIGNED> {
         static_assert(K_EACH % 4 == 0 && EACH * THREADS == OUTER * DEEP, "");
         const int32_t outer = first + of_row() * COUNT;
         left = row_width - outer;
+        short_rows = row_width < COUNT;
         // (a piece that is outside of the rows: any piece that is not)
         from = memory + (left > 0 ? outer : 0);
         next = static_cast<size_t>(DEEP * COUNT) * row_width;
@@ -292,13 +329,13 @@ struct TurnedLoader : public Pieces<T, OUTER, DEEP, THREADS, ALIGNED> {
     /// Piece j of the next step of consecutive rows (after begin_rows), of which the matrix has rows_left.
     __device__ __forceinline__ void begin_rows() { from += static_cast<size_t>(k(0)) * (between / K_EACH); }
     template <bool WHOLE> __device__ __forceinline__ void load(int j, int32_t rows_left, char* lds, int wave) {
-        this->template take<WHOLE>(j, from + j * between, k(j) < rows_left ? left : 0, lds, wave);
+        this->template take<WHOLE>(j, from + j * between, k(j) < rows_left ? left : 0, short_rows, lds, wave);
         from += j == EACH - 1 ? next : 0;
     }
     /// Piece j of a step whose row is `row` there (negative: none; not with WHOLE).
     template <bool WHOLE> __device__ __forceinline__ void load_row(int j, int32_t row, char* lds, int wave) {
         const size_t at = static_cast<size_t>(WHOLE ? row : max(row, 0)) * (between / K_EACH);
-        this->template take<WHOLE>(j, from + at, row >= 0 ? left : 0, lds, wave);
+        this->template take<WHOLE>(j, from + at, row >= 0 ? left : 0, short_rows, lds, wave);
     }
 };
 
@@ -630,7 +667,7 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
             };
         };
         if (unit.of_group > 1) { // (uniform)
-            put(wide_t<T>(), row_of(g.partial + unit_index * size));
+            put(wide_t<T>(), row_of(g.partial + unit_index * partial_size(g.m_size, g.n_size)));
         } else {
             put(T(), row_of(g.out + unit.group * size));
         }
@@ -639,49 +676,64 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
     }
 }
 
-/// out[g, :] := the sum of its units' partial results, for groups of more than one unit; blockIdx.x: the group. A lane
-/// has JOINED numbers (four where partial results of four numbers begin on 16-byte boundaries), a wavefront every
-/// fourth of the partial results.
-constexpr int JOIN_WAVES = 4;
-template <typename T, int JOINED>
-__global__ __launch_bounds__(JOIN_WAVES* WAVE) void join_units_kernel(Product<T> g) {
+/// out[g, :] := the sum of its units' partial results, for groups of more than one unit, each shared out over all
+/// workgroups. A lane has four numbers; of many partial results, a wavefront has every fourth.
+constexpr int JOIN_WAVES = 4, JOINED = 4;
+template <typename T> __global__ __launch_bounds__(JOIN_WAVES* WAVE) void join_units_kernel(Product<T> g) {
     typedef wide_t<T> Wide __attribute__((ext_vector_type(JOINED)));
     typedef T Narrow __attribute__((ext_vector_type(JOINED), aligned(sizeof(T))));
     __shared__ Wide shared[JOIN_WAVES][WAVE];
-    const GroupUnit unit =
-        UnitsOfGroups<Units::OF_GROUPS>(g.groups, g.step).of(static_cast<int32_t>(blockIdx.x));
-    if (unit.group < 0 || unit.of_group < 2 || unit.index >= g.most_units) {
-        return; // (uniform)
-    }
     const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
-    const int32_t parts = min(unit.of_group, g.most_units - unit.index);
-    const size_t size = static_cast<size_t>(g.m_size) * g.n_size / JOINED;
-    const Wide* from = reinterpret_cast<const Wide*>(g.partial) + unit.index * size;
-    for (size_t first = blockIdx.y * static_cast<size_t>(WAVE); first < size; first += static_cast<size_t>(gridDim.y) * WAVE) {
-        const size_t i = first + lane;
-        Wide sum{};
-        if (i < size) {
+    const size_t size = static_cast<size_t>(g.m_size) * g.n_size, pieces = partial_size(g.m_size, g.n_size) / JOINED;
+    UnitsOfGroups<Units::OF_GROUPS> of_groups(g.groups, g.step);
+    int32_t turn = static_cast<int32_t>(blockIdx.x); // (another workgroup begins with each group)
+    of_groups.for_split_groups([&](const GroupUnit& unit) {
+        const int32_t parts = min(unit.of_group, g.most_units - unit.index);
+        const int32_t sharing = parts >= 4 * JOIN_WAVES ? JOIN_WAVES : 1;
+        const size_t at_once = JOIN_WAVES / sharing * WAVE;
+        const Wide* from = reinterpret_cast<const Wide*>(g.partial) + unit.index * pieces;
+        T* const to = g.out + unit.group * size;
+        size_t first = turn * at_once;
+        for (; first < pieces; first += gridDim.x * at_once) {
+            const size_t i = first + (sharing > 1 ? lane : threadIdx.x);
+            Wide sum{};
+            if (i < pieces) {
 #pragma unroll 8
-            for (int32_t u = wave; u < parts; u += JOIN_WAVES) {
-                sum += from[u * size + i];
+                for (int32_t u = sharing > 1 ? wave : 0; u < parts; u += sharing) {
+                    sum += from[u * pieces + i];
+                }
+            }
+            if (sharing > 1) { // (uniform)
+                __syncthreads();
+                shared[wave][lane] = sum;
+                __syncthreads();
+                if (wave == 0) {
+#pragma unroll
+                    for (int w = 1; w < JOIN_WAVES; w++) {
+                        sum += shared[w][lane];
+                    }
+                }
+            }
+            if (i < pieces && (sharing == 1 || wave == 0)) {
+                Narrow narrow;
+#pragma unroll
+                for (int j = 0; j < JOINED; j++) {
+                    narrow[j] = static_cast<T>(sum[j]);
+                }
+                if ((i + 1) * JOINED <= size) {
+                    *reinterpret_cast<Narrow*>(to + i * JOINED) = narrow;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < JOINED; j++) {
+                        if (i * JOINED + j < size) {
+                            to[i * JOINED + j] = narrow[j];
+                        }
+                    }
+                }
             }
         }
-        shared[wave][lane] = sum;
-        __syncthreads();
-        if (wave == 0 && i < size) {
-            Narrow narrow;
-#pragma unroll
-            for (int w = 1; w < JOIN_WAVES; w++) {
-                sum += shared[w][lane];
-            }
-#pragma unroll
-            for (int j = 0; j < JOINED; j++) {
-                narrow[j] = static_cast<T>(sum[j]);
-            }
-            *reinterpret_cast<Narrow*>(g.out + (unit.group * size + i) * JOINED) = narrow;
-        }
-        __syncthreads();
-    }
+        turn = static_cast<int32_t>((first - pieces) / at_once % gridDim.x);
+    });
 }
 
 } // namespace mops::amd::grouped_product
