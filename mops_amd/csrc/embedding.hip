@@ -22,6 +22,7 @@
 #include "numbers.hpp"
 #include "runtime.hpp"
 #include "sender_buckets.hpp"
+#include "wave_sort.hpp"
 
 namespace mops::amd {
 namespace embedding {
@@ -29,10 +30,12 @@ namespace {
 
 constexpr int THREADS = 256;
 constexpr int AHEAD = 8;            // rows that a team has on their way
-constexpr int32_t PLACES_EACH = 32; // of a chunk, per team
+constexpr int32_t PLACES_EACH = 32; // of a chunk, per team, at most
+constexpr int32_t CHUNKS = 1024;    // that there should be, and at least CHUNK_PLACES places in each
+constexpr int32_t CHUNK_PLACES = 64;
 constexpr int32_t ALONE = 64;       // places that a team sums up by itself
 constexpr int32_t FEW = 16;         // rows per table row from which on a workgroup has one table row
-constexpr int32_t ROWS_PER_TEAM = 4;
+constexpr int32_t ROWS_PER_TEAM = 4; // at most
 
 /// How a row's pieces are shared out: `team` lanes (a power of two) hold a piece each.
 struct Teams {
@@ -40,11 +43,11 @@ struct Teams {
     int32_t team, teams; // lanes per team, teams per workgroup
     unsigned tiles;      // workgroups beside each other that hold a row
 
-    template <int N> static Teams make(int32_t columns) {
+    template <int N> static Teams make(int32_t columns, int32_t most_lanes = THREADS) {
         Teams t;
         t.row = PiecesOfRow::make<N>(columns);
         t.team = 1;
-        while (t.team < THREADS && t.team < t.row.pieces) {
+        while (t.team < most_lanes && t.team < t.row.pieces) {
             t.team *= 2;
         }
         t.teams = THREADS / t.team;
@@ -89,38 +92,56 @@ __global__ __launch_bounds__(THREADS) void lookup_kernel(
     }
 }
 
-/// sum[j] += rows order[begin], order[begin + step], ... before `end`, at `column`. A team's lanes read the order side by
-/// side and hand it round, so that a row waits for its place once per `team` rows, not each time.
+/// sum[j] += rows row[0], row[1], .. (outside [0, n_rows): none) at `column`.
+template <typename T, int N>
+__device__ __forceinline__ void add_batch(
+    wide_t<T> (&sum)[N], const T* __restrict__ rows, const int32_t (&row)[AHEAD], int32_t n_rows, size_t columns,
+    int32_t column
+) {
+    Piece<T, N> value[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; u++) {
+        value[u] = Piece<T, N>::load(rows + (in_bounds(row[u], n_rows) ? row[u] : 0) * columns + column);
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; u++) {
+        if (in_bounds(row[u], n_rows)) {
+#pragma unroll
+            for (int j = 0; j < N; j++) {
+                sum[j] += value[u].get(j);
+            }
+        }
+    }
+}
+
+/// sum[j] += rows order[begin], order[begin + step], ... before `end`, at `column`. The lanes of a team read the order
+/// side by side and hand it round, so that a row waits for its place once per `team` rows, not each time.
 template <typename T, int N>
 __device__ __forceinline__ void add_rows(
     wide_t<T> (&sum)[N], const T* __restrict__ rows, const int32_t* __restrict__ order, int32_t n_rows, int32_t begin,
     int32_t end, int32_t step, size_t columns, int32_t column, int32_t team
 ) {
+    int32_t row[AHEAD];
+    if (team < AHEAD) {
+        for (int32_t p = begin; p < end; p += AHEAD * step) {
+#pragma unroll
+            for (int u = 0; u < AHEAD; u++) {
+                row[u] = p + u * step < end ? order[p + u * step] : -1;
+            }
+            add_batch<T, N>(sum, rows, row, n_rows, columns, column);
+        }
+        return;
+    }
     const int32_t width = min(team, WAVE), lane = threadIdx.x & (width - 1);
     for (int32_t p = begin; p < end; p += width * step) {
         const int32_t left = min((end - p + step - 1) / step, width); // rows of this round
         const int32_t mine = lane < left ? order[p + lane * step] : -1;
         for (int32_t first = 0; first < left; first += AHEAD) {
-            int32_t row[AHEAD];
-            Piece<T, N> value[AHEAD];
 #pragma unroll
             for (int u = 0; u < AHEAD; u++) {
-                row[u] = __shfl(mine, min(first + u, width - 1), width);
-                row[u] = first + u < left && in_bounds(row[u], n_rows) ? row[u] : -1;
+                row[u] = __shfl(mine, first + u, width); // (lanes behind the last place have none; AHEAD divides width)
             }
-#pragma unroll
-            for (int u = 0; u < AHEAD; u++) {
-                value[u] = Piece<T, N>::load(rows + max(row[u], 0) * columns + column);
-            }
-#pragma unroll
-            for (int u = 0; u < AHEAD; u++) {
-                if (row[u] >= 0) {
-#pragma unroll
-                    for (int j = 0; j < N; j++) {
-                        sum[j] += value[u].get(j);
-                    }
-                }
-            }
+            add_batch<T, N>(sum, rows, row, n_rows, columns, column);
         }
     }
 }
@@ -178,20 +199,18 @@ __global__ __launch_bounds__(THREADS) void chunk_kernel(
     }
 }
 
-/// grad_table[v, :] for `each` rows of the table per team: a team per row where few rows name it, the workgroup
-/// together where many do.
+/// Rows row0 .. row_end - 1 of the gradient, by a workgroup: a team per row of the table where few rows name it (at most
+/// `alone`), all teams together where many do. places[v - row0]: the first place of row v in `order`, which has n_places.
 template <typename T, int N>
-__global__ __launch_bounds__(THREADS) void gradient_kernel(
-    T* __restrict__ grad_table, const T* __restrict__ grad_output, const wide_t<T>* __restrict__ partial,
-    const int32_t* __restrict__ order, const int32_t* __restrict__ offsets, int32_t n_rows, int32_t table_rows,
-    Teams teams, int32_t chunk, int32_t each, int32_t alone, wide_t<T> scale
+__device__ __forceinline__ void sum_table_rows(
+    wide_t<T>* joined, T* __restrict__ grad_table, const T* __restrict__ grad_output, const wide_t<T>* __restrict__ partial,
+    const int32_t* order, const int32_t* places, int32_t n_places, int32_t n_rows, int32_t row0, int32_t row_end,
+    const Teams& teams, int32_t chunk, int32_t alone, wide_t<T> scale
 ) {
-    __shared__ wide_t<T> joined[N * THREADS];
     const int32_t piece = blockIdx.y * teams.team + (threadIdx.x & (teams.team - 1));
     const bool holds = piece < teams.row.pieces;
     const int32_t column = teams.row.start<N>(min(piece, teams.row.pieces - 1));
     const int32_t mine = threadIdx.x / teams.team;
-    const int32_t row0 = blockIdx.x * each, row_end = min(row0 + each, table_rows);
     auto store = [&](int32_t row, const wide_t<T>(&sum)[N]) {
         Piece<T, N> value;
 #pragma unroll
@@ -202,7 +221,7 @@ __global__ __launch_bounds__(THREADS) void gradient_kernel(
     };
     bool many = false;
     for (int32_t row = row0 + mine; row < row_end; row += teams.teams) {
-        const int32_t begin = max(offsets[row], 0), end = min(offsets[row + 1], n_rows);
+        const int32_t begin = max(places[row - row0], 0), end = min(places[row - row0 + 1], n_places);
         if (end - begin > alone) {
             many = true;
         } else {
@@ -217,7 +236,7 @@ __global__ __launch_bounds__(THREADS) void gradient_kernel(
         return;
     }
     for (int32_t row = row0; row < row_end; row++) {
-        const int32_t begin = max(offsets[row], 0), end = min(offsets[row + 1], n_rows);
+        const int32_t begin = max(places[row - row0], 0), end = min(places[row - row0 + 1], n_places);
         if (end - begin <= alone) { // (uniform)
             continue;
         }
@@ -261,6 +280,61 @@ __global__ __launch_bounds__(THREADS) void gradient_kernel(
     }
 }
 
+template <typename T, int N>
+__global__ __launch_bounds__(THREADS) void gradient_kernel(
+    T* __restrict__ grad_table, const T* __restrict__ grad_output, const wide_t<T>* __restrict__ partial,
+    const int32_t* __restrict__ order, const int32_t* __restrict__ offsets, int32_t n_rows, int32_t table_rows,
+    Teams teams, int32_t chunk, int32_t each, int32_t alone, wide_t<T> scale
+) {
+    __shared__ wide_t<T> joined[N * THREADS];
+    const int32_t row0 = blockIdx.x * each, row_end = min(row0 + each, table_rows);
+    sum_table_rows<T, N>(
+        joined, grad_table, grad_output, partial, order, offsets + row0, n_rows, n_rows, row0, row_end, teams, chunk,
+        alone, scale
+    );
+}
+
+/// The same for at most THREADS rows, without an order in memory: every workgroup looks at all indices and puts the rows
+/// that name its part of the table in order in LDS. One launch instead of three or four (10 rows, 5 table rows: 9.9 us
+/// with the sort).
+constexpr int32_t FEW_TABLE_ROWS = 1024; // of a workgroup, at most
+template <typename T, int N>
+__global__ __launch_bounds__(THREADS) void few_rows_kernel(
+    T* __restrict__ grad_table, const T* __restrict__ grad_output, const int32_t* __restrict__ indices, int32_t n_rows,
+    int32_t table_rows, Teams teams, int32_t each, int32_t alone, wide_t<T> scale
+) {
+    constexpr int WAVES = THREADS / WAVE;
+    __shared__ wide_t<T> joined[N * THREADS];
+    __shared__ int32_t places[FEW_TABLE_ROWS + 1], key[THREADS], order[THREADS], of_wave[WAVES];
+    const int32_t row0 = blockIdx.x * each, row_end = min(row0 + each, table_rows), tid = threadIdx.x;
+    for (int32_t i = tid; i <= each; i += THREADS) {
+        places[i] = 0;
+    }
+    const int32_t index = tid < n_rows ? indices[tid] : -1;
+    const bool here = index >= row0 && index < row_end;
+    key[tid] = here ? index - row0 : -1;
+    __syncthreads();
+    if (here) {
+        atomicAdd(&places[index - row0], 1);
+    }
+    __syncthreads();
+    const int32_t listed = scan_in_place<WAVES>(places, each, 0, of_wave);
+    if (tid == 0) {
+        places[each] = listed;
+    }
+    if (here) { // (among the rows of the same index, in ascending order)
+        int32_t place = places[index - row0];
+        for (int32_t earlier = 0; earlier < tid; earlier++) {
+            place += key[earlier] == index - row0 ? 1 : 0;
+        }
+        order[place] = tid;
+    }
+    __syncthreads();
+    sum_table_rows<T, N>(
+        joined, grad_table, grad_output, nullptr, order, places, listed, n_rows, row0, row_end, teams, 1, alone, scale
+    );
+}
+
 /// body(number of columns in a piece): 16 bytes, or single numbers for rows shorter than that.
 template <typename T, typename Body> void by_width(int32_t columns, Body&& body) {
     if (columns >= PIECE<T>) {
@@ -300,9 +374,37 @@ void gradient(
 ) {
     by_width<T>(columns, [&](auto width) {
         constexpr int N = decltype(width)::value;
+        const size_t units = static_cast<size_t>(compute_units());
+        // Rows of the table per workgroup: one where many rows name each on average (200 000 rows, 94 table rows, 128
+        // floats: 73 us for the whole gradient with one row per team), else some per team if there are enough of them,
+        // for workgroups that have nothing but zeros to store come and go faster than they are started.
+        const bool many = static_cast<size_t>(n_rows) > static_cast<size_t>(table_rows) * FEW;
+        const int32_t alone = many ? 0 : ALONE;
         const Teams teams = Teams::make<N>(columns);
-        const int32_t chunk = PLACES_EACH * teams.teams;
-        const int32_t chunks = n_rows / chunk;
+        auto rows_each = [&](const Teams& t) {
+            const size_t by_team = static_cast<size_t>(table_rows) * t.tiles / t.teams;
+            return static_cast<size_t>(many ? 1 : t.teams) *
+                   std::min<size_t>(ROWS_PER_TEAM, many ? 1 : std::max<size_t>(by_team / (8 * units), 1));
+        };
+        // few workgroups: fewer columns in each of more
+        Teams summing = teams;
+        while (many && summing.team > 8 && static_cast<size_t>(table_rows) * summing.tiles < units) {
+            summing = Teams::make<N>(columns, summing.team / 2);
+        }
+        const size_t each = rows_each(summing);
+        const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<size_t>(table_rows), each)), summing.tiles);
+        if (n_rows <= THREADS) { // (also where the caller has a plan: reading it would take longer)
+            few_rows_kernel<T, N><<<grid, THREADS, 0, stream>>>(
+                grad_table, grad_output, indices, n_rows, table_rows, summing, static_cast<int32_t>(each), alone,
+                static_cast<wide_t<T>>(scale)
+            );
+            return;
+        }
+        const int32_t chunk = std::min<int32_t>(
+            PLACES_EACH * teams.teams,
+            static_cast<int32_t>(ceil_div(static_cast<size_t>(n_rows), CHUNKS * CHUNK_PLACES)) * CHUNK_PLACES
+        );
+        const int32_t chunks = n_rows / std::max(chunk, 1);
         const size_t partial_bytes =
             n_rows > ALONE ? align256(static_cast<size_t>(chunks) * columns * sizeof(wide_t<T>)) : 0;
         const size_t order_bytes = order == nullptr ? align256(static_cast<size_t>(n_rows) * 4) : 0;
@@ -328,16 +430,9 @@ void gradient(
                 partial, grad_output, indices, order, n_rows, table_rows, teams, chunk
             );
         }
-        // Rows of the table per workgroup: one where many rows name each on average (200 000 rows, 94 table rows, 128
-        // floats: 73 us for the whole gradient with one row per team, 4 x as long as this kernel needs otherwise), else
-        // some per team, for workgroups that have nothing but zeros to store come and go faster than they are started.
-        const bool many = static_cast<size_t>(n_rows) > static_cast<size_t>(table_rows) * FEW;
-        const size_t rows_each = many ? 1 : static_cast<size_t>(teams.teams) * ROWS_PER_TEAM;
-        const int32_t alone = many ? 0 : ALONE;
-        const size_t blocks = ceil_div(static_cast<size_t>(table_rows), rows_each);
-        gradient_kernel<T, N><<<dim3(static_cast<unsigned>(blocks), teams.tiles), THREADS, 0, stream>>>(
-            grad_table, grad_output, partial, order, offsets, n_rows, table_rows, teams, chunk,
-            static_cast<int32_t>(rows_each), alone, static_cast<wide_t<T>>(scale)
+        gradient_kernel<T, N><<<grid, THREADS, 0, stream>>>(
+            grad_table, grad_output, partial, order, offsets, n_rows, table_rows, summing, chunk,
+            static_cast<int32_t>(each), alone, static_cast<wide_t<T>>(scale)
         );
     });
     MOPS_HIP_CHECK(hipGetLastError());
