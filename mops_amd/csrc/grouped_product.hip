@@ -28,84 +28,120 @@ unsigned tiles(int32_t size, int tile) { return static_cast<unsigned>(ceil_div(s
 template <typename T> bool aligned(const T* data, int32_t width) {
     return reinterpret_cast<uintptr_t>(data) % 16 == 0 && static_cast<size_t>(width) * sizeof(T) % 16 == 0;
 }
-template <typename T, Form FORM> int32_t q_width(const Product<T>& g) {
-    return FORM == Form::GRAD_SUMS ? g.m_size : g.k_size;
-}
-template <typename T, Form FORM> int32_t p_width(const Product<T>& g) {
-    return FORM == Form::GRAD_ROWS ? g.k_size : g.n_size;
+template <typename T, Form FORM> bool aligned(const Product<T>& g) {
+    return aligned(g.q, FORM == Form::GRAD_SUMS ? g.m_size : g.k_size) &&
+           aligned(g.p, FORM == Form::GRAD_ROWS ? g.k_size : g.n_size);
 }
 
-template <typename T, Form FORM, int BM, int BN, int WM, int WN, int DEEP = 8, int STAGES = 2> void launch(Product<T> g, hipStream_t stream) {
-    constexpr bool SUMS = FORM == Form::GRAD_SUMS;
-    g.m_tiles = SUMS ? static_cast<int32_t>(tiles(g.m_size, BM)) : 1;
-    g.n_tiles = static_cast<int32_t>(tiles(g.n_size, BN));
-    if (!SUMS) {
-        g.step = BM;
+/// The extents of a call's tiles: TILE x TILE numbers.
+template <Form FORM, typename T> unsigned set_tiles(Product<T>& g, int tile) {
+    g.m_tiles = FORM == Form::GRAD_SUMS ? static_cast<int32_t>(tiles(g.m_size, tile)) : 1;
+    g.n_tiles = static_cast<int32_t>(tiles(g.n_size, tile));
+    if (FORM != Form::GRAD_SUMS) {
+        g.step = tile;
     }
     g.most_units = narrow_i32(most_units(g.groups.n_rows, g.groups.n_groups, g.step), "number of units of rows");
     const size_t workgroups = ceil_div(static_cast<size_t>(g.most_units) * g.m_tiles * g.n_tiles, 8) * 8;
-    const unsigned blocks = static_cast<unsigned>(narrow_i32(workgroups, "number of tiles"));
-    if (BM == 256 || (aligned(g.q, q_width<T, FORM>(g)) && aligned(g.p, p_width<T, FORM>(g)))) {
-        tiles_kernel<T, FORM, BM, BN, WM, WN, DEEP, STAGES, true><<<blocks, WM * WN * WAVE, 0, stream>>>(g);
-    } else if constexpr (BM < 256) {
-        tiles_kernel<T, FORM, BM, BN, WM, WN, 8, 2, false><<<blocks, WM * WN * WAVE, 0, stream>>>(g);
-    }
+    return static_cast<unsigned>(narrow_i32(workgroups, "number of tiles"));
 }
 
-template <typename T, Form FORM> void rows_times(const Product<T>& g, hipStream_t stream) {
-    const size_t rows = static_cast<size_t>(g.groups.n_rows);
-    const size_t big = ceil_div(rows, 256) * tiles(g.n_size, 256), middle = ceil_div(rows, 128) * tiles(g.n_size, 128);
+/// body(tile, wavefronts of its rows, of its columns, rows aligned): the kernels there are. Tiles of 256 are for 16-bit
+/// types with aligned rows (through registers they leave none for the pieces that are on their way).
+template <typename T, typename Body> void with_tile(int tile, bool in_place, Body&& body) {
+    std::integral_constant<int, 2> two;
+    std::integral_constant<int, 4> four;
+    if (tile == 256) {
+        if constexpr (sizeof(T) == 2) {
+            body(std::integral_constant<int, 256>{}, two, four, std::true_type{});
+        }
+    } else if (tile == 128) {
+        in_place ? body(std::integral_constant<int, 128>{}, two, two, std::true_type{})
+                 : body(std::integral_constant<int, 128>{}, two, two, std::false_type{});
+    } else {
+        in_place ? body(std::integral_constant<int, 64>{}, two, two, std::true_type{})
+                 : body(std::integral_constant<int, 64>{}, two, two, std::false_type{});
+    }
+}
+constexpr int DEEP = 8, STAGES = 2;
+
+template <typename T, Form FORM> void launch(Product<T> g, int tile, hipStream_t stream) {
+    const unsigned workgroups = set_tiles<FORM>(g, tile);
+    with_tile<T>(tile, aligned<T, FORM>(g), [&](auto size, auto m, auto n, auto in_place) {
+        constexpr int TILE = decltype(size)::value, WM = decltype(m)::value, WN = decltype(n)::value;
+        constexpr bool ALIGNED = decltype(in_place)::value;
+        tiles_kernel<T, FORM, TILE, TILE, WM, WN, DEEP, STAGES, ALIGNED><<<workgroups, WM * WN * WAVE, 0, stream>>>(g);
+    });
+    MOPS_HIP_CHECK(hipGetLastError());
+}
+
+/// The tiles of FORWARD and GRAD_ROWS: the largest that keep all compute units busy and, on average, are half full.
+template <typename T, Form FORM> int tile_of_rows(const Product<T>& g) {
+    const size_t rows = static_cast<size_t>(g.groups.n_rows), groups = static_cast<size_t>(g.groups.n_groups);
     const size_t units = static_cast<size_t>(compute_units());
-    // (through registers the tiles of 256 leave none for the pieces that are on their way)
-    const bool in_place = aligned(g.q, q_width<T, FORM>(g)) && aligned(g.p, p_width<T, FORM>(g));
-    if (sizeof(T) == 2 && in_place && big >= units && rows >= 128 * static_cast<size_t>(g.groups.n_groups)) {
-        if constexpr (sizeof(T) == 2) {
-            launch<T, FORM, 256, 256, 2, 4, 8, 2>(g, stream);
-        }
-    } else if (middle >= units && rows >= 64 * static_cast<size_t>(g.groups.n_groups)) {
-        launch<T, FORM, 128, 128, 2, 2>(g, stream);
-    } else {
-        launch<T, FORM, 64, 64, 2, 2>(g, stream);
-    }
-    MOPS_HIP_CHECK(hipGetLastError());
+    auto fits = [&](int tile) {
+        return ceil_div(rows, tile) * tiles(g.n_size, tile) >= units && rows >= tile / 2 * groups;
+    };
+    return sizeof(T) == 2 && aligned<T, FORM>(g) && fits(256) ? 256 : fits(128) ? 128 : 64;
 }
 
-template <typename T> void sum_of_rows(Product<T> g, hipStream_t stream) {
-    const size_t units = static_cast<size_t>(compute_units()), groups = static_cast<size_t>(g.groups.n_groups);
-    const size_t rows = static_cast<size_t>(std::max(g.groups.n_rows, 1));
-    const size_t big = static_cast<size_t>(tiles(g.m_size, 256)) * tiles(g.n_size, 256);
-    const size_t middle = static_cast<size_t>(tiles(g.m_size, 128)) * tiles(g.n_size, 128);
-    // (big tiles: one workgroup per compute unit, in groups that can be split if there are too few of them)
-    const bool use_big = sizeof(T) == 2 && aligned(g.q, g.m_size) && aligned(g.p, g.n_size) && g.m_size >= 256 && g.n_size >= 256 &&
-                         big * std::max(groups, ceil_div(rows, 2048)) >= units;
-    const bool use_middle = g.m_size > 64 && g.n_size > 64;
-    const size_t tiles_of_unit =
-        use_big ? big : use_middle ? middle : static_cast<size_t>(tiles(g.m_size, 64)) * tiles(g.n_size, 64);
-    // Rows per unit: what every workgroup that the GPU has room for would have if the work were shared out evenly. Larger
-    // groups than that are split, smaller ones are not.
-    const size_t room = (use_big ? 1 : 2) * units;
-    size_t step = std::max<size_t>(ceil_div(rows * tiles_of_unit, room), 256);
-    step = std::min(ceil_div(step, 64) * 64, ceil_div(rows, 64) * 64);
-    g.step = static_cast<int32_t>(step);
-    const bool splits = step < rows;
-    const size_t most = most_units(g.groups.n_rows, g.groups.n_groups, g.step);
+/// The tiles of GRAD_SUMS, and its rows per unit: what every workgroup that the GPU has room for would have if the work
+/// were shared out evenly. Larger groups than that are split, smaller ones are not.
+template <typename T> int tile_of_sums(Product<T>& g) {
+    const size_t rows = static_cast<size_t>(std::max(g.groups.n_rows, 1)), groups = static_cast<size_t>(g.groups.n_groups);
+    const size_t units = static_cast<size_t>(compute_units());
+    auto of_unit = [&](int tile) { return static_cast<size_t>(tiles(g.m_size, tile)) * tiles(g.n_size, tile); };
+    auto fits = [&](int tile) {
+        return g.m_size > tile / 2 && g.n_size > tile / 2 &&
+               of_unit(tile) * std::max(groups, ceil_div(rows, 8 * tile)) >= units;
+    };
+    const int tile = sizeof(T) == 2 && aligned<T, Form::GRAD_SUMS>(g) && fits(256) ? 256 : fits(128) ? 128 : 64;
+    const size_t room = (tile == 256 ? 1 : 2) * units;
+    const size_t step = std::max<size_t>(ceil_div(rows * of_unit(tile), room), 256);
+    g.step = static_cast<int32_t>(std::min(ceil_div(step, 64) * 64, ceil_div(rows, 64) * 64));
+    return tile;
+}
+
+template <typename T> void forward(const Product<T>& g, hipStream_t stream) {
+    launch<T, Form::FORWARD>(g, tile_of_rows<T, Form::FORWARD>(g), stream);
+}
+
+/// Either may be without an `out`: not wanted.
+template <typename T> void gradients(Product<T> sums, Product<T> rows, hipStream_t stream) {
+    const int of_sums = sums.out != nullptr ? tile_of_sums(sums) : 0;
+    const int of_rows = rows.out != nullptr ? tile_of_rows<T, Form::GRAD_ROWS>(rows) : 0;
+    const bool splits = of_sums != 0 && sums.step < sums.groups.n_rows;
     if (splits) {
-        g.partial = static_cast<wide_t<T>*>(scratch(most * partial_size(g.m_size, g.n_size) * sizeof(wide_t<T>)));
+        const size_t most = most_units(sums.groups.n_rows, sums.groups.n_groups, sums.step);
+        sums.partial =
+            static_cast<wide_t<T>*>(scratch(most * partial_size(sums.m_size, sums.n_size) * sizeof(wide_t<T>)));
     }
-    if (use_big) {
-        if constexpr (sizeof(T) == 2) {
-            launch<T, Form::GRAD_SUMS, 256, 256, 2, 4, 8, 2>(g, stream);
-        }
-    } else if (use_middle) {
-        launch<T, Form::GRAD_SUMS, 128, 128, 2, 2>(g, stream);
+    const bool in_place = of_sums != 0 && aligned<T, Form::GRAD_SUMS>(sums);
+    if (of_sums == of_rows && in_place == aligned<T, Form::GRAD_ROWS>(rows)) {
+        const unsigned for_sums = set_tiles<Form::GRAD_SUMS>(sums, of_sums);
+        const unsigned for_rows = set_tiles<Form::GRAD_ROWS>(rows, of_rows);
+        with_tile<T>(of_sums, in_place, [&](auto size, auto m, auto n, auto is_aligned) {
+            constexpr int TILE = decltype(size)::value, WM = decltype(m)::value, WN = decltype(n)::value;
+            constexpr bool ALIGNED = decltype(is_aligned)::value;
+            gradients_kernel<T, TILE, TILE, WM, WN, DEEP, STAGES, ALIGNED>
+                <<<for_sums + for_rows, WM * WN * WAVE, 0, stream>>>(sums, rows, for_sums);
+        });
+        MOPS_HIP_CHECK(hipGetLastError());
     } else {
-        launch<T, Form::GRAD_SUMS, 64, 64, 2, 2>(g, stream);
+        if (of_sums != 0) {
+            launch<T, Form::GRAD_SUMS>(sums, of_sums, stream);
+        }
+        if (of_rows != 0) {
+            launch<T, Form::GRAD_ROWS>(rows, of_rows, stream);
+        }
     }
     if (splits) {
-        g.most_units = narrow_i32(most, "number of units of rows");
-        join_units_kernel<T><<<static_cast<unsigned>(4 * units), JOIN_WAVES * WAVE, 0, stream>>>(g);
+        sums.most_units = narrow_i32(
+            most_units(sums.groups.n_rows, sums.groups.n_groups, sums.step), "number of units of rows"
+        );
+        const unsigned workgroups = 4 * static_cast<unsigned>(compute_units());
+        join_units_kernel<T><<<workgroups, JOIN_WAVES * WAVE, 0, stream>>>(sums);
+        MOPS_HIP_CHECK(hipGetLastError());
     }
-    MOPS_HIP_CHECK(hipGetLastError());
 }
 
 } // namespace
@@ -160,7 +196,7 @@ void grouped_matrix_product(
         g.groups = groups;
         g.n_size = L;
         g.k_size = K;
-        grouped_product::rows_times<T, grouped_product::Form::FORWARD>(g, current_stream());
+        grouped_product::forward(g, current_stream());
     }
     finish_call("grouped_matrix_product");
 }
@@ -186,25 +222,25 @@ void grouped_matrix_product_vjp(
     }
     const int32_t K = count_i32(W.shape[1], "W.shape[1]"), L = count_i32(W.shape[2], "W.shape[2]");
     typedef device_t<scalar_t> T;
-    if (grad_A.data != nullptr && groups.n_rows > 0 && K > 0) {
-        grouped_product::Product<T> g{};
-        g.out = data_of(grad_A);
-        g.q = data_of(grad_output);
-        g.p = data_of(W);
-        g.groups = groups;
-        g.n_size = K;
-        g.k_size = L;
-        grouped_product::rows_times<T, grouped_product::Form::GRAD_ROWS>(g, current_stream());
-    }
+    grouped_product::Product<T> sums{}, rows{};
     if (grad_W.data != nullptr && groups.n_groups > 0 && K > 0 && L > 0) {
-        grouped_product::Product<T> g{};
-        g.out = data_of(grad_W);
-        g.q = data_of(A);
-        g.p = data_of(grad_output);
-        g.groups = groups;
-        g.m_size = K;
-        g.n_size = L;
-        grouped_product::sum_of_rows(g, current_stream());
+        sums.out = data_of(grad_W);
+        sums.q = data_of(A);
+        sums.p = data_of(grad_output);
+        sums.groups = groups;
+        sums.m_size = K;
+        sums.n_size = L;
+    }
+    if (grad_A.data != nullptr && groups.n_rows > 0 && K > 0) {
+        rows.out = data_of(grad_A);
+        rows.q = data_of(grad_output);
+        rows.p = data_of(W);
+        rows.groups = groups;
+        rows.n_size = K;
+        rows.k_size = L;
+    }
+    if (sums.out != nullptr || rows.out != nullptr) {
+        grouped_product::gradients(sums, rows, current_stream());
     }
     finish_call("grouped_matrix_product_vjp");
 }

@@ -347,8 +347,14 @@ template <int LATER> __device__ __forceinline__ void meet() {
 
 /// WM x WN wavefronts; every one of them makes BM / WM x BN / WN numbers, in steps of DEEP pieces of k of which STAGES
 /// are in LDS or on their way there.
+template <int BM, int BN, int DEEP, int STAGES> struct TileLds {
+    char stages[STAGES * (BM + BN) * DEEP * 16] __attribute__((aligned(16)));
+    int32_t rows[BM];
+};
 template <typename T, Form FORM, int BM, int BN, int WM, int WN, int DEEP, int STAGES, bool ALIGNED>
-__global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
+__device__ __forceinline__ void make_tile(
+    const Product<T>& g, const uint32_t block, TileLds<BM, BN, DEEP, STAGES>& lds
+) {
     typedef Matrix<T> M;
     constexpr int THREADS = WM * WN * WAVE, COUNT = M::COUNT, BLOCK = M::BLOCK;
     constexpr int STEP = DEEP * COUNT, STEPS = DEEP * BLOCK / WAVE;
@@ -361,8 +367,8 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
         P_TURNED, TurnedLoader<T, BN, DEEP, THREADS, ALIGNED>, StraightLoader<T, BN, DEEP, THREADS, ALIGNED>>;
     constexpr int P_AT = BM * DEEP * 16, BYTES = P_AT + BN * DEEP * 16;
     static_assert(ALIGNED || STAGES == 2, "through registers: one step on its way, one in LDS beside the present one");
-    __shared__ __attribute__((aligned(16))) char stages[STAGES * BYTES];
-    __shared__ int32_t rows[SUMS ? 1 : BM];
+    char* const stages = lds.stages;
+    int32_t* const rows = lds.rows;
 
     // Workgroups b, b + 8, .. run on the same XCD. Tiles of rows take the same time each: an XCD gets consecutive ones, so
     // that its L2 holds what they share. A unit of GRAD_SUMS takes as long as it has rows: its tiles go to all XCDs (24
@@ -372,8 +378,8 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
     const int32_t units = min(of_groups.total(), g.most_units);
     const int64_t tiles = static_cast<int64_t>(units) * tiles_of_unit;
     const int32_t per_xcd = static_cast<int32_t>((tiles + 7) / 8);
-    const int64_t tile = SUMS ? blockIdx.x : static_cast<int64_t>(blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
-    if (static_cast<int32_t>(blockIdx.x / 8) >= per_xcd || tile >= tiles) {
+    const int64_t tile = SUMS ? block : static_cast<int64_t>(block % 8) * per_xcd + block / 8;
+    if (static_cast<int32_t>(block / 8) >= per_xcd || tile >= tiles) {
         return; // (uniform)
     }
     int32_t unit_index, m0, n0;
@@ -608,7 +614,7 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
         typedef decltype(zero) To;
         constexpr int COLUMNS = BN / WN, OF_PIECE = 16 / sizeof(To), RUN = M::RUN, PIECES = COLUMNS / OF_PIECE;
         constexpr int ROWS_ABREAST = PIECES >= 16 ? 1 : 16 / PIECES; // rows in 256 bytes, all banks
-        static_assert(BLOCK * COLUMNS * sizeof(To) * WM * WN <= sizeof(stages), "");
+        static_assert(BLOCK * COLUMNS * sizeof(To) * WM * WN <= sizeof(lds.stages), "");
         typedef To Run __attribute__((ext_vector_type(RUN)));
         typedef To Piece __attribute__((ext_vector_type(OF_PIECE), aligned(sizeof(To))));
         char* const mine = stages + wave * (BLOCK * COLUMNS * sizeof(To));
@@ -673,6 +679,24 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
         }
     } else {
         put(T(), [&](int m) { return m < unit.count ? g.out + static_cast<size_t>(rows[m]) * g.n_size : nullptr; });
+    }
+}
+
+template <typename T, Form FORM, int BM, int BN, int WM, int WN, int DEEP, int STAGES, bool ALIGNED>
+__global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
+    __shared__ TileLds<BM, BN, DEEP, STAGES> lds;
+    make_tile<T, FORM, BM, BN, WM, WN, DEEP, STAGES, ALIGNED>(g, blockIdx.x, lds);
+}
+
+/// Both gradients in one launch, the sums' tiles (of which there are `of_sums` workgroups, a multiple of 8) in front: they
+/// take longer, and the rows' tiles fill in behind them.
+template <typename T, int BM, int BN, int WM, int WN, int DEEP, int STAGES, bool ALIGNED>
+__global__ __launch_bounds__(WM* WN* WAVE) void gradients_kernel(Product<T> sums, Product<T> rows, uint32_t of_sums) {
+    __shared__ TileLds<BM, BN, DEEP, STAGES> lds;
+    if (blockIdx.x < of_sums) {
+        make_tile<T, Form::GRAD_SUMS, BM, BN, WM, WN, DEEP, STAGES, ALIGNED>(sums, blockIdx.x, lds);
+    } else {
+        make_tile<T, Form::GRAD_ROWS, BM, BN, WM, WN, DEEP, STAGES, ALIGNED>(rows, blockIdx.x - of_sums, lds);
     }
 }
 
