@@ -7,6 +7,7 @@ second derivatives; every call goes through the interpreter (and the backward pa
 """
 import torch
 
+from . import layers as _layers
 from . import ops as _ops
 
 
@@ -390,3 +391,93 @@ for _name, _backward, _setup in [
     torch.library.register_autograd(f"mops::{_name}", _backward, setup_context=_setup, lib=_library)
 
 
+
+
+# ------------------------------------------------------ layers' operators --
+_library.define("order_by_group(Tensor indices, int n_groups) -> (Tensor, Tensor)")
+_library.define("scaled_embedding(Tensor table, Tensor indices, float scale=1.) -> Tensor")
+_library.define("grouped_matrix_product(Tensor A, Tensor W, Tensor offsets, Tensor? order=None) -> Tensor")
+_library.define(
+    "gated_residual_norm(Tensor residual, Tensor block, Tensor gate, Tensor weight_block, Tensor weight_next, "
+    "float residual_scale=1., float epsilon=1e-06) -> (Tensor, Tensor)"
+)
+
+
+def _grouped(A, W, offsets, order=None):
+    return _layers.grouped_matrix_product(A, W, offsets, order)
+
+
+def _update(residual, block, gate, weight_block, weight_next, residual_scale=1.0, epsilon=1e-6):
+    return _layers.gated_residual_norm(residual, block, gate, weight_block, weight_next, residual_scale, epsilon)
+
+
+for _name, _kernel in [
+    ("order_by_group", _layers.order_by_group),
+    ("scaled_embedding", lambda table, indices, scale=1.0: _layers.scaled_embedding(table, indices, scale)),
+    ("grouped_matrix_product", _grouped),
+    ("gated_residual_norm", _update),
+]:
+    _library.impl(_name, _kernel, "CUDA")
+    _library.impl(_name, _refuse_host(_name), "CPU")
+
+_register_fake(
+    "order_by_group",
+    lambda indices, n_groups: (
+        indices.new_empty(indices.shape, dtype=torch.int32), indices.new_empty((n_groups + 1,), dtype=torch.int32),
+    ),
+)  # fmt: skip
+_register_fake(
+    "scaled_embedding", lambda table, indices, scale=1.0: table.new_empty((indices.shape[0], table.shape[1]))
+)
+_register_fake(
+    "grouped_matrix_product", lambda A, W, offsets, order=None: A.new_empty((A.shape[0], W.shape[2]))
+)
+_register_fake(
+    "gated_residual_norm",
+    lambda residual, block, gate, weight_block, weight_next, residual_scale=1.0, epsilon=1e-6: (
+        residual.new_empty(residual.shape), residual.new_empty(residual.shape),
+    ),
+)  # fmt: skip
+
+
+def _embedding_setup(ctx, inputs, output):
+    table, indices, ctx.scale = inputs
+    ctx.save_for_backward(table, indices)
+
+
+def _embedding_backward(ctx, grad_output):
+    table, indices = ctx.saved_tensors
+    return _layers.scaled_embedding_vjp(grad_output.contiguous(), table, indices, ctx.scale), None, None
+
+
+def _grouped_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs)
+
+
+def _grouped_backward(ctx, grad_output):
+    A, W, offsets, order = ctx.saved_tensors
+    wanted = {"compute_grad_A": ctx.needs_input_grad[0], "compute_grad_W": ctx.needs_input_grad[1]}
+    grads = _layers.grouped_matrix_product_vjp(grad_output.contiguous(), A, W, offsets, order, **wanted)
+    return (*grads, None, None)
+
+
+def _update_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs[:5])
+    ctx.residual_scale, ctx.epsilon = inputs[5:]
+    ctx.set_materialize_grads(False)
+
+
+def _update_backward(ctx, grad_state, grad_next):
+    names = ("residual", "block", "gate", "weight_block", "weight_next")
+    wanted = {"compute_grad_" + name: want for name, want in zip(names, ctx.needs_input_grad)}
+    cotangents = [None if grad is None else grad.contiguous() for grad in (grad_state, grad_next)]
+    grads = _layers.gated_residual_norm_vjp(*cotangents, *ctx.saved_tensors, ctx.residual_scale, ctx.epsilon, **wanted)
+    return (*grads, None, None)
+
+
+for _name, _backward, _setup in [
+    ("scaled_embedding", _embedding_backward, _embedding_setup),
+    ("grouped_matrix_product", _grouped_backward, _grouped_setup),
+    ("gated_residual_norm", _update_backward, _update_setup),
+]:
+    torch.library.register_autograd(f"mops::{_name}", _backward, setup_context=_setup, lib=_library)

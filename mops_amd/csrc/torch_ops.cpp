@@ -16,6 +16,9 @@
 // reference) the vjp is itself a Function whose backward is the library's
 // vjp_vjp. There is no gradient with respect to C or to index tensors.
 //
+// The operators of the layers (mops/layers.h) follow the same pattern, for 16-bit
+// types as well.
+//
 // mops_amd/torch.py loads this library when it has been built and registers
 // the same operators from Python otherwise.
 #include <array>
@@ -506,7 +509,233 @@ struct SasawFunction : public Function<SasawFunction> {
     }
 };
 
+// -------------------------------------------------- layers' operators --
+/// `like`: the tensor whose type and device all others have, by its name.
+at::Tensor layer_values(
+    const at::Tensor& tensor, const at::Tensor& like, const char* name, const char* like_name, const char* operation
+) {
+    require_device(tensor, name, operation);
+    if (!is_layer_dtype(tensor.scalar_type())) {
+        throw std::runtime_error(
+            std::string("mops::") + operation + ": " + name + " must be float32, float64, bfloat16 or float16"
+        );
+    }
+    if (tensor.scalar_type() != like.scalar_type() || tensor.device() != like.device()) {
+        throw std::runtime_error(
+            std::string("mops::") + operation + ": " + name + " must have the dtype and the device of " + like_name
+        );
+    }
+    return tensor.contiguous();
+}
+/// (undefined stays undefined: not given)
+at::Tensor layer_indices(const at::Tensor& tensor, const at::Tensor& like, const char* name, const char* operation) {
+    if (!tensor.defined()) {
+        return tensor;
+    }
+    require_device(tensor, name, operation);
+    if (tensor.device() != like.device() || !at::isIntegralType(tensor.scalar_type(), /*includeBool=*/false)) {
+        throw std::runtime_error(
+            std::string("mops::") + operation + ": " + name + " must hold integers, on the device of the other tensors"
+        );
+    }
+    return tensor.to(at::kInt).contiguous();
+}
+
+std::tuple<at::Tensor, at::Tensor> order_by_group(const at::Tensor& indices_, int64_t n_groups) {
+    const char* op = "order_by_group";
+    require_device(indices_, "indices", op);
+    const at::Tensor indices = layer_indices(indices_, indices_, "indices", op);
+    if (n_groups < 0) {
+        throw std::runtime_error("mops::order_by_group: n_groups must not be negative");
+    }
+    OnTorchStream stream(indices);
+    at::Tensor order = new_like(indices), offsets = new_tensor({n_groups + 1}, indices);
+    mops::cuda::order_by_group(
+        view<int32_t, 1>(order, "order"), view<int32_t, 1>(offsets, "offsets"), view<int32_t, 1>(indices, "indices")
+    );
+    return {order, offsets};
+}
+
+at::Tensor embedding_forward(const at::Tensor& table_, const at::Tensor& indices_, double scale) {
+    const char* op = "scaled_embedding";
+    const at::Tensor table = layer_values(table_, table_, "table", "table", op);
+    const at::Tensor indices = layer_indices(indices_, table_, "indices", op);
+    OnTorchStream stream(table);
+    at::Tensor output = new_tensor({indices.dim() == 1 ? indices.size(0) : 0, table.dim() == 2 ? table.size(1) : 0}, table);
+    by_layer_dtype(table, [&](auto zero) {
+        using T = decltype(zero);
+        mops::cuda::scaled_embedding<T>(
+            view<T, 2>(output, "output"), view<T, 2>(table, "table"), view<int32_t, 1>(indices, "indices"), scale
+        );
+    });
+    return output;
+}
+
+struct EmbeddingFunction : public Function<EmbeddingFunction> {
+    static at::Tensor forward(AutogradContext* ctx, at::Tensor table, at::Tensor indices, double scale) {
+        ctx->save_for_backward({table, indices});
+        ctx->saved_data["scale"] = scale;
+        return embedding_forward(table, indices, scale);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const char* op = "scaled_embedding_vjp";
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor& table = saved[0];
+        const at::Tensor indices = layer_indices(saved[1], table, "indices", op);
+        const at::Tensor grad_output = layer_values(grads[0], table, "grad_output", "table", op);
+        OnTorchStream stream(table);
+        at::Tensor grad_table = new_like(table);
+        by_layer_dtype(table, [&](auto zero) {
+            using T = decltype(zero);
+            mops::cuda::scaled_embedding_vjp<T>(
+                view<T, 2>(grad_table, "grad_table"), view<T, 2>(grad_output, "grad_output"),
+                view<int32_t, 1>(indices, "indices"), mops::Tensor<int32_t, 1>{nullptr, {0}},
+                mops::Tensor<int32_t, 1>{nullptr, {0}}, ctx->saved_data["scale"].toDouble()
+            );
+        });
+        return {grad_table, at::Tensor(), at::Tensor()};
+    }
+};
+
+at::Tensor grouped_forward(
+    const at::Tensor& A_, const at::Tensor& W_, const at::Tensor& offsets_, const at::Tensor& order_
+) {
+    const char* op = "grouped_matrix_product";
+    const at::Tensor A = layer_values(A_, A_, "A", "A", op), W = layer_values(W_, A_, "W", "A", op);
+    const at::Tensor offsets = layer_indices(offsets_, A_, "offsets", op), order = layer_indices(order_, A_, "order", op);
+    OnTorchStream stream(A);
+    at::Tensor output = new_tensor({A.dim() == 2 ? A.size(0) : 0, W.dim() == 3 ? W.size(2) : 0}, A);
+    by_layer_dtype(A, [&](auto zero) {
+        using T = decltype(zero);
+        mops::cuda::grouped_matrix_product<T>(
+            view<T, 2>(output, "output"), view<T, 2>(A, "A"), view<T, 3>(W, "W"), view<int32_t, 1>(offsets, "offsets"),
+            view<int32_t, 1>(order, "order")
+        );
+    });
+    return output;
+}
+
+struct GroupedFunction : public Function<GroupedFunction> {
+    static at::Tensor forward(AutogradContext* ctx, at::Tensor A, at::Tensor W, at::Tensor offsets, at::Tensor order) {
+        ctx->save_for_backward({A, W, offsets, order});
+        return grouped_forward(A, W, offsets, order);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const char* op = "grouped_matrix_product_vjp";
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor A = layer_values(saved[0], saved[0], "A", "A", op), W = layer_values(saved[1], saved[0], "W", "A", op);
+        const at::Tensor offsets = layer_indices(saved[2], A, "offsets", op), order = layer_indices(saved[3], A, "order", op);
+        const at::Tensor grad_output = layer_values(grads[0], A, "grad_output", "A", op);
+        OnTorchStream stream(A);
+        at::Tensor grad_A = ctx->needs_input_grad(0) ? new_like(A) : at::Tensor();
+        at::Tensor grad_W = ctx->needs_input_grad(1) ? new_like(W) : at::Tensor();
+        by_layer_dtype(A, [&](auto zero) {
+            using T = decltype(zero);
+            mops::cuda::grouped_matrix_product_vjp<T>(
+                view<T, 2>(grad_A, "grad_A"), view<T, 3>(grad_W, "grad_W"), view<T, 2>(grad_output, "grad_output"),
+                view<T, 2>(A, "A"), view<T, 3>(W, "W"), view<int32_t, 1>(offsets, "offsets"),
+                view<int32_t, 1>(order, "order")
+            );
+        });
+        return {grad_A, grad_W, at::Tensor(), at::Tensor()};
+    }
+};
+
+/// residual, block, gate, weight_block, weight_next
+std::array<at::Tensor, 5> update_inputs(const std::array<at::Tensor, 5>& tensors, const char* op) {
+    const char* names[5] = {"residual", "block", "gate", "weight_block", "weight_next"};
+    std::array<at::Tensor, 5> inputs;
+    for (size_t i = 0; i < 5; i++) {
+        inputs[i] = layer_values(tensors[i], tensors[0], names[i], names[0], op);
+    }
+    return inputs;
+}
+
+std::tuple<at::Tensor, at::Tensor> update_forward(
+    const std::array<at::Tensor, 5>& tensors, double residual_scale, double epsilon
+) {
+    const auto in = update_inputs(tensors, "gated_residual_norm");
+    OnTorchStream stream(in[0]);
+    at::Tensor state = new_like(in[0]), next = new_like(in[0]);
+    by_layer_dtype(in[0], [&](auto zero) {
+        using T = decltype(zero);
+        mops::cuda::gated_residual_norm<T>(
+            view<T, 2>(state, "state"), view<T, 2>(next, "next"), view<T, 2>(in[0], "residual"),
+            view<T, 2>(in[1], "block"), view<T, 2>(in[2], "gate"), view<T, 1>(in[3], "weight_block"),
+            view<T, 1>(in[4], "weight_next"), residual_scale, epsilon
+        );
+    });
+    return {state, next};
+}
+
+struct UpdateFunction : public Function<UpdateFunction> {
+    static variable_list forward(
+        AutogradContext* ctx, at::Tensor residual, at::Tensor block, at::Tensor gate, at::Tensor weight_block,
+        at::Tensor weight_next, double residual_scale, double epsilon
+    ) {
+        ctx->save_for_backward({residual, block, gate, weight_block, weight_next});
+        ctx->saved_data["residual_scale"] = residual_scale;
+        ctx->saved_data["epsilon"] = epsilon;
+        ctx->set_materialize_grads(false); // (a gradient that is not there is not read)
+        const auto [state, next] =
+            update_forward({residual, block, gate, weight_block, weight_next}, residual_scale, epsilon);
+        return {state, next};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const char* op = "gated_residual_norm_vjp";
+        const auto saved = ctx->get_saved_variables();
+        const auto in = update_inputs({saved[0], saved[1], saved[2], saved[3], saved[4]}, op);
+        std::array<at::Tensor, 2> cotangent;
+        for (size_t i = 0; i < 2; i++) {
+            cotangent[i] = grads[i].defined()
+                               ? layer_values(grads[i], in[0], i == 0 ? "grad_state" : "grad_next", "residual", op)
+                               : at::Tensor();
+        }
+        OnTorchStream stream(in[0]);
+        std::array<at::Tensor, 5> out;
+        for (size_t i = 0; i < 5; i++) {
+            out[i] = ctx->needs_input_grad(i) ? new_like(in[i]) : at::Tensor();
+        }
+        by_layer_dtype(in[0], [&](auto zero) {
+            using T = decltype(zero);
+            mops::cuda::gated_residual_norm_vjp<T>(
+                view<T, 2>(out[0], "grad_residual"), view<T, 2>(out[1], "grad_block"), view<T, 2>(out[2], "grad_gate"),
+                view<T, 1>(out[3], "grad_weight_block"), view<T, 1>(out[4], "grad_weight_next"),
+                view<T, 2>(cotangent[0], "grad_state"), view<T, 2>(cotangent[1], "grad_next"),
+                view<T, 2>(in[0], "residual"), view<T, 2>(in[1], "block"), view<T, 2>(in[2], "gate"),
+                view<T, 1>(in[3], "weight_block"), view<T, 1>(in[4], "weight_next"),
+                ctx->saved_data["residual_scale"].toDouble(), ctx->saved_data["epsilon"].toDouble()
+            );
+        });
+        return {out[0], out[1], out[2], out[3], out[4], at::Tensor(), at::Tensor()};
+    }
+};
+
 // ------------------------------------------------------------ operators --
+at::Tensor scaled_embedding(const at::Tensor& table, const at::Tensor& indices, double scale) {
+    return recorded({&table}) ? EmbeddingFunction::apply(table, indices, scale)
+                              : embedding_forward(table, indices, scale);
+}
+
+at::Tensor grouped_matrix_product(
+    const at::Tensor& A, const at::Tensor& W, const at::Tensor& offsets, const c10::optional<at::Tensor>& order
+) {
+    const at::Tensor rows = order.has_value() ? *order : at::Tensor();
+    return recorded({&A, &W}) ? GroupedFunction::apply(A, W, offsets, rows) : grouped_forward(A, W, offsets, rows);
+}
+
+std::tuple<at::Tensor, at::Tensor> gated_residual_norm(
+    const at::Tensor& residual, const at::Tensor& block, const at::Tensor& gate, const at::Tensor& weight_block,
+    const at::Tensor& weight_next, double residual_scale, double epsilon
+) {
+    if (!recorded({&residual, &block, &gate, &weight_block, &weight_next})) {
+        return update_forward({residual, block, gate, weight_block, weight_next}, residual_scale, epsilon);
+    }
+    const variable_list results =
+        UpdateFunction::apply(residual, block, gate, weight_block, weight_next, residual_scale, epsilon);
+    return {results[0], results[1]};
+}
+
 at::Tensor homogeneous_polynomial_evaluation(const at::Tensor& A, const at::Tensor& C, const at::Tensor& indices_A) {
     return recorded({&A, &C}) ? Hpe::apply(A, C, indices_A) : hpe_forward(A, C, indices_A);
 }
@@ -553,6 +782,17 @@ at::Tensor sparse_accumulation_scatter_add_with_weights(
 } // namespace
 
 TORCH_LIBRARY(mops, m) {
+    m.def("order_by_group(Tensor indices, int n_groups) -> (Tensor, Tensor)", order_by_group);
+    m.def("scaled_embedding(Tensor table, Tensor indices, float scale=1.) -> Tensor", scaled_embedding);
+    m.def(
+        "grouped_matrix_product(Tensor A, Tensor W, Tensor offsets, Tensor? order=None) -> Tensor",
+        grouped_matrix_product
+    );
+    m.def(
+        "gated_residual_norm(Tensor residual, Tensor block, Tensor gate, Tensor weight_block, Tensor weight_next, "
+        "float residual_scale=1., float epsilon=1e-06) -> (Tensor, Tensor)",
+        gated_residual_norm
+    );
     m.def(
         "homogeneous_polynomial_evaluation(Tensor A, Tensor C, Tensor indices_A) -> Tensor",
         homogeneous_polynomial_evaluation

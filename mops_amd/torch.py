@@ -21,6 +21,11 @@ library's ``*_vjp_vjp`` functions (the operations for which the reference
 has one, ``mops-torch/src/{hpe,sap,opsa}.cpp``); the two weighted operations
 have none, as in the reference.
 
+The operators of the layers around them (``mops_amd.layers``; not part of the
+reference) are registered beside them, with first derivatives, for ``bfloat16``
+and ``float16`` as well: ``order_by_group``, ``scaled_embedding``,
+``grouped_matrix_product``, ``gated_residual_norm``.
+
 Host tensors are refused: this library is the device path only.
 """
 import os
@@ -35,6 +40,10 @@ __all__ = [
     "outer_product_scatter_add",
     "outer_product_scatter_add_with_weights",
     "sparse_accumulation_scatter_add_with_weights",
+    "order_by_group",
+    "scaled_embedding",
+    "grouped_matrix_product",
+    "gated_residual_norm",
     "OPERATORS_FROM",
 ]
 
@@ -53,3 +62,7 @@ sparse_accumulation_of_products = torch.ops.mops.sparse_accumulation_of_products
 outer_product_scatter_add = torch.ops.mops.outer_product_scatter_add
 outer_product_scatter_add_with_weights = torch.ops.mops.outer_product_scatter_add_with_weights
 sparse_accumulation_scatter_add_with_weights = torch.ops.mops.sparse_accumulation_scatter_add_with_weights
+order_by_group = torch.ops.mops.order_by_group
+scaled_embedding = torch.ops.mops.scaled_embedding
+grouped_matrix_product = torch.ops.mops.grouped_matrix_product
+gated_residual_norm = torch.ops.mops.gated_residual_norm

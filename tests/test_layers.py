@@ -153,6 +153,16 @@ PRODUCTS = [
 ]  # fmt: skip
 
 
+# every extent of tiles with rows on 16-byte boundaries and off them, groups that are split into few and into many units,
+# more groups than a wavefront has lanes
+LARGE_PRODUCTS = [
+    (8300, 3, 72, 2056, "padded", True), (8300, 3, 2056, 72, "frequent", True), (5000, 20, 1040, 1032, "frequent", True),
+    (5000, 20, 1040, 1032, "uniform", False), (30000, 2, 64, 64, "frequent", False),
+    (6000, 130, 70, 90, "frequent", True), (9000, 200, 256, 256, "uniform", True),
+    (40000, 2, 130, 514, "padded", True), (4500, 3, 515, 777, "frequent", False), (70000, 3, 5, 3, "uniform", True),
+]  # fmt: skip
+
+
 def product_case(rows, groups, K, L, kind, dtype):
     generator = generator_of(rows, groups, K, L)
     A, W = random(generator, (rows, K), dtype), random(generator, (groups, K, L), dtype)
@@ -171,7 +181,7 @@ def product_plan(index, groups, ordered):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("tag", list(DTYPES))
-@pytest.mark.parametrize("rows,groups,K,L,kind,ordered", PRODUCTS)
+@pytest.mark.parametrize("rows,groups,K,L,kind,ordered", PRODUCTS + LARGE_PRODUCTS)
 def test_grouped_matrix_product(device, rows, groups, K, L, kind, ordered, tag):
     A, W, _, index = product_case(rows, groups, K, L, kind, DTYPES[tag])
     order, offsets, index = product_plan(index, groups, ordered)
@@ -190,7 +200,7 @@ def test_grouped_matrix_product(device, rows, groups, K, L, kind, ordered, tag):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("tag", list(DTYPES))
-@pytest.mark.parametrize("rows,groups,K,L,kind,ordered", PRODUCTS)
+@pytest.mark.parametrize("rows,groups,K,L,kind,ordered", PRODUCTS + LARGE_PRODUCTS)
 def test_grouped_matrix_product_vjp(device, rows, groups, K, L, kind, ordered, tag):
     A, W, grad_output, index = product_case(rows, groups, K, L, kind, DTYPES[tag])
     order, offsets, index = product_plan(index, groups, ordered)
@@ -341,6 +351,64 @@ def test_gated_residual_norm_vjp(device, rows, columns, gate_rows, tag):
         same = mops_amd.gated_residual_norm_vjp(*[g.to(device) for g in with_zero], *on_device, SCALE, EPSILON)
         for a, b in zip(some, same):
             assert torch.equal(a, b)
+
+
+# ------------------------------------------------- offsets beyond 32 bits ----
+HUGE_ROWS, HUGE_COLUMNS = 70000, 32768  # 2.3e9 numbers
+
+
+def huge(device, fill):
+    tensor = torch.empty(HUGE_ROWS, HUGE_COLUMNS, dtype=torch.bfloat16, device=device)
+    return tensor.fill_(fill)
+
+
+@pytest.mark.gpu
+def test_tables_of_more_than_two_to_the_31_numbers(device):
+    table = huge(device, 0)
+    rows = torch.tensor([HUGE_ROWS - 1, 3, HUGE_ROWS - 1, -1, 65537], dtype=torch.int32, device=device)
+    table[-1], table[3], table[65537] = 2.0, 3.0, 5.0
+    output = mops_amd.scaled_embedding(table, rows, 0.5)
+    assert [output[i].unique().tolist() for i in range(5)] == [[1.0], [1.5], [1.0], [0.0], [2.5]]
+    for repeats in (1, 60):  # (without an order in memory, and with one)
+        grad = mops_amd.scaled_embedding_vjp(output.repeat(repeats, 1), table, rows.repeat(repeats), 1.0)
+        assert [grad[i].unique().tolist() for i in (-1, 3, 65537, 0)] == [[2.0 * repeats], [1.5 * repeats], [2.5 * repeats], [0.0]]
+        assert torch.count_nonzero(grad.sum(1)).item() == 3
+        del grad
+
+
+@pytest.mark.gpu
+def test_products_of_more_than_two_to_the_31_numbers(device):
+    A = huge(device, 0)
+    A[-1], A[65537] = 1.0, 2.0
+    offsets = torch.tensor([0, 10, HUGE_ROWS], dtype=torch.int32, device=device)
+    for width in (8, 3):  # (rows of W on 16-byte boundaries and off them)
+        W = torch.full((2, HUGE_COLUMNS, width), 0.5, dtype=torch.bfloat16, device=device)
+        output = mops_amd.grouped_matrix_product(A, W, offsets)
+        assert output[-1].unique().tolist() == [HUGE_COLUMNS / 2] and output[65537].unique().tolist() == [HUGE_COLUMNS]
+        assert torch.count_nonzero(output).item() == 2 * width
+        grad_output = torch.zeros(HUGE_ROWS, width, dtype=torch.bfloat16, device=device)
+        grad_output[-1], grad_output[65537] = 4.0, 1.0
+        grad_A, grad_W = mops_amd.grouped_matrix_product_vjp(grad_output, A, W, offsets)
+        assert grad_A[-1].unique().tolist() == [2.0 * width] and grad_A[65537].unique().tolist() == [0.5 * width]
+        assert torch.count_nonzero(grad_A[:65537]).item() == 0
+        assert grad_W[1].unique().tolist() == [6.0] and not grad_W[0].any()
+        del grad_A
+
+
+@pytest.mark.gpu
+def test_updates_of_more_than_two_to_the_31_numbers(device):
+    residual, block, gate = huge(device, 1.0), huge(device, 1.0), huge(device, 2.0)
+    weight = torch.ones(HUGE_COLUMNS, dtype=torch.bfloat16, device=device)
+    residual[-1], gate[-1] = 0.0, 4.0
+    state, following = mops_amd.gated_residual_norm(residual, block, gate, weight, weight, 0.5, 0.0)
+    # (norm(1) = 1: state = residual + gate / 2)
+    assert state[-1].unique().tolist() == [2.0] and state[-2].unique().tolist() == [2.0]
+    assert state[0].unique().tolist() == [2.0] and following[-1].unique().tolist() == [1.0]
+    del state, following
+    grads = mops_amd.gated_residual_norm_vjp(
+        gate, None, residual, block, gate, weight, weight, 0.5, 0.0, compute_grad_block=False, compute_grad_gate=False
+    )
+    assert grads[0][-1].unique().tolist() == [4.0] and grads[0][65537].unique().tolist() == [2.0]
 
 
 # ---------------------------------------------------------- differences ----
@@ -558,3 +626,163 @@ def test_refusals(device):
         mops_amd.gated_residual_norm_vjp(rows, floats(4, 4), rows, rows, one, row, row)
     # (a refused call leaves nothing behind: the next one is right)
     assert mops_amd.scaled_embedding(floats(3, 4) + 1, integers(5), 2.0).eq(2).all()
+
+
+# ------------------------------------------------------ PyTorch operators ----
+def operators():
+    import mops_amd.torch  # noqa: F401  (registers the operators)
+
+    return torch.ops.mops
+
+
+SCHEMAS = {
+    "order_by_group": "mops::order_by_group(Tensor indices, int n_groups) -> (Tensor, Tensor)",
+    "scaled_embedding": "mops::scaled_embedding(Tensor table, Tensor indices, float scale=1.) -> Tensor",
+    "grouped_matrix_product": "mops::grouped_matrix_product(Tensor A, Tensor W, Tensor offsets, Tensor? order=None) -> Tensor",
+    "gated_residual_norm": "mops::gated_residual_norm(Tensor residual, Tensor block, Tensor gate, Tensor weight_block, Tensor weight_next, float residual_scale=1., float epsilon=9.9999999999999995e-07) -> (Tensor, Tensor)",
+}  # fmt: skip
+
+
+@pytest.mark.parametrize("name", list(SCHEMAS))
+def test_operator_schemas(name):
+    assert str(getattr(operators(), name).default._schema) == SCHEMAS[name]
+
+
+def test_operators_refuse_host_tensors():
+    index, values = torch.zeros(3, dtype=torch.int32), torch.zeros(3, 4)
+    with pytest.raises(RuntimeError, match="device path only"):
+        operators().order_by_group(index, 2)
+    with pytest.raises(RuntimeError, match="device path only"):
+        operators().scaled_embedding(values, index, 1.0)
+    with pytest.raises(RuntimeError, match="device path only"):
+        operators().grouped_matrix_product(values, torch.zeros(1, 4, 2), index[:2])
+    with pytest.raises(RuntimeError, match="device path only"):
+        operators().gated_residual_norm(values, values, values, values[0], values[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tag", list(DTYPES))
+def test_operators_with_autograd(device, tag):
+    """Values and gradients of the operators: what the functions of the package give, bit for bit."""
+    ops, dtype = operators(), DTYPES[tag]
+    generator = generator_of(21)
+
+    def rand(*shape):
+        return random(generator, shape, dtype).to(device)
+
+    index = indices_of("padded", 50, 4).to(device)
+    order, offsets = ops.order_by_group(index.long(), 4)
+    assert same((order, offsets), mops_amd.order_by_group(index, 4))
+    table, A, W, gate = rand(4, 24), rand(50, 24), rand(4, 24, 10), rand(1, 24)
+    rows, weights = [rand(50, 24), rand(50, 24)], [rand(24), rand(24)]
+    grad, grads = rand(50, 10), [rand(50, 24), rand(50, 24)]
+
+    leaf = table.clone().requires_grad_(True)
+    output = ops.scaled_embedding(leaf, index, 0.7)
+    output.backward(grads[0])
+    assert same(output.detach(), mops_amd.scaled_embedding(table, index, 0.7))
+    assert same(leaf.grad, mops_amd.scaled_embedding_vjp(grads[0], table, index, 0.7))
+
+    leaves = [A.clone().requires_grad_(True), W.clone().requires_grad_(True)]
+    output = ops.grouped_matrix_product(*leaves, offsets, order)
+    output.backward(grad)
+    assert same(output.detach(), mops_amd.grouped_matrix_product(A, W, offsets, order))
+    expected = mops_amd.grouped_matrix_product_vjp(grad, A, W, offsets, order)
+    assert same(tuple(t.grad for t in leaves), expected)
+    # rows that lie in the order of their group already
+    in_order = mops_amd.grouped_matrix_product(A, W, offsets)
+    assert same(ops.grouped_matrix_product(A, W, offsets), in_order)
+
+    inputs = [*rows, gate, *weights]
+    leaves = [t.clone().requires_grad_(True) for t in inputs]
+    state, following = ops.gated_residual_norm(*leaves, 0.4, 1e-5)
+    assert same((state.detach(), following.detach()), mops_amd.gated_residual_norm(*inputs, 0.4, 1e-5))
+    torch.autograd.backward([state, following], grads)
+    assert same(tuple(t.grad for t in leaves), mops_amd.gated_residual_norm_vjp(*grads, *inputs, 0.4, 1e-5))
+    # only one result used, only some inputs recorded
+    block = rows[1].clone().requires_grad_(True)
+    ops.gated_residual_norm(rows[0], block, gate, *weights, 0.4, 1e-5)[1].backward(grads[1])
+    assert same(block.grad, mops_amd.gated_residual_norm_vjp(None, grads[1], *inputs, 0.4, 1e-5)[1])
+
+
+@pytest.mark.gpu
+def test_operators_registered_from_python():
+    """The same tests with the operators of mops_amd/_torch_python_ops.py, in a process of their own."""
+    import os
+    import subprocess
+    import sys
+
+    if os.environ.get("MOPS_AMD_TORCH_PYTHON_OPS", "0") not in ("", "0"):
+        pytest.skip("this process already runs them")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run(
+        [sys.executable, "-m", "pytest", os.path.join(root, "tests", "test_layers.py"), "-q", "-x", "-k", "operator",
+         "-p", "no:cacheprovider"],
+        cwd=root, env=dict(os.environ, MOPS_AMD_TORCH_PYTHON_OPS="1"), capture_output=True, text=True,
+    )  # fmt: skip
+    assert done.returncode == 0, done.stdout[-3000:] + done.stderr[-2000:]
+    assert " passed" in done.stdout
+
+
+# ---------------------------------------------------------------- example ----
+class PlainOperators:
+    """The operators of the example in elementary torch operations."""
+
+    @staticmethod
+    def order_by_group(indices, n_groups):
+        order, offsets = plan_of(indices.cpu(), n_groups)
+        return order.to(indices.device), offsets.to(indices.device)
+
+    @staticmethod
+    def scaled_embedding(table, indices, scale):
+        inside = indices >= 0
+        return torch.where(inside[:, None], table[torch.where(inside, indices, 0).long()] * scale, 0.0)
+
+    @staticmethod
+    def outer_product_scatter_add_with_weights(A, B, W, indices_W, indices_output):
+        terms = A[:, :, None] * (B * W[indices_W.long()])[:, None, :]
+        zeros = torch.zeros(W.shape[0], A.shape[1], B.shape[1], dtype=A.dtype, device=A.device)
+        return zeros.index_add(0, indices_output.long(), terms)
+
+    @staticmethod
+    def grouped_matrix_product(A, W, offsets, order):
+        output = torch.zeros(A.shape[0], W.shape[2], dtype=A.dtype, device=A.device)
+        for g in range(W.shape[0]):
+            rows = order[int(offsets[g]) : int(offsets[g + 1])].long()
+            output = output.index_add(0, rows, A[rows] @ W[g])
+        return output
+
+    @staticmethod
+    def gated_residual_norm(residual, block, gate, weight_block, weight_next, scale, epsilon):
+        def norm(x):
+            return x / torch.sqrt((x**2).mean(1, keepdim=True) + epsilon)
+
+        state = residual + scale * gate * norm(block) * weight_block
+        return state, norm(state) * weight_next
+
+
+@pytest.mark.gpu
+def test_example_network(device):
+    """The operators together, with the sums over edges: energy and all gradients in float64 against elementary torch
+    operations (rounding errors of some 1e4 terms, 1e-16 each, grow through the layers; held to 1e-10 of each gradient's
+    largest value), and a loss that falls."""
+    import importlib.util
+    import os
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    spec = importlib.util.spec_from_file_location("element_network", os.path.join(root, "examples", "element_network.py"))
+    network = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(network)
+    s = network.structure(device, torch.float64)
+    results = []
+    for ops in (torch.ops.mops, PlainOperators):
+        p = network.parameters(device, torch.float64)
+        value = network.energy(p, s, ops)
+        value.backward()
+        results.append((value.detach(), {name: t.grad for name, t in p.items()}))
+    assert abs(results[0][0] - results[1][0]) <= 1e-10 * abs(results[1][0])
+    for name, gradient in results[0][1].items():
+        expected = results[1][1][name]
+        assert (gradient - expected).abs().max() <= 1e-10 * expected.abs().max(), name
+    losses = network.train(steps=15, device=device)
+    assert losses[-1] < 0.2 * losses[0]
