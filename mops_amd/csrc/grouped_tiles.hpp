@@ -227,50 +227,44 @@ __device__ __forceinline__ void fetch(const void* from, char* lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "m0");
 }
 
-/// A side of the product on its way to LDS: piece i = threadIdx.x + j * THREADS, j < EACH.
-template <typename T, int OUTER, int DEEP, int THREADS, bool ALIGNED> struct Pieces {
+/// A side of the product on its way to LDS: piece i = threadIdx.x + j * THREADS, j < EACH. Through registers: SETS steps
+/// are on their way at once, each in a set of registers.
+template <typename T, int OUTER, int DEEP, int THREADS, int SETS> struct Pieces {
     static constexpr int EACH = OUTER * DEEP / THREADS, COUNT = Matrix<T>::COUNT;
-    Numbers<T> piece[ALIGNED ? 1 : EACH];
-    int32_t missing[ALIGNED ? 1 : EACH]; // of the piece's numbers, which then hold `missing` of the row's earlier ones in front
-    bool complete;                       // no piece of the step misses any (uniform)
+    static constexpr bool ALIGNED = SETS == 0;
+    Numbers<T> piece[ALIGNED ? 1 : SETS][ALIGNED ? 1 : EACH];
 
-    /// piece j: numbers `from` .. of a row, of which `left` are in the row (at most 0: none). WHOLE: all of them are,
-    /// or the side's row does not matter. Through registers, the last piece of a row is the row's last COUNT numbers
+    /// piece j of a step: numbers `from` .. of a row, of which `left` are in the row (at most 0: none). WHOLE: all of them
+    /// are, or the side's row does not matter. Through registers, the last piece of a row is the row's last COUNT numbers
     /// (`short_rows`: there are fewer), of which it drops those of the piece before when it is stored.
     template <bool WHOLE>
-    __device__ __forceinline__ void take(int j, const T* from, int32_t left, bool short_rows, char* lds, int wave) {
+    __device__ __forceinline__ void take(int set, int j, const T* from, int32_t left, bool short_rows, char* lds, int wave) {
         if constexpr (ALIGNED) {
             const void* at = WHOLE || left > 0 ? static_cast<const void*>(from) : &zeros_in_memory;
             fetch(at, lds + (wave * WAVE + j * THREADS) * 16);
         } else if constexpr (WHOLE) {
-            complete = true;
-            piece[j] = load_numbers<T>(from);
+            piece[set][j] = load_numbers<T>(from);
         } else if (short_rows) { // (uniform)
-            complete = true;
-            piece[j] = load_some_numbers<T>(from, left);
+            piece[set][j] = load_some_numbers<T>(from, left);
         } else {
-            complete = false;
-            missing[j] = min(max(COUNT - left, 0), COUNT);
-            if (missing[j] < COUNT) {
-                piece[j] = load_numbers<T>(from - missing[j]);
+            const int32_t missing = min(max(COUNT - left, 0), COUNT);
+            if (missing < COUNT) {
+                piece[set][j] = load_numbers<T>(from - missing);
             }
         }
     }
-    /// the pieces that came through registers
-    __device__ __forceinline__ void store(char* lds) const {
+    /// a piece that came through registers
+    __device__ __forceinline__ void put(int set, int j, int32_t left, bool complete, char* lds) const {
         if constexpr (!ALIGNED) {
-#pragma unroll
-            for (int j = 0; j < EACH; j++) {
-                *reinterpret_cast<Numbers<T>*>(lds + (threadIdx.x + j * THREADS) * 16) =
-                    complete ? piece[j] : without_first<T>(piece[j], missing[j]);
-            }
+            *reinterpret_cast<Numbers<T>*>(lds + (threadIdx.x + j * THREADS) * 16) =
+                complete ? piece[set][j] : without_first<T>(piece[set][j], min(max(COUNT - left, 0), COUNT));
         }
     }
 };
 
-template <typename T, int OUTER, int DEEP, int THREADS, bool ALIGNED>
-struct StraightLoader : public Pieces<T, OUTER, DEEP, THREADS, ALIGNED> {
-    typedef Pieces<T, OUTER, DEEP, THREADS, ALIGNED> Base;
+template <typename T, int OUTER, int DEEP, int THREADS, int SETS>
+struct StraightLoader : public Pieces<T, OUTER, DEEP, THREADS, SETS> {
+    typedef Pieces<T, OUTER, DEEP, THREADS, SETS> Base;
     typedef Straight<T, OUTER, DEEP> Layout;
     using Base::COUNT;
     using Base::EACH;
@@ -289,17 +283,25 @@ struct StraightLoader : public Pieces<T, OUTER, DEEP, THREADS, ALIGNED> {
         }
     }
     /// Piece j of the next step, which begins at k0 (steps are asked for in order).
-    template <bool WHOLE> __device__ __forceinline__ void load(int j, int32_t k0, char* lds, int wave) {
-        this->template take<WHOLE>(j, from[j], k_size - k0 - of_row(j) * COUNT, k_size < COUNT, lds, wave);
+    template <bool WHOLE> __device__ __forceinline__ void load(int set, int j, int32_t k0, char* lds, int wave) {
+        this->template take<WHOLE>(set, j, from[j], k_size - k0 - of_row(j) * COUNT, k_size < COUNT, lds, wave);
         from[j] += DEEP * COUNT;
+    }
+    /// The pieces of a step that came through registers (`whole`: it was loaded with WHOLE).
+    __device__ __forceinline__ void store(int set, int32_t k0, bool whole, char* lds) const {
+#pragma unroll
+        for (int j = 0; j < EACH; j++) {
+            this->put(set, j, k_size - k0 - of_row(j) * COUNT, whole || k_size < COUNT, lds);
+        }
     }
 };
 
 /// Rows of `width` numbers, of which those from outer0 on are used.
-template <typename T, int OUTER, int DEEP, int THREADS, bool ALIGNED>
-struct TurnedLoader : public Pieces<T, OUTER, DEEP, THREADS, ALIGNED> {
-    typedef Pieces<T, OUTER, DEEP, THREADS, ALIGNED> Base;
+template <typename T, int OUTER, int DEEP, int THREADS, int SETS>
+struct TurnedLoader : public Pieces<T, OUTER, DEEP, THREADS, SETS> {
+    typedef Pieces<T, OUTER, DEEP, THREADS, SETS> Base;
     typedef Turned<T, OUTER, DEEP> Layout;
+    using Base::ALIGNED;
     using Base::COUNT;
     using Base::EACH;
     static constexpr int K_EACH = THREADS / Layout::PIECES; // rows of k between a thread's pieces
@@ -328,21 +330,32 @@ struct TurnedLoader : public Pieces<T, OUTER, DEEP, THREADS, ALIGNED> {
 
     /// Piece j of the next step of consecutive rows (after begin_rows), of which the matrix has rows_left.
     __device__ __forceinline__ void begin_rows() { from += static_cast<size_t>(k(0)) * (between / K_EACH); }
-    template <bool WHOLE> __device__ __forceinline__ void load(int j, int32_t rows_left, char* lds, int wave) {
-        this->template take<WHOLE>(j, from + j * between, k(j) < rows_left ? left : 0, short_rows, lds, wave);
+    template <bool WHOLE> __device__ __forceinline__ void load(int set, int j, int32_t rows_left, char* lds, int wave) {
+        this->template take<WHOLE>(set, j, from + j * between, k(j) < rows_left ? left : 0, short_rows, lds, wave);
         from += j == EACH - 1 ? next : 0;
     }
     /// Piece j of a step whose row is `row` there (negative: none; not with WHOLE).
-    template <bool WHOLE> __device__ __forceinline__ void load_row(int j, int32_t row, char* lds, int wave) {
+    template <bool WHOLE> __device__ __forceinline__ void load_row(int set, int j, int32_t row, char* lds, int wave) {
         const size_t at = static_cast<size_t>(WHOLE ? row : max(row, 0)) * (between / K_EACH);
-        this->template take<WHOLE>(j, from + at, row >= 0 ? left : 0, short_rows, lds, wave);
+        this->template take<WHOLE>(set, j, from + at, row >= 0 ? left : 0, short_rows, lds, wave);
+    }
+    /// The pieces of a step that came through registers, of a side that has rows_left more rows.
+    __device__ __forceinline__ void store(int set, int32_t rows_left, bool whole, char* lds) const {
+#pragma unroll
+        for (int j = 0; j < EACH; j++) {
+            this->put(set, j, k(j) < rows_left ? left : 0, whole || short_rows, lds);
+        }
     }
 };
 
-/// Everything this wavefront has asked of LDS has arrived, and of memory all but the last LATER pieces; then the
-/// workgroup meets.
+/// Everything this wavefront has asked of LDS has arrived, and of what it has asked of memory for LDS all but the last
+/// LATER pieces (negative: nothing goes that way); then the workgroup meets.
 template <int LATER> __device__ __forceinline__ void meet() {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
+    if constexpr (LATER < 0) {
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    } else {
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(LATER) : "memory");
+    }
 }
 
 /// WM x WN wavefronts; every one of them makes BM / WM x BN / WN numbers, in steps of DEEP pieces of k of which STAGES
@@ -361,12 +374,13 @@ __device__ __forceinline__ void make_tile(
     constexpr int MB = BM / WM / BLOCK, NB = BN / WN / BLOCK; // blocks of a wavefront
     constexpr bool SUMS = FORM == Form::GRAD_SUMS, Q_TURNED = SUMS, P_TURNED = FORM != Form::GRAD_ROWS;
     constexpr Units UNITS = SUMS ? Units::OF_GROUPS : Units::OF_ROWS;
+    constexpr int SETS = ALIGNED ? 0 : BM <= 64 ? 3 : sizeof(T) == 8 ? 1 : 2; // (what there is room for in registers)
     using QLoader = std::conditional_t<
-        Q_TURNED, TurnedLoader<T, BM, DEEP, THREADS, ALIGNED>, StraightLoader<T, BM, DEEP, THREADS, ALIGNED>>;
+        Q_TURNED, TurnedLoader<T, BM, DEEP, THREADS, SETS>, StraightLoader<T, BM, DEEP, THREADS, SETS>>;
     using PLoader = std::conditional_t<
-        P_TURNED, TurnedLoader<T, BN, DEEP, THREADS, ALIGNED>, StraightLoader<T, BN, DEEP, THREADS, ALIGNED>>;
+        P_TURNED, TurnedLoader<T, BN, DEEP, THREADS, SETS>, StraightLoader<T, BN, DEEP, THREADS, SETS>>;
     constexpr int P_AT = BM * DEEP * 16, BYTES = P_AT + BN * DEEP * 16;
-    static_assert(ALIGNED || STAGES == 2, "through registers: one step on its way, one in LDS beside the present one");
+    static_assert(ALIGNED || STAGES == 2, "through registers: one step in LDS beside the present one");
     char* const stages = lds.stages;
     int32_t* const rows = lds.rows;
 
@@ -456,18 +470,18 @@ __device__ __forceinline__ void make_tile(
             }
         };
         // Piece `piece` of the step that begins at k0 (find_rows of it before).
-        auto load_piece = [&](auto is_whole, int piece, int32_t k0, char* buffer) {
+        auto load_piece = [&](auto is_whole, int set, int piece, int32_t k0, char* buffer) {
             constexpr bool WHOLE = decltype(is_whole)::value;
             if constexpr (SUMS) {
                 if (piece < Q_EACH) {
-                    q.template load_row<WHOLE>(piece, row_of_piece[piece], buffer, wave);
+                    q.template load_row<WHOLE>(set, piece, row_of_piece[piece], buffer, wave);
                 } else {
-                    p.template load_row<WHOLE>(piece - Q_EACH, row_of_piece[piece], buffer + P_AT, wave);
+                    p.template load_row<WHOLE>(set, piece - Q_EACH, row_of_piece[piece], buffer + P_AT, wave);
                 }
             } else if (piece < Q_EACH) {
-                q.template load<WHOLE>(piece, k0, buffer, wave);
+                q.template load<WHOLE>(set, piece, k0, buffer, wave);
             } else {
-                p.template load<WHOLE>(piece - Q_EACH, P_TURNED ? k_size - k0 : k0, buffer + P_AT, wave);
+                p.template load<WHOLE>(set, piece - Q_EACH, P_TURNED ? k_size - k0 : k0, buffer + P_AT, wave);
             }
         };
         // through registers, no step but the last one needs to look where the matrices end
@@ -485,23 +499,28 @@ __device__ __forceinline__ void make_tile(
 #pragma unroll
             for (int piece = 0; piece < EACH; piece++) {
                 if (piece >= from && piece < upto) {
-                    load_piece(std::false_type(), piece, k0, buffer);
+                    load_piece(std::false_type(), 0, piece, k0, buffer);
                 }
             }
         };
-        auto load = [&](int32_t k0, char* buffer) {
-            if (!ALIGNED && whole && k0 + STEP <= k_size) { // (uniform)
+        // through registers: a step from memory to a set of them, and from there to LDS
+        auto is_whole = [&](int32_t k0) { return whole && k0 + STEP <= k_size; }; // (uniform)
+        auto load = [&](int set, int32_t k0) {
+            if (is_whole(k0)) {
 #pragma unroll
                 for (int piece = 0; piece < EACH; piece++) {
-                    load_piece(std::true_type(), piece, k0, buffer);
+                    load_piece(std::true_type(), set, piece, k0, nullptr);
                 }
             } else {
-                load_some(0, EACH, k0, buffer);
+#pragma unroll
+                for (int piece = 0; piece < EACH; piece++) {
+                    load_piece(std::false_type(), set, piece, k0, nullptr);
+                }
             }
         };
-        auto store = [&](char* buffer) {
-            q.store(buffer);
-            p.store(buffer + P_AT);
+        auto store = [&](int set, int32_t k0, char* buffer) {
+            q.store(set, Q_TURNED ? k_size - k0 : k0, is_whole(k0), buffer);
+            p.store(set, P_TURNED ? k_size - k0 : k0, is_whole(k0), buffer + P_AT);
         };
         Numbers<T> of_q[2][MB], of_p[2][NB];
         // what a multiplication needs, in the order in which it needs it: q 0, p 0 .. NB - 1, q 1 .. MB - 1
@@ -546,27 +565,30 @@ __device__ __forceinline__ void make_tile(
         auto nothing = [](int, int) {};
         static_assert(STEPS % 2 == 0, "the numbers of step 0 come to the place of the last step but one");
         // Step t is multiplied from stage t % STAGES. Where the workgroup meets in it, step t + 1 has arrived, and the
-        // stage is free for step t + STAGES (ALIGNED: EARLY of its pieces are asked for right then, the others in the next
-        // step's first multiplication), or step t + 1 is put into its stage from registers, which are free for step t + 2.
-        // (ALIGNED: steps behind the last one are asked for like all others: zeros.)
-        constexpr int FIRST = ALIGNED ? STAGES : 1, EARLY = EACH / 2;
+        // stage is free for step t + STAGES: EARLY of its pieces are asked for right then, the others in the next step's
+        // first multiplication. (Steps behind the last one are asked for like all others: zeros.) Through registers: in
+        // front of the meeting step t + 1 is put into its stage, from a set that step t + 1 + SETS comes to.
+        constexpr int EARLY = EACH / 2, UNROLL = ALIGNED ? 1 : SETS;
+        if constexpr (ALIGNED) {
 #pragma unroll
-        for (int t = 0; t < FIRST; t++) {
-            find_rows(t * STEP);
-            if (ALIGNED && t == FIRST - 1) {
-                load_some(0, EARLY, t * STEP, stages + t * BYTES);
-            } else {
-                load(t * STEP, stages + t * BYTES);
+            for (int t = 0; t < STAGES; t++) {
+                find_rows(t * STEP);
+                load_some(0, t == STAGES - 1 ? EARLY : EACH, t * STEP, stages + t * BYTES);
             }
-        }
-        store(stages);
-        meet<ALIGNED ? (STAGES - 2) * EACH + EARLY : 0>();
-        if (!ALIGNED) {
-            find_rows(STEP);
-            if (STEP < k_size) {
-                load(STEP, stages);
+            meet<(STAGES - 2) * EACH + EARLY>();
+        } else {
+            find_rows(0);
+            load(0, 0);
+            store(0, 0, stages);
+#pragma unroll
+            for (int t = 1; t <= SETS; t++) {
+                find_rows(t * STEP);
+                if (t * STEP < k_size) { // (uniform)
+                    load(t % UNROLL, t * STEP);
+                }
             }
-            find_rows(2 * STEP);
+            find_rows((SETS + 1) * STEP);
+            meet<-1>();
         }
         char *before = stages + (STAGES - 1) * BYTES, *buffer = stages;
         if (works) {
@@ -575,7 +597,7 @@ __device__ __forceinline__ void make_tile(
                 read(buffer, 0, r);
             }
         }
-        for (int32_t k0 = 0; k0 < k_size; k0 += STEP) {
+        auto step_at = [&](int32_t k0, int set) {
 #pragma unroll
             for (int step = 0; step < STEPS - 1; step++) {
                 if (ALIGNED && step == 0) {
@@ -588,21 +610,30 @@ __device__ __forceinline__ void make_tile(
                 }
             }
             char* const following = buffer + BYTES < stages + STAGES * BYTES ? buffer + BYTES : stages;
-            store(following);
-            meet<ALIGNED ? (STAGES - 2) * EACH : 0>();
             if constexpr (ALIGNED) {
+                meet<(STAGES - 2) * EACH>();
                 multiply(STEPS - 1, following, 0, 0, EARLY, [&](int from, int upto) {
                     load_some(from, upto, k0 + STAGES * STEP, buffer);
                 });
             } else {
-                if (k0 + 2 * STEP < k_size) { // (uniform)
-                    load(k0 + 2 * STEP, buffer);
-                    find_rows(k0 + 3 * STEP);
+                store(set, k0 + STEP, following);
+                meet<-1>();
+                if (k0 + (SETS + 1) * STEP < k_size) { // (uniform)
+                    load(set, k0 + (SETS + 1) * STEP);
+                    find_rows(k0 + (SETS + 2) * STEP);
                 }
                 multiply(STEPS - 1, following, 0, 0, 0, nothing);
             }
             before = buffer;
             buffer = following;
+        };
+        for (int32_t k0 = 0; k0 < k_size; k0 += UNROLL * STEP) {
+#pragma unroll
+            for (int u = 0; u < UNROLL; u++) {
+                if (k0 + u * STEP < k_size) { // (uniform)
+                    step_at(k0 + u * STEP, (u + 1) % UNROLL);
+                }
+            }
         }
         meet<0>(); // (nothing is on its way to LDS any more)
     }
@@ -683,7 +714,7 @@ __device__ __forceinline__ void make_tile(
 }
 
 template <typename T, Form FORM, int BM, int BN, int WM, int WN, int DEEP, int STAGES, bool ALIGNED>
-__global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
+__global__ __launch_bounds__(WM* WN* WAVE, 2) void tiles_kernel(Product<T> g) {
     __shared__ TileLds<BM, BN, DEEP, STAGES> lds;
     make_tile<T, FORM, BM, BN, WM, WN, DEEP, STAGES, ALIGNED>(g, blockIdx.x, lds);
 }
@@ -691,7 +722,7 @@ __global__ __launch_bounds__(WM* WN* WAVE) void tiles_kernel(Product<T> g) {
 /// Both gradients in one launch, the sums' tiles (of which there are `of_sums` workgroups, a multiple of 8) in front: they
 /// take longer, and the rows' tiles fill in behind them.
 template <typename T, int BM, int BN, int WM, int WN, int DEEP, int STAGES, bool ALIGNED>
-__global__ __launch_bounds__(WM* WN* WAVE) void gradients_kernel(Product<T> sums, Product<T> rows, uint32_t of_sums) {
+__global__ __launch_bounds__(WM* WN* WAVE, 2) void gradients_kernel(Product<T> sums, Product<T> rows, uint32_t of_sums) {
     __shared__ TileLds<BM, BN, DEEP, STAGES> lds;
     if (blockIdx.x < of_sums) {
         make_tile<T, Form::GRAD_SUMS, BM, BN, WM, WN, DEEP, STAGES, ALIGNED>(sums, blockIdx.x, lds);
