@@ -41,7 +41,8 @@ template <Form FORM, typename T> unsigned set_tiles(Product<T>& g, int tile) {
         g.step = tile;
     }
     g.most_units = narrow_i32(most_units(g.groups.n_rows, g.groups.n_groups, g.step), "number of units of rows");
-    const size_t workgroups = ceil_div(static_cast<size_t>(g.most_units) * g.m_tiles * g.n_tiles, 8) * 8;
+    const size_t of_unit = static_cast<size_t>(g.m_tiles) * g.n_tiles * std::max(g.splits, 1);
+    const size_t workgroups = ceil_div(g.most_units * of_unit, 8) * 8;
     return static_cast<unsigned>(narrow_i32(workgroups, "number of tiles"));
 }
 
@@ -101,8 +102,43 @@ template <typename T> int tile_of_sums(Product<T>& g) {
     return tile;
 }
 
-template <typename T> void forward(const Product<T>& g, hipStream_t stream) {
-    launch<T, Form::FORWARD>(g, tile_of_rows<T, Form::FORWARD>(g), stream);
+/// FORWARD and GRAD_ROWS with few tiles and long sums: every compute unit gets a share of k (250 rows of 19 groups, K = 24,
+/// L = 1226 in float, gradients: 20 workgroups, one of 39 steps after the other, are 41 us). At least four steps each.
+template <typename T> void share_k(Product<T>& g, int tile) {
+    g.splits = 1;
+    g.k_each = g.k_size;
+    if (tile != 64) {
+        return;
+    }
+    const size_t step = 16 / sizeof(T) * DEEP, steps = ceil_div(static_cast<size_t>(g.k_size), step);
+    const size_t rows = static_cast<size_t>(g.groups.n_rows), groups = static_cast<size_t>(g.groups.n_groups);
+    const size_t workgroups = std::min(ceil_div(rows, 64) + groups, rows) * tiles(g.n_size, 64);
+    const size_t units = static_cast<size_t>(compute_units());
+    if (workgroups < units && steps >= 8) {
+        const size_t splits = std::min(ceil_div(units, workgroups), steps / 4), each = ceil_div(steps, splits);
+        g.splits = static_cast<int32_t>(ceil_div(steps, each));
+        g.k_each = static_cast<int32_t>(each * step);
+    }
+}
+template <typename T> size_t split_bytes(const Product<T>& g) {
+    return g.splits > 1 ? align256(static_cast<size_t>(g.splits) * g.groups.n_rows * g.n_size * sizeof(wide_t<T>)) : 0;
+}
+template <typename T> void join_splits(const Product<T>& g, hipStream_t stream) {
+    if (g.splits > 1) {
+        const size_t blocks = ceil_div(static_cast<size_t>(g.groups.n_rows) * g.n_size, JOIN_THREADS);
+        join_splits_kernel<T><<<static_cast<unsigned>(blocks), JOIN_THREADS, 0, stream>>>(g);
+        MOPS_HIP_CHECK(hipGetLastError());
+    }
+}
+
+template <typename T> void forward(Product<T> g, hipStream_t stream) {
+    const int tile = tile_of_rows<T, Form::FORWARD>(g);
+    share_k(g, tile);
+    if (g.splits > 1) {
+        g.partial = static_cast<wide_t<T>*>(scratch(split_bytes(g)));
+    }
+    launch<T, Form::FORWARD>(g, tile, stream);
+    join_splits(g, stream);
 }
 
 /// Either may be without an `out`: not wanted.
@@ -110,10 +146,19 @@ template <typename T> void gradients(Product<T> sums, Product<T> rows, hipStream
     const int of_sums = sums.out != nullptr ? tile_of_sums(sums) : 0;
     const int of_rows = rows.out != nullptr ? tile_of_rows<T, Form::GRAD_ROWS>(rows) : 0;
     const bool splits = of_sums != 0 && sums.step < sums.groups.n_rows;
+    if (of_rows != 0) {
+        share_k(rows, of_rows);
+    }
+    const size_t row_bytes = of_rows != 0 ? split_bytes(rows) : 0;
+    size_t sum_bytes = 0;
     if (splits) {
         const size_t most = most_units(sums.groups.n_rows, sums.groups.n_groups, sums.step);
-        sums.partial =
-            static_cast<wide_t<T>*>(scratch(most * partial_size(sums.m_size, sums.n_size) * sizeof(wide_t<T>)));
+        sum_bytes = most * partial_size(sums.m_size, sums.n_size) * sizeof(wide_t<T>);
+    }
+    if (row_bytes + sum_bytes > 0) {
+        char* workspace = static_cast<char*>(scratch(row_bytes + sum_bytes));
+        rows.partial = reinterpret_cast<wide_t<T>*>(workspace);
+        sums.partial = reinterpret_cast<wide_t<T>*>(workspace + row_bytes);
     }
     const bool in_place = of_sums != 0 && aligned<T, Form::GRAD_SUMS>(sums);
     if (of_sums == of_rows && in_place == aligned<T, Form::GRAD_ROWS>(rows)) {
@@ -133,6 +178,9 @@ template <typename T> void gradients(Product<T> sums, Product<T> rows, hipStream
         if (of_rows != 0) {
             launch<T, Form::GRAD_ROWS>(rows, of_rows, stream);
         }
+    }
+    if (of_rows != 0) {
+        join_splits(rows, stream);
     }
     if (splits) {
         sums.most_units = narrow_i32(

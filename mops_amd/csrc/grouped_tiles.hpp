@@ -52,13 +52,16 @@ enum class Form { FORWARD, GRAD_ROWS, GRAD_SUMS };
 /// [rows][m_size], p is [rows][n_size].
 template <typename T> struct Product {
     T* out;
-    wide_t<T>* partial; // GRAD_SUMS: [unit][partial_size(m_size, n_size)], for groups of more than one unit
+    // GRAD_SUMS: [unit][partial_size(m_size, n_size)], for groups of more than one unit; else [split][row][n_size], where
+    // there are several
+    wide_t<T>* partial;
     const T *q, *p;
     RowGroups groups;
     int32_t m_size, n_size, k_size;
     int32_t step;            // places per unit
     int32_t most_units;      // that the grid and `partial` have room for (offsets that are none could give more)
     int32_t m_tiles, n_tiles; // tiles of a unit (m_tiles: GRAD_SUMS)
+    int32_t splits, k_each;   // FORWARD, GRAD_ROWS: shares of k, and how long they are (whole steps)
 };
 
 /// Numbers from one unit's partial result to the next: whole pieces of four.
@@ -222,10 +225,13 @@ __device__ __constant__ const uint4 zeros_in_memory = {0, 0, 0, 0};
 /// 16 bytes from memory to LDS, at `lds` (the same for all lanes) + 16 * lane, without a register. Arrived when the
 /// wavefront's vmcnt says so, which `meet` waits for. (Not the builtin: behind it the compiler waits for vmcnt at the
 /// next read of LDS, of whichever buffer. There is no register here that it could lose track of.)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm" // (m0 as a clobber: reserved, and written here)
 __device__ __forceinline__ void fetch(const void* from, char* lds) {
     const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "m0");
 }
+#pragma clang diagnostic pop
 
 /// A side of the product on its way to LDS: piece i = threadIdx.x + j * THREADS, j < EACH. Through registers: SETS steps
 /// are on their way at once, each in a set of registers.
@@ -387,7 +393,9 @@ __device__ __forceinline__ void make_tile(
     // Workgroups b, b + 8, .. run on the same XCD. Tiles of rows take the same time each: an XCD gets consecutive ones, so
     // that its L2 holds what they share. A unit of GRAD_SUMS takes as long as it has rows: its tiles go to all XCDs (24
     // uneven groups in consecutive tiles: 122 us instead of 88).
-    const int32_t tiles_of_unit = (SUMS ? g.m_tiles : 1) * g.n_tiles;
+    constexpr bool MAY_SPLIT = !SUMS && BM == 64;
+    const int32_t splits = MAY_SPLIT ? g.splits : 1;
+    const int32_t tiles_of_unit = (SUMS ? g.m_tiles : splits) * g.n_tiles;
     UnitsOfGroups<UNITS> of_groups(g.groups, g.step);
     const int32_t units = min(of_groups.total(), g.most_units);
     const int64_t tiles = static_cast<int64_t>(units) * tiles_of_unit;
@@ -396,7 +404,7 @@ __device__ __forceinline__ void make_tile(
     if (static_cast<int32_t>(block / 8) >= per_xcd || tile >= tiles) {
         return; // (uniform)
     }
-    int32_t unit_index, m0, n0;
+    int32_t unit_index, m0, n0, split = 0;
     if (SUMS) {
         unit_index = static_cast<int32_t>(tile / tiles_of_unit);
         const int32_t of_unit = static_cast<int32_t>(tile % tiles_of_unit);
@@ -404,11 +412,13 @@ __device__ __forceinline__ void make_tile(
         n0 = of_unit % g.n_tiles * BN;
     } else {
         // bands of four units: their rows and a tile's columns of the matrix are read together
-        const int32_t band = static_cast<int32_t>(tile / (4 * g.n_tiles)), in_band = static_cast<int32_t>(tile % (4 * g.n_tiles));
+        const int32_t of_band = 4 * tiles_of_unit;
+        const int32_t band = static_cast<int32_t>(tile / of_band), in_band = static_cast<int32_t>(tile % of_band);
         const int32_t height = min(4, units - 4 * band);
         unit_index = 4 * band + in_band % height;
         m0 = 0;
-        n0 = in_band / height * BN;
+        n0 = in_band / height / splits * BN;
+        split = in_band / height % splits;
     }
     const GroupUnit unit = of_groups.find(unit_index);
     if (unit.group < 0) {
@@ -437,23 +447,28 @@ __device__ __forceinline__ void make_tile(
         }
     }
 
-    const int32_t k_size = __builtin_amdgcn_readfirstlane(rest ? 0 : SUMS ? unit.count : g.k_size);
+    const int32_t k_begin = MAY_SPLIT ? split * g.k_each : 0;
+    const int32_t k_size = __builtin_amdgcn_readfirstlane(
+        rest ? 0 : SUMS ? unit.count : splits > 1 ? min(g.k_size - k_begin, g.k_each) : g.k_size
+    );
     if (k_size > 0) {
         QLoader q;
         PLoader p;
         if constexpr (Q_TURNED) {
             q.begin(g.q, g.m_size, m0);
         } else {
-            q.begin(k_size, [&](int i) { return g.q + static_cast<size_t>(rows[i]) * g.k_size; });
+            q.begin(k_size, [&](int i) { return g.q + static_cast<size_t>(rows[i]) * g.k_size + k_begin; });
         }
         const size_t of_group = static_cast<size_t>(unit.group) * g.k_size * g.n_size;
         if constexpr (SUMS) {
             p.begin(g.p, g.n_size, n0);
         } else if constexpr (P_TURNED) {
-            p.begin(g.p + of_group, g.n_size, n0);
+            p.begin(g.p + of_group + static_cast<size_t>(k_begin) * g.n_size, g.n_size, n0);
             p.begin_rows();
         } else {
-            p.begin(k_size, [&](int i) { return g.p + of_group + static_cast<size_t>(min(n0 + i, g.n_size - 1)) * g.k_size; });
+            p.begin(k_size, [&](int i) {
+                return g.p + of_group + static_cast<size_t>(min(n0 + i, g.n_size - 1)) * g.k_size + k_begin;
+            });
         }
         constexpr int Q_EACH = QLoader::EACH, P_EACH = PLoader::EACH, EACH = Q_EACH + P_EACH;
         // GRAD_SUMS: the rows behind the pieces of a step
@@ -709,7 +724,31 @@ __device__ __forceinline__ void make_tile(
             put(T(), row_of(g.out + unit.group * size));
         }
     } else {
-        put(T(), [&](int m) { return m < unit.count ? g.out + static_cast<size_t>(rows[m]) * g.n_size : nullptr; });
+        auto row_of = [&](auto* result) {
+            return [=, &g](int m) { return m < unit.count ? result + static_cast<size_t>(rows[m]) * g.n_size : nullptr; };
+        };
+        if (MAY_SPLIT && splits > 1) { // (uniform)
+            if constexpr (MAY_SPLIT) {
+                put(wide_t<T>(), row_of(g.partial + static_cast<size_t>(split) * g.groups.n_rows * g.n_size));
+            }
+        } else {
+            put(T(), row_of(g.out));
+        }
+    }
+}
+
+/// out := the sum of the shares of k.
+constexpr int JOIN_THREADS = 256;
+template <typename T> __global__ __launch_bounds__(JOIN_THREADS) void join_splits_kernel(Product<T> g) {
+    const size_t size = static_cast<size_t>(g.groups.n_rows) * g.n_size;
+    const size_t i = blockIdx.x * static_cast<size_t>(JOIN_THREADS) + threadIdx.x;
+    if (i < size) {
+        wide_t<T> sum = 0;
+#pragma unroll 8
+        for (int32_t s = 0; s < g.splits; s++) {
+            sum += g.partial[s * size + i];
+        }
+        g.out[i] = static_cast<T>(sum);
     }
 }
 
