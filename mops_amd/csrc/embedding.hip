@@ -35,7 +35,7 @@ constexpr int32_t CHUNKS = 1024;    // that there should be, and at least CHUNK_
 constexpr int32_t CHUNK_PLACES = 64;
 constexpr int32_t ALONE = 64;       // places that a team sums up by itself
 constexpr int32_t FEW = 16;         // rows per table row from which on a workgroup has one table row
-constexpr int32_t ROWS_PER_TEAM = 4; // at most
+constexpr int32_t ROWS_PER_TEAM = 8; // at most
 
 /// How a row's pieces are shared out: `team` lanes (a power of two) hold a piece each.
 struct Teams {
@@ -217,7 +217,7 @@ __device__ __forceinline__ void sum_table_rows(
         for (int j = 0; j < N; j++) {
             value.set(j, scale * sum[j]);
         }
-        value.store(grad_table + static_cast<size_t>(row) * teams.row.columns + column);
+        value.stream_to(grad_table + static_cast<size_t>(row) * teams.row.columns + column);
     };
     bool many = false;
     for (int32_t row = row0 + mine; row < row_end; row += teams.teams) {

@@ -137,9 +137,9 @@ __global__ __launch_bounds__(THREADS_OF<TEAM>) void forward_kernel(Forward<T> f)
         Row block[P], residual[P], gate[P];
 #pragma unroll
         for (int p = 0; p < P; p++) {
-            block[p] = Row::load(f.block + begin + column.at[p]);
-            residual[p] = Row::load(f.residual + begin + column.at[p]);
-            gate[p] = f.gate_per_row ? Row::load(f.gate + begin + column.at[p]) : shared_gate[p];
+            block[p] = Row::stream(f.block + begin + column.at[p]);
+            residual[p] = Row::stream(f.residual + begin + column.at[p]);
+            gate[p] = f.gate_per_row ? Row::stream(f.gate + begin + column.at[p]) : shared_gate[p];
         }
         W sum[1] = {0};
 #pragma unroll
@@ -214,11 +214,11 @@ __global__ __launch_bounds__(THREADS_OF<TEAM>) void gradient_kernel(Gradients<T>
 #pragma unroll
         for (int p = 0; p < P; p++) {
             const size_t at = begin + column.at[p];
-            block[p] = Row::load(g.block + at);
-            residual[p] = Row::load(g.residual + at);
-            gate[p] = g.gate_per_row ? Row::load(g.gate + at) : shared_gate[p];
-            grad_state[p] = g.grad_state != nullptr ? Row::load(g.grad_state + at) : Row{};
-            grad_next[p] = g.grad_next != nullptr ? Row::load(g.grad_next + at) : Row{};
+            block[p] = Row::stream(g.block + at);
+            residual[p] = Row::stream(g.residual + at);
+            gate[p] = g.gate_per_row ? Row::stream(g.gate + at) : shared_gate[p];
+            grad_state[p] = g.grad_state != nullptr ? Row::stream(g.grad_state + at) : Row{};
+            grad_next[p] = g.grad_next != nullptr ? Row::stream(g.grad_next + at) : Row{};
         }
         W sum[1] = {0};
 #pragma unroll
@@ -274,13 +274,13 @@ __global__ __launch_bounds__(THREADS_OF<TEAM>) void gradient_kernel(Gradients<T>
             if (valid && column.holds(p)) {
                 const size_t at = begin + column.at[p];
                 if (g.grad_residual != nullptr) {
-                    to_residual.store(g.grad_residual + at);
+                    to_residual.stream_to(g.grad_residual + at);
                 }
                 if (g.grad_block != nullptr) {
-                    to_block.store(g.grad_block + at);
+                    to_block.stream_to(g.grad_block + at);
                 }
                 if (g.grad_gate != nullptr) {
-                    to_gate.store(g.grad_gate + at);
+                    to_gate.stream_to(g.grad_gate + at);
                 }
             }
         }

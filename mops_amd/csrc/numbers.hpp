@@ -39,6 +39,13 @@ template <typename T, int N> struct Piece {
         return Piece{*reinterpret_cast<const Vector*>(p)};
     }
     __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<Vector*>(p) = v; }
+    /// The same for memory that is passed over once: caches do not keep it.
+    static __device__ __forceinline__ Piece stream(const T* p) {
+        return Piece{__builtin_nontemporal_load(reinterpret_cast<const Vector*>(p))};
+    }
+    __device__ __forceinline__ void stream_to(T* p) const {
+        __builtin_nontemporal_store(v, reinterpret_cast<Vector*>(p));
+    }
     __device__ __forceinline__ wide_t<T> get(int i) const { return static_cast<wide_t<T>>(v[i]); }
     /// (to nearest, ties to even: the one rounding of a result)
     __device__ __forceinline__ void set(int i, wide_t<T> x) { v[i] = static_cast<T>(x); }
@@ -48,6 +55,8 @@ template <typename T> struct Piece<T, 1> {
 
     static __device__ __forceinline__ Piece load(const T* p) { return Piece{*p}; }
     __device__ __forceinline__ void store(T* p) const { *p = v; }
+    static __device__ __forceinline__ Piece stream(const T* p) { return Piece{*p}; }
+    __device__ __forceinline__ void stream_to(T* p) const { *p = v; }
     __device__ __forceinline__ wide_t<T> get(int) const { return static_cast<wide_t<T>>(v); }
     __device__ __forceinline__ void set(int, wide_t<T> x) { v = static_cast<T>(x); }
 };
