@@ -63,14 +63,17 @@ template <typename T, typename Body> void with_tile(int tile, bool in_place, Bod
                  : body(std::integral_constant<int, 64>{}, two, two, std::false_type{});
     }
 }
-constexpr int DEEP = 8, STAGES = 2;
+constexpr int DEEP = 8;
+// Steps in LDS or on their way there. Small tiles have little to compute per step and more need to be on their way (24 rows,
+// 16 groups, K = 2048, L = 1408, bfloat16: 22.2 us with two, 15.8 with three, 17.0 with four); the others fill LDS with two.
+template <int TILE, bool ALIGNED> constexpr int STAGES_OF = TILE == 64 && ALIGNED ? 3 : 2;
 
 template <typename T, Form FORM> void launch(Product<T> g, int tile, hipStream_t stream) {
     const unsigned workgroups = set_tiles<FORM>(g, tile);
     with_tile<T>(tile, aligned<T, FORM>(g), [&](auto size, auto m, auto n, auto in_place) {
         constexpr int TILE = decltype(size)::value, WM = decltype(m)::value, WN = decltype(n)::value;
         constexpr bool ALIGNED = decltype(in_place)::value;
-        tiles_kernel<T, FORM, TILE, TILE, WM, WN, DEEP, STAGES, ALIGNED><<<workgroups, WM * WN * WAVE, 0, stream>>>(g);
+        tiles_kernel<T, FORM, TILE, TILE, WM, WN, DEEP, STAGES_OF<TILE, ALIGNED>, ALIGNED><<<workgroups, WM * WN * WAVE, 0, stream>>>(g);
     });
     MOPS_HIP_CHECK(hipGetLastError());
 }
@@ -167,7 +170,7 @@ template <typename T> void gradients(Product<T> sums, Product<T> rows, hipStream
         with_tile<T>(of_sums, in_place, [&](auto size, auto m, auto n, auto is_aligned) {
             constexpr int TILE = decltype(size)::value, WM = decltype(m)::value, WN = decltype(n)::value;
             constexpr bool ALIGNED = decltype(is_aligned)::value;
-            gradients_kernel<T, TILE, TILE, WM, WN, DEEP, STAGES, ALIGNED>
+            gradients_kernel<T, TILE, TILE, WM, WN, DEEP, STAGES_OF<TILE, ALIGNED>, ALIGNED>
                 <<<for_sums + for_rows, WM * WN * WAVE, 0, stream>>>(sums, rows, for_sums);
         });
         MOPS_HIP_CHECK(hipGetLastError());
