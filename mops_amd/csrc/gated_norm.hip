@@ -479,8 +479,12 @@ template <typename T> __global__ __launch_bounds__(WIDE_COLUMNS) void wide_sums_
     }
 }
 
-/// body(TEAM, P, N): the lanes per row and pieces per lane that hold a row; false: none does.
-template <typename T, typename Body> bool by_columns(int32_t columns, Body&& body) {
+/// A row has the lanes that its pieces fill, and as few pieces per lane as that takes: rows of up to 1024 pieces fit the registers of 256 or 512 lanes. Gradients of 67 million numbers of
+/// bfloat16: 183 us in rows of 256 (32 lanes; with 64, half of them idle, 307), 187 of 1024 (64 lanes with two pieces),
+/// 191 of 4096 (256 with two), 245 of 8192 (512 with two; 256 with four, one workgroup per compute unit, 290).
+/// body(TEAM, P, N): the lanes per row and pieces per lane that hold a row; false: none does, or it has more than MOST
+/// pieces.
+template <typename T, int MOST, typename Body> bool by_columns(int32_t columns, Body&& body) {
     auto with = [&](auto team, auto pieces, auto width) {
         body(team, pieces, width);
         return true;
@@ -491,6 +495,7 @@ template <typename T, typename Body> bool by_columns(int32_t columns, Body&& bod
     std::integral_constant<int, 2> two;
     std::integral_constant<int, 4> four;
     std::integral_constant<int, 16> lanes16;
+    std::integral_constant<int, 32> lanes32;
     std::integral_constant<int, 64> lanes64;
     std::integral_constant<int, 256> lanes256;
     std::integral_constant<int, 512> lanes512;
@@ -500,6 +505,9 @@ template <typename T, typename Body> bool by_columns(int32_t columns, Body&& bod
     }
     if (pieces <= 16) {
         return with(lanes16, one, n);
+    }
+    if (pieces <= 32) {
+        return with(lanes32, one, n);
     }
     if (pieces <= 64) {
         return with(lanes64, one, n);
@@ -514,10 +522,12 @@ template <typename T, typename Body> bool by_columns(int32_t columns, Body&& bod
         return with(lanes256, two, n);
     }
     if (pieces <= 1024) {
-        return with(lanes256, four, n);
+        return with(lanes512, two, n);
     }
-    if (pieces <= 2048) {
-        return with(lanes512, four, n);
+    if constexpr (MOST >= 2048) {
+        if (pieces <= 2048) {
+            return with(lanes512, four, n);
+        }
     }
     return false;
 }
@@ -529,7 +539,7 @@ unsigned workgroups(int32_t n_rows, int teams, int resident) {
 }
 
 template <typename T> void forward(Forward<T> f, int32_t columns, hipStream_t stream) {
-    const bool held = by_columns<T>(columns, [&](auto team, auto pieces, auto width) {
+    const bool held = by_columns<T, 2048>(columns, [&](auto team, auto pieces, auto width) {
         constexpr int TEAM = decltype(team)::value, P = decltype(pieces)::value, N = decltype(width)::value;
         f.row = PiecesOfRow::make<N>(columns);
         const int resident = 2048 / THREADS_OF<TEAM>;
@@ -554,10 +564,15 @@ void gradients(
         return wants_sums ? align256(static_cast<size_t>(groups) * which * columns * sizeof(wide_t<T>)) : 0;
     };
     unsigned groups = 0;
-    const bool held = by_columns<T>(columns, [&](auto team, auto pieces, auto width) {
+    // (four pieces of eight numbers do not fit the registers with all that the gradients keep of them: 4096 rows of
+    // 16 384 bfloat16 would be 851 us with 768 bytes of spilled registers per lane, number by number they are 587)
+    constexpr int MOST = sizeof(T) == 2 ? 1024 : 2048;
+    const bool held = by_columns<T, MOST>(columns, [&](auto team, auto pieces, auto width) {
         constexpr int TEAM = decltype(team)::value, P = decltype(pieces)::value, N = decltype(width)::value;
         g.row = PiecesOfRow::make<N>(columns);
-        groups = workgroups(g.n_rows, THREADS_OF<TEAM> / TEAM, 1024 / THREADS_OF<TEAM>);
+        // (two workgroups of 256 per compute unit: 16 384 rows of 4096 bfloat16 are 195 us, with three of them, which do
+        // not all fit, 223 us, with four 198)
+        groups = workgroups(g.n_rows, THREADS_OF<TEAM> / TEAM, 512 / THREADS_OF<TEAM>);
         g.sums = wants_sums ? static_cast<wide_t<T>*>(scratch(sums_bytes(groups))) : nullptr;
         gradient_kernel<T, TEAM, P, N><<<groups, THREADS_OF<TEAM>, 0, stream>>>(g);
     });
