@@ -32,7 +32,8 @@ struct RowGroups {
     }
 };
 
-/// A unit of work: up to `step` places of one group. The rows of no group make up a last group of their own
+/// A unit of work: places of one group, OF_ROWS up to `step` of them, OF_GROUPS about as many (PLACES_TOGETHER at a time,
+/// evenly between the group's units). The rows of no group make up a last group of their own
 /// (group = n_groups, as if its places followed each other: place_of).
 struct GroupUnit {
     int32_t group; // -1: there are fewer units
@@ -45,15 +46,18 @@ enum class Units {
     OF_ROWS,  // no unit for an empty group; units of the rows of no group behind all others
     OF_GROUPS // a unit (of no places) for an empty group; none for the rows of no group
 };
+constexpr int32_t PLACES_TOGETHER = 64;
 
 /// Units there are at most.
 inline size_t most_units(int32_t n_rows, int32_t n_groups, int32_t step) {
     return (static_cast<size_t>(n_rows) + step - 1) / step + static_cast<size_t>(n_groups) + 1;
 }
 
-/// The units of a group with `count` places.
+/// The units of a group with `count` places. OF_GROUPS: rounded down, but for the last quarter, so that equal groups do not
+/// all have a unit more than the GPU has room for (200 000 rows of 8 groups, K = 200, L = 320, gradients of the matrices
+/// in float: 374 us; with all fractions rounded up 456).
 template <Units WHICH> __device__ __forceinline__ int32_t units_of(int32_t count, int32_t step) {
-    return max((count + step - 1) / step, WHICH == Units::OF_GROUPS ? 1 : 0);
+    return WHICH == Units::OF_GROUPS ? max((count + step / 4) / step, 1) : (count + step - 1) / step;
 }
 
 /// (the same in all lanes, and known to be)
@@ -101,10 +105,17 @@ public:
                 const int at = __builtin_ctzll(past);
                 const int32_t of_group = __builtin_amdgcn_readlane(units_, at);
                 const int32_t index = unit - (__builtin_amdgcn_readlane(upto_, at) - of_group);
-                const int32_t first = __builtin_amdgcn_readlane(begin_, at) + index * step_;
-                const int32_t left = __builtin_amdgcn_readlane(count_, at) - index * step_;
+                const int32_t begin = __builtin_amdgcn_readlane(begin_, at);
+                const int32_t count = __builtin_amdgcn_readlane(count_, at);
                 const int32_t group = __builtin_amdgcn_readlane(group_, at);
-                return uniform(GroupUnit{group, first, min(left, step_), index, of_group});
+                int32_t first = index * step_, last = first + step_;
+                if (WHICH == Units::OF_GROUPS) {
+                    const int32_t all = (count + PLACES_TOGETHER - 1) / PLACES_TOGETHER;
+                    const int32_t each = all / of_group, more = all % of_group;
+                    first = (index * each + min(index, more)) * PLACES_TOGETHER;
+                    last = first + (each + (index < more ? 1 : 0)) * PLACES_TOGETHER;
+                }
+                return uniform(GroupUnit{group, begin + first, min(last, count) - first, index, of_group});
             }
             unit -= __builtin_amdgcn_readlane(upto_, WAVE - 1);
         }
