@@ -24,13 +24,45 @@ namespace {
 
 unsigned tiles(int32_t size, int tile) { return static_cast<unsigned>(ceil_div(static_cast<size_t>(size), tile)); }
 
-/// Rows of `width` numbers that all begin on 16-byte boundaries.
-template <typename T> bool aligned(const T* data, int32_t width) {
-    return reinterpret_cast<uintptr_t>(data) % 16 == 0 && static_cast<size_t>(width) * sizeof(T) % 16 == 0;
+/// Rows that follow each other, in memory of the caller.
+template <typename T> struct Matrices {
+    const T* data;
+    size_t n_rows;
+    int32_t width;
+
+    /// They all begin on 16-byte boundaries.
+    bool in_place() const {
+        return reinterpret_cast<uintptr_t>(data) % 16 == 0 && static_cast<size_t>(width) * sizeof(T) % 16 == 0;
+    }
+    int32_t pieces() const { return static_cast<int32_t>(ceil_div(static_cast<size_t>(width), PIECE<T>)); }
+    size_t copied_bytes() const { return in_place() ? 0 : align256(n_rows * pieces() * 16); }
+};
+
+/// Whether rows that begin anywhere are copied to rows that begin on 16-byte boundaries before they are multiplied.
+/// Memory that is read at odd addresses costs the caches twice the time, and tiles that take it through registers are
+/// half as fast as those that do not: what a number of operations gains against what the copy costs, at rates measured
+/// on either side. (8192 rows, K = L = 2047, float16: 159 us without, 92 us with the copy; 37102 rows, 25 groups,
+/// K = 3196, L = 533, gradients: 752 and 585 us; where each number is used less often it is not worth it: 50595
+/// rows, K = 14, L = 1818, 80 us as it is.)
+template <typename T> bool worth_copying(size_t bytes, int matrices, double operations) {
+    constexpr double GAIN = sizeof(T) == 2 ? 1.0 / 700 : sizeof(T) == 4 ? 1.0 / 550 : 1.0 / 150; // us per 10^6
+    return bytes > 0 && operations * 1e-6 * GAIN > static_cast<double>(bytes) / 2.5e6 + 4 * matrices;
 }
-template <typename T, Form FORM> bool aligned(const Product<T>& g) {
-    return aligned(g.q, FORM == Form::GRAD_SUMS ? g.m_size : g.k_size) &&
-           aligned(g.p, FORM == Form::GRAD_ROWS ? g.k_size : g.n_size);
+
+/// The rows of `from`: there, or in `room` (which moves on).
+template <typename T> void place(const T*& data, int32_t& stride, const Matrices<T>& from, char*& room, hipStream_t stream) {
+    data = from.data;
+    stride = from.width;
+    if (room != nullptr && !from.in_place()) {
+        T* to = reinterpret_cast<T*>(room);
+        copy_rows_kernel<T><<<static_cast<unsigned>(ceil_div(from.n_rows, COPY_ROWS)), COPY_THREADS, 0, stream>>>(
+            to, from.data, from.n_rows, from.width, from.pieces()
+        );
+        MOPS_HIP_CHECK(hipGetLastError());
+        data = to;
+        stride = from.pieces() * PIECE<T>;
+        room += from.copied_bytes();
+    }
 }
 
 /// The extents of a call's tiles: TILE x TILE numbers.
@@ -70,35 +102,48 @@ template <int TILE, bool ALIGNED> constexpr int STAGES_OF = TILE == 64 && ALIGNE
 
 template <typename T, Form FORM> void launch(Product<T> g, int tile, hipStream_t stream) {
     const unsigned workgroups = set_tiles<FORM>(g, tile);
-    with_tile<T>(tile, aligned<T, FORM>(g), [&](auto size, auto m, auto n, auto in_place) {
+    with_tile<T>(tile, g.in_place, [&](auto size, auto m, auto n, auto in_place) {
         constexpr int TILE = decltype(size)::value, WM = decltype(m)::value, WN = decltype(n)::value;
         constexpr bool ALIGNED = decltype(in_place)::value;
-        tiles_kernel<T, FORM, TILE, TILE, WM, WN, DEEP, STAGES_OF<TILE, ALIGNED>, ALIGNED><<<workgroups, WM * WN * WAVE, 0, stream>>>(g);
+        tiles_kernel<T, FORM, TILE, TILE, WM, WN, DEEP, STAGES_OF<TILE, ALIGNED>, ALIGNED>
+            <<<workgroups, WM * WN * WAVE, 0, stream>>>(g);
     });
     MOPS_HIP_CHECK(hipGetLastError());
 }
 
+/// Whether what tiles of this extent compute beside the result costs less than smaller tiles, which read more: per number
+/// of a tile, 128 take 1.2 times as long as 256, and 64 more than 1.5 times as long as 128. (61709 rows of 30 groups,
+/// K = 2176, L = 320, float16: 135 us in tiles of 128, 162 in tiles of 256; L = 536: 184 and 175; 60000 rows, L = 40, float:
+/// 81 us in tiles of 64, 140 in tiles of 128.)
+bool filled(int tile, int32_t m, int32_t n = 0) {
+    auto covered = [&](int extent) {
+        return static_cast<double>(tiles(m, extent)) * extent * (n > 0 ? static_cast<double>(tiles(n, extent)) * extent : 1);
+    };
+    return covered(tile) <= (tile == 256 ? 1.3 : 1.5) * covered(tile / 2);
+}
+
 /// The tiles of FORWARD and GRAD_ROWS: the largest that keep all compute units busy and, on average, are half full.
-template <typename T, Form FORM> int tile_of_rows(const Product<T>& g) {
+template <typename T> int tile_of_rows(const Product<T>& g) {
     const size_t rows = static_cast<size_t>(g.groups.n_rows), groups = static_cast<size_t>(g.groups.n_groups);
     const size_t units = static_cast<size_t>(compute_units());
     auto fits = [&](int tile) {
-        return ceil_div(rows, tile) * tiles(g.n_size, tile) >= units && rows >= tile / 2 * groups;
+        return ceil_div(rows, tile) * tiles(g.n_size, tile) >= units && rows >= tile / 2 * groups &&
+               filled(tile, g.n_size);
     };
-    return sizeof(T) == 2 && aligned<T, FORM>(g) && fits(256) ? 256 : fits(128) ? 128 : 64;
+    return sizeof(T) == 2 && g.in_place && fits(256) ? 256 : fits(128) ? 128 : 64;
 }
 
 /// The tiles of GRAD_SUMS, and its rows per unit: what every workgroup that the GPU has room for would have if the work
-/// were shared out evenly. Larger groups than that are split, smaller ones are not.
+/// were shared out evenly. Larger groups than that are split (UnitsOfGroups), smaller ones are not.
 template <typename T> int tile_of_sums(Product<T>& g) {
     const size_t rows = static_cast<size_t>(std::max(g.groups.n_rows, 1)), groups = static_cast<size_t>(g.groups.n_groups);
     const size_t units = static_cast<size_t>(compute_units());
     auto of_unit = [&](int tile) { return static_cast<size_t>(tiles(g.m_size, tile)) * tiles(g.n_size, tile); };
     auto fits = [&](int tile) {
-        return g.m_size > tile / 2 && g.n_size > tile / 2 &&
+        return g.m_size > tile / 2 && g.n_size > tile / 2 && filled(tile, g.m_size, g.n_size) &&
                of_unit(tile) * std::max(groups, ceil_div(rows, 8 * tile)) >= units;
     };
-    const int tile = sizeof(T) == 2 && aligned<T, Form::GRAD_SUMS>(g) && fits(256) ? 256 : fits(128) ? 128 : 64;
+    const int tile = sizeof(T) == 2 && g.in_place && fits(256) ? 256 : fits(128) ? 128 : 64;
     const size_t room = (tile == 256 ? 1 : 2) * units;
     const size_t step = std::max<size_t>(ceil_div(rows * of_unit(tile), room), 256);
     g.step = static_cast<int32_t>(std::min(ceil_div(step, 64) * 64, ceil_div(rows, 64) * 64));
@@ -134,40 +179,78 @@ template <typename T> void join_splits(const Product<T>& g, hipStream_t stream) 
     }
 }
 
-template <typename T> void forward(Product<T> g, hipStream_t stream) {
-    const int tile = tile_of_rows<T, Form::FORWARD>(g);
-    share_k(g, tile);
-    if (g.splits > 1) {
-        g.partial = static_cast<wide_t<T>*>(scratch(split_bytes(g)));
+template <typename T> void forward(Product<T> g, const Matrices<T>& A, const Matrices<T>& W, hipStream_t stream) {
+    size_t copies = A.copied_bytes() + W.copied_bytes();
+    const double operations = 2.0 * A.n_rows * g.k_size * g.n_size;
+    g.in_place = copies == 0;
+    if (worth_copying<T>(copies, !A.in_place() + !W.in_place(), operations) && scratch_ready(copies)) {
+        g.in_place = true;
+    } else {
+        copies = 0;
     }
+    const int tile = tile_of_rows(g);
+    share_k(g, tile);
+    char* room = nullptr;
+    if (copies + split_bytes(g) > 0) {
+        char* workspace = static_cast<char*>(scratch(copies + split_bytes(g)));
+        g.partial = reinterpret_cast<wide_t<T>*>(workspace + copies);
+        room = copies > 0 ? workspace : nullptr;
+    }
+    place(g.q, g.q_stride, A, room, stream);
+    place(g.p, g.p_stride, W, room, stream);
     launch<T, Form::FORWARD>(g, tile, stream);
     join_splits(g, stream);
 }
 
 /// Either may be without an `out`: not wanted.
-template <typename T> void gradients(Product<T> sums, Product<T> rows, hipStream_t stream) {
-    const int of_sums = sums.out != nullptr ? tile_of_sums(sums) : 0;
-    const int of_rows = rows.out != nullptr ? tile_of_rows<T, Form::GRAD_ROWS>(rows) : 0;
-    const bool splits = of_sums != 0 && sums.step < sums.groups.n_rows;
-    if (of_rows != 0) {
+template <typename T>
+void gradients(
+    Product<T> sums, Product<T> rows, const Matrices<T>& grad_output, const Matrices<T>& A, const Matrices<T>& W,
+    hipStream_t stream
+) {
+    const bool of_A = rows.out != nullptr, of_W = sums.out != nullptr;
+    size_t copies = grad_output.copied_bytes() + (of_W ? A.copied_bytes() : 0) + (of_A ? W.copied_bytes() : 0);
+    const int matrices = !grad_output.in_place() + (of_W && !A.in_place()) + (of_A && !W.in_place());
+    const double operations = (of_A + of_W) * 2.0 * A.n_rows * A.width * W.width;
+    sums.in_place = grad_output.in_place() && A.in_place();
+    rows.in_place = grad_output.in_place() && W.in_place();
+    if (worth_copying<T>(copies, matrices, operations) && scratch_ready(copies)) {
+        sums.in_place = rows.in_place = true;
+    } else {
+        copies = 0;
+    }
+    const int of_sums = of_W ? tile_of_sums(sums) : 0;
+    const int of_rows = of_A ? tile_of_rows(rows) : 0;
+    const bool splits = of_W && sums.step < sums.groups.n_rows;
+    if (of_A) {
         share_k(rows, of_rows);
     }
-    const size_t row_bytes = of_rows != 0 ? split_bytes(rows) : 0;
+    const size_t row_bytes = of_A ? split_bytes(rows) : 0;
     size_t sum_bytes = 0;
     if (splits) {
         const size_t most = most_units(sums.groups.n_rows, sums.groups.n_groups, sums.step);
         sum_bytes = most * partial_size(sums.m_size, sums.n_size) * sizeof(wide_t<T>);
     }
-    if (row_bytes + sum_bytes > 0) {
-        char* workspace = static_cast<char*>(scratch(row_bytes + sum_bytes));
-        rows.partial = reinterpret_cast<wide_t<T>*>(workspace);
-        sums.partial = reinterpret_cast<wide_t<T>*>(workspace + row_bytes);
+    char* room = nullptr;
+    if (copies + row_bytes + sum_bytes > 0) {
+        char* workspace = static_cast<char*>(scratch(copies + row_bytes + sum_bytes));
+        rows.partial = reinterpret_cast<wide_t<T>*>(workspace + copies);
+        sums.partial = reinterpret_cast<wide_t<T>*>(workspace + copies + row_bytes);
+        room = copies > 0 ? workspace : nullptr;
     }
-    const bool in_place = of_sums != 0 && aligned<T, Form::GRAD_SUMS>(sums);
-    if (of_sums == of_rows && in_place == aligned<T, Form::GRAD_ROWS>(rows)) {
+    place(rows.q, rows.q_stride, grad_output, room, stream);
+    sums.p = rows.q;
+    sums.p_stride = rows.q_stride;
+    if (of_W) {
+        place(sums.q, sums.q_stride, A, room, stream);
+    }
+    if (of_A) {
+        place(rows.p, rows.p_stride, W, room, stream);
+    }
+    if (of_sums == of_rows && sums.in_place == rows.in_place) {
         const unsigned for_sums = set_tiles<Form::GRAD_SUMS>(sums, of_sums);
         const unsigned for_rows = set_tiles<Form::GRAD_ROWS>(rows, of_rows);
-        with_tile<T>(of_sums, in_place, [&](auto size, auto m, auto n, auto is_aligned) {
+        with_tile<T>(of_sums, sums.in_place, [&](auto size, auto m, auto n, auto is_aligned) {
             constexpr int TILE = decltype(size)::value, WM = decltype(m)::value, WN = decltype(n)::value;
             constexpr bool ALIGNED = decltype(is_aligned)::value;
             gradients_kernel<T, TILE, TILE, WM, WN, DEEP, STAGES_OF<TILE, ALIGNED>, ALIGNED>
@@ -175,14 +258,14 @@ template <typename T> void gradients(Product<T> sums, Product<T> rows, hipStream
         });
         MOPS_HIP_CHECK(hipGetLastError());
     } else {
-        if (of_sums != 0) {
+        if (of_W) {
             launch<T, Form::GRAD_SUMS>(sums, of_sums, stream);
         }
-        if (of_rows != 0) {
+        if (of_A) {
             launch<T, Form::GRAD_ROWS>(rows, of_rows, stream);
         }
     }
-    if (of_rows != 0) {
+    if (of_A) {
         join_splits(rows, stream);
     }
     if (splits) {
@@ -242,12 +325,12 @@ void grouped_matrix_product(
         typedef device_t<scalar_t> T;
         grouped_product::Product<T> g{};
         g.out = data_of(output);
-        g.q = data_of(A);
-        g.p = data_of(W);
         g.groups = groups;
         g.n_size = L;
         g.k_size = K;
-        grouped_product::forward(g, current_stream());
+        const grouped_product::Matrices<T> rows{data_of(A), A.shape[0], K};
+        const grouped_product::Matrices<T> matrices{data_of(W), W.shape[0] * W.shape[1], L};
+        grouped_product::forward(g, rows, matrices, current_stream());
     }
     finish_call("grouped_matrix_product");
 }
@@ -276,22 +359,22 @@ void grouped_matrix_product_vjp(
     grouped_product::Product<T> sums{}, rows{};
     if (grad_W.data != nullptr && groups.n_groups > 0 && K > 0 && L > 0) {
         sums.out = data_of(grad_W);
-        sums.q = data_of(A);
-        sums.p = data_of(grad_output);
         sums.groups = groups;
         sums.m_size = K;
         sums.n_size = L;
     }
     if (grad_A.data != nullptr && groups.n_rows > 0 && K > 0) {
         rows.out = data_of(grad_A);
-        rows.q = data_of(grad_output);
-        rows.p = data_of(W);
         rows.groups = groups;
         rows.n_size = K;
         rows.k_size = L;
     }
     if (sums.out != nullptr || rows.out != nullptr) {
-        grouped_product::gradients(sums, rows, current_stream());
+        grouped_product::gradients(
+            sums, rows, grouped_product::Matrices<T>{data_of(grad_output), A.shape[0], L},
+            grouped_product::Matrices<T>{data_of(A), A.shape[0], K},
+            grouped_product::Matrices<T>{data_of(W), W.shape[0] * W.shape[1], L}, current_stream()
+        );
     }
     finish_call("grouped_matrix_product_vjp");
 }

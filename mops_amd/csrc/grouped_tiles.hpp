@@ -56,6 +56,8 @@ template <typename T> struct Product {
     // there are several
     wide_t<T>* partial;
     const T *q, *p;
+    int32_t q_stride, p_stride; // from row to row: their widths, or as much as whole pieces take
+    bool in_place;              // all rows begin on 16-byte boundaries; what a row's last piece has behind it is zero
     RowGroups groups;
     int32_t m_size, n_size, k_size;
     int32_t step;            // places per unit
@@ -455,19 +457,19 @@ __device__ __forceinline__ void make_tile(
         QLoader q;
         PLoader p;
         if constexpr (Q_TURNED) {
-            q.begin(g.q, g.m_size, m0);
+            q.begin(g.q, g.q_stride, m0);
         } else {
-            q.begin(k_size, [&](int i) { return g.q + static_cast<size_t>(rows[i]) * g.k_size + k_begin; });
+            q.begin(k_size, [&](int i) { return g.q + static_cast<size_t>(rows[i]) * g.q_stride + k_begin; });
         }
-        const size_t of_group = static_cast<size_t>(unit.group) * g.k_size * g.n_size;
+        const size_t of_group = static_cast<size_t>(unit.group) * (P_TURNED ? g.k_size : g.n_size) * g.p_stride;
         if constexpr (SUMS) {
-            p.begin(g.p, g.n_size, n0);
+            p.begin(g.p, g.p_stride, n0);
         } else if constexpr (P_TURNED) {
-            p.begin(g.p + of_group + static_cast<size_t>(k_begin) * g.n_size, g.n_size, n0);
+            p.begin(g.p + of_group + static_cast<size_t>(k_begin) * g.p_stride, g.p_stride, n0);
             p.begin_rows();
         } else {
             p.begin(k_size, [&](int i) {
-                return g.p + of_group + static_cast<size_t>(min(n0 + i, g.n_size - 1)) * g.k_size + k_begin;
+                return g.p + of_group + static_cast<size_t>(min(n0 + i, g.n_size - 1)) * g.p_stride + k_begin;
             });
         }
         constexpr int Q_EACH = QLoader::EACH, P_EACH = PLoader::EACH, EACH = Q_EACH + P_EACH;
@@ -740,6 +742,26 @@ __device__ __forceinline__ void make_tile(
         } else {
             put(T(), std::false_type(), row_of(g.out));
         }
+    }
+}
+
+/// The rows of a matrix, each continued with zeros to whole pieces. A workgroup copies COPY_ROWS of them.
+constexpr int COPY_ROWS = 8, COPY_THREADS = 256;
+template <typename T>
+__global__ __launch_bounds__(COPY_THREADS) void copy_rows_kernel(
+    T* __restrict__ to, const T* __restrict__ from, size_t n_rows, int32_t width, int32_t pieces
+) {
+    constexpr int32_t COUNT = Matrix<T>::COUNT;
+    const size_t row0 = static_cast<size_t>(blockIdx.x) * COPY_ROWS;
+    const uint32_t count = static_cast<uint32_t>(min(n_rows - row0, static_cast<size_t>(COPY_ROWS))) * pieces;
+#pragma unroll 4
+    for (uint32_t i = threadIdx.x; i < count; i += COPY_THREADS) {
+        const uint32_t row = i / pieces;
+        const int32_t first = static_cast<int32_t>(i % pieces) * COUNT;
+        const T* at = from + (row0 + row) * width + first;
+        const Numbers<T> numbers =
+            first + COUNT <= width ? load_numbers<T>(at) : load_some_numbers<T>(at, width - first);
+        *reinterpret_cast<Numbers<T>*>(to + ((row0 + row) * pieces + i % pieces) * COUNT) = numbers;
     }
 }
 
