@@ -44,25 +44,25 @@ template <typename T> struct Matrices {
 /// on either side. (8192 rows, K = L = 2047, float16: 159 us without, 92 us with the copy; 37102 rows, 25 groups,
 /// K = 3196, L = 533, gradients: 752 and 585 us; where each number is used less often it is not worth it: 50595
 /// rows, K = 14, L = 1818, 80 us as it is.)
-template <typename T> bool worth_copying(size_t bytes, int matrices, double operations) {
+template <typename T> bool worth_copying(const Matrices<T>& q, const Matrices<T>& p, double operations) {
     constexpr double GAIN = sizeof(T) == 2 ? 1.0 / 700 : sizeof(T) == 4 ? 1.0 / 550 : 1.0 / 150; // us per 10^6
-    return bytes > 0 && operations * 1e-6 * GAIN > static_cast<double>(bytes) / 2.5e6 + 4 * matrices;
+    const double bytes = static_cast<double>(q.copied_bytes() + p.copied_bytes());
+    const int launches = !q.in_place() + !p.in_place();
+    return launches > 0 && operations * 1e-6 * GAIN > bytes / 2.5e6 + 4 * launches;
 }
 
-/// The rows of `from`: there, or in `room` (which moves on).
-template <typename T> void place(const T*& data, int32_t& stride, const Matrices<T>& from, char*& room, hipStream_t stream) {
-    data = from.data;
-    stride = from.width;
-    if (room != nullptr && !from.in_place()) {
-        T* to = reinterpret_cast<T*>(room);
-        copy_rows_kernel<T><<<static_cast<unsigned>(ceil_div(from.n_rows, COPY_ROWS)), COPY_THREADS, 0, stream>>>(
-            to, from.data, from.n_rows, from.width, from.pieces()
-        );
-        MOPS_HIP_CHECK(hipGetLastError());
-        data = to;
-        stride = from.pieces() * PIECE<T>;
-        room += from.copied_bytes();
+/// `matrices` where they are, or their copy in `room` (which moves on).
+template <typename T> Operand<T> place(const Matrices<T>& matrices, char*& room, hipStream_t stream) {
+    if (room == nullptr || matrices.in_place()) {
+        return Operand<T>{matrices.data, matrices.width};
     }
+    T* const to = reinterpret_cast<T*>(room);
+    room += matrices.copied_bytes();
+    copy_rows_kernel<T><<<static_cast<unsigned>(ceil_div(matrices.n_rows, COPY_ROWS)), COPY_THREADS, 0, stream>>>(
+        to, matrices.data, matrices.n_rows, matrices.width, matrices.pieces()
+    );
+    MOPS_HIP_CHECK(hipGetLastError());
+    return Operand<T>{to, matrices.pieces() * PIECE<T>};
 }
 
 /// The extents of a call's tiles: TILE x TILE numbers.
@@ -182,12 +182,9 @@ template <typename T> void join_splits(const Product<T>& g, hipStream_t stream) 
 template <typename T> void forward(Product<T> g, const Matrices<T>& A, const Matrices<T>& W, hipStream_t stream) {
     size_t copies = A.copied_bytes() + W.copied_bytes();
     const double operations = 2.0 * A.n_rows * g.k_size * g.n_size;
-    g.in_place = copies == 0;
-    if (worth_copying<T>(copies, !A.in_place() + !W.in_place(), operations) && scratch_ready(copies)) {
-        g.in_place = true;
-    } else {
-        copies = 0;
-    }
+    const bool copied = worth_copying(A, W, operations) && scratch_ready(copies);
+    g.in_place = copied || copies == 0;
+    copies = copied ? copies : 0;
     const int tile = tile_of_rows(g);
     share_k(g, tile);
     char* room = nullptr;
@@ -196,8 +193,8 @@ template <typename T> void forward(Product<T> g, const Matrices<T>& A, const Mat
         g.partial = reinterpret_cast<wide_t<T>*>(workspace + copies);
         room = copies > 0 ? workspace : nullptr;
     }
-    place(g.q, g.q_stride, A, room, stream);
-    place(g.p, g.p_stride, W, room, stream);
+    g.q = place(A, room, stream);
+    g.p = place(W, room, stream);
     launch<T, Form::FORWARD>(g, tile, stream);
     join_splits(g, stream);
 }
@@ -209,16 +206,18 @@ void gradients(
     hipStream_t stream
 ) {
     const bool of_A = rows.out != nullptr, of_W = sums.out != nullptr;
-    size_t copies = grad_output.copied_bytes() + (of_W ? A.copied_bytes() : 0) + (of_A ? W.copied_bytes() : 0);
-    const int matrices = !grad_output.in_place() + (of_W && !A.in_place()) + (of_A && !W.in_place());
-    const double operations = (of_A + of_W) * 2.0 * A.n_rows * A.width * W.width;
-    sums.in_place = grad_output.in_place() && A.in_place();
-    rows.in_place = grad_output.in_place() && W.in_place();
-    if (worth_copying<T>(copies, matrices, operations) && scratch_ready(copies)) {
-        sums.in_place = rows.in_place = true;
-    } else {
+    // (each as if it were wanted alone: its result does not depend on whether the other one is)
+    const double operations = 2.0 * A.n_rows * A.width * W.width;
+    bool copies_W = of_A && worth_copying(grad_output, W, operations);
+    bool copies_A = of_W && worth_copying(A, grad_output, operations);
+    size_t copies = (copies_A ? A.copied_bytes() : 0) + (copies_W ? W.copied_bytes() : 0) +
+                    (copies_A || copies_W ? grad_output.copied_bytes() : 0);
+    if (!scratch_ready(copies)) {
+        copies_A = copies_W = false;
         copies = 0;
     }
+    sums.in_place = copies_A || (grad_output.in_place() && A.in_place());
+    rows.in_place = copies_W || (grad_output.in_place() && W.in_place());
     const int of_sums = of_W ? tile_of_sums(sums) : 0;
     const int of_rows = of_A ? tile_of_rows(rows) : 0;
     const bool splits = of_W && sums.step < sums.groups.n_rows;
@@ -238,15 +237,13 @@ void gradients(
         sums.partial = reinterpret_cast<wide_t<T>*>(workspace + copies + row_bytes);
         room = copies > 0 ? workspace : nullptr;
     }
-    place(rows.q, rows.q_stride, grad_output, room, stream);
-    sums.p = rows.q;
-    sums.p_stride = rows.q_stride;
-    if (of_W) {
-        place(sums.q, sums.q_stride, A, room, stream);
-    }
-    if (of_A) {
-        place(rows.p, rows.p_stride, W, room, stream);
-    }
+    char* none = nullptr;
+    const Operand<T> copied = place(grad_output, room, stream);
+    const Operand<T> original = place(grad_output, none, stream);
+    sums.p = copies_A ? copied : original;
+    rows.q = copies_W ? copied : original;
+    sums.q = place(A, copies_A ? room : none, stream);
+    rows.p = place(W, copies_W ? room : none, stream);
     if (of_sums == of_rows && sums.in_place == rows.in_place) {
         const unsigned for_sums = set_tiles<Form::GRAD_SUMS>(sums, of_sums);
         const unsigned for_rows = set_tiles<Form::GRAD_ROWS>(rows, of_rows);

@@ -48,6 +48,12 @@ namespace mops::amd::grouped_product {
 
 enum class Form { FORWARD, GRAD_ROWS, GRAD_SUMS };
 
+/// Rows in memory: `stride` numbers from one to the next, their width or as much as whole pieces take.
+template <typename T> struct Operand {
+    const T* data;
+    int32_t stride;
+};
+
 /// The operands of a launch. FORWARD and GRAD_ROWS: q is [rows][k_size], p the matrices of all groups; GRAD_SUMS: q is
 /// [rows][m_size], p is [rows][n_size].
 template <typename T> struct Product {
@@ -55,9 +61,8 @@ template <typename T> struct Product {
     // GRAD_SUMS: [unit][partial_size(m_size, n_size)], for groups of more than one unit; else [split][row][n_size], where
     // there are several
     wide_t<T>* partial;
-    const T *q, *p;
-    int32_t q_stride, p_stride; // from row to row: their widths, or as much as whole pieces take
-    bool in_place;              // all rows begin on 16-byte boundaries; what a row's last piece has behind it is zero
+    Operand<T> q, p;
+    bool in_place; // all rows begin on 16-byte boundaries and have whole pieces, with zeros behind their numbers
     RowGroups groups;
     int32_t m_size, n_size, k_size;
     int32_t step;            // places per unit
@@ -457,19 +462,19 @@ __device__ __forceinline__ void make_tile(
         QLoader q;
         PLoader p;
         if constexpr (Q_TURNED) {
-            q.begin(g.q, g.q_stride, m0);
+            q.begin(g.q.data, g.q.stride, m0);
         } else {
-            q.begin(k_size, [&](int i) { return g.q + static_cast<size_t>(rows[i]) * g.q_stride + k_begin; });
+            q.begin(k_size, [&](int i) { return g.q.data + static_cast<size_t>(rows[i]) * g.q.stride + k_begin; });
         }
-        const size_t of_group = static_cast<size_t>(unit.group) * (P_TURNED ? g.k_size : g.n_size) * g.p_stride;
+        const size_t of_group = static_cast<size_t>(unit.group) * (P_TURNED ? g.k_size : g.n_size) * g.p.stride;
         if constexpr (SUMS) {
-            p.begin(g.p, g.p_stride, n0);
+            p.begin(g.p.data, g.p.stride, n0);
         } else if constexpr (P_TURNED) {
-            p.begin(g.p + of_group + static_cast<size_t>(k_begin) * g.p_stride, g.p_stride, n0);
+            p.begin(g.p.data + of_group + static_cast<size_t>(k_begin) * g.p.stride, g.p.stride, n0);
             p.begin_rows();
         } else {
             p.begin(k_size, [&](int i) {
-                return g.p + of_group + static_cast<size_t>(min(n0 + i, g.n_size - 1)) * g.p_stride + k_begin;
+                return g.p.data + of_group + static_cast<size_t>(min(n0 + i, g.n_size - 1)) * g.p.stride + k_begin;
             });
         }
         constexpr int Q_EACH = QLoader::EACH, P_EACH = PLoader::EACH, EACH = Q_EACH + P_EACH;

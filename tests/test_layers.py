@@ -160,6 +160,7 @@ LARGE_PRODUCTS = [
     (5000, 20, 1040, 1032, "uniform", False), (30000, 2, 64, 64, "frequent", False),
     (6000, 130, 70, 90, "frequent", True), (9000, 200, 256, 256, "uniform", True),
     (40000, 2, 130, 514, "padded", True), (4500, 3, 515, 777, "frequent", False), (70000, 3, 5, 3, "uniform", True),
+    (7000, 2, 1031, 1029, "padded", True), (9001, 3, 1020, 1101, "uniform", False), (9001, 2, 1101, 1024, "padded", True),
 ]  # fmt: skip
 
 
