@@ -52,9 +52,10 @@ template <size_t N> struct Inputs {
                 t.dim() != kinds[i].dimensions || !t.is_contiguous()) {
                 return false;
             }
-            if (i == 0 && !(layers ? is_layer_dtype(t.scalar_type())
-                                   : t.scalar_type() == at::kFloat || t.scalar_type() == at::kDouble)) {
-                return false; // (the first tensor of every function is a floating-point one)
+            if (i == 0 && !(kinds[0].index ? t.scalar_type() == at::kInt
+                            : layers       ? is_layer_dtype(t.scalar_type())
+                                           : t.scalar_type() == at::kFloat || t.scalar_type() == at::kDouble)) {
+                return false; // (the first tensor of every function with values is a floating-point one)
             }
             if (i > 0 && (t.device() != tensor[0]->device() ||
                           t.scalar_type() != (kinds[i].index ? at::kInt : tensor[0]->scalar_type()))) {
@@ -99,6 +100,10 @@ struct OfOperations {
 };
 struct OfLayers {
     template <typename Call> static void with(const at::Tensor& like, Call&& call) { by_layer_dtype(like, call); }
+};
+
+struct OfIndices {
+    template <typename Call> static void with(const at::Tensor&, Call&& call) { call(int32_t()); }
 };
 
 /// outputs(), then call(zero of the element type, outputs) on the tensors' stream and without the
@@ -404,6 +409,22 @@ bool number(PyObject* object, double& value) {
     return true;
 }
 
+PyObject* order_by_group(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
+    Inputs<1> t; // indices
+    int64_t groups;
+    if (n != 2 || !t.take(arguments, {I1}) || !size_of(arguments[1], groups)) {
+        Py_RETURN_NONE;
+    }
+    return run<OfIndices>(
+        t[0], [&] { return std::array<at::Tensor, 2>{new_like(t[0]), new_tensor({groups + 1}, t[0])}; },
+        [&](int32_t, auto& out) {
+            mops::cuda::order_by_group(
+                view<int32_t, 1>(out[0], "order"), view<int32_t, 1>(out[1], "offsets"), view<int32_t, 1>(t[0], "indices")
+            );
+        }
+    );
+}
+
 PyObject* scaled_embedding(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
     Inputs<2> t; // table indices
     double scale;
@@ -540,6 +561,7 @@ PyMethodDef METHODS[] = {
     MOPS_METHOD("outer_product_scatter_add_with_weights_vjp", opsaw_vjp),
     MOPS_METHOD("sparse_accumulation_scatter_add_with_weights", sasaw),
     MOPS_METHOD("sparse_accumulation_scatter_add_with_weights_vjp", sasaw_vjp),
+    MOPS_METHOD("order_by_group", order_by_group),
     MOPS_METHOD("scaled_embedding", scaled_embedding),
     MOPS_METHOD("scaled_embedding_vjp", scaled_embedding_vjp),
     MOPS_METHOD("grouped_matrix_product", grouped_matrix_product),

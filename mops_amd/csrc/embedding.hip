@@ -36,6 +36,7 @@ constexpr int32_t CHUNK_PLACES = 64;
 constexpr int32_t ALONE = 64;       // places that a team sums up by itself
 constexpr int32_t FEW = 16;         // rows per table row from which on a workgroup has one table row
 constexpr int32_t ROWS_PER_TEAM = 8; // at most
+constexpr int32_t TABLE_ROWS = 1024; // of a workgroup, at most
 
 /// How a row's pieces are shared out: `team` lanes (a power of two) hold a piece each.
 struct Teams {
@@ -146,10 +147,17 @@ __device__ __forceinline__ void add_rows(
     }
 }
 
-/// sum[j] of all teams, in the registers of team 0. All threads.
+/// sum[j] of all teams, in the registers of team 0. All threads. (Teams of a wavefront in six steps, the wavefronts one
+/// after the other: 4096 rows, 64 table rows, 8 columns of float16: JOIN1 us, with all 256 teams one after the other 36.)
 template <typename W, int N> __device__ __forceinline__ void join_teams(W (&sum)[N], W* joined, const Teams& teams) {
     if (teams.teams == 1) {
         return;
+    }
+    for (int32_t step = teams.team; step < WAVE; step *= 2) {
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            sum[j] += __shfl_xor(sum[j], step);
+        }
     }
 #pragma unroll
     for (int j = 0; j < N; j++) {
@@ -157,10 +165,10 @@ template <typename W, int N> __device__ __forceinline__ void join_teams(W (&sum)
     }
     __syncthreads();
     if (static_cast<int32_t>(threadIdx.x) < teams.team) {
-        for (int32_t t = 1; t < teams.teams; t++) {
+        for (int32_t t = max(teams.team, WAVE); t < THREADS; t += max(teams.team, WAVE)) {
 #pragma unroll
             for (int j = 0; j < N; j++) {
-                sum[j] += joined[j * THREADS + t * teams.team + threadIdx.x];
+                sum[j] += joined[j * THREADS + t + threadIdx.x];
             }
         }
     }
@@ -203,8 +211,8 @@ __global__ __launch_bounds__(THREADS) void chunk_kernel(
 /// `alone`), all teams together where many do. places[v - row0]: the first place of row v in `order`, which has n_places.
 template <typename T, int N>
 __device__ __forceinline__ void sum_table_rows(
-    wide_t<T>* joined, T* __restrict__ grad_table, const T* __restrict__ grad_output, const wide_t<T>* __restrict__ partial,
-    const int32_t* order, const int32_t* places, int32_t n_places, int32_t n_rows, int32_t row0, int32_t row_end,
+    wide_t<T>* joined, int32_t* many, T* __restrict__ grad_table, const T* __restrict__ grad_output,
+    const wide_t<T>* __restrict__ partial, const int32_t* order, const int32_t* places, int32_t n_places, int32_t n_rows, int32_t row0, int32_t row_end,
     const Teams& teams, int32_t chunk, int32_t alone, wide_t<T> scale
 ) {
     const int32_t piece = blockIdx.y * teams.team + (threadIdx.x & (teams.team - 1));
@@ -219,11 +227,16 @@ __device__ __forceinline__ void sum_table_rows(
         }
         value.stream_to(grad_table + static_cast<size_t>(row) * teams.row.columns + column);
     };
-    bool many = false;
+    if (threadIdx.x == 0) {
+        many[0] = 0;
+    }
+    __syncthreads();
     for (int32_t row = row0 + mine; row < row_end; row += teams.teams) {
         const int32_t begin = max(places[row - row0], 0), end = min(places[row - row0 + 1], n_places);
         if (end - begin > alone) {
-            many = true;
+            if ((threadIdx.x & (teams.team - 1)) == 0) {
+                many[1 + atomicAdd(&many[0], 1)] = row; // (in any order: each is summed up by itself)
+            }
         } else {
             wide_t<T> sum[N] = {};
             add_rows<T, N>(sum, grad_output, order, n_rows, begin, end, 1, teams.row.columns, column, teams.team);
@@ -232,14 +245,11 @@ __device__ __forceinline__ void sum_table_rows(
             }
         }
     }
-    if (!__syncthreads_or(many)) {
-        return;
-    }
-    for (int32_t row = row0; row < row_end; row++) {
+    __syncthreads();
+    const int32_t n_many = many[0];
+    for (int32_t m = 0; m < n_many; m++) { // (uniform)
+        const int32_t row = many[1 + m];
         const int32_t begin = max(places[row - row0], 0), end = min(places[row - row0 + 1], n_places);
-        if (end - begin <= alone) { // (uniform)
-            continue;
-        }
         wide_t<T> sum[N] = {};
         const int32_t first_chunk = (begin + chunk - 1) / chunk, past_chunk = end / chunk;
         const bool chunks = partial != nullptr && first_chunk < past_chunk;
@@ -287,9 +297,10 @@ __global__ __launch_bounds__(THREADS) void gradient_kernel(
     Teams teams, int32_t chunk, int32_t each, int32_t alone, wide_t<T> scale
 ) {
     __shared__ wide_t<T> joined[N * THREADS];
+    __shared__ int32_t many[TABLE_ROWS + 1];
     const int32_t row0 = blockIdx.x * each, row_end = min(row0 + each, table_rows);
     sum_table_rows<T, N>(
-        joined, grad_table, grad_output, partial, order, offsets + row0, n_rows, n_rows, row0, row_end, teams, chunk,
+        joined, many, grad_table, grad_output, partial, order, offsets + row0, n_rows, n_rows, row0, row_end, teams, chunk,
         alone, scale
     );
 }
@@ -297,7 +308,6 @@ __global__ __launch_bounds__(THREADS) void gradient_kernel(
 /// The same for at most THREADS rows, without an order in memory: every workgroup looks at all indices and puts the rows
 /// that name its part of the table in order in LDS. One launch instead of three or four (10 rows, 5 table rows: 9.9 us
 /// with the sort).
-constexpr int32_t FEW_TABLE_ROWS = 1024; // of a workgroup, at most
 template <typename T, int N>
 __global__ __launch_bounds__(THREADS) void few_rows_kernel(
     T* __restrict__ grad_table, const T* __restrict__ grad_output, const int32_t* __restrict__ indices, int32_t n_rows,
@@ -305,7 +315,7 @@ __global__ __launch_bounds__(THREADS) void few_rows_kernel(
 ) {
     constexpr int WAVES = THREADS / WAVE;
     __shared__ wide_t<T> joined[N * THREADS];
-    __shared__ int32_t places[FEW_TABLE_ROWS + 1], key[THREADS], order[THREADS], of_wave[WAVES];
+    __shared__ int32_t many[TABLE_ROWS + 1], places[TABLE_ROWS + 1], key[THREADS], order[THREADS], of_wave[WAVES];
     const int32_t row0 = blockIdx.x * each, row_end = min(row0 + each, table_rows), tid = threadIdx.x;
     for (int32_t i = tid; i <= each; i += THREADS) {
         places[i] = 0;
@@ -331,7 +341,7 @@ __global__ __launch_bounds__(THREADS) void few_rows_kernel(
     }
     __syncthreads();
     sum_table_rows<T, N>(
-        joined, grad_table, grad_output, nullptr, order, places, listed, n_rows, row0, row_end, teams, 1, alone, scale
+        joined, many, grad_table, grad_output, nullptr, order, places, listed, n_rows, row0, row_end, teams, 1, alone, scale
     );
 }
 
@@ -383,8 +393,8 @@ void gradient(
         const Teams teams = Teams::make<N>(columns);
         auto rows_each = [&](const Teams& t) {
             const size_t by_team = static_cast<size_t>(table_rows) * t.tiles / t.teams;
-            return static_cast<size_t>(many ? 1 : t.teams) *
-                   std::min<size_t>(ROWS_PER_TEAM, many ? 1 : std::max<size_t>(by_team / (8 * units), 1));
+            return many ? size_t(1)
+                        : std::min<size_t>(t.teams * std::clamp<size_t>(by_team / (8 * units), 1, ROWS_PER_TEAM), TABLE_ROWS);
         };
         // few workgroups: fewer columns in each of more
         Teams summing = teams;
@@ -454,7 +464,8 @@ void order_by_group(Tensor<int32_t, 1> order, Tensor<int32_t, 1> offsets, Tensor
     }
     const int32_t n_rows = count_i32(indices.shape[0], "number of rows");
     const int32_t groups = count_i32(offsets.shape[0], "number of groups + 1") - 1;
-    void* workspace = n_rows > 0 ? scratch(order_all_by_group_bytes(groups, n_rows)) : nullptr;
+    const size_t bytes = n_rows > 0 ? order_all_by_group_bytes(groups, n_rows) : 0;
+    void* workspace = bytes > 0 ? scratch(bytes) : nullptr;
     order_all_by_group(order.data, offsets.data, indices.data, n_rows, groups, workspace, current_stream());
     finish_call("order_by_group");
 }

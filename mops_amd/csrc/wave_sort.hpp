@@ -103,6 +103,9 @@ __device__ __forceinline__ void place_keys(
     int32_t* mine = counters + static_cast<size_t>(wave) * keys;
     auto place_one = [&](const Item& item, int32_t at) {
         const bool valid = at < share.end && item.key >= 0;
+        if (!__any(valid)) {
+            return; // (uniform)
+        }
         const Ranked ranked = rank_in_wave(item.key, valid, bits, lane);
         const int32_t place = valid ? mine[item.key] + static_cast<int32_t>(ranked.before) : 0;
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");

@@ -149,6 +149,9 @@ def order_by_group(indices, n_groups):
     is outside ``[0, n_groups)`` (negative: padding) come last and belong to no group. One plan per batch serves
     ``grouped_matrix_product`` in every layer and the gradient of ``scaled_embedding``.
     """
+    result = _native.order_by_group(indices, n_groups)
+    if result is not None:
+        return result
     function = "order_by_group"
     _check_tensors_index(function, indices)
     check_scalar(n_groups, function, "n_groups")

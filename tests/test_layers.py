@@ -75,7 +75,7 @@ def plan_of(index, groups):
 @pytest.mark.parametrize(
     "rows,groups",
     [(0, 5), (1, 1), (7, 3), (1000, 1), (5000, 94), (4097, 511), (4097, 512), (9000, 5000), (70001, 100003),
-     (300000, 7), (200, 3000000)],
+     (300000, 7), (200, 3000000), (4096, 511), (4097, 64), (16384, 600), (16385, 600), (3001, 70000), (900, 20)],
 )  # fmt: skip
 def test_order_by_group(device, rows, groups, kind):
     index = indices_of(kind, rows, groups)
@@ -98,6 +98,7 @@ EMBEDDINGS = [
     (0, 5, 8, "uniform"), (1, 1, 1, "uniform"), (3, 4, 7, "padded"), (33, 10, 16, "uniform"), (65, 100, 3, "frequent"),
     (600, 4, 128, "uniform"), (5000, 94, 64, "frequent"), (700, 5000, 513, "frequent"), (129, 3, 2049, "one"),
     (3000, 2, 130, "padded"), (500, 40, 4099, "nowhere"), (20000, 5, 9, "one"), (1500, 7, 5000, "frequent"),
+    (200, 3000000, 1, "uniform"), (50000, 60000, 8, "frequent"), (4096, 64, 8, "uniform"), (40000, 30000, 40, "frequent"),
 ]  # fmt: skip
 
 
