@@ -148,7 +148,7 @@ __device__ __forceinline__ void add_rows(
 }
 
 /// sum[j] of all teams, in the registers of team 0. All threads. (Teams of a wavefront in six steps, the wavefronts one
-/// after the other: 4096 rows, 64 table rows, 8 columns of float16: JOIN1 us, with all 256 teams one after the other 36.)
+/// after the other: 4096 rows, 64 table rows, 8 columns of float16: 15 us, with all 256 teams one after the other 36.)
 template <typename W, int N> __device__ __forceinline__ void join_teams(W (&sum)[N], W* joined, const Teams& teams) {
     if (teams.teams == 1) {
         return;
@@ -207,50 +207,49 @@ __global__ __launch_bounds__(THREADS) void chunk_kernel(
     }
 }
 
-/// Rows row0 .. row_end - 1 of the gradient, by a workgroup: a team per row of the table where few rows name it (at most
-/// `alone`), all teams together where many do. places[v - row0]: the first place of row v in `order`, which has n_places.
-template <typename T, int N>
-__device__ __forceinline__ void sum_table_rows(
-    wide_t<T>* joined, int32_t* many, T* __restrict__ grad_table, const T* __restrict__ grad_output,
-    const wide_t<T>* __restrict__ partial, const int32_t* order, const int32_t* places, int32_t n_places, int32_t n_rows, int32_t row0, int32_t row_end,
-    const Teams& teams, int32_t chunk, int32_t alone, wide_t<T> scale
-) {
-    const int32_t piece = blockIdx.y * teams.team + (threadIdx.x & (teams.team - 1));
-    const bool holds = piece < teams.row.pieces;
-    const int32_t column = teams.row.start<N>(min(piece, teams.row.pieces - 1));
-    const int32_t mine = threadIdx.x / teams.team;
-    auto store = [&](int32_t row, const wide_t<T>(&sum)[N]) {
+/// The gradient's rows, as a workgroup makes them.
+template <typename T, int N> struct TableRows {
+    typedef wide_t<T> W;
+    T* grad_table;
+    const T* grad_output;
+    const W* partial; // (null: none)
+    const int32_t* order;
+    int32_t n_rows, chunk;
+    const Teams& teams;
+    W scale;
+    bool holds;     // the lane has a piece of the row
+    int32_t column, mine;
+
+    __device__ __forceinline__ TableRows(
+        T* grad_table, const T* grad_output, const W* partial, const int32_t* order, int32_t n_rows, int32_t chunk,
+        const Teams& teams, W scale
+    ) : grad_table(grad_table), grad_output(grad_output), partial(partial), order(order), n_rows(n_rows), chunk(chunk),
+        teams(teams), scale(scale) {
+        const int32_t piece = blockIdx.y * teams.team + (threadIdx.x & (teams.team - 1));
+        holds = piece < teams.row.pieces;
+        column = teams.row.start<N>(min(piece, teams.row.pieces - 1));
+        mine = threadIdx.x / teams.team;
+    }
+
+    __device__ __forceinline__ void store(int32_t row, const W (&sum)[N]) const {
         Piece<T, N> value;
 #pragma unroll
         for (int j = 0; j < N; j++) {
             value.set(j, scale * sum[j]);
         }
         value.stream_to(grad_table + static_cast<size_t>(row) * teams.row.columns + column);
-    };
-    if (threadIdx.x == 0) {
-        many[0] = 0;
     }
-    __syncthreads();
-    for (int32_t row = row0 + mine; row < row_end; row += teams.teams) {
-        const int32_t begin = max(places[row - row0], 0), end = min(places[row - row0 + 1], n_places);
-        if (end - begin > alone) {
-            if ((threadIdx.x & (teams.team - 1)) == 0) {
-                many[1 + atomicAdd(&many[0], 1)] = row; // (in any order: each is summed up by itself)
-            }
-        } else {
-            wide_t<T> sum[N] = {};
-            add_rows<T, N>(sum, grad_output, order, n_rows, begin, end, 1, teams.row.columns, column, teams.team);
-            if (holds) {
-                store(row, sum);
-            }
+    /// Row `row`, which has the places begin .. end - 1, by the team alone.
+    __device__ __forceinline__ void by_team(int32_t row, int32_t begin, int32_t end) const {
+        W sum[N] = {};
+        add_rows<T, N>(sum, grad_output, order, n_rows, begin, end, 1, teams.row.columns, column, teams.team);
+        if (holds) {
+            store(row, sum);
         }
     }
-    __syncthreads();
-    const int32_t n_many = many[0];
-    for (int32_t m = 0; m < n_many; m++) { // (uniform)
-        const int32_t row = many[1 + m];
-        const int32_t begin = max(places[row - row0], 0), end = min(places[row - row0 + 1], n_places);
-        wide_t<T> sum[N] = {};
+    /// The same by all teams of the workgroup, with the sums of the chunks that lie inside.
+    __device__ __forceinline__ void by_all(W* joined, int32_t row, int32_t begin, int32_t end) const {
+        W sum[N] = {};
         const int32_t first_chunk = (begin + chunk - 1) / chunk, past_chunk = end / chunk;
         const bool chunks = partial != nullptr && first_chunk < past_chunk;
         add_rows<T, N>(
@@ -259,7 +258,7 @@ __device__ __forceinline__ void sum_table_rows(
         );
         if (chunks) {
             for (int32_t c = first_chunk + mine; c < past_chunk; c += AHEAD * teams.teams) {
-                wide_t<T> value[AHEAD][N];
+                W value[AHEAD][N];
 #pragma unroll
                 for (int u = 0; u < AHEAD; u++) {
                     const size_t from = min(c + u * teams.teams, past_chunk - 1);
@@ -283,26 +282,51 @@ __device__ __forceinline__ void sum_table_rows(
                 teams.team
             );
         }
-        join_teams<wide_t<T>, N>(sum, joined, teams);
+        join_teams<W, N>(sum, joined, teams);
         if (mine == 0 && holds) {
             store(row, sum);
         }
     }
-}
+};
 
-template <typename T, int N>
+/// ONE_EACH: a workgroup per row of the table. Else workgroups that have `each` rows of it, a team per row, and in front of
+/// them ceil(n_rows / ALONE) others for the rows of more than ALONE places: the places of such a row include a multiple of
+/// ALONE, and the workgroup of the first one makes it. (The most frequent ones are often neighbours. 44 721 rows of
+/// 33 749, 223 columns, float16: 26 us with a plan; 72 where the workgroup that has them makes them one after the other.)
+template <typename T, int N, bool ONE_EACH>
 __global__ __launch_bounds__(THREADS) void gradient_kernel(
     T* __restrict__ grad_table, const T* __restrict__ grad_output, const wide_t<T>* __restrict__ partial,
-    const int32_t* __restrict__ order, const int32_t* __restrict__ offsets, int32_t n_rows, int32_t table_rows,
-    Teams teams, int32_t chunk, int32_t each, int32_t alone, wide_t<T> scale
+    const int32_t* __restrict__ indices, const int32_t* __restrict__ order, const int32_t* __restrict__ offsets,
+    int32_t n_rows, int32_t table_rows, Teams teams, int32_t chunk, int32_t each, wide_t<T> scale
 ) {
     __shared__ wide_t<T> joined[N * THREADS];
-    __shared__ int32_t many[TABLE_ROWS + 1];
-    const int32_t row0 = blockIdx.x * each, row_end = min(row0 + each, table_rows);
-    sum_table_rows<T, N>(
-        joined, many, grad_table, grad_output, partial, order, offsets + row0, n_rows, n_rows, row0, row_end, teams, chunk,
-        alone, scale
-    );
+    const TableRows<T, N> rows(grad_table, grad_output, partial, order, n_rows, chunk, teams, scale);
+    auto begin_of = [&](int32_t row) { return max(offsets[row], 0); };
+    auto end_of = [&](int32_t row) { return min(offsets[row + 1], n_rows); };
+    if (ONE_EACH) {
+        const int32_t row = blockIdx.x;
+        rows.by_all(joined, row, begin_of(row), end_of(row));
+        return;
+    }
+    const int32_t others = (n_rows + ALONE - 1) / ALONE, block = static_cast<int32_t>(blockIdx.x);
+    if (block < others) {
+        const int32_t place = block * ALONE, listed = order[place];
+        const int32_t row = in_bounds(listed, n_rows) ? indices[listed] : -1;
+        if (in_bounds(row, table_rows)) { // (uniform, like the next one)
+            const int32_t begin = begin_of(row), end = end_of(row);
+            if (end - begin > ALONE && (begin + ALONE - 1) / ALONE == block) {
+                rows.by_all(joined, row, begin, end);
+            }
+        }
+        return;
+    }
+    const int32_t row0 = (block - others) * each, row_end = min(row0 + each, table_rows);
+    for (int32_t row = row0 + rows.mine; row < row_end; row += teams.teams) {
+        const int32_t begin = begin_of(row), end = end_of(row);
+        if (end - begin <= ALONE) {
+            rows.by_team(row, begin, end);
+        }
+    }
 }
 
 /// The same for at most THREADS rows, without an order in memory: every workgroup looks at all indices and puts the rows
@@ -311,11 +335,11 @@ __global__ __launch_bounds__(THREADS) void gradient_kernel(
 template <typename T, int N>
 __global__ __launch_bounds__(THREADS) void few_rows_kernel(
     T* __restrict__ grad_table, const T* __restrict__ grad_output, const int32_t* __restrict__ indices, int32_t n_rows,
-    int32_t table_rows, Teams teams, int32_t each, int32_t alone, wide_t<T> scale
+    int32_t table_rows, Teams teams, int32_t each, bool one_each, wide_t<T> scale
 ) {
     constexpr int WAVES = THREADS / WAVE;
     __shared__ wide_t<T> joined[N * THREADS];
-    __shared__ int32_t many[TABLE_ROWS + 1], places[TABLE_ROWS + 1], key[THREADS], order[THREADS], of_wave[WAVES];
+    __shared__ int32_t places[TABLE_ROWS + 1], key[THREADS], order[THREADS], of_wave[WAVES];
     const int32_t row0 = blockIdx.x * each, row_end = min(row0 + each, table_rows), tid = threadIdx.x;
     for (int32_t i = tid; i <= each; i += THREADS) {
         places[i] = 0;
@@ -340,9 +364,14 @@ __global__ __launch_bounds__(THREADS) void few_rows_kernel(
         order[place] = tid;
     }
     __syncthreads();
-    sum_table_rows<T, N>(
-        joined, many, grad_table, grad_output, nullptr, order, places, listed, n_rows, row0, row_end, teams, 1, alone, scale
-    );
+    const TableRows<T, N> rows(grad_table, grad_output, nullptr, order, n_rows, 1, teams, scale);
+    if (one_each) { // (uniform)
+        rows.by_all(joined, row0, places[0], places[1]);
+        return;
+    }
+    for (int32_t row = row0 + rows.mine; row < row_end; row += teams.teams) {
+        rows.by_team(row, places[row - row0], places[row - row0 + 1]);
+    }
 }
 
 /// body(number of columns in a piece): 16 bytes, or single numbers for rows shorter than that.
@@ -389,7 +418,6 @@ void gradient(
         // floats: 73 us for the whole gradient with one row per team), else some per team if there are enough of them,
         // for workgroups that have nothing but zeros to store come and go faster than they are started.
         const bool many = static_cast<size_t>(n_rows) > static_cast<size_t>(table_rows) * FEW;
-        const int32_t alone = many ? 0 : ALONE;
         const Teams teams = Teams::make<N>(columns);
         auto rows_each = [&](const Teams& t) {
             const size_t by_team = static_cast<size_t>(table_rows) * t.tiles / t.teams;
@@ -405,7 +433,7 @@ void gradient(
         const dim3 grid(static_cast<unsigned>(ceil_div(static_cast<size_t>(table_rows), each)), summing.tiles);
         if (n_rows <= THREADS) { // (also where the caller has a plan: reading it would take longer)
             few_rows_kernel<T, N><<<grid, THREADS, 0, stream>>>(
-                grad_table, grad_output, indices, n_rows, table_rows, summing, static_cast<int32_t>(each), alone,
+                grad_table, grad_output, indices, n_rows, table_rows, summing, static_cast<int32_t>(each), many,
                 static_cast<wide_t<T>>(scale)
             );
             return;
@@ -440,10 +468,17 @@ void gradient(
                 partial, grad_output, indices, order, n_rows, table_rows, teams, chunk
             );
         }
-        gradient_kernel<T, N><<<grid, THREADS, 0, stream>>>(
-            grad_table, grad_output, partial, order, offsets, n_rows, table_rows, summing, chunk,
-            static_cast<int32_t>(each), alone, static_cast<wide_t<T>>(scale)
-        );
+        auto launch = [&](auto one_each, dim3 workgroups) {
+            gradient_kernel<T, N, decltype(one_each)::value><<<workgroups, THREADS, 0, stream>>>(
+                grad_table, grad_output, partial, indices, order, offsets, n_rows, table_rows, summing, chunk,
+                static_cast<int32_t>(each), static_cast<wide_t<T>>(scale)
+            );
+        };
+        if (many) {
+            launch(std::true_type{}, grid);
+        } else {
+            launch(std::false_type{}, dim3(grid.x + static_cast<unsigned>(ceil_div(n_rows, ALONE)), grid.y));
+        }
     });
     MOPS_HIP_CHECK(hipGetLastError());
 }
