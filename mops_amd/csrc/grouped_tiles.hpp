@@ -140,12 +140,13 @@ template <typename T> __device__ __forceinline__ Numbers<T> load_numbers(const T
     }
     return v;
 }
-/// The first `count` numbers, zeros behind them.
+/// The first `count` numbers (at least one), zeros behind them.
 template <typename T> __device__ __forceinline__ Numbers<T> load_some_numbers(const T* from, int32_t count) {
     Numbers<T> v;
 #pragma unroll
     for (int i = 0; i < Matrix<T>::COUNT; i++) {
-        v[i] = i < count ? from[i] : static_cast<T>(0.f);
+        const T number = from[min(i, count - 1)];
+        v[i] = i < count ? number : static_cast<T>(0.f);
     }
     return v;
 }
@@ -163,12 +164,11 @@ template <typename T> __device__ __forceinline__ Numbers<T> without_first(Number
     return both.numbers;
 }
 
-/// LDS of a straight side of OUTER rows: [OUTER][DEEP pieces], DEEP 4 or 8, permuted so that 16 lanes that read the same
-/// piece of 16 rows reach all banks.
+/// LDS of a straight side of OUTER rows: [OUTER][DEEP pieces], permuted so that 16 lanes that read the same piece of 16
+/// rows reach all banks.
 template <typename T, int OUTER, int DEEP> struct Straight {
-    static __device__ __forceinline__ int permuted(int row, int piece) {
-        return DEEP == 8 ? piece ^ (row >> 1 & 7) : piece ^ (row >> 2 & 3);
-    }
+    static_assert(DEEP == 8, "pieces of 128 bytes");
+    static __device__ __forceinline__ int permuted(int row, int piece) { return piece ^ (row >> 1 & 7); }
     static __device__ __forceinline__ int place(int row, int piece) { return (row * DEEP + permuted(row, piece)) * 16; }
     /// which piece of its row lies at place i
     static __device__ __forceinline__ int piece(int i) { return permuted(i / DEEP, i % DEEP); }
@@ -240,6 +240,10 @@ __device__ __forceinline__ void fetch(const void* from, char* lds) {
 }
 #pragma clang diagnostic pop
 
+/// How the pieces of a step are loaded to registers. WHOLE: all of them lie inside of their rows, or do not matter. ALL: those
+/// outside as well, from somewhere. SOME: not those.
+enum class Take { WHOLE, ALL, SOME };
+
 /// A side of the product on its way to LDS: piece i = threadIdx.x + j * THREADS, j < EACH. Through registers: SETS steps
 /// are on their way at once, each in a set of registers.
 template <typename T, int OUTER, int DEEP, int THREADS, int SETS> struct Pieces {
@@ -247,23 +251,25 @@ template <typename T, int OUTER, int DEEP, int THREADS, int SETS> struct Pieces 
     static constexpr bool ALIGNED = SETS == 0;
     Numbers<T> piece[ALIGNED ? 1 : SETS][ALIGNED ? 1 : EACH];
 
-    /// piece j of a step: numbers `from` .. of a row, of which `left` are in the row (at most 0: none). WHOLE: all of them
-    /// are, or the side's row does not matter. Through registers, the last piece of a row is the row's last COUNT numbers
-    /// (`short_rows`: there are fewer), of which it drops those of the piece before when it is stored.
-    template <bool WHOLE>
+    /// piece j of a step: numbers `from` .. of a row, of which `left` are in the row (at most 0: none). Through registers,
+    /// the last piece of a row is the row's last COUNT numbers (`short_rows`: there are fewer), of which it drops those of
+    /// the piece before when it is stored.
+    template <Take HOW>
     __device__ __forceinline__ void take(int set, int j, const T* from, int32_t left, bool short_rows, char* lds, int wave) {
+        const void* const nowhere = &zeros_in_memory;
+        const int32_t missing = max(COUNT - left, 0);
         if constexpr (ALIGNED) {
-            const void* at = WHOLE || left > 0 ? static_cast<const void*>(from) : &zeros_in_memory;
-            fetch(at, lds + (wave * WAVE + j * THREADS) * 16);
-        } else if constexpr (WHOLE) {
+            fetch(left > 0 ? static_cast<const void*>(from) : nowhere, lds + (wave * WAVE + j * THREADS) * 16);
+        } else if constexpr (HOW == Take::WHOLE) {
             piece[set][j] = load_numbers<T>(from);
+        } else if constexpr (HOW == Take::ALL) {
+            const T* const any = static_cast<const T*>(nowhere);
+            piece[set][j] = short_rows ? load_some_numbers<T>(left > 0 ? from : any, left > 0 ? left : COUNT)
+                                       : load_numbers<T>(missing < COUNT ? from - missing : any);
         } else if (short_rows) { // (uniform)
-            piece[set][j] = load_some_numbers<T>(from, left);
-        } else {
-            const int32_t missing = min(max(COUNT - left, 0), COUNT);
-            if (missing < COUNT) {
-                piece[set][j] = load_numbers<T>(from - missing);
-            }
+            piece[set][j] = left > 0 ? load_some_numbers<T>(from, left) : Numbers<T>{};
+        } else if (missing < COUNT) {
+            piece[set][j] = load_numbers<T>(from - missing);
         }
     }
     /// a piece that came through registers
@@ -296,11 +302,11 @@ struct StraightLoader : public Pieces<T, OUTER, DEEP, THREADS, SETS> {
         }
     }
     /// Piece j of the next step, which begins at k0 (steps are asked for in order).
-    template <bool WHOLE> __device__ __forceinline__ void load(int set, int j, int32_t k0, char* lds, int wave) {
-        this->template take<WHOLE>(set, j, from[j], k_size - k0 - of_row(j) * COUNT, k_size < COUNT, lds, wave);
+    template <Take HOW> __device__ __forceinline__ void load(int set, int j, int32_t k0, char* lds, int wave) {
+        this->template take<HOW>(set, j, from[j], k_size - k0 - of_row(j) * COUNT, k_size < COUNT, lds, wave);
         from[j] += DEEP * COUNT;
     }
-    /// The pieces of a step that came through registers (`whole`: it was loaded with WHOLE).
+    /// The pieces of a step that came through registers (`whole`: as WHOLE).
     __device__ __forceinline__ void store(int set, int32_t k0, bool whole, char* lds) const {
 #pragma unroll
         for (int j = 0; j < EACH; j++) {
@@ -343,14 +349,14 @@ struct TurnedLoader : public Pieces<T, OUTER, DEEP, THREADS, SETS> {
 
     /// Piece j of the next step of consecutive rows (after begin_rows), of which the matrix has rows_left.
     __device__ __forceinline__ void begin_rows() { from += static_cast<size_t>(k(0)) * (between / K_EACH); }
-    template <bool WHOLE> __device__ __forceinline__ void load(int set, int j, int32_t rows_left, char* lds, int wave) {
-        this->template take<WHOLE>(set, j, from + j * between, k(j) < rows_left ? left : 0, short_rows, lds, wave);
+    template <Take HOW> __device__ __forceinline__ void load(int set, int j, int32_t rows_left, char* lds, int wave) {
+        this->template take<HOW>(set, j, from + j * between, k(j) < rows_left ? left : 0, short_rows, lds, wave);
         from += j == EACH - 1 ? next : 0;
     }
     /// Piece j of a step whose row is `row` there (negative: none; not with WHOLE).
-    template <bool WHOLE> __device__ __forceinline__ void load_row(int set, int j, int32_t row, char* lds, int wave) {
-        const size_t at = static_cast<size_t>(WHOLE ? row : max(row, 0)) * (between / K_EACH);
-        this->template take<WHOLE>(set, j, from + at, row >= 0 ? left : 0, short_rows, lds, wave);
+    template <Take HOW> __device__ __forceinline__ void load_row(int set, int j, int32_t row, char* lds, int wave) {
+        const size_t at = static_cast<size_t>(HOW == Take::WHOLE ? row : max(row, 0)) * (between / K_EACH);
+        this->template take<HOW>(set, j, from + at, row >= 0 ? left : 0, short_rows, lds, wave);
     }
     /// The pieces of a step that came through registers, of a side that has rows_left more rows.
     __device__ __forceinline__ void store(int set, int32_t rows_left, bool whole, char* lds) const {
@@ -387,7 +393,7 @@ __device__ __forceinline__ void make_tile(
     constexpr int MB = BM / WM / BLOCK, NB = BN / WN / BLOCK; // blocks of a wavefront
     constexpr bool SUMS = FORM == Form::GRAD_SUMS, Q_TURNED = SUMS, P_TURNED = FORM != Form::GRAD_ROWS;
     constexpr Units UNITS = SUMS ? Units::OF_GROUPS : Units::OF_ROWS;
-    constexpr int SETS = ALIGNED ? 0 : BM <= 64 ? 3 : sizeof(T) == 8 ? 1 : 2; // (what there is room for in registers)
+    constexpr int SETS = ALIGNED ? 0 : BM > 64 && sizeof(T) == 8 ? 1 : 2; // (what there is room for in registers)
     using QLoader = std::conditional_t<
         Q_TURNED, TurnedLoader<T, BM, DEEP, THREADS, SETS>, StraightLoader<T, BM, DEEP, THREADS, SETS>>;
     using PLoader = std::conditional_t<
@@ -399,7 +405,7 @@ __device__ __forceinline__ void make_tile(
 
     // Workgroups b, b + 8, .. run on the same XCD. Tiles of rows take the same time each: an XCD gets consecutive ones, so
     // that its L2 holds what they share. A unit of GRAD_SUMS takes as long as it has rows: its tiles go to all XCDs (24
-    // uneven groups in consecutive tiles: 122 us instead of 88).
+    // uneven groups, 1280 x 1000, in consecutive tiles: 122 us instead of 115).
     constexpr bool MAY_SPLIT = !SUMS && BM == 64;
     const int32_t splits = MAY_SPLIT ? g.splits : 1;
     const int32_t tiles_of_unit = (SUMS ? g.m_tiles : splits) * g.n_tiles;
@@ -478,34 +484,39 @@ __device__ __forceinline__ void make_tile(
             });
         }
         constexpr int Q_EACH = QLoader::EACH, P_EACH = PLoader::EACH, EACH = Q_EACH + P_EACH;
-        // GRAD_SUMS: the rows behind the pieces of a step
-        [[maybe_unused]] int32_t row_of_piece[SUMS ? EACH : 1];
-        auto find_rows = [&](int32_t k0) {
+        // GRAD_SUMS: the rows behind the pieces of a step, found SETS steps before its pieces are asked for (what waits for
+        // them then waits for no pieces that were asked for later)
+        constexpr int ROW_SETS = ALIGNED ? 1 : SETS;
+        [[maybe_unused]] int32_t row_of_piece[ROW_SETS][SUMS ? EACH : 1];
+        auto find_rows = [&](int set, int32_t k0) {
             if constexpr (SUMS) {
                 auto row_at = [&](int k) { return k0 + k < k_size ? g.groups.row_at(unit.begin + k0 + k) : -1; };
 #pragma unroll
                 for (int j = 0; j < EACH; j++) {
-                    row_of_piece[j] = j >= Q_EACH && QLoader::K_EACH == PLoader::K_EACH
-                                          ? row_of_piece[j - Q_EACH]
-                                          : row_at(j < Q_EACH ? QLoader::k(j) : PLoader::k(j - Q_EACH));
+                    row_of_piece[set][j] = j >= Q_EACH && QLoader::K_EACH == PLoader::K_EACH
+                                               ? row_of_piece[set][j - Q_EACH]
+                                               : row_at(j < Q_EACH ? QLoader::k(j) : PLoader::k(j - Q_EACH));
                 }
             }
         };
         // Piece `piece` of the step that begins at k0 (find_rows of it before).
-        auto load_piece = [&](auto is_whole, int set, int piece, int32_t k0, char* buffer) {
-            constexpr bool WHOLE = decltype(is_whole)::value;
+        auto load_piece = [&](auto take, int set, int piece, int32_t k0, char* buffer) {
+            constexpr Take HOW = decltype(take)::value;
             if constexpr (SUMS) {
                 if (piece < Q_EACH) {
-                    q.template load_row<WHOLE>(set, piece, row_of_piece[piece], buffer, wave);
+                    q.template load_row<HOW>(set, piece, row_of_piece[set][piece], buffer, wave);
                 } else {
-                    p.template load_row<WHOLE>(set, piece - Q_EACH, row_of_piece[piece], buffer + P_AT, wave);
+                    p.template load_row<HOW>(set, piece - Q_EACH, row_of_piece[set][piece], buffer + P_AT, wave);
                 }
             } else if (piece < Q_EACH) {
-                q.template load<WHOLE>(set, piece, k0, buffer, wave);
+                q.template load<HOW>(set, piece, k0, buffer, wave);
             } else {
-                p.template load<WHOLE>(set, piece - Q_EACH, P_TURNED ? k_size - k0 : k0, buffer + P_AT, wave);
+                p.template load<HOW>(set, piece - Q_EACH, P_TURNED ? k_size - k0 : k0, buffer + P_AT, wave);
             }
         };
+        typedef std::integral_constant<Take, Take::WHOLE> Whole;
+        typedef std::integral_constant<Take, Take::ALL> All;
+        typedef std::integral_constant<Take, Take::SOME> Some;
         // through registers, no step but the last one needs to look where the matrices end
         bool whole = true;
         if constexpr (!ALIGNED) {
@@ -521,22 +532,22 @@ __device__ __forceinline__ void make_tile(
 #pragma unroll
             for (int piece = 0; piece < EACH; piece++) {
                 if (piece >= from && piece < upto) {
-                    load_piece(std::false_type(), 0, piece, k0, buffer);
+                    load_piece(Some(), 0, piece, k0, buffer);
                 }
             }
         };
         // through registers: a step from memory to a set of them, and from there to LDS
         auto is_whole = [&](int32_t k0) { return whole && k0 + STEP <= k_size; }; // (uniform)
-        auto load = [&](int set, int32_t k0) {
+        auto load = [&](auto otherwise, int set, int32_t k0) {
             if (is_whole(k0)) {
 #pragma unroll
                 for (int piece = 0; piece < EACH; piece++) {
-                    load_piece(std::true_type(), set, piece, k0, nullptr);
+                    load_piece(Whole(), set, piece, k0, nullptr);
                 }
             } else {
 #pragma unroll
                 for (int piece = 0; piece < EACH; piece++) {
-                    load_piece(std::false_type(), set, piece, k0, nullptr);
+                    load_piece(otherwise, set, piece, k0, nullptr);
                 }
             }
         };
@@ -590,70 +601,116 @@ __device__ __forceinline__ void make_tile(
         // stage is free for step t + STAGES: EARLY of its pieces are asked for right then, the others in the next step's
         // first multiplication. (Steps behind the last one are asked for like all others: zeros.) Through registers: in
         // front of the meeting step t + 1 is put into its stage, from a set that step t + 1 + SETS comes to.
-        constexpr int EARLY = EACH / 2, UNROLL = ALIGNED ? 1 : SETS;
+        constexpr int EARLY = EACH / 2;
+        char *before = stages + (STAGES - 1) * BYTES, *buffer = stages;
+        auto read_first = [&] {
+            if (works) {
+#pragma unroll
+                for (int r = 0; r < READS; r++) {
+                    read(buffer, 0, r);
+                }
+            }
+        };
         if constexpr (ALIGNED) {
 #pragma unroll
             for (int t = 0; t < STAGES; t++) {
-                find_rows(t * STEP);
+                find_rows(0, t * STEP);
                 load_some(0, t == STAGES - 1 ? EARLY : EACH, t * STEP, stages + t * BYTES);
             }
             meet<(STAGES - 2) * EACH + EARLY>();
-        } else {
-            find_rows(0);
-            load(0, 0);
-            store(0, 0, stages);
+            read_first();
+            for (int32_t k0 = 0; k0 < k_size; k0 += STEP) {
 #pragma unroll
-            for (int t = 1; t <= SETS; t++) {
-                find_rows(t * STEP);
-                if (t * STEP < k_size) { // (uniform)
-                    load(t % UNROLL, t * STEP);
+                for (int step = 0; step < STEPS - 1; step++) {
+                    if (step == 0) {
+                        multiply(step, buffer, step + 1, EARLY, EACH, [&](int from, int upto) {
+                            load_some(from, upto, k0 + (STAGES - 1) * STEP, before);
+                        });
+                        find_rows(0, k0 + STAGES * STEP);
+                    } else {
+                        multiply(step, buffer, step + 1, 0, 0, nothing);
+                    }
                 }
-            }
-            find_rows((SETS + 1) * STEP);
-            meet<-1>();
-        }
-        char *before = stages + (STAGES - 1) * BYTES, *buffer = stages;
-        if (works) {
-#pragma unroll
-            for (int r = 0; r < READS; r++) {
-                read(buffer, 0, r);
-            }
-        }
-        auto step_at = [&](int32_t k0, int set) {
-#pragma unroll
-            for (int step = 0; step < STEPS - 1; step++) {
-                if (ALIGNED && step == 0) {
-                    multiply(step, buffer, step + 1, EARLY, EACH, [&](int from, int upto) {
-                        load_some(from, upto, k0 + (STAGES - 1) * STEP, before);
-                    });
-                    find_rows(k0 + STAGES * STEP);
-                } else {
-                    multiply(step, buffer, step + 1, 0, 0, nothing);
-                }
-            }
-            char* const following = buffer + BYTES < stages + STAGES * BYTES ? buffer + BYTES : stages;
-            if constexpr (ALIGNED) {
+                char* const following = buffer + BYTES < stages + STAGES * BYTES ? buffer + BYTES : stages;
                 meet<(STAGES - 2) * EACH>();
                 multiply(STEPS - 1, following, 0, 0, EARLY, [&](int from, int upto) {
                     load_some(from, upto, k0 + STAGES * STEP, buffer);
                 });
-            } else {
+                before = buffer;
+                buffer = following;
+            }
+        } else {
+            // Long sums have a loop in which every step loads all of its pieces: the compiler counts what is on its way, and
+            // behind a load that may not have been issued it can only wait for everything (4402 rows of 24 groups,
+            // K = 1797, L = 269, float16: 37 us instead of 61). Their last steps, and sums that have no more, load what
+            // there is (53740 rows, K = 9, L = 2389: 124 us instead of 145).
+            constexpr int LOOKS = (SUMS ? 2 * SETS : SETS) + 1; // steps behind the present one that a step has to do with
+            auto begin_with = [&](auto take) {
+                constexpr bool ALL = decltype(take)::value == Take::ALL;
+                // (SOME: the first step is not to wait for the others)
+                constexpr int FIRST = ALL ? SETS : 1;
+#pragma unroll
+                for (int t = 0; t < FIRST; t++) {
+                    find_rows(t, t * STEP);
+                    load(take, t, t * STEP);
+                }
+                if (!ALL) {
+                    store(0, 0, stages);
+                }
+#pragma unroll
+                for (int t = FIRST; t < SETS; t++) {
+                    find_rows(t, t * STEP);
+                    if (t * STEP < k_size) { // (uniform)
+                        load(take, t, t * STEP);
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < SETS; t++) {
+                    find_rows(t, (SETS + t) * STEP);
+                }
+                if (ALL) {
+                    store(0, 0, stages);
+                }
+                if (ALL || SETS * STEP < k_size) { // (uniform)
+                    load(take, 0, SETS * STEP);
+                }
+                find_rows(0, 2 * SETS * STEP);
+                meet<-1>();
+                read_first();
+            };
+            auto step_at = [&](auto take, int set, int32_t k0) {
+#pragma unroll
+                for (int step = 0; step < STEPS - 1; step++) {
+                    multiply(step, buffer, step + 1, 0, 0, nothing);
+                }
+                char* const following = buffer == stages ? stages + BYTES : stages;
                 store(set, k0 + STEP, following);
                 meet<-1>();
-                if (k0 + (SETS + 1) * STEP < k_size) { // (uniform)
-                    load(set, k0 + (SETS + 1) * STEP);
-                    find_rows(k0 + (SETS + 2) * STEP);
+                if (decltype(take)::value == Take::ALL || k0 + (SETS + 1) * STEP < k_size) { // (uniform)
+                    load(take, set, k0 + (SETS + 1) * STEP);
+                    find_rows(set, k0 + (2 * SETS + 1) * STEP);
                 }
                 multiply(STEPS - 1, following, 0, 0, 0, nothing);
-            }
-            before = buffer;
-            buffer = following;
-        };
-        for (int32_t k0 = 0; k0 < k_size; k0 += UNROLL * STEP) {
+                buffer = following;
+            };
+            int32_t k0 = 0;
+            if (k_size >= (LOOKS + SETS) * STEP) {
+                begin_with(All());
+                for (; k0 + (LOOKS + SETS) * STEP <= k_size; k0 += SETS * STEP) {
 #pragma unroll
-            for (int u = 0; u < UNROLL; u++) {
-                if (k0 + u * STEP < k_size) { // (uniform)
-                    step_at(k0 + u * STEP, (u + 1) % UNROLL);
+                    for (int u = 0; u < SETS; u++) {
+                        step_at(All(), (u + 1) % SETS, k0 + u * STEP);
+                    }
+                }
+            } else {
+                begin_with(Some());
+            }
+            for (; k0 < k_size; k0 += SETS * STEP) {
+#pragma unroll
+                for (int u = 0; u < SETS; u++) {
+                    if (k0 + u * STEP < k_size) { // (uniform)
+                        step_at(Some(), (u + 1) % SETS, k0 + u * STEP);
+                    }
                 }
             }
         }
@@ -661,7 +718,7 @@ __device__ __forceinline__ void make_tile(
     }
 
     // Every wavefront turns its blocks over in LDS of its own, to store whole pieces of rows side by side (straight from
-    // the registers, 8 bytes of 32 rows per store: 32768 rows, K = 2048, L = 4096, bfloat16: 657 us instead of 446).
+    // the registers, 8 bytes of 32 rows per store: 32768 rows, K = 2048, L = 4096, bfloat16: 657 us instead of 613).
     __syncthreads();
     auto put = [&](auto zero, auto is_partial, auto&& row_at) {
         typedef decltype(zero) To;
@@ -785,8 +842,12 @@ template <typename T> __global__ __launch_bounds__(JOIN_THREADS) void join_split
     }
 }
 
+/// Wavefronts per SIMD: small tiles through registers wait for memory most of the time and have room for four (60094 rows,
+/// K = 107, L = 31, float16: 9.4 us, with three and more pieces on their way in each 12.0).
+template <typename T, int BM, bool ALIGNED> constexpr int ABREAST = BM == 64 && !ALIGNED && sizeof(T) < 8 ? 4 : 2;
+
 template <typename T, Form FORM, int BM, int BN, int WM, int WN, int DEEP, int STAGES, bool ALIGNED>
-__global__ __launch_bounds__(WM* WN* WAVE, 2) void tiles_kernel(Product<T> g) {
+__global__ __launch_bounds__(WM* WN* WAVE, (ABREAST<T, BM, ALIGNED>)) void tiles_kernel(Product<T> g) {
     __shared__ TileLds<BM, BN, DEEP, STAGES> lds;
     make_tile<T, FORM, BM, BN, WM, WN, DEEP, STAGES, ALIGNED>(g, blockIdx.x, lds);
 }

@@ -513,8 +513,9 @@ namespace {
 
 /// The order of few rows in one launch: a workgroup looks at all of them, counts those of the groups in front of its own
 /// `each` (where its first place is), and places those of its own. What it reads comes from L2, and no launch waits for
-/// another (rows / groups, with this and with the three launches above: 465 / 3268: FEW1 and 23 us, 14 901 / 1803: FEW2 and
-/// 26, 32 768 / 100 003: FEW3 and 35, 65 536 / 1000: FEW4 and FEW5).
+/// another (rows / groups, with this and with the launches above: 465 / 3268: 5 and 15 us, 14 901 / 1803: 10 and 17,
+/// 4096 / 64: 6 and 8). More rows are too many for every workgroup to look at: 65 536 / 1000: 42 and 21 us, and, where one
+/// level of buckets does, 16 384 / 64: 13 and 8.
 /// LDS: counters[wavefronts][each], start[each], of_wave[wavefronts].
 constexpr int32_t FEW_ROWS = 16384, FEW_ROWS_ONE_LEVEL = 4096;
 constexpr int64_t FEW_LOOKS = 1 << 24;           // at rows, by all workgroups
