@@ -7,8 +7,8 @@
 //
 // and its gradients. Everything is bound by memory: a row is read once, held in
 // registers (a team of lanes per row, up to four pieces of 16 bytes per lane),
-// and its results are written once. Rows of more than 2048 pieces are read
-// three times instead (`wide` kernels).
+// and its results are written once. Rows of more than 2048 pieces (the
+// gradients of 16-bit rows: 1024) are read three times instead (`wide` kernels).
 //
 // Gradients. With b = block, y = norm(b) = b rb, a = s gate y weight_block,
 // t = residual + a, rt = 1 / sqrt(mean(t^2) + epsilon), h = grad_next weight_next:
@@ -113,6 +113,8 @@ template <int TEAM, int P, int N> struct Columns {
 /// Threads of a workgroup whose teams have TEAM lanes.
 template <int TEAM> constexpr int THREADS_OF = TEAM > 256 ? TEAM : 256;
 
+/// Both results, bound by memory: three reads and two writes per number (four with a shared gate), 16 384 rows of 4096
+/// bfloat16 with a gate each in 101 us, 6.6 TB/s. What is read once streams past the caches (127 us through them).
 template <typename T, int TEAM, int P, int N>
 __global__ __launch_bounds__(THREADS_OF<TEAM>) void forward_kernel(Forward<T> f) {
     typedef wide_t<T> W;
@@ -183,6 +185,9 @@ __global__ __launch_bounds__(THREADS_OF<TEAM>) void forward_kernel(Forward<T> f)
     }
 }
 
+/// All gradients of a row in one pass, bound by memory: five reads and three writes per number, 16 384 rows of 4096 bfloat16
+/// in 188 us, 5.7 TB/s; 50 021 rows of 384 floats with a shared gate in 86, 5.4 TB/s. The sums over the rows stay in
+/// registers, which is what limits the lanes' pieces.
 template <typename T, int TEAM, int P, int N>
 __global__ __launch_bounds__(THREADS_OF<TEAM>) void gradient_kernel(Gradients<T> g) {
     typedef wide_t<T> W;
@@ -325,7 +330,8 @@ __global__ __launch_bounds__(THREADS_OF<TEAM>) void gradient_kernel(Gradients<T>
     }
 }
 
-/// to[column] := the sum over the workgroups of what they have: 16 lanes side by side for 16 columns, and 16 shares of
+/// to[column] := the sum over the workgroups of what they have (512 of them and 4096 columns of two sums: 17 MB, read from the
+/// caches, 6 us): 16 lanes side by side for 16 columns, and 16 shares of
 /// the workgroups.
 constexpr int JOIN_COLUMNS = 16, JOIN_SHARES = 16;
 template <typename T>
@@ -357,7 +363,8 @@ __global__ __launch_bounds__(JOIN_COLUMNS* JOIN_SHARES) void join_kernel(
     }
 }
 
-// Rows that do not fit the registers of a workgroup: read again for every step, number by number.
+// Rows that do not fit the registers of a workgroup: read again for every step, number by number, from the caches (3300
+// rows of 20 000 bfloat16: 270 us, 2.0 TB/s of what has to move; gradients 624, 1.7).
 constexpr int WIDE_THREADS = 1024;
 
 template <typename T> __global__ __launch_bounds__(WIDE_THREADS) void wide_forward_kernel(Forward<T> f) {

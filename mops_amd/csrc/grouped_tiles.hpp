@@ -32,6 +32,13 @@
 // by then, the workgroup meets: the step's buffer is free for the step after
 // the next, the next step's has arrived. So there is one barrier per step, and
 // nothing waits for LDS or memory behind it.
+//
+// Large products are bound by the matrix units (and, in 16 bits, by the clock
+// that the power of random numbers leaves): one group of 8192 rows, K = L =
+// 8192: bfloat16 1040 to 1170 TFLOP/s, float 130, double 65; K = L = 2048 1080
+// (float16), at odd addresses, with the copy, 750. Tiles of 128 read memory and
+// LDS twice as often for the same work: 890 there. Few rows are bound by the
+// matrices' bytes: 24 rows, 16 experts of 2048 x 1408 bfloat16, 15.8 us, 5.8 TB/s.
 #ifndef MOPS_AMD_GROUPED_TILES_HPP
 #define MOPS_AMD_GROUPED_TILES_HPP
 
