@@ -79,7 +79,8 @@ template <Form FORM, typename T> unsigned set_tiles(Product<T>& g, int tile) {
 }
 
 /// body(tile, wavefronts of its rows, of its columns, rows aligned): the kernels there are. Tiles of 256 are for 16-bit
-/// types with aligned rows (through registers they leave none for the pieces that are on their way).
+/// types with aligned rows (through registers they leave none for the pieces that are on their way, nor do tiles of 128 in
+/// double: 43 221 rows, K = 235, L = 95: 69 us in tiles of 64, 121 in tiles of 128, which spill).
 template <typename T, typename Body> void with_tile(int tile, bool in_place, Body&& body) {
     std::integral_constant<int, 2> two;
     std::integral_constant<int, 4> four;
@@ -88,8 +89,11 @@ template <typename T, typename Body> void with_tile(int tile, bool in_place, Bod
             body(std::integral_constant<int, 256>{}, two, four, std::true_type{});
         }
     } else if (tile == 128) {
-        in_place ? body(std::integral_constant<int, 128>{}, two, two, std::true_type{})
-                 : body(std::integral_constant<int, 128>{}, two, two, std::false_type{});
+        if (in_place) {
+            body(std::integral_constant<int, 128>{}, two, two, std::true_type{});
+        } else if constexpr (sizeof(T) < 8) {
+            body(std::integral_constant<int, 128>{}, two, two, std::false_type{});
+        }
     } else {
         in_place ? body(std::integral_constant<int, 64>{}, two, two, std::true_type{})
                  : body(std::integral_constant<int, 64>{}, two, two, std::false_type{});
@@ -122,15 +126,20 @@ bool filled(int tile, int32_t m, int32_t n = 0) {
     return covered(tile) <= (tile == 256 ? 1.3 : 1.5) * covered(tile / 2);
 }
 
+/// Whether there are tiles of this extent (with_tile).
+template <typename T> bool exists(int tile, bool in_place) {
+    return tile == 256 ? sizeof(T) == 2 && in_place : sizeof(T) < 8 || in_place;
+}
+
 /// The tiles of FORWARD and GRAD_ROWS: the largest that keep all compute units busy and, on average, are half full.
 template <typename T> int tile_of_rows(const Product<T>& g) {
     const size_t rows = static_cast<size_t>(g.groups.n_rows), groups = static_cast<size_t>(g.groups.n_groups);
     const size_t units = static_cast<size_t>(compute_units());
     auto fits = [&](int tile) {
-        return ceil_div(rows, tile) * tiles(g.n_size, tile) >= units && rows >= tile / 2 * groups &&
-               filled(tile, g.n_size);
+        return exists<T>(tile, g.in_place) && ceil_div(rows, tile) * tiles(g.n_size, tile) >= units &&
+               rows >= tile / 2 * groups && filled(tile, g.n_size);
     };
-    return sizeof(T) == 2 && g.in_place && fits(256) ? 256 : fits(128) ? 128 : 64;
+    return fits(256) ? 256 : fits(128) ? 128 : 64;
 }
 
 /// The tiles of GRAD_SUMS, and its rows per unit: what every workgroup that the GPU has room for would have if the work
@@ -140,10 +149,11 @@ template <typename T> int tile_of_sums(Product<T>& g) {
     const size_t units = static_cast<size_t>(compute_units());
     auto of_unit = [&](int tile) { return static_cast<size_t>(tiles(g.m_size, tile)) * tiles(g.n_size, tile); };
     auto fits = [&](int tile) {
-        return g.m_size > tile / 2 && g.n_size > tile / 2 && filled(tile, g.m_size, g.n_size) &&
+        return exists<T>(tile, g.in_place) && g.m_size > tile / 2 && g.n_size > tile / 2 &&
+               filled(tile, g.m_size, g.n_size) &&
                of_unit(tile) * std::max(groups, ceil_div(rows, 8 * tile)) >= units;
     };
-    const int tile = sizeof(T) == 2 && g.in_place && fits(256) ? 256 : fits(128) ? 128 : 64;
+    const int tile = fits(256) ? 256 : fits(128) ? 128 : 64;
     const size_t room = (tile == 256 ? 1 : 2) * units;
     const size_t step = std::max<size_t>(ceil_div(rows * of_unit(tile), room), 256);
     g.step = static_cast<int32_t>(std::min(ceil_div(step, 64) * 64, ceil_div(rows, 64) * 64));

@@ -400,7 +400,7 @@ __device__ __forceinline__ void make_tile(
     constexpr int MB = BM / WM / BLOCK, NB = BN / WN / BLOCK; // blocks of a wavefront
     constexpr bool SUMS = FORM == Form::GRAD_SUMS, Q_TURNED = SUMS, P_TURNED = FORM != Form::GRAD_ROWS;
     constexpr Units UNITS = SUMS ? Units::OF_GROUPS : Units::OF_ROWS;
-    constexpr int SETS = ALIGNED ? 0 : BM > 64 && sizeof(T) == 8 ? 1 : 2; // (what there is room for in registers)
+    constexpr int SETS = ALIGNED ? 0 : 2; // (what there is room for in registers)
     using QLoader = std::conditional_t<
         Q_TURNED, TurnedLoader<T, BM, DEEP, THREADS, SETS>, StraightLoader<T, BM, DEEP, THREADS, SETS>>;
     using PLoader = std::conditional_t<
