@@ -48,7 +48,8 @@ template <typename T> bool worth_copying(const Matrices<T>& q, const Matrices<T>
     constexpr double GAIN = sizeof(T) == 2 ? 1.0 / 700 : sizeof(T) == 4 ? 1.0 / 550 : 1.0 / 150; // us per 10^6
     const double bytes = static_cast<double>(q.copied_bytes() + p.copied_bytes());
     const int launches = !q.in_place() + !p.in_place();
-    return launches > 0 && operations * 1e-6 * GAIN > bytes / 2.5e6 + 4 * launches;
+    constexpr double MOST = double(size_t(1) << 31); // (memory that the thread keeps)
+    return launches > 0 && bytes <= MOST && operations * 1e-6 * GAIN > bytes / 2.5e6 + 4 * launches;
 }
 
 /// `matrices` where they are, or their copy in `room` (which moves on).
