@@ -431,7 +431,8 @@ __device__ __forceinline__ void make_tile(
         m0 = of_unit / g.n_tiles * BM;
         n0 = of_unit % g.n_tiles * BN;
     } else {
-        // bands of four units: their rows and a tile's columns of the matrix are read together
+        // bands of four units: their rows and a tile's columns of the matrix are read together (of two or eight: the same
+        // time)
         const int32_t of_band = 4 * tiles_of_unit;
         const int32_t band = static_cast<int32_t>(tile / of_band), in_band = static_cast<int32_t>(tile % of_band);
         const int32_t height = min(4, units - 4 * band);
@@ -607,7 +608,8 @@ __device__ __forceinline__ void make_tile(
         // Step t is multiplied from stage t % STAGES. Where the workgroup meets in it, step t + 1 has arrived, and the
         // stage is free for step t + STAGES: EARLY of its pieces are asked for right then, the others in the next step's
         // first multiplication. (Steps behind the last one are asked for like all others: zeros.) Through registers: in
-        // front of the meeting step t + 1 is put into its stage, from a set that step t + 1 + SETS comes to.
+        // front of the meeting step t + 1 is put into its stage, from a set that step t + 1 + SETS comes to. (32768 rows of
+        // 32 groups, K = 2048, L = 4096, bfloat16: 585 us with half of the pieces early, 600 with a quarter.)
         constexpr int EARLY = EACH / 2;
         char *before = stages + (STAGES - 1) * BYTES, *buffer = stages;
         auto read_first = [&] {
