@@ -21,6 +21,7 @@
 #include "checks.hpp"
 #include "device_common.hpp"
 #include "numbers.hpp"
+#include "plan_bounds.hpp"
 #include "runtime.hpp"
 #include "sender_buckets.hpp"
 #include "wave_sort.hpp"
@@ -241,29 +242,29 @@ template <typename T, int N> struct TableRows {
         }
         value.stream_to(grad_table + static_cast<size_t>(row) * teams.row.columns + column);
     }
-    /// Row `row`, which has the places begin .. end - 1, by the team alone.
-    __device__ __forceinline__ void by_team(int32_t row, int32_t begin, int32_t end) const {
+    /// Row `row`, which has these places, by the team alone.
+    __device__ __forceinline__ void by_team(int32_t row, Range places) const {
         W sum[N] = {};
-        add_rows<T, N>(sum, grad_output, order, n_rows, begin, end, 1, teams.row.columns, column, teams.team);
+        add_rows<T, N>(sum, grad_output, order, n_rows, places.begin, places.end, 1, teams.row.columns, column, teams.team);
         if (holds) {
             store(row, sum);
         }
     }
     /// The same by all teams of the workgroup, with the sums of the chunks that lie inside.
-    __device__ __forceinline__ void by_all(W* joined, int32_t row, int32_t begin, int32_t end) const {
+    __device__ __forceinline__ void by_all(W* joined, int32_t row, Range places) const {
         W sum[N] = {};
-        const int32_t first_chunk = (begin + chunk - 1) / chunk, past_chunk = end / chunk;
-        const bool chunks = partial != nullptr && first_chunk < past_chunk;
+        const Range inside = chunks_inside(places, chunk);
+        const bool chunks = partial != nullptr && inside.begin < inside.end;
         add_rows<T, N>(
-            sum, grad_output, order, n_rows, begin + mine, chunks ? first_chunk * chunk : end, teams.teams,
-            teams.row.columns, column, teams.team
+            sum, grad_output, order, n_rows, places.begin + mine, chunks ? inside.begin * chunk : places.end,
+            teams.teams, teams.row.columns, column, teams.team
         );
         if (chunks) {
-            for (int32_t c = first_chunk + mine; c < past_chunk; c += AHEAD * teams.teams) {
+            for (int32_t c = inside.begin + mine; c < inside.end; c += AHEAD * teams.teams) {
                 W value[AHEAD][N];
 #pragma unroll
                 for (int u = 0; u < AHEAD; u++) {
-                    const size_t from = min(c + u * teams.teams, past_chunk - 1);
+                    const size_t from = min(c + u * teams.teams, inside.end - 1);
 #pragma unroll
                     for (int j = 0; j < N; j++) {
                         value[u][j] = partial[from * teams.row.columns + column + j];
@@ -271,7 +272,7 @@ template <typename T, int N> struct TableRows {
                 }
 #pragma unroll
                 for (int u = 0; u < AHEAD; u++) {
-                    if (c + u * teams.teams < past_chunk) {
+                    if (c + u * teams.teams < inside.end) {
 #pragma unroll
                         for (int j = 0; j < N; j++) {
                             sum[j] += value[u][j];
@@ -280,8 +281,8 @@ template <typename T, int N> struct TableRows {
                 }
             }
             add_rows<T, N>(
-                sum, grad_output, order, n_rows, past_chunk * chunk + mine, end, teams.teams, teams.row.columns, column,
-                teams.team
+                sum, grad_output, order, n_rows, inside.end * chunk + mine, places.end, teams.teams,
+                teams.row.columns, column, teams.team
             );
         }
         join_teams<W, N>(sum, joined, teams);
@@ -305,11 +306,10 @@ __global__ __launch_bounds__(THREADS) void gradient_kernel(
 ) {
     __shared__ wide_t<T> joined[N * THREADS];
     const TableRows<T, N> rows(grad_table, grad_output, partial, order, n_rows, chunk, teams, scale);
-    auto begin_of = [&](int32_t row) { return max(offsets[row], 0); };
-    auto end_of = [&](int32_t row) { return min(offsets[row + 1], n_rows); };
+    auto places_of = [&](int32_t row) { return places_between(offsets[row], offsets[row + 1], n_rows); };
     if (ONE_EACH) {
         const int32_t row = blockIdx.x;
-        rows.by_all(joined, row, begin_of(row), end_of(row));
+        rows.by_all(joined, row, places_of(row));
         return;
     }
     const int32_t others = (n_rows + ALONE - 1) / ALONE, block = static_cast<int32_t>(blockIdx.x);
@@ -317,18 +317,18 @@ __global__ __launch_bounds__(THREADS) void gradient_kernel(
         const int32_t place = block * ALONE, listed = order[place];
         const int32_t row = in_bounds(listed, n_rows) ? indices[listed] : -1;
         if (in_bounds(row, table_rows)) { // (uniform, like the next one)
-            const int32_t begin = begin_of(row), end = end_of(row);
-            if (end - begin > ALONE && (begin + ALONE - 1) / ALONE == block) {
-                rows.by_all(joined, row, begin, end);
+            const Range places = places_of(row);
+            if (places.end - places.begin > ALONE && chunks_inside(places, ALONE).begin == block) {
+                rows.by_all(joined, row, places);
             }
         }
         return;
     }
     const int32_t row0 = (block - others) * each, row_end = min(row0 + each, table_rows);
     for (int32_t row = row0 + rows.mine; row < row_end; row += teams.teams) {
-        const int32_t begin = begin_of(row), end = end_of(row);
-        if (end - begin <= ALONE) {
-            rows.by_team(row, begin, end);
+        const Range places = places_of(row);
+        if (places.end - places.begin <= ALONE) {
+            rows.by_team(row, places);
         }
     }
 }
@@ -370,11 +370,11 @@ __global__ __launch_bounds__(THREADS) void few_rows_kernel(
     __syncthreads();
     const TableRows<T, N> rows(grad_table, grad_output, nullptr, order, n_rows, 1, teams, scale);
     if (one_each) { // (uniform)
-        rows.by_all(joined, row0, places[0], places[1]);
+        rows.by_all(joined, row0, Range{places[0], places[1]});
         return;
     }
     for (int32_t row = row0 + rows.mine; row < row_end; row += teams.teams) {
-        rows.by_team(row, places[row - row0], places[row - row0 + 1]);
+        rows.by_team(row, Range{places[row - row0], places[row - row0 + 1]});
     }
 }
 

@@ -8,6 +8,7 @@
 #include <hip/hip_runtime.h>
 
 #include "device_common.hpp"
+#include "plan_bounds.hpp"
 
 namespace mops::amd {
 
@@ -20,10 +21,10 @@ struct RowGroups {
     int32_t n_groups, n_rows;
 
     __device__ __forceinline__ int32_t begin_of(int32_t group) const {
-        return min(max(offsets[group], 0), n_rows);
+        return within(offsets[group], 0, n_rows);
     }
     __device__ __forceinline__ int32_t end_of(int32_t group, int32_t begin) const {
-        return min(max(offsets[group + 1], begin), n_rows);
+        return within(offsets[group + 1], begin, n_rows);
     }
     /// (an order that is none gives some row, never one outside)
     __device__ __forceinline__ int32_t row_at(int32_t place) const {
