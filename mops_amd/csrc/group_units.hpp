@@ -40,6 +40,7 @@ struct GroupUnit {
     int32_t group; // -1: there are fewer units
     int32_t begin, count; // places
     int32_t index, of_group; // which unit of its group this is, and how many the group has
+    int32_t slot;            // OF_GROUPS, of_group > 1: which unit of all groups of more than one unit this is
 };
 
 /// What becomes of a group without rows, and of the rows without a group.
@@ -54,11 +55,9 @@ inline size_t most_units(int32_t n_rows, int32_t n_groups, int32_t step) {
     return (static_cast<size_t>(n_rows) + step - 1) / step + static_cast<size_t>(n_groups) + 1;
 }
 
-/// The units of a group with `count` places. OF_GROUPS: rounded down, but for the last quarter, so that equal groups do not
-/// all have a unit more than the GPU has room for (200 000 rows of 8 groups, K = 200, L = 320, gradients of the matrices
-/// in float: 374 us; with all fractions rounded up 456).
+/// The units of a group with `count` places.
 template <Units WHICH> __device__ __forceinline__ int32_t units_of(int32_t count, int32_t step) {
-    return WHICH == Units::OF_GROUPS ? max((count + step / 4) / step, 1) : (count + step - 1) / step;
+    return WHICH == Units::OF_GROUPS ? units_to_sum(count, step) : (count + step - 1) / step;
 }
 
 /// (the same in all lanes, and known to be)
@@ -66,7 +65,7 @@ __device__ __forceinline__ GroupUnit uniform(const GroupUnit& unit) {
     return GroupUnit{
         __builtin_amdgcn_readfirstlane(unit.group), __builtin_amdgcn_readfirstlane(unit.begin),
         __builtin_amdgcn_readfirstlane(unit.count), __builtin_amdgcn_readfirstlane(unit.index),
-        __builtin_amdgcn_readfirstlane(unit.of_group),
+        __builtin_amdgcn_readfirstlane(unit.of_group), __builtin_amdgcn_readfirstlane(unit.slot),
     };
 }
 
@@ -97,13 +96,15 @@ public:
 
     /// Unit number `unit`.
     __device__ __forceinline__ GroupUnit find(int32_t unit) {
+        int32_t slot = unit; // less the groups of one unit in front (OF_GROUPS: no group has none)
         for (int32_t base = 0; base < groups_.n_groups; base += WAVE) {
             if (base != base_) {
                 look(base);
             }
-            const uint64_t past = __ballot(upto_ > unit);
+            const uint64_t past = __ballot(upto_ > unit), alone = __ballot(units_ == 1);
             if (past != 0) {
                 const int at = __builtin_ctzll(past);
+                slot -= __popcll(alone & ((uint64_t(1) << at) - 1));
                 const int32_t of_group = __builtin_amdgcn_readlane(units_, at);
                 const int32_t index = unit - (__builtin_amdgcn_readlane(upto_, at) - of_group);
                 const int32_t begin = __builtin_amdgcn_readlane(begin_, at);
@@ -116,24 +117,26 @@ public:
                     first = (index * each + min(index, more)) * PLACES_TOGETHER;
                     last = first + (each + (index < more ? 1 : 0)) * PLACES_TOGETHER;
                 }
-                return uniform(GroupUnit{group, begin + first, min(last, count) - first, index, of_group});
+                return uniform(GroupUnit{group, begin + first, min(last, count) - first, index, of_group, slot});
             }
+            slot -= __popcll(alone);
             unit -= __builtin_amdgcn_readlane(upto_, WAVE - 1);
         }
         if (WHICH == Units::OF_ROWS) {
             const int32_t rest_rows = rest(), units = (rest_rows + step_ - 1) / step_;
             if (unit < units) {
                 return uniform(
-                    GroupUnit{groups_.n_groups, unit * step_, min(rest_rows - unit * step_, step_), unit, units}
+                    GroupUnit{groups_.n_groups, unit * step_, min(rest_rows - unit * step_, step_), unit, units, 0}
                 );
             }
         }
-        return GroupUnit{-1, 0, 0, 0, 0};
+        return GroupUnit{-1, 0, 0, 0, 0, 0};
     }
 
-    /// body(unit) for every group of more than one unit: its first one (index: its number), without its places.
+    /// body(unit) for every group of more than one unit: its first one, without its places.
     template <typename Body> __device__ __forceinline__ void for_split_groups(Body&& body) {
-        int32_t before = 0;
+        constexpr int32_t MANY = 1 << 30; // (more than any plan has: offsets that are none could give numbers beyond 32 bits)
+        int32_t slot = 0;
         for (int32_t base = 0; base < groups_.n_groups; base += WAVE) {
             if (base != base_) {
                 look(base);
@@ -143,10 +146,9 @@ public:
                 const int at = __builtin_ctzll(split);
                 split &= split - 1;
                 const int32_t of_group = __builtin_amdgcn_readlane(units_, at);
-                const int32_t first = before + __builtin_amdgcn_readlane(upto_, at) - of_group;
-                body(uniform(GroupUnit{__builtin_amdgcn_readlane(group_, at), 0, 0, first, of_group}));
+                body(uniform(GroupUnit{__builtin_amdgcn_readlane(group_, at), 0, 0, 0, of_group, slot}));
+                slot = min(slot + of_group, MANY);
             }
-            before += __builtin_amdgcn_readlane(upto_, WAVE - 1);
         }
     }
 

@@ -231,16 +231,13 @@ void gradients(
     rows.in_place = copies_W || (grad_output.in_place() && W.in_place());
     const int of_sums = of_W ? tile_of_sums(sums) : 0;
     const int of_rows = of_A ? tile_of_rows(rows) : 0;
-    const bool splits = of_W && sums.step < sums.groups.n_rows;
+    sums.most_slots = of_W ? most_split_units(sums.groups.n_rows, sums.step) : 0;
     if (of_A) {
         share_k(rows, of_rows);
     }
     const size_t row_bytes = of_A ? split_bytes(rows) : 0;
-    size_t sum_bytes = 0;
-    if (splits) {
-        const size_t most = most_units(sums.groups.n_rows, sums.groups.n_groups, sums.step);
-        sum_bytes = most * partial_size(sums.m_size, sums.n_size) * sizeof(wide_t<T>);
-    }
+    // (few, and of no more numbers than the tiles that the GPU has room for: 80 MB at most)
+    const size_t sum_bytes = sums.most_slots * partial_size(sums.m_size, sums.n_size) * sizeof(wide_t<T>);
     char* room = nullptr;
     if (copies + row_bytes + sum_bytes > 0) {
         char* workspace = static_cast<char*>(scratch(copies + row_bytes + sum_bytes));
@@ -276,10 +273,7 @@ void gradients(
     if (of_A) {
         join_splits(rows, stream);
     }
-    if (splits) {
-        sums.most_units = narrow_i32(
-            most_units(sums.groups.n_rows, sums.groups.n_groups, sums.step), "number of units of rows"
-        );
+    if (sums.most_slots > 0) {
         const unsigned workgroups = 4 * static_cast<unsigned>(compute_units());
         join_units_kernel<T><<<workgroups, JOIN_WAVES * WAVE, 0, stream>>>(sums);
         MOPS_HIP_CHECK(hipGetLastError());

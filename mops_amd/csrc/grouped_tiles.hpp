@@ -65,7 +65,7 @@ template <typename T> struct Operand {
 /// [rows][m_size], p is [rows][n_size].
 template <typename T> struct Product {
     T* out;
-    // GRAD_SUMS: [unit][partial_size(m_size, n_size)], for groups of more than one unit; else [split][row][n_size], where
+    // GRAD_SUMS: [slot][partial_size(m_size, n_size)], for the units of groups of more than one; else [split][row][n_size], where
     // there are several
     wide_t<T>* partial;
     Operand<T> q, p;
@@ -73,7 +73,8 @@ template <typename T> struct Product {
     RowGroups groups;
     int32_t m_size, n_size, k_size;
     int32_t step;            // places per unit
-    int32_t most_units;      // that the grid and `partial` have room for (offsets that are none could give more)
+    int32_t most_units;      // that the grid has room for (offsets that are none could give more)
+    int32_t most_slots;      // GRAD_SUMS: that `partial` has room for (likewise)
     int32_t m_tiles, n_tiles; // tiles of a unit (m_tiles: GRAD_SUMS)
     int32_t splits, k_each;   // FORWARD, GRAD_ROWS: shares of k, and how long they are (whole steps)
 };
@@ -798,7 +799,9 @@ __device__ __forceinline__ void make_tile(
             };
         };
         if (unit.of_group > 1) { // (uniform)
-            put(wide_t<T>(), std::true_type(), row_of(g.partial + unit_index * partial_size(g.m_size, g.n_size)));
+            if (unit.slot < g.most_slots) {
+                put(wide_t<T>(), std::true_type(), row_of(g.partial + unit.slot * partial_size(g.m_size, g.n_size)));
+            }
         } else {
             put(T(), std::false_type(), row_of(g.out + unit.group * size));
         }
@@ -885,10 +888,10 @@ template <typename T> __global__ __launch_bounds__(JOIN_WAVES* WAVE) void join_u
     UnitsOfGroups<Units::OF_GROUPS> of_groups(g.groups, g.step);
     int32_t turn = static_cast<int32_t>(blockIdx.x); // (another workgroup begins with each group)
     of_groups.for_split_groups([&](const GroupUnit& unit) {
-        const int32_t parts = min(unit.of_group, g.most_units - unit.index);
+        const int32_t parts = min(unit.of_group, g.most_slots - unit.slot);
         const int32_t sharing = parts >= 4 * JOIN_WAVES ? JOIN_WAVES : 1;
         const size_t at_once = JOIN_WAVES / sharing * WAVE;
-        const Wide* from = reinterpret_cast<const Wide*>(g.partial) + unit.index * pieces;
+        const Wide* from = reinterpret_cast<const Wide*>(g.partial) + unit.slot * pieces;
         T* const to = g.out + unit.group * size;
         size_t first = turn * at_once;
         for (; first < pieces; first += gridDim.x * at_once) {

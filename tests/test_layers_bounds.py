@@ -1,8 +1,14 @@
 """Plans that are none, and memory that is not there: what the layers' operators read and take then."""
 import os
 import subprocess
+import sys
 
 import numpy as np
+import pytest
+import torch
+
+import mops_amd
+from tests.test_layers import assert_within, random
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -57,3 +63,108 @@ def test_offsets_that_are_none_stay_within_the_rows(tmp_path):
     assert (got[:, :2] + 256 * 64).max() <= high and (got * np.array([1, 1, 0, 0])).min() >= 0
     inside = got[:, 2] < got[:, 3]
     assert ((got[:, 3] * chunk)[inside] <= n_rows[inside]).all()
+
+
+UNITS = """
+#include <cstdio>
+#include <cstdlib>
+#include "plan_bounds.hpp"
+using namespace mops::amd;
+static_assert(units_to_sum(2147418111, 2147418112) == 1, "");
+int main(int n, char** a) {
+    const int step = atoi(a[1]);
+    long long rows = 0;
+    int split = 0;
+    for (int i = 2; i < n; i++) { // the groups' sizes
+        const int units = units_to_sum(atoi(a[i]), step);
+        rows += atoi(a[i]);
+        split += units > 1 ? units : 0;
+    }
+    printf("%d %d\\n", split, most_split_units(int(rows), step));
+}
+"""
+
+
+def test_units_of_split_groups_are_few(tmp_path):
+    """Room for partial results is for the units of groups of more than one unit: never too little, none where no group
+    can have two, and not more for more groups."""
+    rng = np.random.default_rng(1)
+    reached = 0
+    for step, sizes in [
+        (256, [447]), (256, [448]), (256, [0, 448, 448, 448, 447]), (64, [112] * 50), (64, [111] * 50), (320, [0] * 100),
+        (57344, [256] * 256), (57344, [65536]), (1 << 20, [(1 << 20) * 7 // 4 - 1]),
+        *[(64 * int(rng.integers(1, 20)), rng.integers(0, 4000, 40).tolist()) for _ in range(20)],
+    ]:  # fmt: skip
+        split, most = run_on_host(tmp_path, UNITS, step, *sizes)[0]
+        assert split <= most <= 8 * sum(sizes) / (7 * step)
+        assert most == 0 or sum(sizes) >= 1.75 * step
+        reached += split == most
+    assert reached >= 6
+
+
+GROUPS = {  # sizes of the groups: some of several units in front, between and behind those of one, of more and fewer groups than a wavefront has lanes
+    "wide": [700] + [0, 1, 3] * 23 + [900, 2] + [1] * 60 + [2048, 5, 0, 600],
+    "narrow": [1, 900, 0, 2, 448, 447, 3000, 0],
+    "many": [0] * 300 + [1500] + [1, 0] * 150 + [449, 512],
+}
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64], ids=str)
+@pytest.mark.parametrize("columns", [(64, 72), (31, 33)], ids=str)
+@pytest.mark.parametrize("sizes", list(GROUPS))
+def test_gradients_of_groups_of_several_units(device, sizes, columns, dtype):
+    K, L = columns
+    sizes = torch.tensor(GROUPS[sizes])
+    rows, groups = int(sizes.sum()), len(sizes)
+    generator = torch.Generator().manual_seed(rows + K)
+    A, grad_output = [random(generator, (rows, width), dtype) for width in (K, L)]
+    W = random(generator, (groups, K, L), dtype)
+    offsets = torch.zeros(groups + 1, dtype=torch.int32)
+    offsets[1:] = sizes.cumsum(0)
+    order = torch.randperm(rows, generator=generator).int()
+    arguments = [x.to(device) for x in (grad_output, A, W, offsets, order)]
+    _, grad_W = mops_amd.grouped_matrix_product_vjp(*arguments, compute_grad_A=False)
+    exact, magnitude = torch.zeros(2, groups, K, L, dtype=torch.float64)
+    for g in range(groups):
+        mine = order[offsets[g] : offsets[g + 1]].long()
+        a, c = A[mine].double(), grad_output[mine].double()
+        exact[g], magnitude[g] = a.t() @ c, a.abs().t() @ c.abs()
+    assert_within(grad_W, exact, magnitude, int(sizes.max()), "grad_W")
+    assert torch.equal(mops_amd.grouped_matrix_product_vjp(*arguments)[1], grad_W)
+
+
+MANY_GROUPS = """
+import ctypes
+import torch
+import mops_amd
+from mops_amd._c_lib import device_library
+
+capacity = device_library().cdll.mops_amd_scratch_capacity
+capacity.restype = ctypes.c_int64
+device = torch.device("cuda:0")
+torch.manual_seed(0)
+rows, groups, K, L = 1000, 512, 256, 256
+A, grad_output = torch.randn(rows, K, device=device), torch.randn(rows, L, device=device)
+W = torch.randn(groups, K, L, device=device)
+for index in (torch.arange(rows, device=device) % groups, torch.zeros(rows, device=device)):
+    order, offsets = mops_amd.order_by_group(index.int(), groups)
+    grad_A, grad_W = mops_amd.grouped_matrix_product_vjp(grad_output, A, W, offsets, order)
+    exact = torch.zeros(groups, K, L, dtype=torch.float64)
+    for row in range(rows):
+        exact[int(index[row])] += torch.outer(A[row].cpu().double(), grad_output[row].cpu().double())
+    error = (grad_W.cpu().double() - exact).abs().max().item()
+    assert error < 0.05, error  # (1016 2^-24 times the magnitudes of 1000 products, which add up to some 640)
+    print("ok", capacity(), flush=True)
+# the groups that can be split at all, of 256 rows or more, have four units
+assert 0 < capacity() <= 4 << 20, capacity()
+"""
+
+
+@pytest.mark.gpu
+def test_many_groups_take_no_scratch_memory_each(device):
+    """Partial results need room for the groups that are split, not for every group. In a process of its own, whose thread
+    has no scratch memory from other calls."""
+    done = subprocess.run([sys.executable, "-c", MANY_GROUPS], cwd=ROOT, capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0, done.stdout + done.stderr[-3000:]
+    assert done.stdout.count("ok ") == 2, done.stdout
