@@ -191,13 +191,18 @@ template <typename T> void join_splits(const Product<T>& g, hipStream_t stream) 
 }
 
 template <typename T> void forward(Product<T> g, const Matrices<T>& A, const Matrices<T>& W, hipStream_t stream) {
-    size_t copies = A.copied_bytes() + W.copied_bytes();
-    const double operations = 2.0 * A.n_rows * g.k_size * g.n_size;
-    const bool copied = worth_copying(A, W, operations) && scratch_ready(copies);
-    g.in_place = copied || copies == 0;
-    copies = copied ? copies : 0;
-    const int tile = tile_of_rows(g);
-    share_k(g, tile);
+    size_t copies = 0;
+    int tile = 0;
+    auto choose = [&](bool copied) {
+        copies = copied ? A.copied_bytes() + W.copied_bytes() : 0;
+        g.in_place = copied || (A.in_place() && W.in_place());
+        tile = tile_of_rows(g);
+        share_k(g, tile);
+    };
+    choose(worth_copying(A, W, 2.0 * A.n_rows * g.k_size * g.n_size));
+    if (copies > 0 && !scratch_ready(copies + split_bytes(g))) {
+        choose(false);
+    }
     char* room = nullptr;
     if (copies + split_bytes(g) > 0) {
         char* workspace = static_cast<char*>(scratch(copies + split_bytes(g)));
@@ -219,25 +224,32 @@ void gradients(
     const bool of_A = rows.out != nullptr, of_W = sums.out != nullptr;
     // (each as if it were wanted alone: its result does not depend on whether the other one is)
     const double operations = 2.0 * A.n_rows * A.width * W.width;
-    bool copies_W = of_A && worth_copying(grad_output, W, operations);
-    bool copies_A = of_W && worth_copying(A, grad_output, operations);
-    size_t copies = (copies_A ? A.copied_bytes() : 0) + (copies_W ? W.copied_bytes() : 0) +
-                    (copies_A || copies_W ? grad_output.copied_bytes() : 0);
-    if (!scratch_ready(copies)) {
-        copies_A = copies_W = false;
-        copies = 0;
+    bool copies_W = false, copies_A = false;
+    int of_sums = 0, of_rows = 0;
+    size_t copies = 0, row_bytes = 0, sum_bytes = 0;
+    auto choose = [&](bool copied) {
+        copies_W = copied && of_A && worth_copying(grad_output, W, operations);
+        copies_A = copied && of_W && worth_copying(A, grad_output, operations);
+        copies = (copies_A ? A.copied_bytes() : 0) + (copies_W ? W.copied_bytes() : 0) +
+                 (copies_A || copies_W ? grad_output.copied_bytes() : 0);
+        sums.in_place = copies_A || (grad_output.in_place() && A.in_place());
+        rows.in_place = copies_W || (grad_output.in_place() && W.in_place());
+        if (of_W) {
+            of_sums = tile_of_sums(sums);
+            sums.most_slots = most_split_units(sums.groups.n_rows, sums.step);
+            // (few, and of no more numbers than the tiles that the GPU has room for: 80 MB at most)
+            sum_bytes = sums.most_slots * partial_size(sums.m_size, sums.n_size) * sizeof(wide_t<T>);
+        }
+        if (of_A) {
+            of_rows = tile_of_rows(rows);
+            share_k(rows, of_rows);
+            row_bytes = split_bytes(rows);
+        }
+    };
+    choose(true);
+    if (copies > 0 && !scratch_ready(copies + row_bytes + sum_bytes)) {
+        choose(false);
     }
-    sums.in_place = copies_A || (grad_output.in_place() && A.in_place());
-    rows.in_place = copies_W || (grad_output.in_place() && W.in_place());
-    const int of_sums = of_W ? tile_of_sums(sums) : 0;
-    const int of_rows = of_A ? tile_of_rows(rows) : 0;
-    sums.most_slots = of_W ? most_split_units(sums.groups.n_rows, sums.step) : 0;
-    if (of_A) {
-        share_k(rows, of_rows);
-    }
-    const size_t row_bytes = of_A ? split_bytes(rows) : 0;
-    // (few, and of no more numbers than the tiles that the GPU has room for: 80 MB at most)
-    const size_t sum_bytes = sums.most_slots * partial_size(sums.m_size, sums.n_size) * sizeof(wide_t<T>);
     char* room = nullptr;
     if (copies + row_bytes + sum_bytes > 0) {
         char* workspace = static_cast<char*>(scratch(copies + row_bytes + sum_bytes));

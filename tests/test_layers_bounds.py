@@ -168,3 +168,102 @@ def test_many_groups_take_no_scratch_memory_each(device):
     done = subprocess.run([sys.executable, "-c", MANY_GROUPS], cwd=ROOT, capture_output=True, text=True, timeout=100)
     assert done.returncode == 0, done.stdout + done.stderr[-3000:]
     assert done.stdout.count("ok ") == 2, done.stdout
+
+
+THREADS = """
+import ctypes, threading
+import torch
+import mops_amd
+from mops_amd._c_lib import device_library
+
+library = device_library().cdll
+library.mops_amd_scratch_capacity.restype = ctypes.c_int64
+library.mops_amd_reserve_scratch.argtypes = [ctypes.c_int64]
+device = torch.device("cuda:0")
+end = threading.Event()
+
+def in_a_thread(function):
+    \"\"\"The result in a new thread, which lives on and so keeps its scratch memory.\"\"\"
+    results, done = [], threading.Event()
+    def work():
+        try:
+            results.append(function())
+        except BaseException as error:
+            results.append(error)
+        done.set()
+        end.wait()
+    threading.Thread(target=work, daemon=True).start()
+    assert done.wait(60)
+    if isinstance(results[0], BaseException):
+        raise results[0]
+    return results[0]
+
+def case(rows, K, L, dtype):
+    generator = torch.Generator().manual_seed(K)
+    A, W, grad_output = [
+        torch.randn(shape, generator=generator, dtype=torch.float32).to(device, dtype)
+        for shape in ((rows, K), (1, K, L), (rows, L))
+    ]
+    offsets = torch.tensor([0, rows], dtype=torch.int32, device=device)
+    exact = [A.double() @ W[0].double(), grad_output.double() @ W[0].double().t(), A.double().t() @ grad_output.double()]
+    vjp = lambda *wanted: mops_amd.grouped_matrix_product_vjp(grad_output, A, W, offsets, None, *wanted)
+    return {
+        "product": (lambda: [mops_amd.grouped_matrix_product(A, W, offsets)], exact[:1], K),
+        "grad_A": (lambda: [vjp(True, False)[0]], exact[1:2], L),
+        "grad_W": (lambda: [vjp(False, True)[1].squeeze(0)], exact[2:], rows),
+        "gradients": (lambda: [x.squeeze(0) for x in vjp()], exact[1:], max(L, rows)),
+    }
+
+def check(results, exact, unit, terms):
+    for result, wanted in zip(results, exact, strict=True):
+        # (numbers of size 1: the magnitudes of a sum of n terms add up to less than n)
+        error = (result.double() - wanted).abs().max().item()
+        assert error <= (terms + 16) * unit[0] * terms + unit[1] * wanted.abs().max().item(), (error, terms)
+"""
+
+CAPTURED = THREADS + """
+def eager(call):
+    results = call()
+    torch.cuda.synchronize()
+    return results, library.mops_amd_scratch_capacity()
+
+def captured(call, capacity):
+    assert library.mops_amd_reserve_scratch(int(capacity / 1.5)) == 0
+    torch.cuda.synchronize()
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.stream(stream), torch.cuda.graph(graph, stream=stream):
+        results = call()
+    for _ in range(2):
+        for result in results:
+            result.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+    return results, library.mops_amd_scratch_capacity()
+
+# the product and grad_A share out a long sum, grad_W the rows of its group
+for name, sizes in [
+    ("product", (768, 20001, 767)), ("grad_A", (768, 767, 20001)), ("grad_W", (20001, 767, 767)),
+    ("gradients", (20001, 767, 767)), ("gradients", (768, 767, 20001)),
+]:
+    call, exact, terms = case(*sizes, torch.float64)[name]
+    results, capacity = in_a_thread(lambda: eager(call))
+    check(results, exact, (2.0**-53, 2.0**-53), terms)
+    print("eager", name, capacity, flush=True)
+    # a block that holds the copies, but not all of the partial results as well (blocks are made half as large again as
+    # what is asked for)
+    room = capacity / 1.5 - (3 << 20)
+    results, got = in_a_thread(lambda: captured(call, room))
+    check(results, exact, (2.0**-53, 2.0**-53), terms)
+    assert got <= room, (got, room)
+    print("ok", name, got, flush=True)
+end.set()
+"""
+
+
+@pytest.mark.gpu
+def test_a_captured_call_whose_block_holds_the_copies_only(device):
+    """Products at odd addresses copy their operands where there is room; during a capture the block has to hold the
+    copies and the partial results, or the call does without copies."""
+    done = subprocess.run([sys.executable, "-c", CAPTURED], cwd=ROOT, capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0, done.stdout + done.stderr[-3000:]
+    assert done.stdout.count("ok ") == 5, done.stdout
