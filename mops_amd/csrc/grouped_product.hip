@@ -200,12 +200,16 @@ template <typename T> void forward(Product<T> g, const Matrices<T>& A, const Mat
         share_k(g, tile);
     };
     choose(worth_copying(A, W, 2.0 * A.n_rows * g.k_size * g.n_size));
-    if (copies > 0 && !scratch_ready(copies + split_bytes(g))) {
-        choose(false);
+    char* workspace = nullptr;
+    if (copies > 0) {
+        workspace = static_cast<char*>(scratch_or_null(copies + split_bytes(g)));
+        if (workspace == nullptr) {
+            choose(false);
+        }
     }
     char* room = nullptr;
     if (copies + split_bytes(g) > 0) {
-        char* workspace = static_cast<char*>(scratch(copies + split_bytes(g)));
+        workspace = workspace != nullptr ? workspace : static_cast<char*>(scratch(split_bytes(g)));
         g.partial = reinterpret_cast<wide_t<T>*>(workspace + copies);
         room = copies > 0 ? workspace : nullptr;
     }
@@ -247,12 +251,16 @@ void gradients(
         }
     };
     choose(true);
-    if (copies > 0 && !scratch_ready(copies + row_bytes + sum_bytes)) {
-        choose(false);
+    char* workspace = nullptr;
+    if (copies > 0) {
+        workspace = static_cast<char*>(scratch_or_null(copies + row_bytes + sum_bytes));
+        if (workspace == nullptr) {
+            choose(false);
+        }
     }
     char* room = nullptr;
     if (copies + row_bytes + sum_bytes > 0) {
-        char* workspace = static_cast<char*>(scratch(copies + row_bytes + sum_bytes));
+        workspace = workspace != nullptr ? workspace : static_cast<char*>(scratch(row_bytes + sum_bytes));
         rows.partial = reinterpret_cast<wide_t<T>*>(workspace + copies);
         sums.partial = reinterpret_cast<wide_t<T>*>(workspace + copies + row_bytes);
         room = copies > 0 ? workspace : nullptr;

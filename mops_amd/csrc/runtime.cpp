@@ -274,7 +274,36 @@ void collect_kernel_time(double* milliseconds, int64_t* launches) {
     st.recorded.clear();
 }
 
-void* scratch(size_t bytes) {
+namespace {
+
+constexpr size_t COUNTER_BYTES = SCRATCH_COUNTERS * sizeof(int32_t);
+
+/// What a block of at least `bytes` is made with: half as much again, so that a slowly growing shape does not make a new
+/// block with every call, 1 MiB at least.
+size_t block_capacity(size_t bytes) { return std::max(bytes + bytes / 2, size_t(1) << 20); }
+
+/// What a block can have at most, as far as a test wants it (MOPS_AMD_TEST_SCRATCH_LIMIT, bytes): beyond it the device
+/// is taken to be full.
+size_t memory_limit() {
+    const char* limit = std::getenv("MOPS_AMD_TEST_SCRATCH_LIMIT");
+    return limit == nullptr ? std::numeric_limits<size_t>::max() : std::strtoull(limit, nullptr, 10);
+}
+
+hipError_t allocate_block(void** block, size_t bytes) {
+    if (bytes > memory_limit()) {
+        *block = nullptr;
+        return hipErrorOutOfMemory;
+    }
+    const hipError_t status = hipMalloc(block, bytes);
+    if (status != hipSuccess) {
+        *block = nullptr;
+        (void)hipGetLastError(); // (or the next launch would be taken for the one that failed)
+    }
+    return status;
+}
+
+/// scratch(bytes); null instead of an error where `needed` is false and the device has not as much memory.
+void* take_block(size_t bytes, bool needed) {
     auto& st = state();
     Resources& res = st.res();
     int device = 0;
@@ -315,14 +344,18 @@ void* scratch(size_t bytes) {
                 "captured into a graph; make one call with the largest shapes on this thread before capturing"
             );
         }
-        size_t capacity = bytes + bytes / 2;
-        if (capacity < (size_t(1) << 20)) {
-            capacity = size_t(1) << 20;
+        size_t capacity = block_capacity(bytes);
+        if (allocate_block(&res.block, COUNTER_BYTES + capacity) != hipSuccess) {
+            // (a device that is nearly full: no more than the call needs)
+            capacity = align256(bytes);
+            const hipError_t status = allocate_block(&res.block, COUNTER_BYTES + capacity);
+            if (status != hipSuccess && !needed) {
+                return nullptr;
+            }
+            check_hip(status, "hipMalloc of scratch memory");
         }
-        constexpr size_t counter_bytes = SCRATCH_COUNTERS * sizeof(int32_t);
-        MOPS_HIP_CHECK(hipMalloc(&res.block, counter_bytes + capacity));
         // (not in a captured graph: a stream that is being captured got its error above)
-        MOPS_HIP_CHECK(hipMemsetAsync(res.block, 0, counter_bytes, st.stream));
+        MOPS_HIP_CHECK(hipMemsetAsync(res.block, 0, COUNTER_BYTES, st.stream));
         res.capacity = capacity;
         res.device = device;
         res.counters_dirty = false;
@@ -359,7 +392,31 @@ void* scratch(size_t bytes) {
     }
     res.block_in_graph = res.block_in_graph || st.capturing;
     st.used_scratch = true;
-    return static_cast<char*>(res.block) + SCRATCH_COUNTERS * sizeof(int32_t);
+    return static_cast<char*>(res.block) + COUNTER_BYTES;
+}
+
+} // namespace
+
+void* scratch(size_t bytes) { return take_block(bytes, true); }
+
+void* scratch_or_null(size_t bytes) {
+    if (!scratch_ready(bytes)) {
+        return nullptr;
+    }
+    const Resources& res = state().res();
+    int device = 0;
+    MOPS_HIP_CHECK(hipGetDevice(&device));
+    if (res.block == nullptr || device != res.device || bytes > res.capacity) { // (not while capturing: scratch_ready)
+        size_t left = 0, total = 0;
+        MOPS_HIP_CHECK(hipMemGetInfo(&left, &total));
+        if (res.block != nullptr && device == res.device && !res.block_in_graph) {
+            left += COUNTER_BYTES + res.capacity; // what growing frees
+        }
+        if (COUNTER_BYTES + block_capacity(bytes) > std::min(left, memory_limit())) {
+            return nullptr;
+        }
+    }
+    return take_block(bytes, false);
 }
 
 bool scratch_ready(size_t bytes) {

@@ -49,6 +49,10 @@ void* scratch(size_t bytes);
 /// the thread has no block of that size. For kernels that are the faster ones for a shape which
 /// others serve without scratch memory: a call that is captured first thing must not fail for them.
 bool scratch_ready(size_t bytes);
+/// scratch(bytes), or null where the thread's block is smaller and cannot grow: during a capture, or
+/// because the device has not as much memory left (the block then stays as it is). For memory that a
+/// call can do without.
+void* scratch_or_null(size_t bytes);
 /// Bytes of the calling thread's scratch block (0: none yet).
 size_t scratch_capacity();
 

@@ -267,3 +267,47 @@ def test_a_captured_call_whose_block_holds_the_copies_only(device):
     done = subprocess.run([sys.executable, "-c", CAPTURED], cwd=ROOT, capture_output=True, text=True, timeout=100)
     assert done.returncode == 0, done.stdout + done.stderr[-3000:]
     assert done.stdout.count("ok ") == 5, done.stdout
+
+
+FULL_DEVICE = THREADS + """
+import os
+LIMIT = "MOPS_AMD_TEST_SCRATCH_LIMIT"  # what a nearly full device has left for the block
+os.environ[LIMIT] = str(200 << 20)
+
+def calls():
+    for name, sizes in [
+        ("product", (768, 20001, 767)), ("grad_A", (768, 767, 20001)), ("grad_W", (20001, 767, 767)),
+        ("gradients", (20001, 767, 767)), ("gradients", (768, 767, 20001)),
+    ]:
+        call, exact, terms = case(*sizes, torch.float64)[name]
+        check(call(), exact, (2.0**-53, 2.0**-53), terms)
+        print("ok", name, library.mops_amd_scratch_capacity(), flush=True)
+        assert library.mops_amd_scratch_capacity() < 200 << 20
+    capacity = library.mops_amd_scratch_capacity()
+    assert 0 < capacity
+    # memory that a call cannot do without: an error, and no trace of it in the next call
+    assert library.mops_amd_reserve_scratch(400 << 20) == 1
+    check(call(), exact, (2.0**-53, 2.0**-53), terms)
+    # no room for half as much again: what is asked for
+    assert library.mops_amd_reserve_scratch(180 << 20) == 0
+    assert library.mops_amd_scratch_capacity() == 180 << 20
+    check(call(), exact, (2.0**-53, 2.0**-53), terms)
+    assert library.mops_amd_scratch_capacity() == 180 << 20
+    # memory again
+    del os.environ[LIMIT]
+    check(call(), exact, (2.0**-53, 2.0**-53), terms)
+    assert library.mops_amd_scratch_capacity() > 300 << 20
+    print("ok", flush=True)
+
+in_a_thread(calls)
+end.set()
+"""
+
+
+@pytest.mark.gpu
+def test_products_on_a_device_that_is_nearly_full(device):
+    """Copies of operands are memory that a call can do without: where the device has none left, the call runs as it would
+    at odd addresses."""
+    done = subprocess.run([sys.executable, "-c", FULL_DEVICE], cwd=ROOT, capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0, done.stdout + done.stderr[-3000:]
+    assert done.stdout.count("ok") == 6, done.stdout
