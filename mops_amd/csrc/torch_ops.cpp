@@ -22,6 +22,7 @@
 // mops_amd/torch.py loads this library when it has been built and registers
 // the same operators from Python otherwise.
 #include <array>
+#include <limits>
 #include <stdexcept>
 #include <string>
 #include <vector>
@@ -527,7 +528,8 @@ at::Tensor layer_values(
     }
     return tensor.contiguous();
 }
-/// (undefined stays undefined: not given)
+/// (undefined stays undefined: not given.) A number that does not fit 32 bits is outside of every range, and has to stay
+/// outside: it becomes -1 or the largest one, not what its lower half happens to be.
 at::Tensor layer_indices(const at::Tensor& tensor, const at::Tensor& like, const char* name, const char* operation) {
     if (!tensor.defined()) {
         return tensor;
@@ -537,6 +539,9 @@ at::Tensor layer_indices(const at::Tensor& tensor, const at::Tensor& like, const
         throw std::runtime_error(
             std::string("mops::") + operation + ": " + name + " must hold integers, on the device of the other tensors"
         );
+    }
+    if (tensor.element_size() > 4) {
+        return tensor.to(at::kLong).clamp(-1, std::numeric_limits<int32_t>::max()).to(at::kInt).contiguous();
     }
     return tensor.to(at::kInt).contiguous();
 }

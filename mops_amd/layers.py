@@ -132,8 +132,16 @@ def _values(*tensors):
     return [None if t is None else _dispatch.contiguous(t) for t in tensors]
 
 
+def _int32(tensor):
+    """A number that does not fit 32 bits is outside of every range, and has to stay outside: it becomes -1 or the
+    largest one, not what its lower half happens to be."""
+    if tensor.dtype.itemsize > 4:
+        tensor = tensor.long().clamp(-1, 2**31 - 1)
+    return _dispatch.as_int32(tensor)
+
+
 def _indices(*tensors):
-    return [None if t is None else _dispatch.as_int32(t) for t in tensors]
+    return [None if t is None else _int32(t) for t in tensors]
 
 
 def _like(wanted, tensor):

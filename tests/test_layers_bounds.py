@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import mops_amd
+from mops_amd import layers
 from tests.test_layers import assert_within, random
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -311,3 +312,48 @@ def test_products_on_a_device_that_is_nearly_full(device):
     done = subprocess.run([sys.executable, "-c", FULL_DEVICE], cwd=ROOT, capture_output=True, text=True, timeout=100)
     assert done.returncode == 0, done.stdout + done.stderr[-3000:]
     assert done.stdout.count("ok") == 6, done.stdout
+
+
+WIDE_INDICES = [
+    0, 4, 5, -1, 2, 3, 2**31 - 1, 2**31, 2**31 + 2, 2**32 - 1, 2**32, 2**32 + 3, -(2**31), -(2**31) - 1, -(2**32), 1, 2**33 + 1,
+    -(2**32) + 2, -(2**63), -(2**63) + 1, 2**63 - 1, 2**62 + 4, 3,
+]  # fmt: skip
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.uint64, torch.uint32, torch.int16, torch.uint8], ids=str)
+def test_wide_indices_in_32_bits(dtype):
+    """An index outside of 32 bits is outside of every range: no other index of 32 bits stands for it."""
+    low, high = (0, 2 ** (8 * dtype.itemsize)) if "uint" in str(dtype) else [s * 2 ** (8 * dtype.itemsize - 1) for s in (-1, 1)]
+    values = [v for v in [*WIDE_INDICES, 2**63, 2**63 + 3, 2**64 - 1, 200] if low <= v < high]
+    got = layers._int32(torch.tensor(values, dtype=dtype))
+    assert got.dtype == torch.int32
+    for value, index in zip(values, got.tolist()):
+        assert index == value if 0 <= value < 2**31 - 1 else index < 0 or index == 2**31 - 1, (value, index)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("where", ["package", "operators"])
+def test_indices_beyond_32_bits_are_outside(device, where):
+    """In every function that takes them, through the package and as an operator."""
+    import mops_amd.torch
+
+    ops = mops_amd if where == "package" else torch.ops.mops
+    groups, columns = 5, 12
+    index = torch.tensor(WIDE_INDICES, device=device)
+    inside = (index >= 0) & (index < groups)
+    narrow = torch.where(inside, index, -1).int()
+    order, offsets = ops.order_by_group(index, groups)
+    assert all(torch.equal(x, y) for x, y in zip((order, offsets), mops_amd.order_by_group(narrow, groups)))
+    assert offsets[-1].item() == int(inside.sum())
+    table = torch.randn(groups, columns, device=device)
+    output = ops.scaled_embedding(table, index, 2.0)
+    assert torch.equal(output, mops_amd.scaled_embedding(table, narrow, 2.0)) and not output[~inside].any()
+    grad_output = torch.randn(len(index), columns, device=device)
+    expected = mops_amd.scaled_embedding_vjp(grad_output, table, narrow, 2.0)
+    if where == "package":
+        assert torch.equal(mops_amd.scaled_embedding_vjp(grad_output, table, index, 2.0), expected)
+        assert torch.equal(mops_amd.scaled_embedding_vjp(grad_output, table, index, 2.0, order, offsets), expected)
+    else:
+        leaf = table.clone().requires_grad_(True)
+        ops.scaled_embedding(leaf, index, 2.0).backward(grad_output)
+        assert torch.equal(leaf.grad, expected)
