@@ -620,10 +620,18 @@ at::Tensor grouped_forward(
     return output;
 }
 
+/// An argument of a Function that may be missing: undefined tensors are none it takes.
+c10::optional<at::Tensor> optional(const at::Tensor& tensor) {
+    return tensor.defined() ? c10::optional<at::Tensor>(tensor) : c10::nullopt;
+}
+at::Tensor or_undefined(const c10::optional<at::Tensor>& tensor) { return tensor.has_value() ? *tensor : at::Tensor(); }
+
 struct GroupedFunction : public Function<GroupedFunction> {
-    static at::Tensor forward(AutogradContext* ctx, at::Tensor A, at::Tensor W, at::Tensor offsets, at::Tensor order) {
-        ctx->save_for_backward({A, W, offsets, order});
-        return grouped_forward(A, W, offsets, order);
+    static at::Tensor forward(
+        AutogradContext* ctx, at::Tensor A, at::Tensor W, at::Tensor offsets, c10::optional<at::Tensor> order
+    ) {
+        ctx->save_for_backward({A, W, offsets, or_undefined(order)});
+        return grouped_forward(A, W, offsets, or_undefined(order));
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const char* op = "grouped_matrix_product_vjp";
@@ -725,8 +733,9 @@ at::Tensor scaled_embedding(const at::Tensor& table, const at::Tensor& indices, 
 at::Tensor grouped_matrix_product(
     const at::Tensor& A, const at::Tensor& W, const at::Tensor& offsets, const c10::optional<at::Tensor>& order
 ) {
-    const at::Tensor rows = order.has_value() ? *order : at::Tensor();
-    return recorded({&A, &W}) ? GroupedFunction::apply(A, W, offsets, rows) : grouped_forward(A, W, offsets, rows);
+    const at::Tensor rows = or_undefined(order);
+    return recorded({&A, &W}) ? GroupedFunction::apply(A, W, offsets, optional(rows))
+                              : grouped_forward(A, W, offsets, rows);
 }
 
 std::tuple<at::Tensor, at::Tensor> gated_residual_norm(
