@@ -401,6 +401,16 @@ _library.define(
     "gated_residual_norm(Tensor residual, Tensor block, Tensor gate, Tensor weight_block, Tensor weight_next, "
     "float residual_scale=1., float epsilon=1e-06) -> (Tensor, Tensor)"
 )
+_library.define("scaled_embedding_vjp(Tensor grad_output, Tensor table, Tensor indices, float scale) -> Tensor")
+_library.define(
+    "grouped_matrix_product_vjp(Tensor grad_output, Tensor A, Tensor W, Tensor offsets, Tensor? order, "
+    "bool[2] wanted) -> (Tensor, Tensor)"
+)
+_library.define(
+    "gated_residual_norm_vjp(Tensor? grad_state, Tensor? grad_next, Tensor residual, Tensor block, Tensor gate, "
+    "Tensor weight_block, Tensor weight_next, float residual_scale, float epsilon, bool[5] wanted) "
+    "-> (Tensor, Tensor, Tensor, Tensor, Tensor)"
+)
 
 
 def _grouped(A, W, offsets, order=None):
@@ -411,11 +421,25 @@ def _update(residual, block, gate, weight_block, weight_next, residual_scale=1.0
     return _layers.gated_residual_norm(residual, block, gate, weight_block, weight_next, residual_scale, epsilon)
 
 
+def _grouped_vjp(grad_output, A, W, offsets, order, wanted):
+    grad_A, grad_W = _layers.grouped_matrix_product_vjp(grad_output, A, W, offsets, order, *wanted)
+    return _or_empty(grad_A, A), _or_empty(grad_W, W)
+
+
+def _update_vjp(grad_state, grad_next, *arguments):
+    *arguments, wanted = arguments
+    grads = _layers.gated_residual_norm_vjp(grad_state, grad_next, *arguments, *wanted)
+    return tuple(_or_empty(grad, arguments[0]) for grad in grads)
+
+
 for _name, _kernel in [
     ("order_by_group", _layers.order_by_group),
     ("scaled_embedding", lambda table, indices, scale=1.0: _layers.scaled_embedding(table, indices, scale)),
     ("grouped_matrix_product", _grouped),
     ("gated_residual_norm", _update),
+    ("scaled_embedding_vjp", _layers.scaled_embedding_vjp),
+    ("grouped_matrix_product_vjp", _grouped_vjp),
+    ("gated_residual_norm_vjp", _update_vjp),
 ]:
     _library.impl(_name, _kernel, "CUDA")
     _library.impl(_name, _refuse_host(_name), "CPU")
@@ -447,7 +471,17 @@ def _embedding_setup(ctx, inputs, output):
 
 def _embedding_backward(ctx, grad_output):
     table, indices = ctx.saved_tensors
-    return _layers.scaled_embedding_vjp(grad_output.contiguous(), table, indices, ctx.scale), None, None
+    return torch.ops.mops.scaled_embedding_vjp(grad_output.contiguous(), table, indices, ctx.scale), None, None
+
+
+def _embedding_vjp_setup(ctx, inputs, output):
+    _, _, indices, ctx.scale = inputs
+    ctx.save_for_backward(indices)
+
+
+def _embedding_vjp_backward(ctx, grad_table):
+    (indices,) = ctx.saved_tensors
+    return torch.ops.mops.scaled_embedding(grad_table.contiguous(), indices, ctx.scale), None, None, None
 
 
 def _grouped_setup(ctx, inputs, output):
@@ -455,10 +489,31 @@ def _grouped_setup(ctx, inputs, output):
 
 
 def _grouped_backward(ctx, grad_output):
-    A, W, offsets, order = ctx.saved_tensors
-    wanted = {"compute_grad_A": ctx.needs_input_grad[0], "compute_grad_W": ctx.needs_input_grad[1]}
-    grads = _layers.grouped_matrix_product_vjp(grad_output.contiguous(), A, W, offsets, order, **wanted)
-    return (*grads, None, None)
+    wanted = list(ctx.needs_input_grad[:2])
+    grads = torch.ops.mops.grouped_matrix_product_vjp(grad_output.contiguous(), *ctx.saved_tensors, wanted)
+    return (*(grad if want else None for grad, want in zip(grads, wanted)), None, None)
+
+
+def _grouped_vjp_setup(ctx, inputs, output):
+    *tensors, ctx.computed = inputs
+    ctx.save_for_backward(*tensors)
+    ctx.set_materialize_grads(False)
+
+
+def _grouped_vjp_backward(ctx, u, v):
+    """With c = grad_output, by group: grad_A = c W^T and grad_W = A^T c."""
+    grad_output, A, W, offsets, order = ctx.saved_tensors
+    u, v = [x.contiguous() if _given(x, computed) else None for x, computed in zip((u, v), ctx.computed)]
+    product, vjp = torch.ops.mops.grouped_matrix_product, torch.ops.mops.grouped_matrix_product_vjp
+    grads = [None, None, None]
+    if ctx.needs_input_grad[0]:
+        parts = [product(a, w, offsets, order) for a, w in ((u, W), (A, v)) if a is not None and w is not None]
+        grads[0] = sum(parts[1:], parts[0]) if parts else None
+    if ctx.needs_input_grad[1] and v is not None:
+        grads[1] = vjp(grad_output, A, v, offsets, order, [True, False])[0]
+    if ctx.needs_input_grad[2] and u is not None:
+        grads[2] = vjp(grad_output, u, W, offsets, order, [False, True])[1]
+    return (*grads, None, None, None)
 
 
 def _update_setup(ctx, inputs, output):
@@ -468,14 +523,26 @@ def _update_setup(ctx, inputs, output):
 
 
 def _update_backward(ctx, grad_state, grad_next):
-    names = ("residual", "block", "gate", "weight_block", "weight_next")
-    wanted = {"compute_grad_" + name: want for name, want in zip(names, ctx.needs_input_grad)}
+    wanted = list(ctx.needs_input_grad[:5])
     cotangents = [None if grad is None else grad.contiguous() for grad in (grad_state, grad_next)]
-    grads = _layers.gated_residual_norm_vjp(*cotangents, *ctx.saved_tensors, ctx.residual_scale, ctx.epsilon, **wanted)
-    return (*grads, None, None)
+    grads = torch.ops.mops.gated_residual_norm_vjp(
+        *cotangents, *ctx.saved_tensors, ctx.residual_scale, ctx.epsilon, wanted
+    )
+    return (*(grad if want else None for grad, want in zip(grads, wanted)), None, None)
+
+
+def _update_vjp_setup(ctx, inputs, output):
+    pass
+
+
+def _update_vjp_backward(ctx, *grads):
+    raise RuntimeError("mops::gated_residual_norm: second derivatives are not supported")
 
 
 for _name, _backward, _setup in [
+    ("scaled_embedding_vjp", _embedding_vjp_backward, _embedding_vjp_setup),
+    ("grouped_matrix_product_vjp", _grouped_vjp_backward, _grouped_vjp_setup),
+    ("gated_residual_norm_vjp", _update_vjp_backward, _update_vjp_setup),
     ("scaled_embedding", _embedding_backward, _embedding_setup),
     ("grouped_matrix_product", _grouped_backward, _grouped_setup),
     ("gated_residual_norm", _update_backward, _update_setup),

@@ -17,10 +17,14 @@
 // vjp_vjp. There is no gradient with respect to C or to index tensors.
 //
 // The operators of the layers (mops/layers.h) follow the same pattern, for 16-bit
-// types as well.
+// types as well. The embedding and the products by group are linear in each
+// argument, so derivatives of their gradients, of any order, are calls of the same
+// operators; of the residual update's gradients there is none, and asking for one
+// is an error.
 //
 // mops_amd/torch.py loads this library when it has been built and registers
 // the same operators from Python otherwise.
+#include <algorithm>
 #include <array>
 #include <limits>
 #include <stdexcept>
@@ -576,28 +580,56 @@ at::Tensor embedding_forward(const at::Tensor& table_, const at::Tensor& indices
     return output;
 }
 
+at::Tensor embedding_vjp(const at::Tensor& grad_output_, const at::Tensor& indices_, int64_t table_rows, double scale) {
+    const char* op = "scaled_embedding_vjp";
+    const at::Tensor grad_output = layer_values(grad_output_, grad_output_, "grad_output", "grad_output", op);
+    const at::Tensor indices = layer_indices(indices_, grad_output_, "indices", op);
+    OnTorchStream stream(grad_output);
+    at::Tensor grad_table = new_tensor({table_rows, grad_output.dim() == 2 ? grad_output.size(1) : 0}, grad_output);
+    by_layer_dtype(grad_output, [&](auto zero) {
+        using T = decltype(zero);
+        mops::cuda::scaled_embedding_vjp<T>(
+            view<T, 2>(grad_table, "grad_table"), view<T, 2>(grad_output, "grad_output"),
+            view<int32_t, 1>(indices, "indices"), mops::Tensor<int32_t, 1>{nullptr, {0}},
+            mops::Tensor<int32_t, 1>{nullptr, {0}}, scale
+        );
+    });
+    return grad_table;
+}
+
+at::Tensor scaled_embedding(const at::Tensor& table, const at::Tensor& indices, double scale);
+
+struct EmbeddingVjp : public Function<EmbeddingVjp> {
+    static at::Tensor forward(
+        AutogradContext* ctx, at::Tensor grad_output, at::Tensor indices, int64_t table_rows, double scale
+    ) {
+        ctx->save_for_backward({indices});
+        ctx->saved_data["scale"] = scale;
+        return embedding_vjp(grad_output, indices, table_rows, scale);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const at::Tensor indices = ctx->get_saved_variables()[0];
+        return {
+            scaled_embedding(grads[0], indices, ctx->saved_data["scale"].toDouble()), at::Tensor(), at::Tensor(),
+            at::Tensor(),
+        };
+    }
+};
+
 struct EmbeddingFunction : public Function<EmbeddingFunction> {
     static at::Tensor forward(AutogradContext* ctx, at::Tensor table, at::Tensor indices, double scale) {
-        ctx->save_for_backward({table, indices});
+        ctx->save_for_backward({indices});
+        ctx->saved_data["table_rows"] = table.dim() == 2 ? table.size(0) : 0;
         ctx->saved_data["scale"] = scale;
         return embedding_forward(table, indices, scale);
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const char* op = "scaled_embedding_vjp";
-        const auto saved = ctx->get_saved_variables();
-        const at::Tensor& table = saved[0];
-        const at::Tensor indices = layer_indices(saved[1], table, "indices", op);
-        const at::Tensor grad_output = layer_values(grads[0], table, "grad_output", "table", op);
-        OnTorchStream stream(table);
-        at::Tensor grad_table = new_like(table);
-        by_layer_dtype(table, [&](auto zero) {
-            using T = decltype(zero);
-            mops::cuda::scaled_embedding_vjp<T>(
-                view<T, 2>(grad_table, "grad_table"), view<T, 2>(grad_output, "grad_output"),
-                view<int32_t, 1>(indices, "indices"), mops::Tensor<int32_t, 1>{nullptr, {0}},
-                mops::Tensor<int32_t, 1>{nullptr, {0}}, ctx->saved_data["scale"].toDouble()
-            );
-        });
+        const at::Tensor indices = ctx->get_saved_variables()[0];
+        const int64_t table_rows = ctx->saved_data["table_rows"].toInt();
+        const double scale = ctx->saved_data["scale"].toDouble();
+        const at::Tensor grad_table = recorded({&grads[0]})
+                                          ? EmbeddingVjp::apply(grads[0], indices, table_rows, scale)
+                                          : embedding_vjp(grads[0], indices, table_rows, scale);
         return {grad_table, at::Tensor(), at::Tensor()};
     }
 };
@@ -626,6 +658,81 @@ c10::optional<at::Tensor> optional(const at::Tensor& tensor) {
 }
 at::Tensor or_undefined(const c10::optional<at::Tensor>& tensor) { return tensor.has_value() ? *tensor : at::Tensor(); }
 
+/// grad_A, grad_W; a gradient that is not wanted comes back undefined.
+std::array<at::Tensor, 2> grouped_vjp(
+    const at::Tensor& grad_output_, const at::Tensor& A_, const at::Tensor& W_, const at::Tensor& offsets_,
+    const at::Tensor& order_, bool want_A, bool want_W
+) {
+    const char* op = "grouped_matrix_product_vjp";
+    const at::Tensor A = layer_values(A_, A_, "A", "A", op), W = layer_values(W_, A_, "W", "A", op);
+    const at::Tensor offsets = layer_indices(offsets_, A_, "offsets", op), order = layer_indices(order_, A_, "order", op);
+    const at::Tensor grad_output = layer_values(grad_output_, A_, "grad_output", "A", op);
+    OnTorchStream stream(A);
+    at::Tensor grad_A = want_A ? new_like(A) : at::Tensor(), grad_W = want_W ? new_like(W) : at::Tensor();
+    by_layer_dtype(A, [&](auto zero) {
+        using T = decltype(zero);
+        mops::cuda::grouped_matrix_product_vjp<T>(
+            view<T, 2>(grad_A, "grad_A"), view<T, 3>(grad_W, "grad_W"), view<T, 2>(grad_output, "grad_output"),
+            view<T, 2>(A, "A"), view<T, 3>(W, "W"), view<int32_t, 1>(offsets, "offsets"),
+            view<int32_t, 1>(order, "order")
+        );
+    });
+    return {grad_A, grad_W};
+}
+
+at::Tensor grouped_product(const at::Tensor& A, const at::Tensor& W, const at::Tensor& offsets, const at::Tensor& order);
+std::array<at::Tensor, 2> grouped_gradients(
+    const at::Tensor& grad_output, const at::Tensor& A, const at::Tensor& W, const at::Tensor& offsets,
+    const at::Tensor& order, bool want_A, bool want_W
+);
+
+struct GroupedVjp : public Function<GroupedVjp> {
+    static variable_list forward(
+        AutogradContext* ctx, at::Tensor grad_output, at::Tensor A, at::Tensor W, at::Tensor offsets,
+        c10::optional<at::Tensor> order_, bool want_A, bool want_W
+    ) {
+        const at::Tensor order = or_undefined(order_);
+        ctx->save_for_backward({grad_output, A, W, offsets, order});
+        ctx->saved_data["want_A"] = want_A;
+        ctx->saved_data["want_W"] = want_W;
+        ctx->set_materialize_grads(false);
+        const auto gradients = grouped_vjp(grad_output, A, W, offsets, order, want_A, want_W);
+        return {want_A ? gradients[0] : nothing(A), want_W ? gradients[1] : nothing(W)};
+    }
+    /// With u, v for grad_A = c W^T and grad_W = A^T c (c: grad_output), all of them by group: the gradient for c is
+    /// u W + A v (each rounded by itself, as autograd adds up gradients), that for A is c v^T, that for W is u^T c.
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &grad_output = saved[0], &A = saved[1], &W = saved[2], &offsets = saved[3], &order = saved[4];
+        const at::Tensor u = or_undefined(grads[0], ctx->saved_data["want_A"].toBool());
+        const at::Tensor v = or_undefined(grads[1], ctx->saved_data["want_W"].toBool());
+        variable_list result(7);
+        if (ctx->needs_input_grad(0)) {
+            const at::Tensor from_u = u.defined() ? grouped_product(u, W, offsets, order) : at::Tensor();
+            const at::Tensor from_v = v.defined() ? grouped_product(A, v, offsets, order) : at::Tensor();
+            result[0] = from_u.defined() && from_v.defined() ? from_u + from_v : from_u.defined() ? from_u : from_v;
+        }
+        if (ctx->needs_input_grad(1) && v.defined()) {
+            result[1] = grouped_gradients(grad_output, A, v, offsets, order, true, false)[0];
+        }
+        if (ctx->needs_input_grad(2) && u.defined()) {
+            result[2] = grouped_gradients(grad_output, u, W, offsets, order, false, true)[1];
+        }
+        return result;
+    }
+};
+
+std::array<at::Tensor, 2> grouped_gradients(
+    const at::Tensor& grad_output, const at::Tensor& A, const at::Tensor& W, const at::Tensor& offsets,
+    const at::Tensor& order, bool want_A, bool want_W
+) {
+    if (!recorded({&grad_output, &A, &W})) {
+        return grouped_vjp(grad_output, A, W, offsets, order, want_A, want_W);
+    }
+    const variable_list gradients = GroupedVjp::apply(grad_output, A, W, offsets, optional(order), want_A, want_W);
+    return {or_undefined(gradients[0], want_A), or_undefined(gradients[1], want_W)};
+}
+
 struct GroupedFunction : public Function<GroupedFunction> {
     static at::Tensor forward(
         AutogradContext* ctx, at::Tensor A, at::Tensor W, at::Tensor offsets, c10::optional<at::Tensor> order
@@ -634,23 +741,11 @@ struct GroupedFunction : public Function<GroupedFunction> {
         return grouped_forward(A, W, offsets, or_undefined(order));
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const char* op = "grouped_matrix_product_vjp";
         const auto saved = ctx->get_saved_variables();
-        const at::Tensor A = layer_values(saved[0], saved[0], "A", "A", op), W = layer_values(saved[1], saved[0], "W", "A", op);
-        const at::Tensor offsets = layer_indices(saved[2], A, "offsets", op), order = layer_indices(saved[3], A, "order", op);
-        const at::Tensor grad_output = layer_values(grads[0], A, "grad_output", "A", op);
-        OnTorchStream stream(A);
-        at::Tensor grad_A = ctx->needs_input_grad(0) ? new_like(A) : at::Tensor();
-        at::Tensor grad_W = ctx->needs_input_grad(1) ? new_like(W) : at::Tensor();
-        by_layer_dtype(A, [&](auto zero) {
-            using T = decltype(zero);
-            mops::cuda::grouped_matrix_product_vjp<T>(
-                view<T, 2>(grad_A, "grad_A"), view<T, 3>(grad_W, "grad_W"), view<T, 2>(grad_output, "grad_output"),
-                view<T, 2>(A, "A"), view<T, 3>(W, "W"), view<int32_t, 1>(offsets, "offsets"),
-                view<int32_t, 1>(order, "order")
-            );
-        });
-        return {grad_A, grad_W, at::Tensor(), at::Tensor()};
+        const auto gradients = grouped_gradients(
+            grads[0], saved[0], saved[1], saved[2], saved[3], ctx->needs_input_grad(0), ctx->needs_input_grad(1)
+        );
+        return {gradients[0], gradients[1], at::Tensor(), at::Tensor()};
     }
 };
 
@@ -681,6 +776,61 @@ std::tuple<at::Tensor, at::Tensor> update_forward(
     return {state, next};
 }
 
+typedef std::array<bool, 5> Wanted;
+
+/// The gradients; undefined where not wanted. grad_state, grad_next: undefined for zero.
+std::array<at::Tensor, 5> update_vjp(
+    const at::Tensor& grad_state, const at::Tensor& grad_next, const std::array<at::Tensor, 5>& tensors,
+    double residual_scale, double epsilon, const Wanted& wanted
+) {
+    const char* op = "gated_residual_norm_vjp";
+    const auto in = update_inputs(tensors, op);
+    const std::array<at::Tensor, 2> grads = {grad_state, grad_next};
+    std::array<at::Tensor, 2> cotangent;
+    for (size_t i = 0; i < 2; i++) {
+        cotangent[i] = grads[i].defined()
+                           ? layer_values(grads[i], in[0], i == 0 ? "grad_state" : "grad_next", "residual", op)
+                           : at::Tensor();
+    }
+    OnTorchStream stream(in[0]);
+    std::array<at::Tensor, 5> out;
+    for (size_t i = 0; i < 5; i++) {
+        out[i] = wanted[i] ? new_like(in[i]) : at::Tensor();
+    }
+    by_layer_dtype(in[0], [&](auto zero) {
+        using T = decltype(zero);
+        mops::cuda::gated_residual_norm_vjp<T>(
+            view<T, 2>(out[0], "grad_residual"), view<T, 2>(out[1], "grad_block"), view<T, 2>(out[2], "grad_gate"),
+            view<T, 1>(out[3], "grad_weight_block"), view<T, 1>(out[4], "grad_weight_next"),
+            view<T, 2>(cotangent[0], "grad_state"), view<T, 2>(cotangent[1], "grad_next"),
+            view<T, 2>(in[0], "residual"), view<T, 2>(in[1], "block"), view<T, 2>(in[2], "gate"),
+            view<T, 1>(in[3], "weight_block"), view<T, 1>(in[4], "weight_next"), residual_scale, epsilon
+        );
+    });
+    return out;
+}
+
+/// The gradients where they are recorded themselves: there is no derivative of them, which whoever asks for one is told.
+struct UpdateVjp : public Function<UpdateVjp> {
+    static variable_list forward(
+        AutogradContext*, c10::optional<at::Tensor> grad_state_, c10::optional<at::Tensor> grad_next_, at::Tensor residual,
+        at::Tensor block, at::Tensor gate, at::Tensor weight_block, at::Tensor weight_next, double residual_scale,
+        double epsilon, Wanted wanted
+    ) {
+        const at::Tensor grad_state = or_undefined(grad_state_), grad_next = or_undefined(grad_next_);
+        const std::array<at::Tensor, 5> in = {residual, block, gate, weight_block, weight_next};
+        const auto gradients = update_vjp(grad_state, grad_next, in, residual_scale, epsilon, wanted);
+        variable_list results;
+        for (size_t i = 0; i < 5; i++) {
+            results.push_back(wanted[i] ? gradients[i] : nothing(residual));
+        }
+        return results;
+    }
+    static variable_list backward(AutogradContext*, variable_list) {
+        throw std::runtime_error("mops::gated_residual_norm: second derivatives are not supported");
+    }
+};
+
 struct UpdateFunction : public Function<UpdateFunction> {
     static variable_list forward(
         AutogradContext* ctx, at::Tensor residual, at::Tensor block, at::Tensor gate, at::Tensor weight_block,
@@ -695,32 +845,26 @@ struct UpdateFunction : public Function<UpdateFunction> {
         return {state, next};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        const char* op = "gated_residual_norm_vjp";
-        const auto saved = ctx->get_saved_variables();
-        const auto in = update_inputs({saved[0], saved[1], saved[2], saved[3], saved[4]}, op);
-        std::array<at::Tensor, 2> cotangent;
-        for (size_t i = 0; i < 2; i++) {
-            cotangent[i] = grads[i].defined()
-                               ? layer_values(grads[i], in[0], i == 0 ? "grad_state" : "grad_next", "residual", op)
-                               : at::Tensor();
-        }
-        OnTorchStream stream(in[0]);
-        std::array<at::Tensor, 5> out;
+        const auto in = ctx->get_saved_variables();
+        const double scale = ctx->saved_data["residual_scale"].toDouble(), epsilon = ctx->saved_data["epsilon"].toDouble();
+        Wanted wanted;
         for (size_t i = 0; i < 5; i++) {
-            out[i] = ctx->needs_input_grad(i) ? new_like(in[i]) : at::Tensor();
+            wanted[i] = ctx->needs_input_grad(i);
         }
-        by_layer_dtype(in[0], [&](auto zero) {
-            using T = decltype(zero);
-            mops::cuda::gated_residual_norm_vjp<T>(
-                view<T, 2>(out[0], "grad_residual"), view<T, 2>(out[1], "grad_block"), view<T, 2>(out[2], "grad_gate"),
-                view<T, 1>(out[3], "grad_weight_block"), view<T, 1>(out[4], "grad_weight_next"),
-                view<T, 2>(cotangent[0], "grad_state"), view<T, 2>(cotangent[1], "grad_next"),
-                view<T, 2>(in[0], "residual"), view<T, 2>(in[1], "block"), view<T, 2>(in[2], "gate"),
-                view<T, 1>(in[3], "weight_block"), view<T, 1>(in[4], "weight_next"),
-                ctx->saved_data["residual_scale"].toDouble(), ctx->saved_data["epsilon"].toDouble()
-            );
-        });
-        return {out[0], out[1], out[2], out[3], out[4], at::Tensor(), at::Tensor()};
+        variable_list result(7);
+        if (recorded({&grads[0], &grads[1], &in[0], &in[1], &in[2], &in[3], &in[4]})) {
+            const variable_list gradients =
+                UpdateVjp::apply(
+                    optional(grads[0]), optional(grads[1]), in[0], in[1], in[2], in[3], in[4], scale, epsilon, wanted
+                );
+            for (size_t i = 0; i < 5; i++) {
+                result[i] = or_undefined(gradients[i], wanted[i]);
+            }
+        } else {
+            const auto gradients = update_vjp(grads[0], grads[1], {in[0], in[1], in[2], in[3], in[4]}, scale, epsilon, wanted);
+            std::copy(gradients.begin(), gradients.end(), result.begin());
+        }
+        return result;
     }
 };
 
@@ -730,12 +874,15 @@ at::Tensor scaled_embedding(const at::Tensor& table, const at::Tensor& indices, 
                               : embedding_forward(table, indices, scale);
 }
 
+at::Tensor grouped_product(const at::Tensor& A, const at::Tensor& W, const at::Tensor& offsets, const at::Tensor& order) {
+    return recorded({&A, &W}) ? GroupedFunction::apply(A, W, offsets, optional(order))
+                              : grouped_forward(A, W, offsets, order);
+}
+
 at::Tensor grouped_matrix_product(
     const at::Tensor& A, const at::Tensor& W, const at::Tensor& offsets, const c10::optional<at::Tensor>& order
 ) {
-    const at::Tensor rows = or_undefined(order);
-    return recorded({&A, &W}) ? GroupedFunction::apply(A, W, offsets, optional(rows))
-                              : grouped_forward(A, W, offsets, rows);
+    return grouped_product(A, W, offsets, or_undefined(order));
 }
 
 std::tuple<at::Tensor, at::Tensor> gated_residual_norm(

@@ -22,9 +22,12 @@ has one, ``mops-torch/src/{hpe,sap,opsa}.cpp``); the two weighted operations
 have none, as in the reference.
 
 The operators of the layers around them (``mops_amd.layers``; not part of the
-reference) are registered beside them, with first derivatives, for ``bfloat16``
-and ``float16`` as well: ``order_by_group``, ``scaled_embedding``,
-``grouped_matrix_product``, ``gated_residual_norm``.
+reference) are registered beside them, for ``bfloat16`` and ``float16`` as well:
+``order_by_group``, ``scaled_embedding``, ``grouped_matrix_product``,
+``gated_residual_norm``. The gradients of the embedding and of the products are
+calls of the same operators and can be differentiated again (a loss on forces);
+``gated_residual_norm`` has first derivatives, and differentiating its gradients
+raises an error.
 
 Host tensors are refused: this library is the device path only.
 """
