@@ -40,10 +40,17 @@ constexpr int AHEAD = 8;            // rows that a team has on their way
 constexpr int32_t PLACES_EACH = 32;
 constexpr int32_t CHUNKS = 1024;
 constexpr int32_t CHUNK_PLACES = 64;
-constexpr int32_t ALONE = 64;       // places that a team sums up by itself
-constexpr int32_t FEW = 16;         // rows per table row from which on a workgroup has one table row
+// Places that a team sums up by itself (with 32, 64 and 128, a plan given: 32 768 tokens of 100 003, 2048 bfloat16: 90, 90 and
+// 134 us; 44 721 rows of 33 749, 223 float16: 19, 26 and 42; 65 536 of 50 000, 512 bfloat16, skewed: 40, 50 and 66).
+constexpr int32_t ALONE = 64;
+// Rows per table row from which on a workgroup has one table row (with 4, 16 and 64, a plan given: 30 000 rows of 5000, 256
+// floats: 12.2, 8.5 and 8.0 us; 200 000 of them: 34, 34 and 37; 20 000 rows of 1000, 64 floats, skewed: 8.3, 8.8 and 10.8;
+// 12 000 of them: 7.7, 10.3 and 10.2; 80 000 of 2000, 8 floats, skewed: 8.8, 8.4 and 12.8).
+constexpr int32_t FEW = 16;
 constexpr int32_t ROWS_PER_TEAM = 8; // at most
-constexpr int32_t TABLE_ROWS = 1024; // of a workgroup, at most
+// Table rows of a workgroup, at most: their places in LDS (few_rows_kernel). They matter where rows are a few numbers wide
+// (200 rows of 3 000 000, 2 floats: 15.0 us, with 256 of them 18.3; 18 050 of 1 000 000, 3 float16: 11.5 and 11.2).
+constexpr int32_t TABLE_ROWS = 1024;
 
 /// How a row's pieces are shared out: `team` lanes (a power of two) hold a piece each.
 struct Teams {

@@ -41,9 +41,13 @@ template <typename T> struct Matrices {
 /// Whether rows that begin anywhere are copied to rows that begin on 16-byte boundaries before they are multiplied.
 /// Memory that is read at odd addresses costs the caches twice the time, and tiles that take it through registers are
 /// half as fast as those that do not: what a number of operations gains against what the copy costs, at rates measured
-/// on either side. (8192 rows, K = L = 2047, float16: 159 us without, 92 us with the copy; 37102 rows, 25 groups,
-/// K = 3196, L = 533, gradients: 752 and 585 us; where each number is used less often it is not worth it: 50595
-/// rows, K = 14, L = 1818, 80 us as it is.)
+/// on either side. As they are / copied, us, where the rule copies: 8192 rows, one group, K = L = 2047, the product: float16
+/// 158 / 91, float 642 / 579, double 1195 / 1129; K = L = 1023: 43 / 39, 170 / 162, 318 / 298; 37102 rows, 25 groups,
+/// K = 3196, L = 533, float16, gradients: 752 / 585. Where it does not: K = L = 511: float16 20 / 22, float 58 / 56; 255:
+/// 10 / 14, 20 / 24, double 32 / 38; 60 000 rows of 4 groups, 65 x 63: 10 / 22, 17 / 30, 28 / 39; 50 595 rows, K = 15,
+/// L = 1817: 84 / 95, 149 / 156. It looks at sums of operations and bytes only, and costs time where the copied form's
+/// tiles fit worse: gradients of the rows in float and double (8192 x 1023 squared 138 / 160, 262 / 295; 30 000 rows of
+/// 8 groups, 401 x 601 double 264 / 374), the product of 60 000 rows of 20 groups, 101 x 1001 float16 (70 / 81).
 template <typename T> bool worth_copying(const Matrices<T>& q, const Matrices<T>& p, double operations) {
     constexpr double GAIN = sizeof(T) == 2 ? 1.0 / 700 : sizeof(T) == 4 ? 1.0 / 550 : 1.0 / 150; // us per 10^6
     const double bytes = static_cast<double>(q.copied_bytes() + p.copied_bytes());
