@@ -352,6 +352,16 @@ struct TurnedLoader : public Pieces<T, OUTER, DEEP, THREADS, SETS> {
         next = static_cast<size_t>(DEEP * COUNT) * row_width;
         between = static_cast<size_t>(K_EACH) * row_width;
     }
+    /// The same for rows of two halves of row_width numbers, of which blocks of columns come in turn: the first half's
+    /// numbers first .., as many of the second half's, and so on. A wavefront then has the numbers of both halves that
+    /// belong to a column of the result in the same lane.
+    __device__ __forceinline__ void begin_pairs(const T* memory, int32_t row_width, int32_t first) {
+        constexpr int BLOCK = Matrix<T>::BLOCK;
+        const int32_t outer = of_row() * COUNT, column = first + outer / (2 * BLOCK) * BLOCK + outer % BLOCK;
+        begin(memory + (outer / BLOCK % 2 != 0 ? row_width : 0), row_width, column - outer);
+        next *= 2;
+        between *= 2;
+    }
     /// Every piece of the step inside of its row, or outside as a whole.
     __device__ __forceinline__ bool whole() const { return ALIGNED || left >= COUNT || left <= 0; }
 
@@ -385,21 +395,204 @@ template <int LATER> __device__ __forceinline__ void meet() {
     }
 }
 
+/// What a workgroup has of a tile when its sums are complete: what a finish (below) makes results of.
+template <typename T, int BM, int BN, int WM, int WN> struct TileOf {
+    typedef Matrix<T> M;
+    static constexpr int BLOCK = M::BLOCK, MB = BM / WM / BLOCK, NB = BN / WN / BLOCK; // blocks of a wavefront
+    static constexpr int THREADS = WM * WN * WAVE, TILE_ROWS = BM, ACROSS = WN;
+    typename M::Sums (&sums)[MB][NB];
+    char* lds;           // of the steps, free by now (as many bytes as they had)
+    const int32_t* rows; // behind the tile's (not GRAD_SUMS)
+    const GroupUnit& unit;
+    int lane, wave, wave_m; // wave_m: the wavefront's first row of the tile
+    int32_t m0, n0, split;
+
+    static constexpr int HELD = M::HELD;
+    /// Number e of a block: its row of the tile (block i), and its column of the block.
+    __device__ __forceinline__ int row(int i) const { return wave_m + i * BLOCK + lane % BLOCK; }
+    __device__ __forceinline__ int column(int e) const { return M::row_of(lane, e); }
+    /// Which of the wavefronts that share the tile's rows this is.
+    __device__ __forceinline__ int across() const { return wave % WN; }
+};
+
+/// 16 bytes of numbers, in memory at any address that holds numbers.
+template <typename To> struct Packed {
+    static constexpr int COUNT = 16 / sizeof(To);
+    typedef To Numbers __attribute__((ext_vector_type(COUNT)));
+    typedef To Anywhere __attribute__((ext_vector_type(COUNT), aligned(sizeof(To))));
+};
+
+/// LDS in which a wavefront turns over a row of its BLOCKS blocks, to have whole pieces of rows side by side (stored
+/// straight from the registers, 8 bytes of 32 rows per store: 32768 rows, K = 2048, L = 4096, bfloat16: 657 us instead of
+/// 613).
+template <typename T, typename To, int BLOCKS> struct TurnedOver {
+    typedef Matrix<T> M;
+    typedef typename Packed<To>::Numbers Piece;
+    static constexpr int BLOCK = M::BLOCK, COLUMNS = BLOCKS * BLOCK, OF_PIECE = Packed<To>::COUNT, RUN = M::RUN;
+    static constexpr int PIECES = COLUMNS / OF_PIECE, BYTES = BLOCK * COLUMNS * sizeof(To); // of a wavefront
+    static constexpr int ROWS_ABREAST = PIECES >= 16 ? 1 : 16 / PIECES; // rows in 256 bytes, all banks
+    char* mine;
+    int lane;
+
+    static __device__ __forceinline__ int place(int row, int piece) {
+        return (row * PIECES + (piece ^ (row / ROWS_ABREAST & (PIECES - 1)))) * 16;
+    }
+    /// What has been written can be read, or what has been read can be written over.
+    static __device__ __forceinline__ void settle() {
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    }
+    /// value(j, e): number e of block j.
+    template <typename Value> __device__ __forceinline__ void write(Value&& value) const {
+        typedef To Run __attribute__((ext_vector_type(RUN)));
+#pragma unroll
+        for (int j = 0; j < BLOCKS; j++) {
+#pragma unroll
+            for (int e = 0; e < M::HELD; e += RUN) {
+                const int column = j * BLOCK + M::row_of(lane, e);
+                Run run;
+#pragma unroll
+                for (int r = 0; r < RUN; r++) {
+                    run[r] = static_cast<To>(value(j, e + r));
+                }
+                *reinterpret_cast<Run*>(
+                    mine + place(lane % BLOCK, column / OF_PIECE) + column % OF_PIECE * sizeof(To)
+                ) = run;
+            }
+        }
+        settle();
+    }
+    __device__ __forceinline__ Piece read(int row, int piece) const {
+        return *reinterpret_cast<const Piece*>(mine + place(row, piece));
+    }
+};
+
+/// A wavefront's results by pieces. value(i, j, e): number e of block (i, j), j < BLOCKS; store(row, column, numbers): a
+/// piece of 16 bytes of To, its row in the tile and its first column (every wavefront has BLOCKS blocks of columns).
+template <typename To, int BLOCKS, int LDS_BYTES, typename T, int BM, int BN, int WM, int WN, typename Value, typename Store>
+__device__ __forceinline__ void turn_over(const TileOf<T, BM, BN, WM, WN>& t, Value&& value, Store&& store) {
+    typedef TurnedOver<T, To, BLOCKS> Turned;
+    static_assert(Turned::BYTES * WM * WN <= LDS_BYTES, "");
+    const Turned turned{t.lds + t.wave * Turned::BYTES, t.lane};
+#pragma unroll
+    for (int i = 0; i < TileOf<T, BM, BN, WM, WN>::MB; i++) {
+        turned.write([&](int j, int e) { return value(i, j, e); });
+#pragma unroll
+        for (int at = 0; at < Turned::BLOCK * Turned::PIECES; at += WAVE) {
+            const int row = (at + t.lane) / Turned::PIECES, piece = (at + t.lane) % Turned::PIECES;
+            store(
+                t.wave_m + i * Turned::BLOCK + row, t.across() * Turned::COLUMNS + piece * Turned::OF_PIECE,
+                turned.read(row, piece)
+            );
+        }
+        Turned::settle();
+    }
+}
+
+/// A piece to place `n` of a row of n_size numbers (null: no such row). STREAMED: past the caches (a result: 20011 rows,
+/// K = 1280, L = 1000, gradients: 182 us instead of 191; partial results are read again at once).
+template <bool STREAMED, typename To>
+__device__ __forceinline__ void store_piece(
+    To* row, int32_t n, int32_t n_size, const typename Packed<To>::Numbers& numbers
+) {
+    constexpr int OF_PIECE = Packed<To>::COUNT;
+    typedef typename Packed<To>::Anywhere Anywhere;
+    if (row != nullptr && n < n_size) {
+        if (n + OF_PIECE <= n_size) {
+            Anywhere piece;
+#pragma unroll
+            for (int r = 0; r < OF_PIECE; r++) {
+                piece[r] = numbers[r];
+            }
+            if constexpr (STREAMED) {
+                __builtin_nontemporal_store(piece, reinterpret_cast<Anywhere*>(row + n));
+            } else {
+                *reinterpret_cast<Anywhere*>(row + n) = piece;
+            }
+        } else {
+#pragma unroll
+            for (int r = 0; r < OF_PIECE; r++) {
+                if (n + r < n_size) {
+                    row[n + r] = numbers[r];
+                }
+            }
+        }
+    }
+}
+
+/// A finish makes results of a workgroup's sums. PAIRS: p has rows of two halves (Operand::stride numbers each), and a tile
+/// BN / 2 columns of both, block of a wavefront 2 j the first half's, 2 j + 1 the second's. RESTS: the rows of no group have
+/// results as well (of sums that are zero).
+///
+/// This one stores the sums, scaled and rounded to T; where a group or k is split, they are not rounded yet.
+struct AsTheyAre {
+    template <typename Wide> __device__ __forceinline__ Wide operator()(Wide sum) const { return sum; }
+};
+template <typename T, Form FORM, typename Scale = AsTheyAre> struct StoreSums {
+    static constexpr bool PAIRS = false, RESTS = true;
+    [[no_unique_address]] Scale scale;
+
+    template <bool MAY_SPLIT, int LDS_BYTES, int BM, int BN, int WM, int WN>
+    __device__ __forceinline__ void operator()(const Product<T>& g, const TileOf<T, BM, BN, WM, WN>& t) const {
+        auto put = [&](auto zero, auto is_partial, auto&& row_at) {
+            typedef decltype(zero) To;
+            turn_over<To, TileOf<T, BM, BN, WM, WN>::NB, LDS_BYTES>(
+                t, [&](int i, int j, int e) { return scale(t.sums[i][j][e]); },
+                [&](int row, int column, const typename Packed<To>::Numbers& numbers) {
+                    store_piece<!decltype(is_partial)::value, To>(row_at(row), t.n0 + column, g.n_size, numbers);
+                }
+            );
+        };
+        if constexpr (FORM == Form::GRAD_SUMS) {
+            const size_t size = static_cast<size_t>(g.m_size) * g.n_size;
+            auto row_of = [&](auto* result) {
+                return [=, &g, &t](int m) {
+                    return t.m0 + m < g.m_size ? result + static_cast<size_t>(t.m0 + m) * g.n_size : nullptr;
+                };
+            };
+            if (t.unit.of_group > 1) { // (uniform)
+                if (t.unit.slot < g.most_slots) {
+                    put(wide_t<T>(), std::true_type(), row_of(g.partial + t.unit.slot * partial_size(g.m_size, g.n_size)));
+                }
+            } else {
+                put(T(), std::false_type(), row_of(g.out + t.unit.group * size));
+            }
+        } else {
+            auto row_of = [&](auto* result) {
+                return [=, &g, &t](int m) {
+                    return m < t.unit.count ? result + static_cast<size_t>(t.rows[m]) * g.n_size : nullptr;
+                };
+            };
+            if (MAY_SPLIT && g.splits > 1) { // (uniform)
+                if constexpr (MAY_SPLIT) {
+                    put(wide_t<T>(), std::true_type(),
+                        row_of(g.partial + static_cast<size_t>(t.split) * g.groups.n_rows * g.n_size));
+                }
+            } else {
+                put(T(), std::false_type(), row_of(g.out));
+            }
+        }
+    }
+};
+
 /// WM x WN wavefronts; every one of them makes BM / WM x BN / WN numbers, in steps of DEEP pieces of k of which STAGES
 /// are in LDS or on their way there.
 template <int BM, int BN, int DEEP, int STAGES> struct TileLds {
     char stages[STAGES * (BM + BN) * DEEP * 16] __attribute__((aligned(16)));
     int32_t rows[BM];
 };
-template <typename T, Form FORM, int BM, int BN, int WM, int WN, int DEEP, int STAGES, bool ALIGNED>
+template <typename T, Form FORM, int BM, int BN, int WM, int WN, int DEEP, int STAGES, bool ALIGNED, typename Finish>
 __device__ __forceinline__ void make_tile(
-    const Product<T>& g, const uint32_t block, TileLds<BM, BN, DEEP, STAGES>& lds
+    const Product<T>& g, const Finish& finish, const uint32_t block, TileLds<BM, BN, DEEP, STAGES>& lds
 ) {
     typedef Matrix<T> M;
     constexpr int THREADS = WM * WN * WAVE, COUNT = M::COUNT, BLOCK = M::BLOCK;
     constexpr int STEP = DEEP * COUNT, STEPS = DEEP * BLOCK / WAVE;
     constexpr int MB = BM / WM / BLOCK, NB = BN / WN / BLOCK; // blocks of a wavefront
     constexpr bool SUMS = FORM == Form::GRAD_SUMS, Q_TURNED = SUMS, P_TURNED = FORM != Form::GRAD_ROWS;
+    constexpr bool PAIRS = Finish::PAIRS;
+    static_assert(!PAIRS || (FORM == Form::FORWARD && NB % 2 == 0), "pairs of blocks of columns");
     constexpr Units UNITS = SUMS ? Units::OF_GROUPS : Units::OF_ROWS;
     constexpr int SETS = ALIGNED ? 0 : 2; // (what there is room for in registers)
     using QLoader = std::conditional_t<
@@ -439,7 +632,7 @@ __device__ __forceinline__ void make_tile(
         const int32_t height = min(4, units - 4 * band);
         unit_index = 4 * band + in_band % height;
         m0 = 0;
-        n0 = in_band / height / splits * BN;
+        n0 = in_band / height / splits * (PAIRS ? BN / 2 : BN);
         split = in_band / height % splits;
     }
     const GroupUnit unit = of_groups.find(unit_index);
@@ -447,6 +640,9 @@ __device__ __forceinline__ void make_tile(
         return; // (uniform; offsets that are none)
     }
     const bool rest = !SUMS && unit.group == g.groups.n_groups;
+    if (!Finish::RESTS && rest) {
+        return; // (uniform)
+    }
     if constexpr (!SUMS) {
         for (int i = threadIdx.x; i < BM; i += THREADS) {
             const int32_t at = min(i, unit.count - 1);
@@ -481,11 +677,17 @@ __device__ __forceinline__ void make_tile(
         } else {
             q.begin(k_size, [&](int i) { return g.q.data + static_cast<size_t>(rows[i]) * g.q.stride + k_begin; });
         }
-        const size_t of_group = static_cast<size_t>(unit.group) * (P_TURNED ? g.k_size : g.n_size) * g.p.stride;
+        constexpr int HALVES = PAIRS ? 2 : 1;
+        const size_t of_group = static_cast<size_t>(unit.group) * (P_TURNED ? g.k_size : g.n_size) * HALVES * g.p.stride;
         if constexpr (SUMS) {
             p.begin(g.p.data, g.p.stride, n0);
         } else if constexpr (P_TURNED) {
-            p.begin(g.p.data + of_group + static_cast<size_t>(k_begin) * g.p.stride, g.p.stride, n0);
+            const T* const from = g.p.data + of_group + static_cast<size_t>(k_begin) * HALVES * g.p.stride;
+            if constexpr (PAIRS) {
+                p.begin_pairs(from, g.p.stride, n0);
+            } else {
+                p.begin(from, g.p.stride, n0);
+            }
             p.begin_rows();
         } else {
             p.begin(k_size, [&](int i) {
@@ -727,96 +929,10 @@ __device__ __forceinline__ void make_tile(
         meet<0>(); // (nothing is on its way to LDS any more)
     }
 
-    // Every wavefront turns its blocks over in LDS of its own, to store whole pieces of rows side by side (straight from
-    // the registers, 8 bytes of 32 rows per store: 32768 rows, K = 2048, L = 4096, bfloat16: 657 us instead of 613).
     __syncthreads();
-    auto put = [&](auto zero, auto is_partial, auto&& row_at) {
-        typedef decltype(zero) To;
-        constexpr int COLUMNS = BN / WN, OF_PIECE = 16 / sizeof(To), RUN = M::RUN, PIECES = COLUMNS / OF_PIECE;
-        constexpr int ROWS_ABREAST = PIECES >= 16 ? 1 : 16 / PIECES; // rows in 256 bytes, all banks
-        static_assert(BLOCK * COLUMNS * sizeof(To) * WM * WN <= sizeof(lds.stages), "");
-        typedef To Run __attribute__((ext_vector_type(RUN)));
-        typedef To Piece __attribute__((ext_vector_type(OF_PIECE), aligned(sizeof(To))));
-        char* const mine = stages + wave * (BLOCK * COLUMNS * sizeof(To));
-        auto place = [](int row, int piece) {
-            return (row * PIECES + (piece ^ (row / ROWS_ABREAST & (PIECES - 1)))) * 16;
-        };
-#pragma unroll
-        for (int i = 0; i < MB; i++) {
-#pragma unroll
-            for (int j = 0; j < NB; j++) {
-#pragma unroll
-                for (int e = 0; e < M::HELD; e += RUN) {
-                    const int column = j * BLOCK + M::row_of(lane, e);
-                    Run run;
-#pragma unroll
-                    for (int r = 0; r < RUN; r++) {
-                        run[r] = static_cast<To>(sums[i][j][e + r]);
-                    }
-                    *reinterpret_cast<Run*>(
-                        mine + place(lane % BLOCK, column / OF_PIECE) + column % OF_PIECE * sizeof(To)
-                    ) = run;
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
-            for (int at = 0; at < BLOCK * PIECES; at += WAVE) {
-                const int row = (at + lane) / PIECES, piece = (at + lane) % PIECES;
-                const int32_t n = n0 + wave_n + piece * OF_PIECE;
-                To* const to = row_at(wave_m + i * BLOCK + row); // (null: no such row)
-                if (to != nullptr && n < g.n_size) {
-                    const Piece numbers = *reinterpret_cast<const Piece*>(mine + place(row, piece));
-                    if (n + OF_PIECE <= g.n_size) {
-                        // (a result streams past the caches: 20011 rows, K = 1280, L = 1000, gradients: 182 us instead of
-                        // 191; partial results are read again at once)
-                        if constexpr (decltype(is_partial)::value) {
-                            *reinterpret_cast<Piece*>(to + n) = numbers;
-                        } else {
-                            __builtin_nontemporal_store(numbers, reinterpret_cast<Piece*>(to + n));
-                        }
-                    } else {
-#pragma unroll
-                        for (int r = 0; r < OF_PIECE; r++) {
-                            if (n + r < g.n_size) {
-                                to[n + r] = numbers[r];
-                            }
-                        }
-                    }
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-        }
-    };
-    if constexpr (SUMS) {
-        const size_t size = static_cast<size_t>(g.m_size) * g.n_size;
-        auto row_of = [&](auto* result) {
-            return [=, &g](int m) {
-                return m0 + m < g.m_size ? result + static_cast<size_t>(m0 + m) * g.n_size : nullptr;
-            };
-        };
-        if (unit.of_group > 1) { // (uniform)
-            if (unit.slot < g.most_slots) {
-                put(wide_t<T>(), std::true_type(), row_of(g.partial + unit.slot * partial_size(g.m_size, g.n_size)));
-            }
-        } else {
-            put(T(), std::false_type(), row_of(g.out + unit.group * size));
-        }
-    } else {
-        auto row_of = [&](auto* result) {
-            return [=, &g](int m) { return m < unit.count ? result + static_cast<size_t>(rows[m]) * g.n_size : nullptr; };
-        };
-        if (MAY_SPLIT && splits > 1) { // (uniform)
-            if constexpr (MAY_SPLIT) {
-                put(wide_t<T>(), std::true_type(), row_of(g.partial + static_cast<size_t>(split) * g.groups.n_rows * g.n_size));
-            }
-        } else {
-            put(T(), std::false_type(), row_of(g.out));
-        }
-    }
+    finish.template operator()<MAY_SPLIT, sizeof(lds.stages), BM, BN, WM, WN>(
+        g, TileOf<T, BM, BN, WM, WN>{sums, stages, rows, unit, lane, wave, wave_m, m0, n0, split}
+    );
 }
 
 /// The rows of a matrix, each continued with zeros to whole pieces. A workgroup copies COPY_ROWS of them.
@@ -856,23 +972,29 @@ template <typename T> __global__ __launch_bounds__(JOIN_THREADS) void join_split
 
 /// Wavefronts per SIMD: small tiles through registers wait for memory most of the time and have room for four (60094 rows,
 /// K = 107, L = 31, float16: 9.4 us, with three and more pieces on their way in each 12.0).
-template <typename T, int BM, bool ALIGNED> constexpr int ABREAST = BM == 64 && !ALIGNED && sizeof(T) < 8 ? 4 : 2;
+template <typename T, int BM, int BN, bool ALIGNED>
+constexpr int ABREAST = BM == 64 && BN == 64 && !ALIGNED && sizeof(T) < 8 ? 4 : 2;
 
-template <typename T, Form FORM, int BM, int BN, int WM, int WN, int DEEP, int STAGES, bool ALIGNED>
-__global__ __launch_bounds__(WM* WN* WAVE, (ABREAST<T, BM, ALIGNED>)) void tiles_kernel(Product<T> g) {
+template <
+    typename T, Form FORM, int BM, int BN, int WM, int WN, int DEEP, int STAGES, bool ALIGNED, typename Finish = StoreSums<T, FORM>>
+__global__ __launch_bounds__(WM* WN* WAVE, (ABREAST<T, BM, BN, ALIGNED>)) void tiles_kernel(Product<T> g, Finish finish) {
     __shared__ TileLds<BM, BN, DEEP, STAGES> lds;
-    make_tile<T, FORM, BM, BN, WM, WN, DEEP, STAGES, ALIGNED>(g, blockIdx.x, lds);
+    make_tile<T, FORM, BM, BN, WM, WN, DEEP, STAGES, ALIGNED>(g, finish, blockIdx.x, lds);
 }
 
 /// Both gradients in one launch, the sums' tiles (of which there are `of_sums` workgroups, a multiple of 8) in front: they
 /// take longer, and the rows' tiles fill in behind them.
-template <typename T, int BM, int BN, int WM, int WN, int DEEP, int STAGES, bool ALIGNED>
-__global__ __launch_bounds__(WM* WN* WAVE, 2) void gradients_kernel(Product<T> sums, Product<T> rows, uint32_t of_sums) {
+template <
+    typename T, int BM, int BN, int WM, int WN, int DEEP, int STAGES, bool ALIGNED, Form OF_ROWS = Form::GRAD_ROWS,
+    typename FinishSums = StoreSums<T, Form::GRAD_SUMS>, typename FinishRows = StoreSums<T, OF_ROWS>>
+__global__ __launch_bounds__(WM* WN* WAVE, 2) void gradients_kernel(
+    Product<T> sums, Product<T> rows, uint32_t of_sums, FinishSums finish_sums, FinishRows finish_rows
+) {
     __shared__ TileLds<BM, BN, DEEP, STAGES> lds;
     if (blockIdx.x < of_sums) {
-        make_tile<T, Form::GRAD_SUMS, BM, BN, WM, WN, DEEP, STAGES, ALIGNED>(sums, blockIdx.x, lds);
+        make_tile<T, Form::GRAD_SUMS, BM, BN, WM, WN, DEEP, STAGES, ALIGNED>(sums, finish_sums, blockIdx.x, lds);
     } else {
-        make_tile<T, Form::GRAD_ROWS, BM, BN, WM, WN, DEEP, STAGES, ALIGNED>(rows, blockIdx.x - of_sums, lds);
+        make_tile<T, OF_ROWS, BM, BN, WM, WN, DEEP, STAGES, ALIGNED>(rows, finish_rows, blockIdx.x - of_sums, lds);
     }
 }
 
