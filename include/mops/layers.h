@@ -1,6 +1,8 @@
 /* The operators of the layers around the sums over edges: a table looked up by
- * an index, products with a matrix per group of rows, and the normalised,
- * gated residual update around a block. None of these exist in
+ * an index, products with a matrix per group of rows, also as gates of each
+ * other, the normalised, gated residual update around a block; and what they
+ * are trained with: the cross entropy of a linear layer to many classes, and
+ * the norm of all gradients, which are clipped by it. None of these exist in
  * lab-cosmo/mops.
  *
  * Device memory only. Conventions as everywhere in this library: contiguous
@@ -52,8 +54,40 @@ MOPS_EXPORT int mops_amd_order_by_group(
     mops_tensor_1d_i32_t order, mops_tensor_1d_i32_t offsets, mops_tensor_1d_i32_t indices
 );
 
-/* For each type S: */
-#define MOPS_LAYERS_DECLARE(S)                                                                     \
+/* Activations of mops_amd_gated_grouped_product. */
+enum { MOPS_AMD_SILU = 0, MOPS_AMD_GELU = 1, MOPS_AMD_SIGMOID = 2 };
+
+/* A tensor of any of the types among others: `size` numbers that follow each
+ * other in memory. */
+enum { MOPS_AMD_F32 = 0, MOPS_AMD_F64 = 1, MOPS_AMD_BF16 = 2, MOPS_AMD_F16 = 3 };
+typedef struct mops_amd_gradient_t {
+    void* data;
+    int64_t size;
+    int32_t type;
+} mops_amd_gradient_t;
+
+/* norm[0] = sqrt(sum of the squares of all numbers of all gradients), added up
+ * in 64 bits in an order that depends on the sizes only. The array is read
+ * before the call returns. */
+#define MOPS_GRADIENTS_DECLARE(W)                                                                  \
+    MOPS_EXPORT int mops_amd_gradient_norm_##W(                                                    \
+        mops_tensor_1d_##W##_t norm, const mops_amd_gradient_t* gradients, int64_t n_gradients     \
+    );                                                                                             \
+    /* And outputs[i] = gradients[i] * min(1, max_norm / norm), of the same size and type. An      \
+     * output is its gradient's own memory (in place), or shares none with any gradient; outputs   \
+     * share none with each other. max_norm is not negative. A norm that is infinite or            \
+     * not-a-number makes of the gradients what the formula does. */                               \
+    MOPS_EXPORT int mops_amd_clip_gradients_##W(                                                   \
+        mops_tensor_1d_##W##_t norm, const mops_amd_gradient_t* outputs,                           \
+        const mops_amd_gradient_t* gradients, int64_t n_gradients, double max_norm                 \
+    );
+MOPS_GRADIENTS_DECLARE(f32)
+MOPS_GRADIENTS_DECLARE(f64)
+
+#undef MOPS_GRADIENTS_DECLARE
+
+/* For each type S (R: what its sums are held in): */
+#define MOPS_LAYERS_DECLARE(S, R)                                                                  \
     /* output[i, :] = scale * table[indices[i], :]; a row of zeros where indices[i] is outside     \
      * the table. */                                                                               \
     MOPS_EXPORT int mops_amd_scaled_embedding_##S(                                                 \
@@ -77,13 +111,48 @@ MOPS_EXPORT int mops_amd_order_by_group(
         mops_tensor_2d_##S##_t output, mops_tensor_2d_##S##_t A, mops_tensor_3d_##S##_t W,         \
         mops_tensor_1d_i32_t offsets, mops_tensor_1d_i32_t order                                   \
     );                                                                                             \
-    /* grad_A[r, :] = grad_output[r, :] W[g, :, :]^T (zeros for a row in no group), grad_W[g, :, :]\
+    /* grad_A[r, :] = grad_output[r, :] W[g, :, :]^T (zeros for a row in no group), grad_W[g, :, :] \
      * = the sum of A[r, :]^T grad_output[r, :] over the rows of group g (zeros for a group        \
      * without rows). */                                                                           \
     MOPS_EXPORT int mops_amd_grouped_matrix_product_vjp_##S(                                       \
         mops_tensor_2d_##S##_t grad_A, mops_tensor_3d_##S##_t grad_W,                              \
         mops_tensor_2d_##S##_t grad_output, mops_tensor_2d_##S##_t A, mops_tensor_3d_##S##_t W,    \
         mops_tensor_1d_i32_t offsets, mops_tensor_1d_i32_t order                                   \
+    );                                                                                             \
+    /* With W = (W_gate, W_up), L columns each, for the rows r of group g as above:                \
+     *   output[r, :] = act(A[r, :] W_gate[g, :, :]) * (A[r, :] W_up[g, :, :])                     \
+     * W.shape[2] = 2 L is even; a row of zeros for a row in no group. act: MOPS_AMD_SILU          \
+     * (x / (1 + e^-x)), MOPS_AMD_GELU (x times the normal distribution's integral up to x),       \
+     * MOPS_AMD_SIGMOID. The projections are never rounded. */                                     \
+    MOPS_EXPORT int mops_amd_gated_grouped_product_##S(                                            \
+        mops_tensor_2d_##S##_t output, mops_tensor_2d_##S##_t A, mops_tensor_3d_##S##_t W,         \
+        mops_tensor_1d_i32_t offsets, mops_tensor_1d_i32_t order, int32_t activation               \
+    );                                                                                             \
+    /* Its gradients. The gradients of the projections, 2 L numbers per row, are held in scratch   \
+     * memory, rounded to the element type. */                                                     \
+    MOPS_EXPORT int mops_amd_gated_grouped_product_vjp_##S(                                        \
+        mops_tensor_2d_##S##_t grad_A, mops_tensor_3d_##S##_t grad_W,                              \
+        mops_tensor_2d_##S##_t grad_output, mops_tensor_2d_##S##_t A, mops_tensor_3d_##S##_t W,    \
+        mops_tensor_1d_i32_t offsets, mops_tensor_1d_i32_t order, int32_t activation               \
+    );                                                                                             \
+    /* With x[r, v] = A[r, :] . W[v, :] for all classes v (rows of W):                             \
+     *   log_sums[r] = log(sum over v of exp(x[r, v]))                                             \
+     *   losses[r] = log_sums[r] - x[r, targets[r]]                                                \
+     * Both zero for a row whose target is negative or too large: padding, of which nothing is     \
+     * read but the target. The logits x are not rounded, and not held in memory. */               \
+    MOPS_EXPORT int mops_amd_linear_cross_entropy_##S(                                             \
+        mops_tensor_1d_##R##_t losses, mops_tensor_1d_##R##_t log_sums, mops_tensor_2d_##S##_t A,  \
+        mops_tensor_2d_##S##_t W, mops_tensor_1d_i32_t targets                                     \
+    );                                                                                             \
+    /* Its gradients, from those of losses and log_sums (either may be a NULL view: zero) and the  \
+     * log_sums that the call returned. The gradients of the logits are held in scratch memory for \
+     * a piece of the classes at a time (about half a gigabyte), rounded to the element type.      \
+     * Zeros for the rows without a target. */                                                     \
+    MOPS_EXPORT int mops_amd_linear_cross_entropy_vjp_##S(                                         \
+        mops_tensor_2d_##S##_t grad_A, mops_tensor_2d_##S##_t grad_W,                              \
+        mops_tensor_1d_##R##_t grad_losses, mops_tensor_1d_##R##_t grad_log_sums,                  \
+        mops_tensor_2d_##S##_t A, mops_tensor_2d_##S##_t W, mops_tensor_1d_i32_t targets,          \
+        mops_tensor_1d_##R##_t log_sums                                                            \
     );                                                                                             \
     /* With norm(x) = x / sqrt(mean of x^2 over the columns + epsilon), row by row:                \
      *   state = residual + residual_scale * gate * norm(block) * weight_block                     \
@@ -107,10 +176,10 @@ MOPS_EXPORT int mops_amd_order_by_group(
         double residual_scale, double epsilon                                                      \
     );
 
-MOPS_LAYERS_DECLARE(f32)
-MOPS_LAYERS_DECLARE(f64)
-MOPS_LAYERS_DECLARE(bf16)
-MOPS_LAYERS_DECLARE(f16)
+MOPS_LAYERS_DECLARE(f32, f32)
+MOPS_LAYERS_DECLARE(f64, f64)
+MOPS_LAYERS_DECLARE(bf16, f32)
+MOPS_LAYERS_DECLARE(f16, f32)
 
 #undef MOPS_LAYERS_DECLARE
 

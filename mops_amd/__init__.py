@@ -1,7 +1,8 @@
 """mops on AMD Instinct MI355X: the five sparse tensor operations of
 lab-cosmo/mops and their vector-Jacobian products, as hand-written HIP kernels
 for gfx950 behind mops' own C ABI, called here on PyTorch-ROCm tensors; and the
-operators of the layers around them (``mops_amd.layers``).
+operators of the layers around them (``mops_amd.layers``) and of networks of
+such layers (``mops_amd.training``).
 
 The public names are those of the reference's Python package
 (``python/mops/src/mops/__init__.py`` of lab-cosmo/mops).
@@ -33,6 +34,15 @@ from .ops import (  # noqa: F401
     sparse_accumulation_scatter_add_with_weights,
     sparse_accumulation_scatter_add_with_weights_vjp,
     sparse_accumulation_scatter_add_with_weights_vjp_vjp,
+)
+from .training import (  # noqa: F401
+    clip_gradients,
+    clip_gradients_,
+    gated_grouped_product,
+    gated_grouped_product_vjp,
+    gradient_norm,
+    linear_cross_entropy,
+    linear_cross_entropy_vjp,
 )
 from .status import MopsError  # noqa: F401
 

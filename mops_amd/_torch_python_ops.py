@@ -8,6 +8,7 @@ second derivatives; every call goes through the interpreter (and the backward pa
 import torch
 
 from . import layers as _layers
+from . import training as _training
 from . import ops as _ops
 
 
@@ -401,6 +402,21 @@ _library.define(
     "gated_residual_norm(Tensor residual, Tensor block, Tensor gate, Tensor weight_block, Tensor weight_next, "
     "float residual_scale=1., float epsilon=1e-06) -> (Tensor, Tensor)"
 )
+_library.define(
+    "gated_grouped_product(Tensor A, Tensor W, Tensor offsets, Tensor? order=None, str activation='silu') -> Tensor"
+)
+_library.define("linear_cross_entropy(Tensor A, Tensor W, Tensor targets) -> (Tensor, Tensor)")
+_library.define("gradient_norm(Tensor[] gradients) -> Tensor")
+_library.define("clip_gradients(Tensor[] gradients, float max_norm) -> (Tensor[], Tensor)")
+_library.define("clip_gradients_(Tensor(a!)[] gradients, float max_norm) -> Tensor")
+_library.define(
+    "gated_grouped_product_vjp(Tensor grad_output, Tensor A, Tensor W, Tensor offsets, Tensor? order, str activation, "
+    "bool[2] wanted) -> (Tensor, Tensor)"
+)
+_library.define(
+    "linear_cross_entropy_vjp(Tensor? grad_losses, Tensor? grad_log_sums, Tensor A, Tensor W, Tensor targets, "
+    "Tensor log_sums, bool[2] wanted) -> (Tensor, Tensor)"
+)
 _library.define("scaled_embedding_vjp(Tensor grad_output, Tensor table, Tensor indices, float scale) -> Tensor")
 _library.define(
     "grouped_matrix_product_vjp(Tensor grad_output, Tensor A, Tensor W, Tensor offsets, Tensor? order, "
@@ -432,7 +448,44 @@ def _update_vjp(grad_state, grad_next, *arguments):
     return tuple(_or_empty(grad, arguments[0]) for grad in grads)
 
 
+def _gated(A, W, offsets, order=None, activation="silu"):
+    return _training.gated_grouped_product(A, W, offsets, order, activation)
+
+
+def _gated_vjp(grad_output, A, W, offsets, order, activation, wanted):
+    grad_A, grad_W = _training.gated_grouped_product_vjp(grad_output, A, W, offsets, order, activation, *wanted)
+    return _or_empty(grad_A, A), _or_empty(grad_W, W)
+
+
+def _cross_entropy_vjp(grad_losses, grad_log_sums, A, W, targets, log_sums, wanted):
+    grad_A, grad_W = _training.linear_cross_entropy_vjp(grad_losses, grad_log_sums, A, W, targets, log_sums, *wanted)
+    return _or_empty(grad_A, A), _or_empty(grad_W, W)
+
+
+def _of_gradients(function):
+    """A function of a list of gradients: of theirs there is none."""
+
+    def call(gradients, *arguments):
+        if torch.is_grad_enabled() and any(gradient.requires_grad for gradient in gradients):
+            raise RuntimeError(
+                f"mops::{function.__name__}: derivatives are not supported, and a gradient requires one"
+            )
+        with torch.no_grad():
+            return function(gradients, *arguments)
+
+    return call
+
+
+for _function in (_training.gradient_norm, _training.clip_gradients, _training.clip_gradients_):
+    _library.impl(_function.__name__, _of_gradients(_function), "CUDA")
+    _library.impl(_function.__name__, _of_gradients(_function), "AutogradCUDA")
+    _library.impl(_function.__name__, _refuse_host(_function.__name__), "CPU")
+
 for _name, _kernel in [
+    ("gated_grouped_product", _gated),
+    ("linear_cross_entropy", _training.linear_cross_entropy),
+    ("gated_grouped_product_vjp", _gated_vjp),
+    ("linear_cross_entropy_vjp", _cross_entropy_vjp),
     ("order_by_group", _layers.order_by_group),
     ("scaled_embedding", lambda table, indices, scale=1.0: _layers.scaled_embedding(table, indices, scale)),
     ("grouped_matrix_product", _grouped),
@@ -456,6 +509,17 @@ _register_fake(
 _register_fake(
     "grouped_matrix_product", lambda A, W, offsets, order=None: A.new_empty((A.shape[0], W.shape[2]))
 )
+_register_fake(
+    "gated_grouped_product",
+    lambda A, W, offsets, order=None, activation="silu": A.new_empty((A.shape[0], W.shape[2] // 2)),
+)
+
+
+def _fake_sums(A):
+    return A.new_empty((A.shape[0],), dtype=torch.float64 if A.dtype == torch.float64 else torch.float32)
+
+
+_register_fake("linear_cross_entropy", lambda A, W, targets: (_fake_sums(A), _fake_sums(A)))
 _register_fake(
     "gated_residual_norm",
     lambda residual, block, gate, weight_block, weight_next, residual_scale=1.0, epsilon=1e-6: (
@@ -539,7 +603,45 @@ def _update_vjp_backward(ctx, *grads):
     raise RuntimeError("mops::gated_residual_norm: second derivatives are not supported")
 
 
+def _gated_setup(ctx, inputs, output):
+    *tensors, ctx.activation = inputs
+    ctx.save_for_backward(*tensors)
+
+
+def _gated_backward(ctx, grad_output):
+    wanted = list(ctx.needs_input_grad[:2])
+    grads = torch.ops.mops.gated_grouped_product_vjp(
+        grad_output.contiguous(), *ctx.saved_tensors, ctx.activation, wanted
+    )
+    return (*(grad if want else None for grad, want in zip(grads, wanted)), None, None, None)
+
+
+def _gated_vjp_backward(ctx, *grads):
+    raise RuntimeError("mops::gated_grouped_product: second derivatives are not supported")
+
+
+def _cross_entropy_setup(ctx, inputs, output):
+    ctx.save_for_backward(*inputs, output[1])
+    ctx.set_materialize_grads(False)
+
+
+def _cross_entropy_backward(ctx, grad_losses, grad_log_sums):
+    wanted = list(ctx.needs_input_grad[:2])
+    cotangents = [None if grad is None else grad.contiguous() for grad in (grad_losses, grad_log_sums)]
+    *tensors, log_sums = ctx.saved_tensors
+    grads = torch.ops.mops.linear_cross_entropy_vjp(*cotangents, *tensors, log_sums.detach(), wanted)
+    return (*(grad if want else None for grad, want in zip(grads, wanted)), None)
+
+
+def _cross_entropy_vjp_backward(ctx, *grads):
+    raise RuntimeError("mops::linear_cross_entropy: second derivatives are not supported")
+
+
 for _name, _backward, _setup in [
+    ("gated_grouped_product_vjp", _gated_vjp_backward, _update_vjp_setup),
+    ("linear_cross_entropy_vjp", _cross_entropy_vjp_backward, _update_vjp_setup),
+    ("gated_grouped_product", _gated_backward, _gated_setup),
+    ("linear_cross_entropy", _cross_entropy_backward, _cross_entropy_setup),
     ("scaled_embedding_vjp", _embedding_vjp_backward, _embedding_vjp_setup),
     ("grouped_matrix_product_vjp", _grouped_vjp_backward, _grouped_vjp_setup),
     ("gated_residual_norm_vjp", _update_vjp_backward, _update_vjp_setup),

@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <array>
+#include <vector>
 
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -545,6 +546,179 @@ PyObject* gated_residual_norm_vjp(PyObject*, PyObject* const* arguments, Py_ssiz
     );
 }
 
+/// The activation's number.
+bool activation_of(PyObject* object, int32_t& which) {
+    constexpr std::array<const char*, 3> NAMES = {"silu", "gelu", "sigmoid"}; // (in the order of mops/layers.h)
+    for (size_t i = 0; PyUnicode_CheckExact(object) && i < NAMES.size(); i++) {
+        if (PyUnicode_CompareWithASCIIString(object, NAMES[i]) == 0) {
+            which = static_cast<int32_t>(i);
+            return true;
+        }
+    }
+    return false;
+}
+
+PyObject* gated_grouped_product(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
+    Inputs<4> t; // A W offsets order
+    int32_t activation;
+    if (n != 5 || !t.take(arguments, {R2, R3, I1, I1}, true, {false, false, false, true}) ||
+        !activation_of(arguments[4], activation)) {
+        Py_RETURN_NONE;
+    }
+    return run<OfLayers>(
+        t[0], [&] { return new_tensor({t[0].size(0), t[1].size(2) / 2}, t[0]); },
+        [&](auto zero, at::Tensor& output) {
+            using T = decltype(zero);
+            mops::cuda::gated_grouped_product<T>(
+                view<T, 2>(output, "output"), view<T, 2>(t[0], "A"), view<T, 3>(t[1], "W"),
+                view<int32_t, 1>(t[2], "offsets"), view<int32_t, 1>(t[3], "order"), activation
+            );
+        }
+    );
+}
+
+PyObject* gated_grouped_product_vjp(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
+    Inputs<5> t; // grad_output A W offsets order
+    int32_t activation;
+    std::array<bool, 2> want;
+    if (n != 8 || !t.take(arguments, {R2, R2, R3, I1, I1}, true, {false, false, false, false, true}) ||
+        !activation_of(arguments[5], activation) || !flags(arguments + 6, want)) {
+        Py_RETURN_NONE;
+    }
+    return run<OfLayers>(
+        t[0], [&] { return std::array<at::Tensor, 2>{like_if(want[0], t[1]), like_if(want[1], t[2])}; },
+        [&](auto zero, auto& out) {
+            using T = decltype(zero);
+            mops::cuda::gated_grouped_product_vjp<T>(
+                view<T, 2>(out[0], "grad_A"), view<T, 3>(out[1], "grad_W"), view<T, 2>(t[0], "grad_output"),
+                view<T, 2>(t[1], "A"), view<T, 3>(t[2], "W"), view<int32_t, 1>(t[3], "offsets"),
+                view<int32_t, 1>(t[4], "order"), activation
+            );
+        }
+    );
+}
+
+PyObject* linear_cross_entropy(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
+    Inputs<3> t; // A W targets
+    if (n != 3 || !t.take(arguments, {R2, R2, I1}, true)) {
+        Py_RETURN_NONE;
+    }
+    return run<OfLayers>(
+        t[0], [&] { return std::array<at::Tensor, 2>{new_sums(t[0]), new_sums(t[0])}; },
+        [&](auto zero, auto& out) {
+            using T = decltype(zero);
+            using Sum = mops::amd::torch_tensors::sum_t<T>;
+            mops::cuda::linear_cross_entropy<T, Sum>(
+                view<Sum, 1>(out[0], "losses"), view<Sum, 1>(out[1], "log_sums"), view<T, 2>(t[0], "A"),
+                view<T, 2>(t[1], "W"), view<int32_t, 1>(t[2], "targets")
+            );
+        }
+    );
+}
+
+PyObject* linear_cross_entropy_vjp(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
+    // grad_losses grad_log_sums A W targets log_sums (the first two may be None)
+    Inputs<3> t;
+    Inputs<3> sums; // log_sums grad_losses grad_log_sums
+    std::array<bool, 2> want;
+    if (n != 8 || !t.take(arguments + 2, {R2, R2, I1}, true) || !flags(arguments + 6, want)) {
+        Py_RETURN_NONE;
+    }
+    PyObject* const of_sums[3] = {arguments[5], arguments[0], arguments[1]};
+    if (!sums.take(of_sums, {R1, R1, R1}, true, {false, true, true}) || sums[0].device() != t[0].device() ||
+        sums[0].scalar_type() != sum_dtype(t[0])) {
+        Py_RETURN_NONE;
+    }
+    return run<OfLayers>(
+        t[0], [&] { return std::array<at::Tensor, 2>{like_if(want[0], t[0]), like_if(want[1], t[1])}; },
+        [&](auto zero, auto& out) {
+            using T = decltype(zero);
+            using Sum = mops::amd::torch_tensors::sum_t<T>;
+            mops::cuda::linear_cross_entropy_vjp<T, Sum>(
+                view<T, 2>(out[0], "grad_A"), view<T, 2>(out[1], "grad_W"), view<Sum, 1>(sums[1], "grad_losses"),
+                view<Sum, 1>(sums[2], "grad_log_sums"), view<T, 2>(t[0], "A"), view<T, 2>(t[1], "W"),
+                view<int32_t, 1>(t[2], "targets"), view<Sum, 1>(sums[0], "log_sums")
+            );
+        }
+    );
+}
+
+/// The gradients of a list or tuple, if a kernel can take all of them as they are.
+bool gradients_of(PyObject* object, std::vector<at::Tensor>& gradients, bool in_place) {
+    if (!PyList_CheckExact(object) && !PyTuple_CheckExact(object)) {
+        return false;
+    }
+    const Py_ssize_t n = PySequence_Fast_GET_SIZE(object);
+    gradients.reserve(static_cast<size_t>(n));
+    for (Py_ssize_t i = 0; i < n; i++) {
+        PyObject* const item = PySequence_Fast_GET_ITEM(object, i);
+        if (!THPVariable_CheckExact(item)) {
+            return false;
+        }
+        const at::Tensor& t = THPVariable_Unpack(item);
+        if (!is_gradient(t) || (i > 0 && t.device() != gradients[0].device()) || (in_place && t.requires_grad())) {
+            return false;
+        }
+        gradients.push_back(t);
+    }
+    return n > 0;
+}
+
+PyObject* gradient_norm(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
+    std::vector<at::Tensor> gradients;
+    if (n != 1 || !gradients_of(arguments[0], gradients, false)) {
+        Py_RETURN_NONE;
+    }
+    return run<OfIndices>(
+        gradients[0], [&] { return new_norm(gradients); },
+        [&](int32_t, at::Tensor& norm) { norm_of_gradients(norm, gradients); }
+    );
+}
+
+/// gradients, max_norm, whether in place: the norm, or the clipped gradients in front of it.
+PyObject* clip_gradients(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
+    std::vector<at::Tensor> gradients, outputs;
+    double max_norm;
+    std::array<bool, 1> in_place;
+    if (n != 3 || !flags(arguments + 2, in_place) || !gradients_of(arguments[0], gradients, in_place[0]) ||
+        !number(arguments[1], max_norm)) {
+        Py_RETURN_NONE;
+    }
+    PyObject* const norm = run<OfIndices>(
+        gradients[0],
+        [&] {
+            for (const at::Tensor& gradient : gradients) {
+                outputs.push_back(in_place[0] ? gradient : new_gradient(gradient));
+            }
+            return new_norm(gradients);
+        },
+        [&](int32_t, at::Tensor& to) { clip_gradients_to(to, outputs, gradients, max_norm); }
+    );
+    if (norm == nullptr || norm == Py_None) {
+        return norm;
+    }
+    if (in_place[0]) {
+        for (const at::Tensor& gradient : gradients) {
+            gradient.unsafeGetTensorImpl()->bump_version();
+        }
+        return norm;
+    }
+    PyObject* const list = PyList_New(static_cast<Py_ssize_t>(outputs.size()));
+    PyObject* const both = PyTuple_New(2);
+    if (list == nullptr || both == nullptr) {
+        Py_XDECREF(list);
+        Py_XDECREF(both);
+        Py_DECREF(norm);
+        return nullptr;
+    }
+    for (size_t i = 0; i < outputs.size(); i++) {
+        PyList_SET_ITEM(list, static_cast<Py_ssize_t>(i), wrap(outputs[i]));
+    }
+    PyTuple_SET_ITEM(both, 0, list);
+    PyTuple_SET_ITEM(both, 1, norm);
+    return both;
+}
+
 #define MOPS_METHOD(NAME, FUNCTION)                                                                 \
     {NAME, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(FUNCTION)), METH_FASTCALL, nullptr}
 PyMethodDef METHODS[] = {
@@ -566,6 +740,12 @@ PyMethodDef METHODS[] = {
     MOPS_METHOD("scaled_embedding_vjp", scaled_embedding_vjp),
     MOPS_METHOD("grouped_matrix_product", grouped_matrix_product),
     MOPS_METHOD("grouped_matrix_product_vjp", grouped_matrix_product_vjp),
+    MOPS_METHOD("gated_grouped_product", gated_grouped_product),
+    MOPS_METHOD("gated_grouped_product_vjp", gated_grouped_product_vjp),
+    MOPS_METHOD("linear_cross_entropy", linear_cross_entropy),
+    MOPS_METHOD("linear_cross_entropy_vjp", linear_cross_entropy_vjp),
+    MOPS_METHOD("gradient_norm", gradient_norm),
+    MOPS_METHOD("clip_gradients", clip_gradients),
     MOPS_METHOD("gated_residual_norm", gated_residual_norm),
     MOPS_METHOD("gated_residual_norm_vjp", gated_residual_norm_vjp),
     {nullptr, nullptr, 0, nullptr},

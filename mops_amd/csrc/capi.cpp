@@ -5,6 +5,7 @@
 // translate exceptions into a status code plus a per-thread message.
 // The wrappers are generated from the parameter lists in
 // mops/detail/signatures.h.
+#include <cstddef>
 #include <cstdint>
 #include <stdexcept>
 #include <string>
@@ -196,7 +197,40 @@ extern "C" int mops_amd_order_by_group(
     MOPS_CATCH_EXCEPTIONS_END
 }
 
-#define MOPS_LAYERS_DEFINE(S, T)                                                                   \
+namespace {
+
+/// The same layout, as the C++ API has it.
+const mops::Gradient* gradients_of(const mops_amd_gradient_t* gradients) {
+    static_assert(sizeof(mops::Gradient) == sizeof(mops_amd_gradient_t), "");
+    static_assert(offsetof(mops::Gradient, size) == offsetof(mops_amd_gradient_t, size), "");
+    static_assert(offsetof(mops::Gradient, type) == offsetof(mops_amd_gradient_t, type), "");
+    return reinterpret_cast<const mops::Gradient*>(gradients);
+}
+
+} // namespace
+
+#define MOPS_GRADIENTS_DEFINE(W, T)                                                                \
+    extern "C" int mops_amd_gradient_norm_##W(                                                     \
+        mops_tensor_1d_##W##_t norm, const mops_amd_gradient_t* gradients, int64_t n_gradients     \
+    ) {                                                                                            \
+        MOPS_CATCH_EXCEPTIONS_BEGIN                                                                \
+        mops::cuda::gradient_norm<T>(view(norm), gradients_of(gradients), extent(n_gradients));    \
+        MOPS_CATCH_EXCEPTIONS_END                                                                  \
+    }                                                                                              \
+    extern "C" int mops_amd_clip_gradients_##W(                                                    \
+        mops_tensor_1d_##W##_t norm, const mops_amd_gradient_t* outputs,                           \
+        const mops_amd_gradient_t* gradients, int64_t n_gradients, double max_norm                 \
+    ) {                                                                                            \
+        MOPS_CATCH_EXCEPTIONS_BEGIN                                                                \
+        mops::cuda::clip_gradients<T>(                                                             \
+            view(norm), gradients_of(outputs), gradients_of(gradients), extent(n_gradients), max_norm \
+        );                                                                                         \
+        MOPS_CATCH_EXCEPTIONS_END                                                                  \
+    }
+MOPS_GRADIENTS_DEFINE(f32, float)
+MOPS_GRADIENTS_DEFINE(f64, double)
+
+#define MOPS_LAYERS_DEFINE(S, T, R, SUM)                                                           \
     extern "C" int mops_amd_scaled_embedding_##S(                                                  \
         mops_tensor_2d_##S##_t output, mops_tensor_2d_##S##_t table, mops_tensor_1d_i32_t indices, \
         double scale                                                                               \
@@ -237,6 +271,51 @@ extern "C" int mops_amd_order_by_group(
         );                                                                                         \
         MOPS_CATCH_EXCEPTIONS_END                                                                  \
     }                                                                                              \
+    extern "C" int mops_amd_gated_grouped_product_##S(                                             \
+        mops_tensor_2d_##S##_t output, mops_tensor_2d_##S##_t A, mops_tensor_3d_##S##_t W,         \
+        mops_tensor_1d_i32_t offsets, mops_tensor_1d_i32_t order, int32_t activation               \
+    ) {                                                                                            \
+        MOPS_CATCH_EXCEPTIONS_BEGIN                                                                \
+        mops::cuda::gated_grouped_product<T>(                                                      \
+            view(output), view(A), view(W), view(offsets), view(order), activation                 \
+        );                                                                                         \
+        MOPS_CATCH_EXCEPTIONS_END                                                                  \
+    }                                                                                              \
+    extern "C" int mops_amd_gated_grouped_product_vjp_##S(                                         \
+        mops_tensor_2d_##S##_t grad_A, mops_tensor_3d_##S##_t grad_W,                              \
+        mops_tensor_2d_##S##_t grad_output, mops_tensor_2d_##S##_t A, mops_tensor_3d_##S##_t W,    \
+        mops_tensor_1d_i32_t offsets, mops_tensor_1d_i32_t order, int32_t activation               \
+    ) {                                                                                            \
+        MOPS_CATCH_EXCEPTIONS_BEGIN                                                                \
+        mops::cuda::gated_grouped_product_vjp<T>(                                                  \
+            view(grad_A), view(grad_W), view(grad_output), view(A), view(W), view(offsets),        \
+            view(order), activation                                                                \
+        );                                                                                         \
+        MOPS_CATCH_EXCEPTIONS_END                                                                  \
+    }                                                                                              \
+    extern "C" int mops_amd_linear_cross_entropy_##S(                                              \
+        mops_tensor_1d_##R##_t losses, mops_tensor_1d_##R##_t log_sums, mops_tensor_2d_##S##_t A,  \
+        mops_tensor_2d_##S##_t W, mops_tensor_1d_i32_t targets                                     \
+    ) {                                                                                            \
+        MOPS_CATCH_EXCEPTIONS_BEGIN                                                                \
+        mops::cuda::linear_cross_entropy<T, SUM>(                                                  \
+            view(losses), view(log_sums), view(A), view(W), view(targets)                          \
+        );                                                                                         \
+        MOPS_CATCH_EXCEPTIONS_END                                                                  \
+    }                                                                                              \
+    extern "C" int mops_amd_linear_cross_entropy_vjp_##S(                                          \
+        mops_tensor_2d_##S##_t grad_A, mops_tensor_2d_##S##_t grad_W,                              \
+        mops_tensor_1d_##R##_t grad_losses, mops_tensor_1d_##R##_t grad_log_sums,                  \
+        mops_tensor_2d_##S##_t A, mops_tensor_2d_##S##_t W, mops_tensor_1d_i32_t targets,          \
+        mops_tensor_1d_##R##_t log_sums                                                            \
+    ) {                                                                                            \
+        MOPS_CATCH_EXCEPTIONS_BEGIN                                                                \
+        mops::cuda::linear_cross_entropy_vjp<T, SUM>(                                              \
+            view(grad_A), view(grad_W), view(grad_losses), view(grad_log_sums), view(A), view(W),  \
+            view(targets), view(log_sums)                                                          \
+        );                                                                                         \
+        MOPS_CATCH_EXCEPTIONS_END                                                                  \
+    }                                                                                              \
     extern "C" int mops_amd_gated_residual_norm_##S(                                               \
         mops_tensor_2d_##S##_t state, mops_tensor_2d_##S##_t next,                                 \
         mops_tensor_2d_##S##_t residual, mops_tensor_2d_##S##_t block,                             \
@@ -268,7 +347,7 @@ extern "C" int mops_amd_order_by_group(
         MOPS_CATCH_EXCEPTIONS_END                                                                  \
     }
 
-MOPS_LAYERS_DEFINE(f32, float)
-MOPS_LAYERS_DEFINE(f64, double)
-MOPS_LAYERS_DEFINE(bf16, mops::bfloat16)
-MOPS_LAYERS_DEFINE(f16, mops::float16)
+MOPS_LAYERS_DEFINE(f32, float, f32, float)
+MOPS_LAYERS_DEFINE(f64, double, f64, double)
+MOPS_LAYERS_DEFINE(bf16, mops::bfloat16, f32, float)
+MOPS_LAYERS_DEFINE(f16, mops::float16, f32, float)

@@ -1,0 +1,47 @@
+// The cross entropy of a linear layer, as the type-independent part of the
+// operator calls it (cross_entropy.hip); the kernels are compiled once per
+// element type.
+#ifndef MOPS_AMD_CROSS_ENTROPY_HPP
+#define MOPS_AMD_CROSS_ENTROPY_HPP
+
+#include <cstdint>
+
+#include <hip/hip_runtime.h>
+
+#include "numbers.hpp"
+
+namespace mops::amd::cross_entropy {
+
+/// A [rows, k_size], W [classes, k_size], targets [rows].
+template <typename T> struct Inputs {
+    const T *A, *W;
+    const int32_t* targets;
+    int32_t rows, classes, k_size;
+};
+
+template <typename T>
+void forward(const Inputs<T>& inputs, wide_t<T>* losses, wide_t<T>* log_sums, hipStream_t stream);
+/// grad_losses and grad_log_sums may be null (zero), either gradient as well (not wanted).
+template <typename T>
+void gradients(
+    const Inputs<T>& inputs, const wide_t<T>* grad_losses, const wide_t<T>* grad_log_sums, const wide_t<T>* log_sums,
+    T* grad_A, T* grad_W, hipStream_t stream
+);
+
+/// The rows with a target in [0, classes) in ascending order, then the others; offsets = {0, how many have one}.
+/// `counts`: room for row_chunks(rows) numbers.
+size_t row_chunks(int32_t rows);
+void rows_with_targets(
+    int32_t* order, int32_t* offsets, int32_t* counts, const int32_t* targets, int32_t rows, int32_t classes,
+    hipStream_t stream
+);
+
+/// scale = {a power of two, its inverse}: see Unscale.
+void find_scale(
+    float* scale, const float* grad_losses, const float* grad_log_sums, const int32_t* targets, int32_t rows,
+    int32_t classes, hipStream_t stream
+);
+
+} // namespace mops::amd::cross_entropy
+
+#endif

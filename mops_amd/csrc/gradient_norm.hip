@@ -1,0 +1,406 @@
+// The norm of all gradients of a network together, and the gradients scaled so
+// that it is at most max_norm:
+//
+//   norm = sqrt(sum over all tensors and numbers of g^2)
+//   output = g min(1, max_norm / norm)
+//
+// Any number of tensors of any sizes and types goes through one launch per
+// TENSORS of them: their addresses and sizes travel as kernel arguments (a
+// captured launch keeps its own), and their numbers are cut into chunks that the
+// workgroups take in turn. Squares are added up in 64 bits, where neither those
+// of the largest 32-bit or bfloat16 number nor a sum of billions of them lose
+// anything that matters; the order depends on the sizes only. Every workgroup of
+// the second launch adds up the partial sums for itself, and goes through the
+// chunks from the last one back: the caches still hold those.
+//
+// Bound by memory: the gradients are read once for the norm, read and written
+// once to be scaled; in place and below max_norm nothing is read again.
+#include "mops/layers.hpp"
+
+#include <algorithm>
+#include <cmath>
+#include <vector>
+
+#include "device_common.hpp"
+#include "numbers.hpp"
+#include "runtime.hpp"
+
+namespace mops::amd::gradient_norm {
+namespace {
+
+using mops::Gradient;
+using mops::GradientType;
+
+constexpr int THREADS = 256;
+constexpr int PIECES_EACH = 8;                                // of 16 bytes, of a thread and chunk
+constexpr int64_t CHUNK_BYTES = int64_t(THREADS) * PIECES_EACH * 16;
+constexpr int TENSORS = 64;                                   // of a launch: 2 KB of arguments
+constexpr int64_t WORKGROUPS_PER_UNIT = 8;                    // all that a compute unit has room for
+
+int64_t size_of(GradientType type) {
+    return type == GradientType::F64 ? 8 : type == GradientType::F32 ? 4 : 2;
+}
+int64_t chunks_of(const Gradient& g) { return static_cast<int64_t>(ceil_div(g.size * size_of(g.type), CHUNK_BYTES)); }
+
+struct Table {
+    const void* from[TENSORS];
+    void* to[TENSORS];
+    int64_t size[TENSORS];
+    int64_t end[TENSORS]; // chunks of the tensors up to this one
+    GradientType type[TENSORS];
+    int32_t count;
+
+    __device__ __forceinline__ int64_t chunks() const { return end[count - 1]; }
+    /// Which tensor has chunk `chunk`.
+    __device__ __forceinline__ int32_t tensor_of(int64_t chunk) const {
+        int32_t low = 0, high = count - 1;
+        while (low < high) {
+            const int32_t middle = (low + high) / 2;
+            if (end[middle] > chunk) {
+                high = middle;
+            } else {
+                low = middle + 1;
+            }
+        }
+        return low;
+    }
+    __device__ __forceinline__ int64_t begin_of(int32_t tensor) const { return tensor > 0 ? end[tensor - 1] : 0; }
+};
+
+/// body(zero of the type).
+template <typename Body> __device__ __forceinline__ void by_type(GradientType type, Body&& body) { // (uniform)
+    if (type == GradientType::F32) {
+        body(0.f);
+    } else if (type == GradientType::BF16) {
+        body(static_cast<__bf16>(0.f));
+    } else if (type == GradientType::F16) {
+        body(static_cast<_Float16>(0.f));
+    } else {
+        body(0.0);
+    }
+}
+
+/// body(whole, i): piece i of the thread, numbers that begin at first(i); whole: all of the chunk's pieces exist.
+template <typename T> struct Chunk {
+    static constexpr int COUNT = PIECE<T>;
+    static constexpr int64_t NUMBERS = CHUNK_BYTES / sizeof(T);
+    int64_t begin, size;
+
+    __device__ __forceinline__ bool whole() const { return begin + NUMBERS <= size; } // (uniform)
+    __device__ __forceinline__ int64_t first(int i) const { return begin + (i * THREADS + threadIdx.x) * COUNT; }
+};
+
+__device__ __forceinline__ double sum_of_wave(double sum) {
+#pragma unroll
+    for (int s = 1; s < WAVE; s *= 2) {
+        sum += __shfl_xor(sum, s);
+    }
+    return sum;
+}
+/// The sum over the workgroup, in all threads.
+__device__ __forceinline__ double sum_of_workgroup(double sum) {
+    __shared__ double of_wave[THREADS / WAVE];
+    sum = sum_of_wave(sum);
+    if (threadIdx.x % WAVE == 0) {
+        of_wave[threadIdx.x / WAVE] = sum;
+    }
+    __syncthreads();
+    sum = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / WAVE; w++) {
+        sum += of_wave[w];
+    }
+    return sum;
+}
+
+__global__ __launch_bounds__(THREADS) void squares_kernel(double* __restrict__ partial, const Table table) {
+    double sums[2] = {0, 0};
+    for (int64_t chunk = blockIdx.x; chunk < table.chunks(); chunk += gridDim.x) {
+        const int32_t tensor = table.tensor_of(chunk);
+        by_type(table.type[tensor], [&](auto zero) {
+            typedef decltype(zero) T;
+            typedef Piece<T, PIECE<T>> Numbers;
+            const T* const from = static_cast<const T*>(table.from[tensor]);
+            const Chunk<T> c{(chunk - table.begin_of(tensor)) * Chunk<T>::NUMBERS, table.size[tensor]};
+            auto add = [&](double x, int i) { sums[i % 2] += x * x; };
+            if (c.whole()) {
+                Numbers numbers[PIECES_EACH];
+#pragma unroll
+                for (int i = 0; i < PIECES_EACH; i++) {
+                    numbers[i] = Numbers::load(from + c.first(i));
+                }
+#pragma unroll
+                for (int i = 0; i < PIECES_EACH; i++) {
+#pragma unroll
+                    for (int e = 0; e < PIECE<T>; e++) {
+                        add(static_cast<double>(numbers[i].get(e)), e);
+                    }
+                }
+            } else {
+                for (int i = 0; i < PIECES_EACH; i++) {
+                    const int64_t first = c.first(i);
+                    if (first + PIECE<T> <= c.size) {
+                        const Numbers numbers = Numbers::load(from + first);
+#pragma unroll
+                        for (int e = 0; e < PIECE<T>; e++) {
+                            add(static_cast<double>(numbers.get(e)), e);
+                        }
+                    } else {
+                        for (int64_t at = first; at < c.size; at++) {
+                            add(static_cast<double>(from[at]), 0);
+                        }
+                    }
+                }
+            }
+        });
+    }
+    const double sum = sum_of_workgroup(sums[0] + sums[1]);
+    if (threadIdx.x == 0) {
+        partial[blockIdx.x] = sum;
+    }
+}
+
+/// The norm, from the partial sums of all workgroups, in all threads.
+__device__ __forceinline__ double norm_of(const double* partial, int32_t parts) {
+    double sum = 0;
+#pragma unroll 4
+    for (int32_t i = threadIdx.x; i < parts; i += THREADS) {
+        sum += partial[i];
+    }
+    return sqrt(sum_of_workgroup(sum));
+}
+
+template <typename Sum>
+__global__ __launch_bounds__(THREADS) void norm_kernel(Sum* __restrict__ norm, const double* __restrict__ partial, int32_t parts) {
+    const double all = norm_of(partial, parts);
+    if (threadIdx.x == 0) {
+        *norm = static_cast<Sum>(all);
+    }
+}
+
+/// norm: null in all launches but one.
+template <typename Sum>
+__global__ __launch_bounds__(THREADS) void scale_kernel(
+    Sum* __restrict__ norm, const double* __restrict__ partial, int32_t parts, double max_norm, bool in_place, const Table table
+) {
+    const double all = norm_of(partial, parts);
+    if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) {
+        *norm = static_cast<Sum>(all);
+    }
+    // (a norm that is none, or infinite, makes of the gradients what the formula does)
+    const double factor = all <= max_norm ? 1.0 : max_norm / all;
+    if (in_place && factor == 1.0) {
+        return; // (uniform)
+    }
+    for (int64_t turn = blockIdx.x; turn < table.chunks(); turn += gridDim.x) {
+        const int64_t chunk = table.chunks() - 1 - turn;
+        const int32_t tensor = table.tensor_of(chunk);
+        by_type(table.type[tensor], [&](auto zero) {
+            typedef decltype(zero) T;
+            typedef Piece<T, PIECE<T>> Numbers;
+            const T* const from = static_cast<const T*>(table.from[tensor]);
+            T* const to = static_cast<T*>(table.to[tensor]);
+            const Chunk<T> c{(chunk - table.begin_of(tensor)) * Chunk<T>::NUMBERS, table.size[tensor]};
+            // (16 bits: a factor of 32 bits is exact enough, 2^-24 beside the result's 2^-9)
+            typedef std::conditional_t<sizeof(T) == 2, float, double> Factor;
+            const Factor by = static_cast<Factor>(factor);
+            auto scaled = [&](const Numbers& numbers) {
+                Numbers result;
+#pragma unroll
+                for (int e = 0; e < PIECE<T>; e++) {
+                    result.v[e] = static_cast<T>(static_cast<Factor>(numbers.get(e)) * by);
+                }
+                return result;
+            };
+            if (c.whole()) {
+                Numbers numbers[PIECES_EACH];
+#pragma unroll
+                for (int i = 0; i < PIECES_EACH; i++) {
+                    numbers[i] = Numbers::load(from + c.first(i));
+                }
+#pragma unroll
+                for (int i = 0; i < PIECES_EACH; i++) {
+                    scaled(numbers[i]).stream_to(to + c.first(i));
+                }
+            } else {
+                for (int i = 0; i < PIECES_EACH; i++) {
+                    const int64_t first = c.first(i);
+                    if (first + PIECE<T> <= c.size) {
+                        scaled(Numbers::load(from + first)).store(to + first);
+                    } else {
+                        for (int64_t at = first; at < c.size; at++) {
+                            to[at] = static_cast<T>(static_cast<Factor>(from[at]) * by);
+                        }
+                    }
+                }
+            }
+        });
+    }
+}
+
+/// The gradients in tables of TENSORS, those without numbers left out.
+std::vector<Table> tables_of(const Gradient* outputs, const Gradient* gradients, size_t n) {
+    std::vector<Table> tables;
+    for (size_t i = 0; i < n; i++) {
+        if (gradients[i].size == 0) {
+            continue;
+        }
+        if (tables.empty() || tables.back().count == TENSORS) {
+            tables.emplace_back();
+            tables.back().count = 0;
+        }
+        Table& table = tables.back();
+        const int32_t at = table.count++;
+        table.from[at] = gradients[i].data;
+        table.to[at] = outputs != nullptr ? outputs[i].data : nullptr;
+        table.size[at] = gradients[i].size;
+        table.type[at] = gradients[i].type;
+        table.end[at] = (at > 0 ? table.end[at - 1] : 0) + chunks_of(gradients[i]);
+    }
+    return tables;
+}
+unsigned workgroups_of(const Table& table) {
+    return static_cast<unsigned>(std::min<int64_t>(table.end[table.count - 1], WORKGROUPS_PER_UNIT * compute_units()));
+}
+
+/// The partial sums, in the thread's scratch memory; how many there are.
+double* sum_squares(const std::vector<Table>& tables, int32_t& parts, hipStream_t stream) {
+    size_t all = 0;
+    for (const Table& table : tables) {
+        all += workgroups_of(table);
+    }
+    double* const partial = static_cast<double*>(scratch(align256(std::max<size_t>(all, 1) * sizeof(double))));
+    parts = 0;
+    for (const Table& table : tables) {
+        squares_kernel<<<workgroups_of(table), THREADS, 0, stream>>>(partial + parts, table);
+        MOPS_HIP_CHECK(hipGetLastError());
+        parts += static_cast<int32_t>(workgroups_of(table));
+    }
+    return partial;
+}
+
+void check(const Gradient* gradients, size_t n, const char* what, const char* operation) {
+    for (size_t i = 0; i < n; i++) {
+        const std::string name = std::string(what) + "[" + std::to_string(i) + "]";
+        const int32_t type = static_cast<int32_t>(gradients[i].type);
+        if (type < 0 || type > static_cast<int32_t>(GradientType::F16)) {
+            throw std::runtime_error(name + " has no known type in " + operation);
+        }
+        if (gradients[i].size < 0 || (gradients[i].size > 0 && gradients[i].data == nullptr)) {
+            throw std::runtime_error(name + " has no memory, or a negative size, in " + operation);
+        }
+    }
+}
+
+/// Every output is its own gradient's memory, or shares none with anything else.
+void check_memory(const Gradient* outputs, const Gradient* gradients, size_t n) {
+    struct Span {
+        const char *begin, *end;
+    };
+    auto span = [](const Gradient& g) {
+        const char* const begin = static_cast<const char*>(g.data);
+        return Span{begin, begin + g.size * size_of(g.type)};
+    };
+    std::vector<Span> written;
+    for (size_t i = 0; i < n; i++) {
+        if (outputs[i].size > 0) {
+            written.push_back(span(outputs[i]));
+        }
+    }
+    std::sort(written.begin(), written.end(), [](const Span& a, const Span& b) { return a.begin < b.begin; });
+    for (size_t i = 1; i < written.size(); i++) {
+        if (written[i].begin < written[i - 1].end) {
+            throw std::runtime_error("outputs must not share memory with each other in clip_gradients");
+        }
+    }
+    for (size_t i = 0; i < n; i++) {
+        const Span read = span(gradients[i]);
+        if (read.begin == read.end || outputs[i].data == gradients[i].data) {
+            continue; // (others that write there would share memory with this output)
+        }
+        auto after = std::lower_bound(written.begin(), written.end(), read.end, [](const Span& a, const char* at) {
+            return a.begin < at;
+        });
+        if (after != written.begin() && std::prev(after)->end > read.begin) {
+            throw std::runtime_error(
+                "an output must be its own gradient's memory, or share none with any gradient, in clip_gradients"
+            );
+        }
+    }
+}
+
+template <typename Sum, typename Norm> Sum* check_norm(const Norm& norm, const char* operation) {
+    if (norm.shape[0] != 1) {
+        throw std::runtime_error(std::string("norm must have one element in ") + operation);
+    }
+    return norm.data;
+}
+
+} // namespace
+} // namespace mops::amd::gradient_norm
+
+namespace mops::cuda {
+
+using namespace mops::amd;
+
+template <typename sum_t>
+void gradient_norm(Tensor<sum_t, 1> norm, const Gradient* gradients, size_t n_gradients) {
+    namespace own = mops::amd::gradient_norm;
+    sum_t* const to = own::check_norm<sum_t>(norm, "gradient_norm");
+    own::check(gradients, n_gradients, "gradients", "gradient_norm");
+    const auto tables = own::tables_of(nullptr, gradients, n_gradients);
+    const hipStream_t stream = current_stream();
+    int32_t parts = 0;
+    const double* const partial = own::sum_squares(tables, parts, stream);
+    own::norm_kernel<sum_t><<<1, own::THREADS, 0, stream>>>(to, partial, parts);
+    finish_call("gradient_norm");
+}
+
+template <typename sum_t>
+void clip_gradients(
+    Tensor<sum_t, 1> norm, const Gradient* outputs, const Gradient* gradients, size_t n_gradients, double max_norm
+) {
+    namespace own = mops::amd::gradient_norm;
+    sum_t* const to = own::check_norm<sum_t>(norm, "clip_gradients");
+    if (!(max_norm >= 0)) {
+        throw std::runtime_error("max_norm must be a number that is not negative in clip_gradients");
+    }
+    own::check(gradients, n_gradients, "gradients", "clip_gradients");
+    own::check(outputs, n_gradients, "outputs", "clip_gradients");
+    for (size_t i = 0; i < n_gradients; i++) {
+        if (outputs[i].size != gradients[i].size || outputs[i].type != gradients[i].type) {
+            throw std::runtime_error(
+                "outputs[" + std::to_string(i) + "] must have the size and the type of its gradient in clip_gradients"
+            );
+        }
+    }
+    own::check_memory(outputs, gradients, n_gradients);
+    const auto tables = own::tables_of(outputs, gradients, n_gradients);
+    const hipStream_t stream = current_stream();
+    int32_t parts = 0;
+    const double* const partial = own::sum_squares(tables, parts, stream);
+    if (tables.empty()) {
+        own::norm_kernel<sum_t><<<1, own::THREADS, 0, stream>>>(to, partial, parts);
+    }
+    // the last tensors first (the caches hold those), the norm with the last launch
+    for (size_t i = tables.size(); i-- > 0;) {
+        const own::Table& table = tables[i];
+        bool in_place = true;
+        for (int32_t t = 0; t < table.count; t++) {
+            in_place = in_place && table.to[t] == table.from[t];
+        }
+        own::scale_kernel<sum_t><<<own::workgroups_of(table), own::THREADS, 0, stream>>>(
+            i == 0 ? to : nullptr, partial, parts, max_norm, in_place, table
+        );
+        MOPS_HIP_CHECK(hipGetLastError());
+    }
+    finish_call("clip_gradients");
+}
+
+#define MOPS_GRADIENT_NORM_INSTANTIATE(T)                                                          \
+    template void gradient_norm<T>(Tensor<T, 1>, const Gradient*, size_t);                         \
+    template void clip_gradients<T>(Tensor<T, 1>, const Gradient*, const Gradient*, size_t, double);
+MOPS_GRADIENT_NORM_INSTANTIATE(float)
+MOPS_GRADIENT_NORM_INSTANTIATE(double)
+
+} // namespace mops::cuda

@@ -19,8 +19,9 @@
 // The operators of the layers (mops/layers.h) follow the same pattern, for 16-bit
 // types as well. The embedding and the products by group are linear in each
 // argument, so derivatives of their gradients, of any order, are calls of the same
-// operators; of the residual update's gradients there is none, and asking for one
-// is an error.
+// operators; of the gradients of the residual update, the gated product and the
+// cross entropy there is none, and asking for one is an error, as is a gradient
+// that requires one in a list that is clipped.
 //
 // mops_amd/torch.py loads this library when it has been built and registers
 // the same operators from Python otherwise.
@@ -868,6 +869,197 @@ struct UpdateFunction : public Function<UpdateFunction> {
     }
 };
 
+// -------------------------------------------------- gated products by group --
+int32_t activation_of(const std::string& name, const char* op) {
+    const std::array<const char*, 3> names = {"silu", "gelu", "sigmoid"}; // (in the order of mops/layers.h)
+    for (size_t i = 0; i < names.size(); i++) {
+        if (name == names[i]) {
+            return static_cast<int32_t>(i);
+        }
+    }
+    throw std::runtime_error(std::string("mops::") + op + ": activation must be silu, gelu or sigmoid, got " + name);
+}
+
+at::Tensor gated_forward(
+    const at::Tensor& A_, const at::Tensor& W_, const at::Tensor& offsets_, const at::Tensor& order_, int64_t activation
+) {
+    const char* op = "gated_grouped_product";
+    const at::Tensor A = layer_values(A_, A_, "A", "A", op), W = layer_values(W_, A_, "W", "A", op);
+    const at::Tensor offsets = layer_indices(offsets_, A_, "offsets", op), order = layer_indices(order_, A_, "order", op);
+    OnTorchStream stream(A);
+    at::Tensor output = new_tensor({A.dim() == 2 ? A.size(0) : 0, W.dim() == 3 ? W.size(2) / 2 : 0}, A);
+    by_layer_dtype(A, [&](auto zero) {
+        using T = decltype(zero);
+        mops::cuda::gated_grouped_product<T>(
+            view<T, 2>(output, "output"), view<T, 2>(A, "A"), view<T, 3>(W, "W"), view<int32_t, 1>(offsets, "offsets"),
+            view<int32_t, 1>(order, "order"), static_cast<int32_t>(activation)
+        );
+    });
+    return output;
+}
+
+/// grad_A, grad_W; a gradient that is not wanted comes back undefined.
+std::array<at::Tensor, 2> gated_vjp(
+    const at::Tensor& grad_output_, const at::Tensor& A_, const at::Tensor& W_, const at::Tensor& offsets_,
+    const at::Tensor& order_, int64_t activation, bool want_A, bool want_W
+) {
+    const char* op = "gated_grouped_product_vjp";
+    const at::Tensor A = layer_values(A_, A_, "A", "A", op), W = layer_values(W_, A_, "W", "A", op);
+    const at::Tensor offsets = layer_indices(offsets_, A_, "offsets", op), order = layer_indices(order_, A_, "order", op);
+    const at::Tensor grad_output = layer_values(grad_output_, A_, "grad_output", "A", op);
+    OnTorchStream stream(A);
+    at::Tensor grad_A = want_A ? new_like(A) : at::Tensor(), grad_W = want_W ? new_like(W) : at::Tensor();
+    by_layer_dtype(A, [&](auto zero) {
+        using T = decltype(zero);
+        mops::cuda::gated_grouped_product_vjp<T>(
+            view<T, 2>(grad_A, "grad_A"), view<T, 3>(grad_W, "grad_W"), view<T, 2>(grad_output, "grad_output"),
+            view<T, 2>(A, "A"), view<T, 3>(W, "W"), view<int32_t, 1>(offsets, "offsets"),
+            view<int32_t, 1>(order, "order"), static_cast<int32_t>(activation)
+        );
+    });
+    return {grad_A, grad_W};
+}
+
+/// Gradients where they are recorded themselves: there is no derivative of them, which whoever asks for one is told.
+struct GatedVjp : public Function<GatedVjp> {
+    static variable_list forward(
+        AutogradContext*, at::Tensor grad_output, at::Tensor A, at::Tensor W, at::Tensor offsets,
+        c10::optional<at::Tensor> order, int64_t activation, bool want_A, bool want_W
+    ) {
+        const auto gradients = gated_vjp(grad_output, A, W, offsets, or_undefined(order), activation, want_A, want_W);
+        return {want_A ? gradients[0] : nothing(A), want_W ? gradients[1] : nothing(W)};
+    }
+    static variable_list backward(AutogradContext*, variable_list) {
+        throw std::runtime_error("mops::gated_grouped_product: second derivatives are not supported");
+    }
+};
+
+struct GatedFunction : public Function<GatedFunction> {
+    static at::Tensor forward(
+        AutogradContext* ctx, at::Tensor A, at::Tensor W, at::Tensor offsets, c10::optional<at::Tensor> order,
+        int64_t activation
+    ) {
+        ctx->save_for_backward({A, W, offsets, or_undefined(order)});
+        ctx->saved_data["activation"] = activation;
+        return gated_forward(A, W, offsets, or_undefined(order), activation);
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &A = saved[0], &W = saved[1], &offsets = saved[2], &order = saved[3];
+        const int64_t activation = ctx->saved_data["activation"].toInt();
+        const bool want_A = ctx->needs_input_grad(0), want_W = ctx->needs_input_grad(1);
+        variable_list result(5);
+        if (recorded({&grads[0], &A, &W})) {
+            const variable_list gradients =
+                GatedVjp::apply(grads[0], A, W, offsets, optional(order), activation, want_A, want_W);
+            result[0] = or_undefined(gradients[0], want_A);
+            result[1] = or_undefined(gradients[1], want_W);
+        } else {
+            const auto gradients = gated_vjp(grads[0], A, W, offsets, order, activation, want_A, want_W);
+            std::copy(gradients.begin(), gradients.end(), result.begin());
+        }
+        return result;
+    }
+};
+
+// ------------------------------------------------------------ cross entropy --
+std::tuple<at::Tensor, at::Tensor> cross_entropy_forward(
+    const at::Tensor& A_, const at::Tensor& W_, const at::Tensor& targets_
+) {
+    const char* op = "linear_cross_entropy";
+    const at::Tensor A = layer_values(A_, A_, "A", "A", op), W = layer_values(W_, A_, "W", "A", op);
+    const at::Tensor targets = layer_indices(targets_, A_, "targets", op);
+    OnTorchStream stream(A);
+    at::Tensor losses = new_sums(A), log_sums = new_sums(A);
+    by_layer_dtype(A, [&](auto zero) {
+        using T = decltype(zero);
+        mops::cuda::linear_cross_entropy<T, sum_t<T>>(
+            view<sum_t<T>, 1>(losses, "losses"), view<sum_t<T>, 1>(log_sums, "log_sums"), view<T, 2>(A, "A"),
+            view<T, 2>(W, "W"), view<int32_t, 1>(targets, "targets")
+        );
+    });
+    return {losses, log_sums};
+}
+
+/// (undefined stays undefined: zero)
+at::Tensor sums_of(const at::Tensor& tensor, const at::Tensor& like, const char* name, const char* op) {
+    if (!tensor.defined()) {
+        return tensor;
+    }
+    require_device(tensor, name, op);
+    if (tensor.device() != like.device() || tensor.scalar_type() != sum_dtype(like)) {
+        throw std::runtime_error(
+            std::string("mops::") + op + ": " + name + " must be on the device of A, and float32 (float64 for float64)"
+        );
+    }
+    return tensor.contiguous();
+}
+
+/// grad_losses, grad_log_sums: undefined for zero. grad_A, grad_W; undefined where not wanted.
+std::array<at::Tensor, 2> cross_entropy_vjp(
+    const at::Tensor& grad_losses_, const at::Tensor& grad_log_sums_, const at::Tensor& A_, const at::Tensor& W_,
+    const at::Tensor& targets_, const at::Tensor& log_sums_, bool want_A, bool want_W
+) {
+    const char* op = "linear_cross_entropy_vjp";
+    const at::Tensor A = layer_values(A_, A_, "A", "A", op), W = layer_values(W_, A_, "W", "A", op);
+    const at::Tensor targets = layer_indices(targets_, A_, "targets", op);
+    const at::Tensor log_sums = sums_of(log_sums_, A_, "log_sums", op);
+    const at::Tensor grad_losses = sums_of(grad_losses_, A_, "grad_losses", op);
+    const at::Tensor grad_log_sums = sums_of(grad_log_sums_, A_, "grad_log_sums", op);
+    OnTorchStream stream(A);
+    at::Tensor grad_A = want_A ? new_like(A) : at::Tensor(), grad_W = want_W ? new_like(W) : at::Tensor();
+    by_layer_dtype(A, [&](auto zero) {
+        using T = decltype(zero);
+        mops::cuda::linear_cross_entropy_vjp<T, sum_t<T>>(
+            view<T, 2>(grad_A, "grad_A"), view<T, 2>(grad_W, "grad_W"), view<sum_t<T>, 1>(grad_losses, "grad_losses"),
+            view<sum_t<T>, 1>(grad_log_sums, "grad_log_sums"), view<T, 2>(A, "A"), view<T, 2>(W, "W"),
+            view<int32_t, 1>(targets, "targets"), view<sum_t<T>, 1>(log_sums, "log_sums")
+        );
+    });
+    return {grad_A, grad_W};
+}
+
+struct CrossEntropyVjp : public Function<CrossEntropyVjp> {
+    static variable_list forward(
+        AutogradContext*, c10::optional<at::Tensor> grad_losses, c10::optional<at::Tensor> grad_log_sums, at::Tensor A,
+        at::Tensor W, at::Tensor targets, at::Tensor log_sums, bool want_A, bool want_W
+    ) {
+        const auto gradients = cross_entropy_vjp(
+            or_undefined(grad_losses), or_undefined(grad_log_sums), A, W, targets, log_sums, want_A, want_W
+        );
+        return {want_A ? gradients[0] : nothing(A), want_W ? gradients[1] : nothing(W)};
+    }
+    static variable_list backward(AutogradContext*, variable_list) {
+        throw std::runtime_error("mops::linear_cross_entropy: second derivatives are not supported");
+    }
+};
+
+struct CrossEntropyFunction : public Function<CrossEntropyFunction> {
+    static variable_list forward(AutogradContext* ctx, at::Tensor A, at::Tensor W, at::Tensor targets) {
+        const auto [losses, log_sums] = cross_entropy_forward(A, W, targets);
+        ctx->save_for_backward({A, W, targets, log_sums});
+        ctx->set_materialize_grads(false); // (a gradient that is not there is not read)
+        return {losses, log_sums};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const at::Tensor &A = saved[0], &W = saved[1], &targets = saved[2], &log_sums = saved[3];
+        const bool want_A = ctx->needs_input_grad(0), want_W = ctx->needs_input_grad(1);
+        variable_list result(3);
+        if (recorded({&grads[0], &grads[1], &A, &W})) {
+            const variable_list gradients = CrossEntropyVjp::apply(
+                optional(grads[0]), optional(grads[1]), A, W, targets, log_sums.detach(), want_A, want_W
+            );
+            result[0] = or_undefined(gradients[0], want_A);
+            result[1] = or_undefined(gradients[1], want_W);
+        } else {
+            const auto gradients = cross_entropy_vjp(grads[0], grads[1], A, W, targets, log_sums, want_A, want_W);
+            std::copy(gradients.begin(), gradients.end(), result.begin());
+        }
+        return result;
+    }
+};
+
 // ------------------------------------------------------------ operators --
 at::Tensor scaled_embedding(const at::Tensor& table, const at::Tensor& indices, double scale) {
     return recorded({&table}) ? EmbeddingFunction::apply(table, indices, scale)
@@ -883,6 +1075,87 @@ at::Tensor grouped_matrix_product(
     const at::Tensor& A, const at::Tensor& W, const at::Tensor& offsets, const c10::optional<at::Tensor>& order
 ) {
     return grouped_product(A, W, offsets, or_undefined(order));
+}
+
+at::Tensor gated_grouped_product(
+    const at::Tensor& A, const at::Tensor& W, const at::Tensor& offsets, const c10::optional<at::Tensor>& order,
+    c10::string_view activation
+) {
+    const int64_t which = activation_of(std::string(activation), "gated_grouped_product");
+    return recorded({&A, &W}) ? GatedFunction::apply(A, W, offsets, order, which)
+                              : gated_forward(A, W, offsets, or_undefined(order), which);
+}
+
+std::tuple<at::Tensor, at::Tensor> linear_cross_entropy(
+    const at::Tensor& A, const at::Tensor& W, const at::Tensor& targets
+) {
+    if (!recorded({&A, &W})) {
+        return cross_entropy_forward(A, W, targets);
+    }
+    const variable_list results = CrossEntropyFunction::apply(A, W, targets);
+    return {results[0], results[1]};
+}
+
+/// The gradients of a list as the kernels take them (in_place: or not at all).
+std::vector<at::Tensor> gradients_of(at::TensorList tensors, const char* op, bool in_place) {
+    std::vector<at::Tensor> gradients;
+    for (const at::Tensor& tensor : tensors) {
+        require_device(tensor, "every gradient", op);
+        if (tensor.layout() != at::kStrided || !is_layer_dtype(tensor.scalar_type()) ||
+            tensor.device() != tensors[0].device()) {
+            throw std::runtime_error(
+                std::string("mops::") + op +
+                ": every gradient must be float32, float64, bfloat16 or float16, and on the device of the first"
+            );
+        }
+        if (recorded({&tensor})) {
+            throw std::runtime_error(
+                std::string("mops::") + op + ": derivatives are not supported, and a gradient requires one"
+            );
+        }
+        if (is_gradient(tensor)) {
+            gradients.push_back(tensor);
+        } else if (in_place) {
+            throw std::runtime_error(std::string("mops::") + op + ": every gradient must fill its memory without gaps");
+        } else {
+            gradients.push_back(tensor.resolve_neg().contiguous());
+        }
+    }
+    if (gradients.empty()) {
+        throw std::runtime_error(std::string("mops::") + op + ": there must be at least one gradient");
+    }
+    return gradients;
+}
+
+at::Tensor gradient_norm(at::TensorList tensors) {
+    const auto gradients = gradients_of(tensors, "gradient_norm", false);
+    OnTorchStream stream(gradients[0]);
+    at::Tensor norm = new_norm(gradients);
+    norm_of_gradients(norm, gradients);
+    return norm;
+}
+
+std::tuple<std::vector<at::Tensor>, at::Tensor> clip_gradients(at::TensorList tensors, double max_norm) {
+    const auto gradients = gradients_of(tensors, "clip_gradients", false);
+    OnTorchStream stream(gradients[0]);
+    std::vector<at::Tensor> outputs;
+    for (const at::Tensor& gradient : gradients) {
+        outputs.push_back(new_gradient(gradient));
+    }
+    at::Tensor norm = new_norm(gradients);
+    clip_gradients_to(norm, outputs, gradients, max_norm);
+    return {outputs, norm};
+}
+
+at::Tensor clip_gradients_in_place(at::TensorList tensors, double max_norm) {
+    const auto gradients = gradients_of(tensors, "clip_gradients_", true);
+    OnTorchStream stream(gradients[0]);
+    at::Tensor norm = new_norm(gradients);
+    clip_gradients_to(norm, gradients, gradients, max_norm);
+    for (const at::Tensor& gradient : gradients) {
+        gradient.unsafeGetTensorImpl()->bump_version();
+    }
+    return norm;
 }
 
 std::tuple<at::Tensor, at::Tensor> gated_residual_norm(
@@ -949,6 +1222,14 @@ TORCH_LIBRARY(mops, m) {
         "grouped_matrix_product(Tensor A, Tensor W, Tensor offsets, Tensor? order=None) -> Tensor",
         grouped_matrix_product
     );
+    m.def(
+        "gated_grouped_product(Tensor A, Tensor W, Tensor offsets, Tensor? order=None, str activation='silu') -> Tensor",
+        gated_grouped_product
+    );
+    m.def("linear_cross_entropy(Tensor A, Tensor W, Tensor targets) -> (Tensor, Tensor)", linear_cross_entropy);
+    m.def("gradient_norm(Tensor[] gradients) -> Tensor", gradient_norm);
+    m.def("clip_gradients(Tensor[] gradients, float max_norm) -> (Tensor[], Tensor)", clip_gradients);
+    m.def("clip_gradients_(Tensor(a!)[] gradients, float max_norm) -> Tensor", clip_gradients_in_place);
     m.def(
         "gated_residual_norm(Tensor residual, Tensor block, Tensor gate, Tensor weight_block, Tensor weight_next, "
         "float residual_scale=1., float epsilon=1e-06) -> (Tensor, Tensor)",

@@ -5,6 +5,8 @@
 
 #include <stdexcept>
 #include <string>
+#include <type_traits>
+#include <vector>
 
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
@@ -82,6 +84,73 @@ inline at::Tensor new_tensor(at::IntArrayRef sizes, const at::Tensor& like) {
     );
 }
 inline at::Tensor new_like(const at::Tensor& like) { return new_tensor(like.sizes(), like); }
+
+/// What the sums of an element type are held in.
+template <typename T> using sum_t = std::conditional_t<std::is_same_v<T, double>, double, float>;
+inline at::ScalarType sum_dtype(const at::Tensor& like) {
+    return like.scalar_type() == at::kDouble ? at::kDouble : at::kFloat;
+}
+/// A sum for each row of `like`.
+inline at::Tensor new_sums(const at::Tensor& like) {
+    return at::detail::empty_cuda(
+        {like.dim() > 0 ? like.size(0) : 0}, sum_dtype(like), c10::nullopt, like.device(), c10::nullopt, c10::nullopt
+    );
+}
+
+// ------------------------------------------------------ lists of gradients --
+/// A tensor whose numbers fill a piece of device memory, in whatever order of dimensions.
+inline bool is_gradient(const at::Tensor& t) {
+    return t.is_cuda() && t.layout() == at::kStrided && t.has_storage() && !t.is_neg() &&
+           is_layer_dtype(t.scalar_type()) && t.is_non_overlapping_and_dense();
+}
+/// Its like, in the same order of dimensions.
+inline at::Tensor new_gradient(const at::Tensor& like) {
+    return like.is_contiguous() ? new_like(like) : at::empty_like(like);
+}
+inline at::Tensor new_norm(const std::vector<at::Tensor>& gradients) {
+    bool wide = false;
+    for (const at::Tensor& gradient : gradients) {
+        wide = wide || gradient.scalar_type() == at::kDouble;
+    }
+    return at::detail::empty_cuda(
+        {}, wide ? at::kDouble : at::kFloat, c10::nullopt, gradients[0].device(), c10::nullopt, c10::nullopt
+    );
+}
+inline std::vector<mops::Gradient> views_of(const std::vector<at::Tensor>& gradients) {
+    std::vector<mops::Gradient> views;
+    views.reserve(gradients.size());
+    for (const at::Tensor& gradient : gradients) {
+        const at::ScalarType type = gradient.scalar_type();
+        views.push_back(mops::Gradient{
+            gradient.data_ptr(), gradient.numel(),
+            type == at::kFloat    ? mops::GradientType::F32
+            : type == at::kDouble ? mops::GradientType::F64
+            : type == at::kHalf   ? mops::GradientType::F16
+                                  : mops::GradientType::BF16,
+        });
+    }
+    return views;
+}
+inline void norm_of_gradients(const at::Tensor& norm, const std::vector<at::Tensor>& gradients) {
+    const auto views = views_of(gradients);
+    by_dtype(norm, [&](auto zero) {
+        using T = decltype(zero);
+        mops::cuda::gradient_norm<T>(mops::Tensor<T, 1>{norm.data_ptr<T>(), {1}}, views.data(), views.size());
+    });
+}
+/// (outputs: the gradients themselves, in place)
+inline void clip_gradients_to(
+    const at::Tensor& norm, const std::vector<at::Tensor>& outputs, const std::vector<at::Tensor>& gradients,
+    double max_norm
+) {
+    const auto to = views_of(outputs), from = views_of(gradients);
+    by_dtype(norm, [&](auto zero) {
+        using T = decltype(zero);
+        mops::cuda::clip_gradients<T>(
+            mops::Tensor<T, 1>{norm.data_ptr<T>(), {1}}, to.data(), from.data(), from.size(), max_norm
+        );
+    });
+}
 
 } // namespace mops::amd::torch_tensors
 

@@ -30,8 +30,11 @@ _STRUCTS = {
     for ndim in (1, 2, 3)
 }
 
-#: function -> ((dimensions or "double", parameter), ...) in the order of the C prototype; a negative number of
-#: dimensions is an index tensor
+#: what the sums of a type are held in
+_WIDE = {"f32": "f32", "f64": "f64", "bf16": "f32", "f16": "f32"}
+
+#: function -> ((dimensions, "double", "int" or "wide", parameter), ...) in the order of the C prototype; a negative
+#: number of dimensions is an index tensor, "wide" one dimension of the type of the sums
 _SIGNATURES = {
     "order_by_group": ((-1, "order"), (-1, "offsets"), (-1, "indices")),
     "scaled_embedding": ((2, "output"), (2, "table"), (-1, "indices"), ("double", "scale")),
@@ -56,33 +59,43 @@ _SIGNATURES = {
 _functions = {}
 
 
-def _function(name, tag):
+def _argument_type(kind, tag):
+    if kind == "double":
+        return ctypes.c_double
+    if kind == "int":
+        return ctypes.c_int32
+    if kind == "wide":
+        return _STRUCTS[(1, _WIDE[tag])]
+    return _STRUCTS[(abs(kind), "i32" if kind < 0 else tag)]
+
+
+def _function(name, tag, signatures=_SIGNATURES):
     symbol = f"mops_amd_{name}" if tag is None else f"mops_amd_{name}_{tag}"
     if symbol not in _functions:
         function = getattr(device_library().cdll, symbol)
         function.restype = ctypes.c_int
-        function.argtypes = [
-            ctypes.c_double if kind == "double" else _STRUCTS[(abs(kind), "i32" if kind < 0 else tag)]
-            for kind, _ in _SIGNATURES[name]
-        ]
+        function.argtypes = [_argument_type(kind, tag) for kind, _ in signatures[name]]
         _functions[symbol] = function
     return _functions[symbol]
 
 
-def _check_tensors(function, tensors, like):
+def _check_tensors(function, tensors, like, signatures=_SIGNATURES):
     """``tensors``: name -> tensor (None: not given). All of them on the device of ``like`` (a name), the
     floating-point ones of its type; first the numbers of dimensions, then types and devices."""
-    kinds = {name: kind for kind, name in _SIGNATURES[function]}
+    kinds = {name: kind for kind, name in signatures[function]}
     for name, tensor in tensors.items():
         if tensor is not None:
-            check_array(tensor, abs(kinds[name]), function, name)
+            check_array(tensor, 1 if kinds[name] == "wide" else abs(kinds[name]), function, name)
     first = tensors[like]
     if not _dispatch.on_device(first):
         raise TypeError(f"`{like}` must be on a ROCm device in {function}: this library implements the device path only")
     for name, tensor in tensors.items():
         if tensor is None:
             continue
-        if kinds[name] < 0:
+        if kinds[name] == "wide":
+            of_first = _WIDE.get(_TAGS.get(_dispatch.dtype_name(first)), "none")
+            correct = _TAGS.get(_dispatch.dtype_name(tensor)) == of_first
+        elif kinds[name] < 0:
             correct = _dispatch.is_integer(tensor)
         else:
             correct = _dispatch.dtype_name(tensor) in _TAGS and tensor.dtype == first.dtype
@@ -100,30 +113,35 @@ def _check_number(function, name, value):
         raise TypeError(f"`{name}` must be a scalar in {function}, got {type(value)}")
 
 
-def _call(function, like, *arguments):
+def _call(function, like, *arguments, signatures=_SIGNATURES):
     """The C function with ``arguments`` in the order of its prototype, on the current stream of ``like``."""
-    import torch
-
     tag = None
     values = []
-    for (kind, _), argument in zip(_SIGNATURES[function], arguments):
-        if kind == "double":
-            values.append(float(argument))
+    for (kind, _), argument in zip(signatures[function], arguments):
+        if kind in ("double", "int"):
+            values.append(float(argument) if kind == "double" else int(argument))
             continue
-        if kind > 0:
+        if kind == "wide" or kind > 0:
             tag = _TAGS[_dispatch.dtype_name(like)]
-        struct = _STRUCTS[(abs(kind), "i32" if kind < 0 else tag)]()
+        struct = _argument_type(kind, tag)()
         if argument is not None:
             element = type(struct.data)
             struct.data = ctypes.cast(ctypes.c_void_p(argument.data_ptr()), element)
             for d, extent in enumerate(argument.shape):
                 struct.shape[d] = extent
         values.append(struct)
+    _on_stream(like, _function(function, tag, signatures), values)
+
+
+def _on_stream(like, function, values):
+    """The C function, on the current stream of the device of ``like``."""
+    import torch
+
     library = device_library()
     with torch.cuda.device(like.device):
         library.cdll.mops_amd_set_stream(torch.cuda.current_stream(like.device).cuda_stream)
         library.cdll.mops_amd_set_synchronous(0)
-        status = _function(function, tag)(*values)
+        status = function(*values)
     if status != 0:
         raise MopsError(library.last_error(), status)
 

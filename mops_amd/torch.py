@@ -24,10 +24,13 @@ have none, as in the reference.
 The operators of the layers around them (``mops_amd.layers``; not part of the
 reference) are registered beside them, for ``bfloat16`` and ``float16`` as well:
 ``order_by_group``, ``scaled_embedding``, ``grouped_matrix_product``,
-``gated_residual_norm``. The gradients of the embedding and of the products are
-calls of the same operators and can be differentiated again (a loss on forces);
-``gated_residual_norm`` has first derivatives, and differentiating its gradients
-raises an error.
+``gated_grouped_product``, ``gated_residual_norm``, ``linear_cross_entropy``, and
+``gradient_norm``, ``clip_gradients``, ``clip_gradients_`` for lists of tensors.
+The gradients of the embedding and of the products are calls of the same
+operators and can be differentiated again (a loss on forces);
+``gated_grouped_product``, ``gated_residual_norm`` and ``linear_cross_entropy``
+have first derivatives, and differentiating their gradients raises an error;
+the functions of lists have none.
 
 Host tensors are refused: this library is the device path only.
 """
@@ -46,7 +49,12 @@ __all__ = [
     "order_by_group",
     "scaled_embedding",
     "grouped_matrix_product",
+    "gated_grouped_product",
     "gated_residual_norm",
+    "linear_cross_entropy",
+    "gradient_norm",
+    "clip_gradients",
+    "clip_gradients_",
     "OPERATORS_FROM",
 ]
 
@@ -68,4 +76,9 @@ sparse_accumulation_scatter_add_with_weights = torch.ops.mops.sparse_accumulatio
 order_by_group = torch.ops.mops.order_by_group
 scaled_embedding = torch.ops.mops.scaled_embedding
 grouped_matrix_product = torch.ops.mops.grouped_matrix_product
+gated_grouped_product = torch.ops.mops.gated_grouped_product
 gated_residual_norm = torch.ops.mops.gated_residual_norm
+linear_cross_entropy = torch.ops.mops.linear_cross_entropy
+gradient_norm = torch.ops.mops.gradient_norm
+clip_gradients = torch.ops.mops.clip_gradients
+clip_gradients_ = torch.ops.mops.clip_gradients_
