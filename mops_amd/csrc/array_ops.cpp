@@ -687,9 +687,7 @@ PyObject* clip_gradients(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
     PyObject* const norm = run<OfIndices>(
         gradients[0],
         [&] {
-            for (const at::Tensor& gradient : gradients) {
-                outputs.push_back(in_place[0] ? gradient : new_gradient(gradient));
-            }
+            outputs = in_place[0] ? gradients : new_gradients(gradients);
             return new_norm(gradients);
         },
         [&](int32_t, at::Tensor& to) { clip_gradients_to(to, outputs, gradients, max_norm); }

@@ -22,6 +22,7 @@
 #define MOPS_AMD_CROSS_ENTROPY_KERNELS_HPP
 
 #include <limits>
+#include <numeric>
 #include <type_traits>
 
 #include "cross_entropy.hpp"
@@ -34,26 +35,40 @@ namespace mops::amd::cross_entropy {
 
 using namespace grouped_product;
 
-__device__ __forceinline__ float power(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504088896341f); }
-__device__ __forceinline__ double power(double x) { return exp(x); }
-__device__ __forceinline__ float logarithm(float x) { return logf(x); }
-__device__ __forceinline__ double logarithm(double x) { return log(x); }
+/// Powers and logarithms of two: a logit enters an exponent as x log2(e) - (what it is relative to), one instruction.
+constexpr double LOG2_E = 1.44269504088896340736, LN_2 = 0.69314718055994530942;
+__device__ __forceinline__ float power(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ double power(double x) { return exp2(x); }
+__device__ __forceinline__ float logarithm(float x) { return log2f(x); }
+__device__ __forceinline__ double logarithm(double x) { return log2(x); }
 __device__ __forceinline__ float larger(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ double larger(double a, double b) { return fmax(a, b); }
+/// 2^(x log2(e) - base)
+__device__ __forceinline__ float power_of(float x, float base) { return power(fmaf(x, static_cast<float>(LOG2_E), -base)); }
+__device__ __forceinline__ double power_of(double x, double base) { return power(fma(x, LOG2_E, -base)); }
 
-/// The largest of some logits and the sum of exp(x - largest). (Not-a-number is never the largest; it makes the sum one.)
+/// The largest of some logits, times log2(e), and the sum of the powers relative to it. (Not-a-number is never the largest;
+/// it makes the sum one.)
 template <typename Wide> struct Sum {
     Wide most, sum;
 
     static __device__ __forceinline__ Wide lowest() { return -std::numeric_limits<Wide>::infinity(); }
     /// What the powers are taken relative to: no difference of infinities where there is nothing.
     static __device__ __forceinline__ Wide base(Wide most) { return most == lowest() ? Wide(0) : most; }
+    /// Of a single logit.
+    static __device__ __forceinline__ Sum of(Wide x) {
+        const Wide most = x == x ? x * static_cast<Wide>(LOG2_E) : lowest();
+        return Sum{most, x == x ? power_of(x, base(most)) : x};
+    }
     __device__ __forceinline__ void join(const Sum& other) {
-        const Wide both = larger(most, other.most);
-        sum = sum * power(most - base(both)) + other.sum * power(other.most - base(both));
+        const Wide both = larger(most, other.most), from = base(both);
+        sum = sum * power(most - from) + other.sum * power(other.most - from);
         most = both;
     }
-    __device__ __forceinline__ Wide logarithm_of_sum() const { return most + logarithm(sum); }
+    /// log(sum of the powers of e), less x.
+    __device__ __forceinline__ Wide logarithm_above(Wide x) const {
+        return most * static_cast<Wide>(LN_2) - x + static_cast<Wide>(LN_2) * logarithm(sum);
+    }
 };
 
 // ----------------------------------------------------------- sums by tiles --
@@ -61,6 +76,7 @@ template <typename Wide> struct Sum {
 template <typename T> struct StorePartialSums {
     typedef wide_t<T> Wide;
     static constexpr bool PAIRS = false, RESTS = false;
+    template <int BM, int BN> static constexpr bool ONCE = BM != BN; // (wide tiles: launch_logits)
     Sum<Wide>* partial;
     Wide* target_logits;
     const int32_t* targets;
@@ -76,56 +92,60 @@ template <typename T> struct StorePartialSums {
         }
         static_assert(WN * BM * sizeof(Sum<Wide>) <= LDS_BYTES, "");
         Sum<Wide>* const shared = reinterpret_cast<Sum<Wide>*>(t.lds);
-        const int32_t first = t.n0 + t.across() * Tile::NB * Tile::BLOCK; // class of the wavefront's first column
-        const bool whole = t.n0 + BN <= g.n_size; // (uniform)
+        constexpr int COLUMNS = Tile::NB * Tile::BLOCK;
+        const int32_t first = t.n0 + t.across() * COLUMNS; // class of the wavefront's first column
+        if (t.n0 + BN > g.n_size) { // (uniform) nothing where there is no class
+            t.for_each([&](int i, int j, int e) {
+                if (first + j * Tile::BLOCK + t.column(e) >= g.n_size) {
+                    t.sums[i][j][e] = Sum<Wide>::lowest();
+                }
+            });
+        }
 #pragma unroll
         for (int i = 0; i < Tile::MB; i++) {
             const int32_t row = t.rows[min(t.row(i), t.unit.count - 1)];
             const int32_t target = targets[row] - first;
-            Sum<Wide> all{Sum<Wide>::lowest(), 0};
-            Wide of_target = 0;
+            // (few wavefronts have a target of their rows among their columns; one lane of all tiles has its logit)
+            if (__any(target >= 0 && target < COLUMNS)) {
+#pragma unroll
+                for (int j = 0; j < Tile::NB; j++) {
+#pragma unroll
+                    for (int e = 0; e < Tile::HELD; e++) {
+                        if (j * Tile::BLOCK + t.column(e) == target && t.row(i) < t.unit.count) {
+                            target_logits[row] = t.sums[i][j][e];
+                        }
+                    }
+                }
+            }
+            Wide most = Sum<Wide>::lowest();
 #pragma unroll
             for (int j = 0; j < Tile::NB; j++) {
 #pragma unroll
                 for (int e = 0; e < Tile::HELD; e++) {
-                    const int at = j * Tile::BLOCK + t.column(e);
-                    const Wide x = t.sums[i][j][e];
-                    all.most = larger(all.most, whole || first + at < g.n_size ? x : Sum<Wide>::lowest());
-                    of_target = at == target ? x : of_target;
+                    most = larger(most, t.sums[i][j][e]);
                 }
             }
 #pragma unroll
             for (int s = Tile::BLOCK; s < WAVE; s *= 2) {
-                all.most = larger(all.most, __shfl_xor(all.most, s));
+                most = larger(most, __shfl_xor(most, s));
             }
-            const Wide base = Sum<Wide>::base(all.most);
+            most *= static_cast<Wide>(LOG2_E);
+            const Wide base = Sum<Wide>::base(most);
+            Wide sum[2] = {0, 0};
 #pragma unroll
             for (int j = 0; j < Tile::NB; j++) {
 #pragma unroll
                 for (int e = 0; e < Tile::HELD; e++) {
-                    const int at = j * Tile::BLOCK + t.column(e);
-                    const Wide one = power(t.sums[i][j][e] - base);
-                    all.sum += whole || first + at < g.n_size ? one : Wide(0);
+                    sum[e % 2] += power_of(t.sums[i][j][e], base);
                 }
             }
+            sum[0] += sum[1];
 #pragma unroll
             for (int s = Tile::BLOCK; s < WAVE; s *= 2) {
-                all.sum += __shfl_xor(all.sum, s);
+                sum[0] += __shfl_xor(sum[0], s);
             }
             if (t.lane < Tile::BLOCK) {
-                shared[t.across() * BM + t.row(i)] = all;
-            }
-            // (one lane of all tiles has the target's column)
-            bool mine = false;
-#pragma unroll
-            for (int j = 0; j < Tile::NB; j++) {
-#pragma unroll
-                for (int e = 0; e < Tile::HELD; e++) {
-                    mine = mine || j * Tile::BLOCK + t.column(e) == target;
-                }
-            }
-            if (mine && t.row(i) < t.unit.count) {
-                target_logits[row] = of_target;
+                shared[t.across() * BM + t.row(i)] = Sum<Wide>{most, sum[0]};
             }
         }
         __syncthreads();
@@ -140,38 +160,41 @@ template <typename T> struct StorePartialSums {
     }
 };
 
-/// losses and log_sums of JOINED_ROWS places per workgroup, JOIN_LANES threads each, from the sums of `parts` tiles; zeros
-/// for the rows without a target.
-constexpr int JOINED_ROWS = 16, JOIN_LANES = 16;
-template <typename T>
-__global__ __launch_bounds__(JOINED_ROWS* JOIN_LANES) void join_sums_kernel(
+/// losses and log_sums of ROWS places per workgroup, as many threads each as there are for them, from the sums of `parts`
+/// tiles; zeros for the rows without a target.
+constexpr int JOIN_SUM_THREADS = 256;
+template <typename T, int ROWS>
+__global__ __launch_bounds__(JOIN_SUM_THREADS) void join_sums_kernel(
     wide_t<T>* __restrict__ losses, wide_t<T>* __restrict__ log_sums, const Sum<wide_t<T>>* __restrict__ partial,
-    const wide_t<T>* __restrict__ target_logits, RowGroups groups, int32_t parts
+    const wide_t<T>* __restrict__ target_logits, const int32_t* __restrict__ targets, RowGroups groups, int32_t parts,
+    int32_t classes
 ) {
     typedef wide_t<T> Wide;
-    __shared__ Sum<Wide> shared[JOIN_LANES][JOINED_ROWS];
-    const int in_block = threadIdx.x % JOINED_ROWS, lane = threadIdx.x / JOINED_ROWS;
-    const int32_t place = blockIdx.x * JOINED_ROWS + in_block, kept = groups.end_of(0, groups.begin_of(0));
+    constexpr int LANES = JOIN_SUM_THREADS / ROWS;
+    __shared__ Sum<Wide> shared[LANES][ROWS];
+    const int in_block = threadIdx.x % ROWS, lane = threadIdx.x / ROWS;
+    const int32_t place = blockIdx.x * ROWS + in_block, kept = groups.end_of(0, groups.begin_of(0));
     Sum<Wide> all{Sum<Wide>::lowest(), 0};
     if (place < kept) {
-        for (int32_t p = lane; p < parts; p += JOIN_LANES) {
+#pragma unroll 4
+        for (int32_t p = lane; p < parts; p += LANES) {
             all.join(partial[static_cast<size_t>(p) * groups.n_rows + place]);
         }
     }
     shared[lane][in_block] = all;
-    __syncthreads();
+#pragma unroll
+    for (int half = LANES / 2; half > 0; half /= 2) {
+        __syncthreads();
+        if (lane < half) {
+            all.join(shared[lane + half][in_block]);
+            shared[lane][in_block] = all;
+        }
+    }
     if (lane == 0 && place < groups.n_rows) {
         const int32_t row = groups.row_at(place);
-        Wide loss = 0, log_sum = 0;
-        if (place < kept) {
-            for (int l = 1; l < JOIN_LANES; l++) {
-                all.join(shared[l][in_block]);
-            }
-            log_sum = all.logarithm_of_sum();
-            loss = all.most - target_logits[row] + logarithm(all.sum);
-        }
-        losses[row] = loss;
-        log_sums[row] = log_sum;
+        const bool has_target = place < kept && in_bounds(targets[row], classes);
+        losses[row] = has_target ? all.logarithm_above(target_logits[row]) : Wide(0);
+        log_sums[row] = has_target ? all.logarithm_above(0) : Wide(0);
     }
 }
 
@@ -185,7 +208,7 @@ __global__ __launch_bounds__(ROW_THREADS) void join_shared_sums_kernel(
     __shared__ Sum<Wide> shared[ROW_THREADS / WAVE];
     __shared__ Wide target_logit;
     const int32_t place = blockIdx.x, kept = g.groups.end_of(0, g.groups.begin_of(0)), row = g.groups.row_at(place);
-    if (place >= kept) { // (uniform)
+    if (place >= kept || !in_bounds(targets[row], g.n_size)) { // (uniform)
         if (threadIdx.x == 0) {
             losses[row] = 0;
             log_sums[row] = 0;
@@ -203,7 +226,7 @@ __global__ __launch_bounds__(ROW_THREADS) void join_shared_sums_kernel(
         if (v == targets[row]) {
             target_logit = x;
         }
-        all.join(Sum<Wide>{x == x ? x : Sum<Wide>::lowest(), x == x ? power(x - Sum<Wide>::base(x)) : x});
+        all.join(Sum<Wide>::of(x));
     }
 #pragma unroll
     for (int s = 1; s < WAVE; s *= 2) {
@@ -217,8 +240,8 @@ __global__ __launch_bounds__(ROW_THREADS) void join_shared_sums_kernel(
         for (int w = 1; w < ROW_THREADS / WAVE; w++) {
             all.join(shared[w]);
         }
-        losses[row] = all.most - target_logit + logarithm(all.sum);
-        log_sums[row] = all.logarithm_of_sum();
+        losses[row] = all.logarithm_above(target_logit);
+        log_sums[row] = all.logarithm_above(0);
     }
 }
 
@@ -254,17 +277,18 @@ template <typename T> struct Weights {
     Unscale<T> scale;
 
     struct OfRow {
-        Wide log_sum, of_power, of_target;
+        Wide base, of_power, of_target; // base: of the powers, log2(e) log_sums
         int32_t target;
 
+        __device__ __forceinline__ Wide at_others(Wide x) const { return of_power * power_of(x, base); }
         __device__ __forceinline__ Wide make(Wide x, int32_t n) const {
-            return of_power * power(x - log_sum) - (n == target ? of_target : Wide(0));
+            return at_others(x) - (n == target ? of_target : Wide(0));
         }
     };
     __device__ __forceinline__ OfRow of_row(int32_t row) const {
         const Wide g = grad_losses != nullptr ? grad_losses[row] : Wide(0);
         const Wide h = grad_log_sums != nullptr ? grad_log_sums[row] : Wide(0);
-        return OfRow{log_sums[row], (g + h) * scale.factor(), g * scale.factor(), targets[row] - first};
+        return OfRow{log_sums[row] * static_cast<Wide>(LOG2_E), (g + h) * scale.factor(), g * scale.factor(), targets[row] - first};
     }
 };
 
@@ -272,6 +296,7 @@ template <typename T> struct Weights {
 template <typename T> struct StoreGradients : Weights<T> {
     typedef wide_t<T> Wide;
     static constexpr bool PAIRS = false, RESTS = false;
+    template <int BM, int BN> static constexpr bool ONCE = BM != BN; // (wide tiles: launch_logits)
     T* d;
     int32_t stride;
 
@@ -284,20 +309,38 @@ template <typename T> struct StoreGradients : Weights<T> {
                 return;
             }
         }
-        typename Weights<T>::OfRow of[Tile::MB];
+        constexpr int COLUMNS = Tile::NB * Tile::BLOCK;
+        const int32_t first = t.n0 + t.across() * COLUMNS;
 #pragma unroll
         for (int i = 0; i < Tile::MB; i++) {
-            of[i] = this->of_row(t.rows[min(t.row(i), t.unit.count - 1)]);
+            const auto of = this->of_row(t.rows[min(t.row(i), t.unit.count - 1)]);
+#pragma unroll
+            for (int j = 0; j < Tile::NB; j++) {
+#pragma unroll
+                for (int e = 0; e < Tile::HELD; e++) {
+                    t.sums[i][j][e] = of.at_others(t.sums[i][j][e]);
+                }
+            }
+            // (few wavefronts have a target of their rows among their columns)
+            if (__any(of.target >= first && of.target < first + COLUMNS)) {
+#pragma unroll
+                for (int j = 0; j < Tile::NB; j++) {
+#pragma unroll
+                    for (int e = 0; e < Tile::HELD; e++) {
+                        t.sums[i][j][e] -= first + j * Tile::BLOCK + t.column(e) == of.target ? of.of_target : Wide(0);
+                    }
+                }
+            }
         }
-        const int32_t first = t.n0 + t.across() * Tile::NB * Tile::BLOCK;
-        const bool whole = t.n0 + BN <= g.n_size; // (uniform)
+        if (t.n0 + BN > g.n_size) { // (uniform) zeros where there is no class
+            t.for_each([&](int i, int j, int e) {
+                if (first + j * Tile::BLOCK + t.column(e) >= g.n_size) {
+                    t.sums[i][j][e] = 0;
+                }
+            });
+        }
         turn_over<T, Tile::NB, LDS_BYTES>(
-            t,
-            [&](int i, int j, int e) {
-                const int32_t n = first + j * Tile::BLOCK + t.column(e);
-                const Wide made = of[i].make(t.sums[i][j][e], n);
-                return whole || n < g.n_size ? made : Wide(0);
-            },
+            t, [&](int i, int j, int e) { return t.sums[i][j][e]; },
             [&](int row, int column, const typename Packed<T>::Numbers& numbers) {
                 T* const to = row < t.unit.count ? d + static_cast<size_t>(t.rows[row]) * stride : nullptr;
                 store_piece<false, T>(to, t.n0 + column, stride, numbers);
@@ -331,6 +374,7 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_shared_gradients_kernel(Pro
 template <typename T> struct AddRows {
     typedef wide_t<T> Wide;
     static constexpr bool PAIRS = false, RESTS = true;
+    template <int BM, int BN> static constexpr bool ONCE = false;
     Wide* sums;
     bool first, last;
     Unscale<T> scale;
@@ -412,6 +456,13 @@ template <typename T> __global__ __launch_bounds__(JOIN_THREADS) void add_shares
 }
 
 // -------------------------------------------------------------------- host --
+/// Rows of which a workgroup joins two, so that there are enough workgroups (64 rows, 391 tiles: 10.8 us with 16 of them in
+/// each of four workgroups, 4.7 like this).
+constexpr unsigned FEW_JOINED = 2048;
+/// Up to so many rows the losses are computed of all of them and those without a target left out at the end: a launch less,
+/// and they are one row of tiles whatever they hold.
+constexpr int32_t FEW_ROWS = 256;
+
 /// The plan of a call's rows, in its workspace.
 struct Plan {
     int32_t *order, *offsets, *counts;
@@ -442,15 +493,25 @@ protected:
         of_logits_ = tile_of_rows(logits_);
         share_k(logits_, of_logits_);
     }
+    /// (wide tiles where square ones of as many columns would be half empty)
+    template <typename Finish> void launch_logits(const Product<T>& g, hipStream_t stream, const Finish& finish) const {
+        if (of_logits_ == WIDE_COLUMNS && g.in_place && in_.rows <= 64) {
+            launch_wide<T, Form::GRAD_ROWS>(g, in_.rows <= LEAST_ROWS<T> ? LEAST_ROWS<T> : 64, WIDE_COLUMNS, stream, finish);
+        } else {
+            launch<T, Form::GRAD_ROWS>(g, of_logits_, stream, finish);
+        }
+    }
     size_t copied_bytes() const { return copied_ ? A_.copied_bytes() + W_.copied_bytes() : 0; }
-    /// The operands, the plan and the groups of everything.
-    RowGroups begin(char*& room, hipStream_t stream) {
+    /// The operands, the plan (if `planned`) and the groups of everything.
+    RowGroups begin(char*& room, bool planned, hipStream_t stream) {
         const Plan plan(room, in_.rows);
-        rows_with_targets(plan.order, plan.offsets, plan.counts, in_.targets, in_.rows, in_.classes, stream);
+        if (planned) {
+            rows_with_targets(plan.order, plan.offsets, plan.counts, in_.targets, in_.rows, in_.classes, stream);
+        }
         char* none = nullptr;
         of_A_ = place(A_, copied_ ? room : none, stream);
         of_W_ = place(W_, copied_ ? room : none, stream);
-        return RowGroups{plan.offsets, plan.order, 1, in_.rows};
+        return planned ? RowGroups{plan.offsets, plan.order, 1, in_.rows} : RowGroups{nullptr, nullptr, 1, in_.rows};
     }
 
     const Inputs<T> in_;
@@ -470,7 +531,7 @@ public:
     void run(wide_t<T>* losses, wide_t<T>* log_sums, char* room, hipStream_t stream) {
         typedef wide_t<T> Wide;
         Product<T> g = this->logits_;
-        g.groups = this->begin(room, stream);
+        g.groups = this->begin(room, this->in_.rows > FEW_ROWS, stream);
         g.q = this->of_A_;
         g.p = this->of_W_;
         Wide* const target_logits = reinterpret_cast<Wide*>(room);
@@ -478,18 +539,22 @@ public:
         Sum<Wide>* const partial = reinterpret_cast<Sum<Wide>*>(room);
         g.partial = reinterpret_cast<Wide*>(room);
         if (g.n_size > 0) {
-            launch<T, Form::GRAD_ROWS>(
-                g, this->of_logits_, stream, StorePartialSums<T>{partial, target_logits, this->in_.targets}
-            );
+            this->launch_logits(g, stream, StorePartialSums<T>{partial, target_logits, this->in_.targets});
         }
         const unsigned rows = static_cast<unsigned>(this->in_.rows);
+        auto join = [&](auto each) {
+            constexpr int ROWS = decltype(each)::value;
+            join_sums_kernel<T, ROWS><<<static_cast<unsigned>(ceil_div(rows, ROWS)), JOIN_SUM_THREADS, 0, stream>>>(
+                losses, log_sums, partial, target_logits, this->in_.targets, g.groups, static_cast<int32_t>(parts()),
+                this->in_.classes
+            );
+        };
         if (g.splits > 1) {
             join_shared_sums_kernel<T><<<rows, ROW_THREADS, 0, stream>>>(losses, log_sums, this->in_.targets, g);
+        } else if (rows <= FEW_JOINED) {
+            join(std::integral_constant<int, 2>{});
         } else {
-            join_sums_kernel<T>
-                <<<static_cast<unsigned>(ceil_div(rows, JOINED_ROWS)), JOINED_ROWS * JOIN_LANES, 0, stream>>>(
-                    losses, log_sums, partial, target_logits, g.groups, static_cast<int32_t>(parts())
-                );
+            join(std::integral_constant<int, 16>{});
         }
         MOPS_HIP_CHECK(hipGetLastError());
     }
@@ -521,21 +586,28 @@ constexpr size_t SMALLEST_PIECE = 256;
 template <typename T> class Backward : Call<T> {
 public:
     Backward(const Inputs<T>& inputs, T* grad_A, T* grad_W) : Call<T>(inputs), grad_A_(grad_A), grad_W_(grad_W) {
-        const size_t classes = inputs.classes, rows = inputs.rows;
-        const size_t pieces = std::max<size_t>(ceil_div(rows * classes * sizeof(T), MOST_BYTES), 1);
-        each_ = std::min(ceil_div(ceil_div(classes, pieces), SMALLEST_PIECE) * SMALLEST_PIECE, classes);
+        const size_t classes = inputs.classes, row_bytes = std::max<size_t>(inputs.rows, 1) * sizeof(T);
+        const size_t most = std::max(MOST_BYTES / row_bytes / SMALLEST_PIECE * SMALLEST_PIECE, SMALLEST_PIECE);
+        // Tiles of grad_W in whole rounds of all compute units, where a piece has room for one (8192 rows, 100003 classes, K =
+        // 2048, bfloat16: 10.3 ms; in four pieces of the same size, 3.06 rounds each, 11.2).
+        constexpr size_t TILE = sizeof(T) == 2 ? 256 : 128;
+        const size_t units = static_cast<size_t>(compute_units());
+        const size_t round = TILE * (units / std::gcd(units, std::max<size_t>(tiles(inputs.k_size, TILE), 1)));
+        each_ = classes <= most ? classes : round <= most ? most / round * round : most;
         stride_ = static_cast<int32_t>(ceil_div(each_, PIECE<T>)) * PIECE<T>;
-        sums_.groups = rows_.groups = this->logits_.groups;
-        sums_.n_size = rows_.n_size = inputs.k_size;
+        sums_.groups = last_sums_.groups = rows_.groups = this->logits_.groups;
+        sums_.n_size = last_sums_.n_size = rows_.n_size = inputs.k_size;
         choose(worth_copying(this->A_, this->W_, 3 * this->operations()));
     }
     void choose(bool copied) {
         this->choose_logits(copied, static_cast<int32_t>(each_));
-        sums_.in_place = copied || this->A_.in_place();
+        sums_.in_place = last_sums_.in_place = copied || this->A_.in_place();
         rows_.in_place = copied || this->W_.in_place();
         sums_.m_size = rows_.k_size = static_cast<int32_t>(each_);
-        of_sums_ = tile_of_sums(sums_);
-        sums_.most_slots = most_split_units(sums_.groups.n_rows, sums_.step);
+        // (the last piece may be a small one, whose rows are shared out further)
+        last_sums_.m_size = static_cast<int32_t>(each_ > 0 ? this->in_.classes - (ceil_div(this->in_.classes, each_) - 1) * each_ : 0);
+        of_sums_ = choose_sums(sums_);
+        of_last_sums_ = choose_sums(last_sums_);
         of_rows_ = tile_of_rows(rows_);
         share_k(rows_, of_rows_);
     }
@@ -550,7 +622,7 @@ public:
     ) {
         typedef wide_t<T> Wide;
         const Inputs<T>& in = this->in_;
-        const RowGroups groups = this->begin(room, stream);
+        const RowGroups groups = this->begin(room, true, stream);
         const Unscale<T> scale{reinterpret_cast<float*>(room)};
         if constexpr (SCALED<T>) {
             find_scale(
@@ -578,24 +650,24 @@ public:
                 {grad_losses, grad_log_sums, log_sums, in.targets, static_cast<int32_t>(first), scale}, d, stride_
             };
             if (count > 0) {
-                launch<T, Form::GRAD_ROWS>(g, this->of_logits_, stream, make);
+                this->launch_logits(g, stream, make);
             }
             if (count > 0 && g.splits > 1) {
                 const size_t blocks = ceil_div(static_cast<size_t>(in.rows) * stride_, JOIN_THREADS);
                 join_shared_gradients_kernel<T><<<static_cast<unsigned>(blocks), JOIN_THREADS, 0, stream>>>(g, make);
                 MOPS_HIP_CHECK(hipGetLastError());
             }
-            Product<T> sums = sums_, rows = rows_;
+            Product<T> sums = last ? last_sums_ : sums_, rows = rows_;
             sums.groups = rows.groups = groups;
             sums.out = grad_W_ != nullptr ? grad_W_ + first * in.k_size : nullptr;
-            sums.m_size = rows.k_size = count;
+            rows.k_size = count;
             sums.q = rows.q = Operand<T>{d, stride_};
             sums.p = this->of_A_;
             rows.out = grad_A_;
             rows.p = g.p;
             rows.partial = reinterpret_cast<Wide*>(room);
             sums.partial = reinterpret_cast<Wide*>(room + row_bytes());
-            multiply(sums, rows, StoreSums<T, Form::GRAD_SUMS, Unscale<T>>{scale}, AddRows<T>{totals, first == 0, last, scale}, stream);
+            multiply(sums, last ? of_last_sums_ : of_sums_, rows, StoreSums<T, Form::GRAD_SUMS, Unscale<T>>{scale}, AddRows<T>{totals, first == 0, last, scale}, stream);
         }
     }
 
@@ -608,18 +680,41 @@ private:
     }
     size_t row_bytes() const { return grad_A_ != nullptr ? split_bytes(rows_) : 0; }
     size_t sum_bytes() const {
-        return grad_W_ != nullptr ? sums_.most_slots * partial_size(sums_.m_size, sums_.n_size) * sizeof(wide_t<T>) : 0;
+        auto of = [](const Product<T>& sums) {
+            return sums.most_slots * partial_size(sums.m_size, sums.n_size) * sizeof(wide_t<T>);
+        };
+        return grad_W_ != nullptr ? std::max(of(sums_), of(last_sums_)) : 0;
+    }
+    static int choose_sums(Product<T>& sums) {
+        const int tile = tile_of_sums(sums);
+        share_rows(sums);
+        sums.most_slots = most_split_units(sums.groups.n_rows, sums.step);
+        return tile;
+    }
+    /// Smaller units than all rows ask for, for rows of which most may have no target: an eighth, or what partial results of
+    /// MOST_PARTIAL bytes allow (200000 rows, 30000 with a target, 94 classes, K = 128, float: 32 us, 63 without).
+    static void share_rows(Product<T>& sums) {
+        constexpr size_t MOST_PARTIAL = size_t(1) << 25;
+        const size_t of_unit = partial_size(sums.m_size, sums.n_size) * sizeof(wide_t<T>);
+        const int32_t least = std::max(sums.step / 8, 256);
+        for (;;) {
+            const int32_t half = static_cast<int32_t>(ceil_div(static_cast<size_t>(sums.step) / 2, 64) * 64);
+            if (half < least || half == sums.step || most_split_units(sums.groups.n_rows, half) * of_unit > MOST_PARTIAL) {
+                return;
+            }
+            sums.step = half;
+        }
     }
     /// Both products with a piece of d, in one launch where their tiles are the same.
     void multiply(
-        Product<T>& sums, Product<T>& rows, const StoreSums<T, Form::GRAD_SUMS, Unscale<T>>& finish_sums,
+        Product<T>& sums, int of_sums, Product<T>& rows, const StoreSums<T, Form::GRAD_SUMS, Unscale<T>>& finish_sums,
         const AddRows<T>& finish_rows, hipStream_t stream
     ) {
         const bool of_W = sums.out != nullptr, of_A = rows.out != nullptr;
-        if (of_W && of_A && of_sums_ == of_rows_ && sums.in_place == rows.in_place) {
-            const unsigned for_sums = set_tiles<Form::GRAD_SUMS>(sums, of_sums_);
+        if (of_W && of_A && of_sums == of_rows_ && sums.in_place == rows.in_place) {
+            const unsigned for_sums = set_tiles<Form::GRAD_SUMS>(sums, of_sums);
             const unsigned for_rows = set_tiles<Form::FORWARD>(rows, of_rows_);
-            with_tile<T>(of_sums_, sums.in_place, [&](auto size, auto m, auto n, auto is_aligned) {
+            with_tile<T>(of_sums, sums.in_place, [&](auto size, auto m, auto n, auto is_aligned) {
                 constexpr int TILE = decltype(size)::value, WM = decltype(m)::value, WN = decltype(n)::value;
                 constexpr bool ALIGNED = decltype(is_aligned)::value;
                 gradients_kernel<
@@ -630,7 +725,7 @@ private:
             MOPS_HIP_CHECK(hipGetLastError());
         } else {
             if (of_W) {
-                launch<T, Form::GRAD_SUMS>(sums, of_sums_, stream, finish_sums);
+                launch<T, Form::GRAD_SUMS>(sums, of_sums, stream, finish_sums);
             }
             if (of_A) {
                 launch<T, Form::FORWARD>(rows, of_rows_, stream, finish_rows);
@@ -651,8 +746,8 @@ private:
     T *const grad_A_, *const grad_W_;
     size_t each_; // classes per piece
     int32_t stride_;
-    Product<T> sums_{}, rows_{};
-    int of_sums_ = 64, of_rows_ = 64;
+    Product<T> sums_{}, last_sums_{}, rows_{};
+    int of_sums_ = 64, of_last_sums_ = 64, of_rows_ = 64;
 };
 
 template <typename T>

@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 #include "device_common.hpp"
@@ -51,6 +52,7 @@ struct Table {
     int32_t count;
 
     __device__ __forceinline__ int64_t chunks() const { return end[count - 1]; }
+    __device__ __forceinline__ int64_t begin_of(int32_t tensor) const { return tensor > 0 ? end[tensor - 1] : 0; }
     /// Which tensor has chunk `chunk`.
     __device__ __forceinline__ int32_t tensor_of(int64_t chunk) const {
         int32_t low = 0, high = count - 1;
@@ -64,7 +66,6 @@ struct Table {
         }
         return low;
     }
-    __device__ __forceinline__ int64_t begin_of(int32_t tensor) const { return tensor > 0 ? end[tensor - 1] : 0; }
 };
 
 /// body(zero of the type).
@@ -80,15 +81,56 @@ template <typename Body> __device__ __forceinline__ void by_type(GradientType ty
     }
 }
 
-/// body(whole, i): piece i of the thread, numbers that begin at first(i); whole: all of the chunk's pieces exist.
-template <typename T> struct Chunk {
+/// Consecutive chunks of a tensor, the workgroup's: numbers begin .. end - 1, whole chunks but for the tensor's last.
+template <typename T> struct Part {
     static constexpr int COUNT = PIECE<T>;
     static constexpr int64_t NUMBERS = CHUNK_BYTES / sizeof(T);
-    int64_t begin, size;
+    typedef Piece<T, COUNT> Numbers;
+    int64_t begin, end;
 
-    __device__ __forceinline__ bool whole() const { return begin + NUMBERS <= size; } // (uniform)
-    __device__ __forceinline__ int64_t first(int i) const { return begin + (i * THREADS + threadIdx.x) * COUNT; }
+    /// chunk(at, count) for every chunk, in order or from the last one back: the thread's first number in it, and how many of
+    /// its pieces exist (compile-time PIECES_EACH in whole chunks). one(at) for numbers behind the last whole piece.
+    template <bool BACK, typename OfChunk, typename One>
+    __device__ __forceinline__ void go(OfChunk&& chunk, One&& one) const {
+        const int64_t all = (end - begin) / NUMBERS;
+        const int64_t rest = begin + all * NUMBERS, pieces = (end - rest) / COUNT;
+        if (rest < end) { // (uniform)
+            const int64_t mine = (pieces - threadIdx.x + THREADS - 1) / THREADS; // (none: 0 or less)
+            chunk(rest + threadIdx.x * COUNT, static_cast<int>(mine));
+            const int64_t at = rest + pieces * COUNT + threadIdx.x;
+            if (at < end) {
+                one(at);
+            }
+        }
+        for (int64_t c = 0; c < all; c++) {
+            chunk(
+                begin + (BACK ? all - 1 - c : c) * NUMBERS + threadIdx.x * COUNT, std::integral_constant<int, PIECES_EACH>{}
+            );
+        }
+    }
+    static __device__ __forceinline__ int64_t of_piece(int i) { return static_cast<int64_t>(i) * THREADS * COUNT; }
 };
+
+/// Every workgroup has consecutive chunks of all tensors (it looks for the first one's tensor once, and the caches see
+/// streams): body(zero of the type, tensor, its part), in order or from the last one back.
+template <bool BACK, typename Body> __device__ __forceinline__ void for_parts(const Table& table, Body&& body) {
+    const int64_t chunks = table.chunks();
+    const int64_t first = chunks * blockIdx.x / gridDim.x, last = chunks * (blockIdx.x + 1) / gridDim.x;
+    if (first >= last) {
+        return;
+    }
+    for (int32_t tensor = table.tensor_of(BACK ? last - 1 : first);; tensor += BACK ? -1 : 1) {
+        const int64_t begin = table.begin_of(tensor);
+        by_type(table.type[tensor], [&](auto zero) {
+            typedef decltype(zero) T;
+            const int64_t from = max(first - begin, int64_t(0)), to = min(last, table.end[tensor]) - begin;
+            body(zero, tensor, Part<T>{from * Part<T>::NUMBERS, min(to * Part<T>::NUMBERS, table.size[tensor])});
+        });
+        if (BACK ? begin <= first : table.end[tensor] >= last) {
+            return;
+        }
+    }
+}
 
 __device__ __forceinline__ double sum_of_wave(double sum) {
 #pragma unroll
@@ -113,47 +155,44 @@ __device__ __forceinline__ double sum_of_workgroup(double sum) {
     return sum;
 }
 
+/// KEPT: the gradients are read again, and the caches should have what they can (616 million bfloat16 numbers, squares and
+/// scaling: 205 + 430 us; streamed past the caches 179 + 478). For the norm alone they stream past (260 million: 77 us, 6.8
+/// TB/s).
+template <bool KEPT>
 __global__ __launch_bounds__(THREADS) void squares_kernel(double* __restrict__ partial, const Table table) {
     double sums[2] = {0, 0};
-    for (int64_t chunk = blockIdx.x; chunk < table.chunks(); chunk += gridDim.x) {
-        const int32_t tensor = table.tensor_of(chunk);
-        by_type(table.type[tensor], [&](auto zero) {
-            typedef decltype(zero) T;
-            typedef Piece<T, PIECE<T>> Numbers;
-            const T* const from = static_cast<const T*>(table.from[tensor]);
-            const Chunk<T> c{(chunk - table.begin_of(tensor)) * Chunk<T>::NUMBERS, table.size[tensor]};
-            auto add = [&](double x, int i) { sums[i % 2] += x * x; };
-            if (c.whole()) {
-                Numbers numbers[PIECES_EACH];
+    for_parts<false>(table, [&](auto zero, int32_t tensor, const auto& part) {
+        typedef decltype(zero) T;
+        typedef typename Part<T>::Numbers Numbers;
+        const T* const from = static_cast<const T*>(table.from[tensor]);
+        auto add = [&](const Numbers& numbers) {
 #pragma unroll
-                for (int i = 0; i < PIECES_EACH; i++) {
-                    numbers[i] = Numbers::load(from + c.first(i));
-                }
-#pragma unroll
-                for (int i = 0; i < PIECES_EACH; i++) {
-#pragma unroll
-                    for (int e = 0; e < PIECE<T>; e++) {
-                        add(static_cast<double>(numbers[i].get(e)), e);
-                    }
-                }
-            } else {
-                for (int i = 0; i < PIECES_EACH; i++) {
-                    const int64_t first = c.first(i);
-                    if (first + PIECE<T> <= c.size) {
-                        const Numbers numbers = Numbers::load(from + first);
-#pragma unroll
-                        for (int e = 0; e < PIECE<T>; e++) {
-                            add(static_cast<double>(numbers.get(e)), e);
-                        }
-                    } else {
-                        for (int64_t at = first; at < c.size; at++) {
-                            add(static_cast<double>(from[at]), 0);
-                        }
-                    }
-                }
+            for (int e = 0; e < PIECE<T>; e++) {
+                const double x = static_cast<double>(numbers.get(e));
+                sums[e % 2] += x * x;
             }
-        });
-    }
+        };
+        part.template go<false>(
+            [&](int64_t at, auto count) {
+                Numbers numbers[PIECES_EACH]{};
+#pragma unroll
+                for (int i = 0; i < PIECES_EACH; i++) {
+                    if (i < count) {
+                        const T* const piece = from + at + part.of_piece(i);
+                        numbers[i] = KEPT ? Numbers::load(piece) : Numbers::stream(piece);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < PIECES_EACH; i++) {
+                    add(numbers[i]);
+                }
+            },
+            [&](int64_t at) {
+                const double x = static_cast<double>(from[at]);
+                sums[0] += x * x;
+            }
+        );
+    });
     const double sum = sum_of_workgroup(sums[0] + sums[1]);
     if (threadIdx.x == 0) {
         partial[blockIdx.x] = sum;
@@ -192,50 +231,41 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(
     if (in_place && factor == 1.0) {
         return; // (uniform)
     }
-    for (int64_t turn = blockIdx.x; turn < table.chunks(); turn += gridDim.x) {
-        const int64_t chunk = table.chunks() - 1 - turn;
-        const int32_t tensor = table.tensor_of(chunk);
-        by_type(table.type[tensor], [&](auto zero) {
-            typedef decltype(zero) T;
-            typedef Piece<T, PIECE<T>> Numbers;
-            const T* const from = static_cast<const T*>(table.from[tensor]);
-            T* const to = static_cast<T*>(table.to[tensor]);
-            const Chunk<T> c{(chunk - table.begin_of(tensor)) * Chunk<T>::NUMBERS, table.size[tensor]};
-            // (16 bits: a factor of 32 bits is exact enough, 2^-24 beside the result's 2^-9)
-            typedef std::conditional_t<sizeof(T) == 2, float, double> Factor;
-            const Factor by = static_cast<Factor>(factor);
-            auto scaled = [&](const Numbers& numbers) {
-                Numbers result;
+    for_parts<true>(table, [&](auto zero, int32_t tensor, const auto& part) {
+        typedef decltype(zero) T;
+        typedef typename Part<T>::Numbers Numbers;
+        const T* const from = static_cast<const T*>(table.from[tensor]);
+        T* const to = static_cast<T*>(table.to[tensor]);
+        // (16 bits: a factor of 32 bits is exact enough, 2^-24 beside the result's 2^-9)
+        typedef std::conditional_t<sizeof(T) == 2, float, double> Factor;
+        const Factor by = static_cast<Factor>(factor);
+        auto scaled = [&](const Numbers& numbers) {
+            Numbers result;
 #pragma unroll
-                for (int e = 0; e < PIECE<T>; e++) {
-                    result.v[e] = static_cast<T>(static_cast<Factor>(numbers.get(e)) * by);
-                }
-                return result;
-            };
-            if (c.whole()) {
+            for (int e = 0; e < PIECE<T>; e++) {
+                result.v[e] = static_cast<T>(static_cast<Factor>(numbers.get(e)) * by);
+            }
+            return result;
+        };
+        part.template go<true>(
+            [&](int64_t at, auto count) {
                 Numbers numbers[PIECES_EACH];
 #pragma unroll
                 for (int i = 0; i < PIECES_EACH; i++) {
-                    numbers[i] = Numbers::load(from + c.first(i));
+                    if (i < count) {
+                        numbers[i] = Numbers::stream(from + at + part.of_piece(i));
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < PIECES_EACH; i++) {
-                    scaled(numbers[i]).stream_to(to + c.first(i));
-                }
-            } else {
-                for (int i = 0; i < PIECES_EACH; i++) {
-                    const int64_t first = c.first(i);
-                    if (first + PIECE<T> <= c.size) {
-                        scaled(Numbers::load(from + first)).store(to + first);
-                    } else {
-                        for (int64_t at = first; at < c.size; at++) {
-                            to[at] = static_cast<T>(static_cast<Factor>(from[at]) * by);
-                        }
+                    if (i < count) {
+                        scaled(numbers[i]).stream_to(to + at + part.of_piece(i));
                     }
                 }
-            }
-        });
-    }
+            },
+            [&](int64_t at) { to[at] = static_cast<T>(static_cast<Factor>(from[at]) * by); }
+        );
+    });
 }
 
 /// The gradients in tables of TENSORS, those without numbers left out.
@@ -264,7 +294,7 @@ unsigned workgroups_of(const Table& table) {
 }
 
 /// The partial sums, in the thread's scratch memory; how many there are.
-double* sum_squares(const std::vector<Table>& tables, int32_t& parts, hipStream_t stream) {
+template <bool KEPT> double* sum_squares(const std::vector<Table>& tables, int32_t& parts, hipStream_t stream) {
     size_t all = 0;
     for (const Table& table : tables) {
         all += workgroups_of(table);
@@ -272,7 +302,7 @@ double* sum_squares(const std::vector<Table>& tables, int32_t& parts, hipStream_
     double* const partial = static_cast<double*>(scratch(align256(std::max<size_t>(all, 1) * sizeof(double))));
     parts = 0;
     for (const Table& table : tables) {
-        squares_kernel<<<workgroups_of(table), THREADS, 0, stream>>>(partial + parts, table);
+        squares_kernel<KEPT><<<workgroups_of(table), THREADS, 0, stream>>>(partial + parts, table);
         MOPS_HIP_CHECK(hipGetLastError());
         parts += static_cast<int32_t>(workgroups_of(table));
     }
@@ -351,7 +381,7 @@ void gradient_norm(Tensor<sum_t, 1> norm, const Gradient* gradients, size_t n_gr
     const auto tables = own::tables_of(nullptr, gradients, n_gradients);
     const hipStream_t stream = current_stream();
     int32_t parts = 0;
-    const double* const partial = own::sum_squares(tables, parts, stream);
+    const double* const partial = own::sum_squares<false>(tables, parts, stream);
     own::norm_kernel<sum_t><<<1, own::THREADS, 0, stream>>>(to, partial, parts);
     finish_call("gradient_norm");
 }
@@ -378,7 +408,7 @@ void clip_gradients(
     const auto tables = own::tables_of(outputs, gradients, n_gradients);
     const hipStream_t stream = current_stream();
     int32_t parts = 0;
-    const double* const partial = own::sum_squares(tables, parts, stream);
+    const double* const partial = own::sum_squares<true>(tables, parts, stream);
     if (tables.empty()) {
         own::norm_kernel<sum_t><<<1, own::THREADS, 0, stream>>>(to, partial, parts);
     }

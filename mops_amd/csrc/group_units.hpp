@@ -14,17 +14,17 @@ namespace mops::amd {
 
 /// The rows of a call in the order of their group: place p holds row order[p] (row p where `order` is null), group g
 /// has the places offsets[g] .. offsets[g + 1] - 1. Whatever the arrays hold, no place outside [0, n_rows) and no
-/// row outside it is ever used.
+/// row outside it is ever used. Without offsets all rows are in one group.
 struct RowGroups {
     const int32_t* offsets;
     const int32_t* order;
     int32_t n_groups, n_rows;
 
     __device__ __forceinline__ int32_t begin_of(int32_t group) const {
-        return within(offsets[group], 0, n_rows);
+        return offsets != nullptr ? within(offsets[group], 0, n_rows) : 0;
     }
     __device__ __forceinline__ int32_t end_of(int32_t group, int32_t begin) const {
-        return within(offsets[group + 1], begin, n_rows);
+        return offsets != nullptr ? within(offsets[group + 1], begin, n_rows) : n_rows;
     }
     /// (an order that is none gives some row, never one outside)
     __device__ __forceinline__ int32_t row_at(int32_t place) const {
@@ -81,18 +81,17 @@ public:
         }
     }
 
-    /// How many there are.
+    /// How many there are, but for those of the rows of no group.
     __device__ __forceinline__ int32_t total() {
         int32_t total = __builtin_amdgcn_readlane(upto_, WAVE - 1);
         for (int32_t base = WAVE; base < groups_.n_groups; base += WAVE) {
             look(base);
             total += __builtin_amdgcn_readlane(upto_, WAVE - 1);
         }
-        if (WHICH == Units::OF_ROWS) {
-            total += (rest() + step_ - 1) / step_;
-        }
         return total;
     }
+    /// OF_ROWS: how many the rows of no group have, numbered behind the others.
+    __device__ __forceinline__ int32_t units_of_rest() { return (rest() + step_ - 1) / step_; }
 
     /// Unit number `unit`.
     __device__ __forceinline__ GroupUnit find(int32_t unit) {

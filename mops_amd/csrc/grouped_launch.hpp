@@ -73,7 +73,9 @@ template <Form FORM, typename T> unsigned set_tiles(Product<T>& g, int tile, int
     }
     g.most_units = narrow_i32(most_units(g.groups.n_rows, g.groups.n_groups, g.step), "number of units of rows");
     const size_t of_unit = static_cast<size_t>(g.m_tiles) * g.n_tiles * std::max(g.splits, 1);
-    const size_t workgroups = ceil_div(g.most_units * of_unit, 8) * 8;
+    const size_t tiles_in_all = g.most_units * of_unit;
+    const size_t workgroups =
+        FORM == Form::GRAD_SUMS ? ceil_div(tiles_in_all, XCDS) * XCDS : workgroups_for(tiles_in_all);
     return static_cast<unsigned>(narrow_i32(workgroups, "number of tiles"));
 }
 
@@ -103,6 +105,25 @@ constexpr int DEEP = 8;
 // 16 groups, K = 2048, L = 1408, bfloat16: 22.2 us with two, 15.8 with three, 17.0 with four); the others fill LDS with two.
 template <int TILE, bool ALIGNED> constexpr int STAGES_OF = TILE == 64 && ALIGNED ? 3 : 2;
 
+/// Tiles of few rows and 128 columns, of rows on 16-byte boundaries, for matrices that are read for few rows: body(rows,
+/// wavefronts of the rows, of the columns). Most of LDS holds what is on its way of the matrices, and two workgroups fit a
+/// compute unit with three steps (64 rows of 50000 classes, K = 2048, bfloat16: 48.5 us with 64 rows, 53 in square tiles of
+/// 128, 59 in those of 64; 24 tokens of 16 experts, 2048 x 2 x 1408: 31.0 us with 32 rows, 33.2 with 64, 41 with 32 rows and
+/// 64 columns, 54 with four steps, of which one workgroup fits).
+constexpr int WIDE_COLUMNS = 128, WIDE_STAGES = 3;
+template <typename T> constexpr int LEAST_ROWS = sizeof(T) < 8 ? 32 : 64; // (double: of 64 only)
+template <typename T, typename Body> void with_wide_tile(int rows, Body&& body) {
+    std::integral_constant<int, 1> one;
+    std::integral_constant<int, 2> two;
+    if (rows < 64) {
+        if constexpr (LEAST_ROWS<T> < 64) {
+            body(std::integral_constant<int, LEAST_ROWS<T>>{}, one, two);
+        }
+    } else {
+        body(std::integral_constant<int, 64>{}, two, two);
+    }
+}
+
 template <typename T, Form FORM, typename Finish = StoreSums<T, FORM>>
 void launch(Product<T> g, int tile, hipStream_t stream, const Finish& finish = {}) {
     const unsigned workgroups = set_tiles<FORM>(g, tile);
@@ -110,6 +131,16 @@ void launch(Product<T> g, int tile, hipStream_t stream, const Finish& finish = {
         constexpr int TILE = decltype(size)::value, WM = decltype(m)::value, WN = decltype(n)::value;
         constexpr bool ALIGNED = decltype(in_place)::value;
         tiles_kernel<T, FORM, TILE, TILE, WM, WN, DEEP, STAGES_OF<TILE, ALIGNED>, ALIGNED, Finish>
+            <<<workgroups, WM * WN * WAVE, 0, stream>>>(g, finish);
+    });
+    MOPS_HIP_CHECK(hipGetLastError());
+}
+template <typename T, Form FORM, typename Finish>
+void launch_wide(Product<T> g, int rows, int columns, hipStream_t stream, const Finish& finish) {
+    const unsigned workgroups = set_tiles<FORM>(g, rows, columns);
+    with_wide_tile<T>(rows, [&](auto size, auto m, auto n) {
+        constexpr int ROWS = decltype(size)::value, WM = decltype(m)::value, WN = decltype(n)::value;
+        tiles_kernel<T, FORM, ROWS, WIDE_COLUMNS, WM, WN, DEEP, WIDE_STAGES, true, Finish>
             <<<workgroups, WM * WN * WAVE, 0, stream>>>(g, finish);
     });
     MOPS_HIP_CHECK(hipGetLastError());

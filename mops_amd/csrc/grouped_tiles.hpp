@@ -50,6 +50,7 @@
 #include "device_common.hpp"
 #include "group_units.hpp"
 #include "numbers.hpp"
+#include "tile_order.hpp"
 
 namespace mops::amd::grouped_product {
 
@@ -239,12 +240,17 @@ __device__ __constant__ const uint4 zeros_in_memory = {0, 0, 0, 0};
 
 /// 16 bytes from memory to LDS, at `lds` (the same for all lanes) + 16 * lane, without a register. Arrived when the
 /// wavefront's vmcnt says so, which `meet` waits for. (Not the builtin: behind it the compiler waits for vmcnt at the
-/// next read of LDS, of whichever buffer. There is no register here that it could lose track of.)
+/// next read of LDS, of whichever buffer. There is no register here that it could lose track of.) ONCE: past the caches
+/// (24 tokens of 16 experts, 2048 x 2 x 1408 bfloat16, other matrices every time: 33.2 us instead of 36.9).
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm" // (m0 as a clobber: reserved, and written here)
-__device__ __forceinline__ void fetch(const void* from, char* lds) {
+template <bool ONCE> __device__ __forceinline__ void fetch(const void* from, char* lds) {
     const uint32_t at = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)lds));
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "m0");
+    if constexpr (ONCE) {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(at), "v"(from) : "m0");
+    } else {
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "m0");
+    }
 }
 #pragma clang diagnostic pop
 
@@ -254,7 +260,7 @@ enum class Take { WHOLE, ALL, SOME };
 
 /// A side of the product on its way to LDS: piece i = threadIdx.x + j * THREADS, j < EACH. Through registers: SETS steps
 /// are on their way at once, each in a set of registers.
-template <typename T, int OUTER, int DEEP, int THREADS, int SETS> struct Pieces {
+template <typename T, int OUTER, int DEEP, int THREADS, int SETS, bool ONCE> struct Pieces {
     static constexpr int EACH = OUTER * DEEP / THREADS, COUNT = Matrix<T>::COUNT;
     static constexpr bool ALIGNED = SETS == 0;
     Numbers<T> piece[ALIGNED ? 1 : SETS][ALIGNED ? 1 : EACH];
@@ -267,7 +273,7 @@ template <typename T, int OUTER, int DEEP, int THREADS, int SETS> struct Pieces 
         const void* const nowhere = &zeros_in_memory;
         const int32_t missing = max(COUNT - left, 0);
         if constexpr (ALIGNED) {
-            fetch(left > 0 ? static_cast<const void*>(from) : nowhere, lds + (wave * WAVE + j * THREADS) * 16);
+            fetch<ONCE>(left > 0 ? static_cast<const void*>(from) : nowhere, lds + (wave * WAVE + j * THREADS) * 16);
         } else if constexpr (HOW == Take::WHOLE) {
             piece[set][j] = load_numbers<T>(from);
         } else if constexpr (HOW == Take::ALL) {
@@ -289,9 +295,9 @@ template <typename T, int OUTER, int DEEP, int THREADS, int SETS> struct Pieces 
     }
 };
 
-template <typename T, int OUTER, int DEEP, int THREADS, int SETS>
-struct StraightLoader : public Pieces<T, OUTER, DEEP, THREADS, SETS> {
-    typedef Pieces<T, OUTER, DEEP, THREADS, SETS> Base;
+template <typename T, int OUTER, int DEEP, int THREADS, int SETS, bool ONCE>
+struct StraightLoader : public Pieces<T, OUTER, DEEP, THREADS, SETS, ONCE> {
+    typedef Pieces<T, OUTER, DEEP, THREADS, SETS, ONCE> Base;
     typedef Straight<T, OUTER, DEEP> Layout;
     using Base::COUNT;
     using Base::EACH;
@@ -324,9 +330,9 @@ struct StraightLoader : public Pieces<T, OUTER, DEEP, THREADS, SETS> {
 };
 
 /// Rows of `width` numbers, of which those from outer0 on are used.
-template <typename T, int OUTER, int DEEP, int THREADS, int SETS>
-struct TurnedLoader : public Pieces<T, OUTER, DEEP, THREADS, SETS> {
-    typedef Pieces<T, OUTER, DEEP, THREADS, SETS> Base;
+template <typename T, int OUTER, int DEEP, int THREADS, int SETS, bool ONCE>
+struct TurnedLoader : public Pieces<T, OUTER, DEEP, THREADS, SETS, ONCE> {
+    typedef Pieces<T, OUTER, DEEP, THREADS, SETS, ONCE> Base;
     typedef Turned<T, OUTER, DEEP> Layout;
     using Base::ALIGNED;
     using Base::COUNT;
@@ -413,6 +419,19 @@ template <typename T, int BM, int BN, int WM, int WN> struct TileOf {
     __device__ __forceinline__ int column(int e) const { return M::row_of(lane, e); }
     /// Which of the wavefronts that share the tile's rows this is.
     __device__ __forceinline__ int across() const { return wave % WN; }
+    /// body(i, j, e) for every number of the lane.
+    template <typename Body> __device__ __forceinline__ void for_each(Body&& body) const {
+#pragma unroll
+        for (int i = 0; i < MB; i++) {
+#pragma unroll
+            for (int j = 0; j < NB; j++) {
+#pragma unroll
+                for (int e = 0; e < HELD; e++) {
+                    body(i, j, e);
+                }
+            }
+        }
+    }
 };
 
 /// 16 bytes of numbers, in memory at any address that holds numbers.
@@ -523,7 +542,8 @@ __device__ __forceinline__ void store_piece(
 
 /// A finish makes results of a workgroup's sums. PAIRS: p has rows of two halves (Operand::stride numbers each), and a tile
 /// BN / 2 columns of both, block of a wavefront 2 j the first half's, 2 j + 1 the second's. RESTS: the rows of no group have
-/// results as well (of sums that are zero).
+/// results as well (of sums that are zero). ONCE<BM, BN>: the matrices are read for one unit of rows only, and need not stay
+/// in the caches.
 ///
 /// This one stores the sums, scaled and rounded to T; where a group or k is split, they are not rounded yet.
 struct AsTheyAre {
@@ -531,6 +551,7 @@ struct AsTheyAre {
 };
 template <typename T, Form FORM, typename Scale = AsTheyAre> struct StoreSums {
     static constexpr bool PAIRS = false, RESTS = true;
+    template <int BM, int BN> static constexpr bool ONCE = false;
     [[no_unique_address]] Scale scale;
 
     template <bool MAY_SPLIT, int LDS_BYTES, int BM, int BN, int WM, int WN>
@@ -591,58 +612,65 @@ __device__ __forceinline__ void make_tile(
     constexpr int STEP = DEEP * COUNT, STEPS = DEEP * BLOCK / WAVE;
     constexpr int MB = BM / WM / BLOCK, NB = BN / WN / BLOCK; // blocks of a wavefront
     constexpr bool SUMS = FORM == Form::GRAD_SUMS, Q_TURNED = SUMS, P_TURNED = FORM != Form::GRAD_ROWS;
+    constexpr Units UNITS = SUMS ? Units::OF_GROUPS : Units::OF_ROWS;
     constexpr bool PAIRS = Finish::PAIRS;
     static_assert(!PAIRS || (FORM == Form::FORWARD && NB % 2 == 0), "pairs of blocks of columns");
-    constexpr Units UNITS = SUMS ? Units::OF_GROUPS : Units::OF_ROWS;
+    constexpr bool ONCE = Finish::template ONCE<BM, BN>;
     constexpr int SETS = ALIGNED ? 0 : 2; // (what there is room for in registers)
     using QLoader = std::conditional_t<
-        Q_TURNED, TurnedLoader<T, BM, DEEP, THREADS, SETS>, StraightLoader<T, BM, DEEP, THREADS, SETS>>;
+        Q_TURNED, TurnedLoader<T, BM, DEEP, THREADS, SETS, false>, StraightLoader<T, BM, DEEP, THREADS, SETS, false>>;
     using PLoader = std::conditional_t<
-        P_TURNED, TurnedLoader<T, BN, DEEP, THREADS, SETS>, StraightLoader<T, BN, DEEP, THREADS, SETS>>;
+        P_TURNED, TurnedLoader<T, BN, DEEP, THREADS, SETS, ONCE>, StraightLoader<T, BN, DEEP, THREADS, SETS, ONCE>>;
     constexpr int P_AT = BM * DEEP * 16, BYTES = P_AT + BN * DEEP * 16;
     static_assert(ALIGNED || STAGES == 2, "through registers: one step in LDS beside the present one");
     char* const stages = lds.stages;
     int32_t* const rows = lds.rows;
 
-    // Workgroups b, b + 8, .. run on the same XCD. Tiles of rows take the same time each: an XCD gets consecutive ones, so
-    // that its L2 holds what they share. A unit of GRAD_SUMS takes as long as it has rows: its tiles go to all XCDs (24
-    // uneven groups, 1280 x 1000, in consecutive tiles: 122 us instead of 115).
-    constexpr bool MAY_SPLIT = !SUMS && BM == 64;
+    // (of GRAD_SUMS, a unit takes as long as it has rows: its tiles go to all XCDs; 24 uneven groups, 1280 x 1000, in
+    // consecutive tiles: 122 us instead of 115)
+    constexpr bool MAY_SPLIT = !SUMS && BM <= 64;
     const int32_t splits = MAY_SPLIT ? g.splits : 1;
     const int32_t tiles_of_unit = (SUMS ? g.m_tiles : splits) * g.n_tiles;
     UnitsOfGroups<UNITS> of_groups(g.groups, g.step);
-    const int32_t units = min(of_groups.total(), g.most_units);
-    const int64_t tiles = static_cast<int64_t>(units) * tiles_of_unit;
-    const int32_t per_xcd = static_cast<int32_t>((tiles + 7) / 8);
-    const int64_t tile = SUMS ? block : static_cast<int64_t>(block % 8) * per_xcd + block / 8;
-    if (static_cast<int32_t>(block / 8) >= per_xcd || tile >= tiles) {
-        return; // (uniform)
-    }
+    // (as many as the grid has room for: offsets that are none could give more)
+    const int32_t units = within(of_groups.total(), 0, g.most_units);
     int32_t unit_index, m0, n0, split = 0;
-    if (SUMS) {
-        unit_index = static_cast<int32_t>(tile / tiles_of_unit);
-        const int32_t of_unit = static_cast<int32_t>(tile % tiles_of_unit);
+    if constexpr (SUMS) {
+        if (block >= static_cast<int64_t>(units) * tiles_of_unit) {
+            return; // (uniform)
+        }
+        unit_index = static_cast<int32_t>(block / tiles_of_unit);
+        const int32_t of_unit = static_cast<int32_t>(block % tiles_of_unit);
         m0 = of_unit / g.n_tiles * BM;
         n0 = of_unit % g.n_tiles * BN;
     } else {
-        // bands of four units: their rows and a tile's columns of the matrix are read together (of two or eight: the same
-        // time)
-        const int32_t of_band = 4 * tiles_of_unit;
-        const int32_t band = static_cast<int32_t>(tile / of_band), in_band = static_cast<int32_t>(tile % of_band);
-        const int32_t height = min(4, units - 4 * band);
-        unit_index = 4 * band + in_band % height;
+        const int32_t of_rest = within(of_groups.units_of_rest(), 0, g.most_units - units);
+        const int32_t tile = tile_of(block, units * tiles_of_unit, Finish::RESTS ? of_rest * tiles_of_unit : 0);
+        if (tile < 0) {
+            return; // (uniform)
+        }
+        int32_t of_unit;
+        if (tile < units * tiles_of_unit) {
+            // bands of four units: their rows and a tile's columns of the matrix are read together (of two or eight: the same
+            // time)
+            const int32_t of_band = 4 * tiles_of_unit;
+            const int32_t band = tile / of_band, in_band = tile % of_band;
+            const int32_t height = min(4, units - 4 * band);
+            unit_index = 4 * band + in_band % height;
+            of_unit = in_band / height;
+        } else {
+            unit_index = tile / tiles_of_unit;
+            of_unit = tile % tiles_of_unit;
+        }
         m0 = 0;
-        n0 = in_band / height / splits * (PAIRS ? BN / 2 : BN);
-        split = in_band / height % splits;
+        n0 = of_unit / splits * (PAIRS ? BN / 2 : BN);
+        split = of_unit % splits;
     }
     const GroupUnit unit = of_groups.find(unit_index);
     if (unit.group < 0) {
         return; // (uniform; offsets that are none)
     }
     const bool rest = !SUMS && unit.group == g.groups.n_groups;
-    if (!Finish::RESTS && rest) {
-        return; // (uniform)
-    }
     if constexpr (!SUMS) {
         for (int i = threadIdx.x; i < BM; i += THREADS) {
             const int32_t at = min(i, unit.count - 1);
@@ -973,7 +1001,7 @@ template <typename T> __global__ __launch_bounds__(JOIN_THREADS) void join_split
 /// Wavefronts per SIMD: small tiles through registers wait for memory most of the time and have room for four (60094 rows,
 /// K = 107, L = 31, float16: 9.4 us, with three and more pieces on their way in each 12.0).
 template <typename T, int BM, int BN, bool ALIGNED>
-constexpr int ABREAST = BM == 64 && BN == 64 && !ALIGNED && sizeof(T) < 8 ? 4 : 2;
+constexpr int ABREAST = BM == 32 ? 1 : BM == 64 && BN == 64 && !ALIGNED && sizeof(T) < 8 ? 4 : 2;
 
 template <
     typename T, Form FORM, int BM, int BN, int WM, int WN, int DEEP, int STAGES, bool ALIGNED, typename Finish = StoreSums<T, FORM>>

@@ -1138,10 +1138,7 @@ at::Tensor gradient_norm(at::TensorList tensors) {
 std::tuple<std::vector<at::Tensor>, at::Tensor> clip_gradients(at::TensorList tensors, double max_norm) {
     const auto gradients = gradients_of(tensors, "clip_gradients", false);
     OnTorchStream stream(gradients[0]);
-    std::vector<at::Tensor> outputs;
-    for (const at::Tensor& gradient : gradients) {
-        outputs.push_back(new_gradient(gradient));
-    }
+    const std::vector<at::Tensor> outputs = new_gradients(gradients);
     at::Tensor norm = new_norm(gradients);
     clip_gradients_to(norm, outputs, gradients, max_norm);
     return {outputs, norm};
