@@ -492,10 +492,15 @@ protected:
         logits_.n_size = classes;
         of_logits_ = tile_of_rows(logits_);
         share_k(logits_, of_logits_);
+        // (classes are read once for few rows: wide tiles, where there are enough to keep the compute units busy)
+        wide_ = logits_.in_place && in_.rows <= 64 && tiles(classes, WIDE_COLUMNS) >= static_cast<unsigned>(compute_units());
+        if (wide_) {
+            of_logits_ = WIDE_COLUMNS;
+            logits_.splits = 1;
+        }
     }
-    /// (wide tiles where square ones of as many columns would be half empty)
     template <typename Finish> void launch_logits(const Product<T>& g, hipStream_t stream, const Finish& finish) const {
-        if (of_logits_ == WIDE_COLUMNS && g.in_place && in_.rows <= 64) {
+        if (wide_) {
             launch_wide<T, Form::GRAD_ROWS>(g, in_.rows <= LEAST_ROWS<T> ? LEAST_ROWS<T> : 64, WIDE_COLUMNS, stream, finish);
         } else {
             launch<T, Form::GRAD_ROWS>(g, of_logits_, stream, finish);
@@ -518,8 +523,8 @@ protected:
     const Matrices<T> A_, W_;
     Operand<T> of_A_{}, of_W_{};
     Product<T> logits_{};
-    int of_logits_ = 64;
-    bool copied_ = false;
+    int of_logits_ = 64; // columns of a tile of logits
+    bool wide_ = false, copied_ = false;
 };
 
 template <typename T> class Forward : Call<T> {

@@ -310,6 +310,9 @@ template <bool KEPT> double* sum_squares(const std::vector<Table>& tables, int32
 }
 
 void check(const Gradient* gradients, size_t n, const char* what, const char* operation) {
+    if (gradients == nullptr && n > 0) {
+        throw std::runtime_error(std::string("there are no ") + what + " in " + operation);
+    }
     for (size_t i = 0; i < n; i++) {
         const std::string name = std::string(what) + "[" + std::to_string(i) + "]";
         const int32_t type = static_cast<int32_t>(gradients[i].type);

@@ -5,6 +5,7 @@ held to its rounding, 2^-q of itself, and to what the errors of the sums in fron
 written down at each operator. A sum of n terms is off by at most (n + 16) 2^-p times the sum of the terms' magnitudes,
 16 for the few operations on each term and for functions that are a few units off (the activations, exp, log).
 """
+import ctypes
 import math
 
 import pytest
@@ -26,6 +27,7 @@ from tests.test_layers import (
     random,
     same,
 )
+from tests.test_layers_bounds import run_on_host
 
 ACTIVATIONS = ["silu", "gelu", "sigmoid"]
 
@@ -73,7 +75,7 @@ def gated_by_definition(A, W, index, activation, grad_output, dtype):
         mask = index == k
         a, w, c = A[mask].double(), W[k].double(), grad_output[mask].double()
         both, most = a @ w, a.abs() @ w.abs()
-        (g, u), (G, U) = both.split(L, 1), most.split(L, 1)
+        g, u, G, U = both[:, :L], both[:, L:], most[:, :L], most[:, L:]
         value, slope, _ = activated(activation, g)
         M = activated(activation, G)[2]
         output[mask], output_bound[mask] = value * u, e * (1.2 * G * U + M * U)
@@ -90,7 +92,9 @@ def gated_by_definition(A, W, index, activation, grad_output, dtype):
 LARGE_GATED = [
     (8300, 3, 72, 1032, "padded", True), (5000, 20, 520, 264, "frequent", True), (4100, 2, 264, 1031, "frequent", True),
     (9000, 2, 50, 299, "uniform", True), (40, 3, 2000, 24, "uniform", True), (30, 2, 1501, 33, "padded", True),
-    (2100, 1, 513, 1027, "uniform", False), (6, 2, 3000, 1, "uniform", True),
+    (2100, 1, 513, 1027, "uniform", False), (6, 2, 3000, 1, "uniform", True), (6, 2, 3000, 16, "uniform", True),
+    (30, 2, 1504, 40, "padded", True), (20, 16, 264, 1032, "uniform", True), (7, 0, 16, 8, "nowhere", True),
+    (70, 3, 24, 0, "padded", True), (50, 2, 0, 40, "uniform", False),
 ]  # fmt: skip
 
 
@@ -201,7 +205,8 @@ LOSSES = [
     (300, 94, 128, "padded"), (40, 3001, 40, "uniform"), (130, 257, 33, "nowhere"), (700, 1000, 24, "one"),
     (33, 90, 1500, "uniform"), (5, 7, 2001, "padded"), (20, 4000, 9, "uniform"), (2000, 40, 72, "padded"),
     (1025, 1030, 64, "frequent"), (513, 2056, 136, "padded"), (17000, 12, 16, "padded"), (4, 0, 6, "nowhere"),
-    (90, 31, 0, "uniform"), (2100, 4100, 1033, "uniform"),
+    (90, 31, 0, "uniform"), (2100, 4100, 1033, "uniform"), (64, 33000, 72, "padded"), (40, 33001, 64, "uniform"),
+    (20, 40000, 16, "frequent"),
 ]  # fmt: skip
 
 
@@ -366,6 +371,59 @@ def test_scale_of_float16_gradients(device):
                                      (grad_W, scaled.t() @ A.double(), scaled.abs().t() @ A.double().abs())):  # fmt: skip
             bound = 2.0**-10 * terms + 2.0**-38 * weight * 600 * 4 * 10 + 2.0**-11 * exact.abs() + 2.0**-25
             assert ((actual.double().cpu() - exact).abs() <= bound).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif("not torch.cuda.is_available() or torch.cuda.mem_get_info()[0] < 60e9")
+def test_operands_of_more_than_two_to_the_31_numbers(device):
+    """Matrices whose offsets pass 32 bits: the last columns, classes and numbers against 64 bits."""
+    generator = torch.Generator(device=device).manual_seed(3)
+
+    def rand(*shape, scale=1.0):
+        return torch.randn(shape, generator=generator, device=device, dtype=torch.bfloat16) * scale
+
+    # (of the rows all but the last 50 numbers are zero: sums of 50 terms, exact zeros beside them)
+    # gated: a matrix of 2.4e9 numbers
+    rows, K, L = 40, 40000, 30000
+    A, W, c = rand(rows, K), rand(1, K, 2 * L, scale=0.1), rand(rows, L)
+    A[:, :-50] = 0
+    offsets = torch.tensor([0, rows], dtype=torch.int32, device=device)
+    output = mops_amd.gated_grouped_product(A, W, offsets)
+    last = slice(L - 40, L)
+    a, w = A[:, -50:].double(), W[0, -50:].double()
+    w_gate, w_up = w[:, :L][:, last].contiguous(), w[:, L:][:, last].contiguous()
+    gate, up, e = a @ w_gate, a @ w_up, (50 + 32) * 2.0**-24
+    G, U = a.abs() @ w_gate.abs(), a.abs() @ w_up.abs()
+    held_to(output[:, last], gate * torch.sigmoid(gate) * up, e * 2.2 * G * U, "output")
+    grad_W = mops_amd.gated_grouped_product_vjp(c, A, W, offsets, compute_grad_A=False)[1]
+    cotangent, value = c[:, last].double(), gate * torch.sigmoid(gate)
+    off = cotangent.abs() * (e * 2.2 * G + 2.0**-8 * value.abs())
+    exact, turned = a.t().contiguous() @ (cotangent * value), a.abs().t().contiguous()
+    bound = turned @ off + (rows + 16) * 2.0**-24 * (turned @ (cotangent * value).abs())
+    held_to(grad_W[0, -50:, L:][:, last], exact, bound, "grad_W")
+    assert not grad_W[0, :-50].any()
+    del W, output, grad_W
+    # cross entropy: classes of 2.3e9 numbers
+    rows, V, K = 30, 70001, 32768
+    A, W = rand(rows, K), rand(V, K, scale=0.1)
+    A[:, :-50] = 0
+    targets = torch.arange(V - rows, V, dtype=torch.int32, device=device)
+    one = torch.ones(rows, device=device)
+    losses, log_sums = mops_amd.linear_cross_entropy(A, W, targets)
+    grad_A, grad_W = mops_amd.linear_cross_entropy_vjp(one, None, A, W, targets, log_sums)
+    results = loss_by_definition(A[:, -50:], W[:, -50:], targets, [one, 0 * one], torch.bfloat16)
+    held_to(losses, *results[0], "losses")
+    held_to(log_sums, *results[1], "log_sums")
+    held_to(grad_A[:, -50:], *results[2], "grad_A")
+    held_to(grad_W[:, -50:], *results[3], "grad_W")
+    assert not grad_W[:, :-50].any()
+    del W, grad_W
+    # gradients: one of 2.2e9 numbers, all of them zero but the last
+    large = torch.zeros((1 << 31) + 100001, dtype=torch.bfloat16, device=device)
+    large[-1] = 4.0
+    clipped, norm = mops_amd.clip_gradients([large, torch.full((1,), 3.0, device=device)], 2.5)
+    assert norm.item() == 5.0 and clipped[0][-1] == 2.0 and clipped[1].item() == 1.5
+    assert clipped[0].count_nonzero() == 1
 
 
 # --------------------------------------------------------- norm of gradients ----
@@ -715,6 +773,78 @@ def test_refusals(device):
         mops_amd.clip_gradients_([floats(3), None], 1.0)
     # (a refused call leaves nothing behind: the next one is right)
     assert mops_amd.gradient_norm([floats(4) + 1]).item() == 2.0
+
+
+def test_refusals_of_lists(tmp_path):
+    """What the C entries for lists refuse before they touch a device."""
+    from mops_amd._c_lib import device_library
+
+    library = device_library()
+    gradient, norm_type = training._Gradient, training._STRUCTS[(1, "f32")]
+    memory = (ctypes.c_float * 64)()
+    at = ctypes.addressof(memory)
+
+    def call(outputs, gradients, max_norm=1.0, extent=1, count=None):
+        norm = norm_type()
+        norm.data = ctypes.cast(ctypes.c_void_p(at), type(norm.data))
+        norm.shape[0] = extent
+        entry = library.cdll.mops_amd_clip_gradients_f32
+        entry.restype = ctypes.c_int
+        arrays = [None if x is None else (gradient * len(x))(*[gradient(*y) for y in x]) for x in (outputs, gradients)]
+        entry.argtypes = [norm_type, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64, ctypes.c_double]
+        addresses = [None if x is None else ctypes.addressof(x) for x in arrays]
+        assert entry(norm, *addresses, len(gradients or []) if count is None else count, max_norm) == 1
+        return library.last_error()
+
+    one = [(at, 8, 0)]
+    assert "norm must have one element" in call(one, one, extent=2)
+    assert "not negative" in call(one, one, max_norm=-0.5)
+    assert "there are no gradients" in call(None, None, count=1)
+    assert "there are no outputs" in call(None, one)
+    assert "does not fit in size_t" in call(one, one, count=-1)
+    assert "gradients[0] has no known type" in call(one, [(at, 8, 4)])
+    assert "gradients[0] has no memory, or a negative size" in call(one, [(at, -1, 0)])
+    assert "gradients[0] has no memory" in call(one, [(None, 8, 0)])
+    assert "outputs[0] must have the size and the type" in call([(at, 8, 2)], one)
+    assert "outputs[0] must have the size and the type" in call([(at, 7, 0)], one)
+    assert "must not share memory with each other" in call([(at, 8, 0), (at + 28, 8, 0)], [(at + 100, 8, 0), (at + 140, 8, 0)])
+    assert "share none with any gradient" in call([(at, 8, 0)], [(at + 16, 8, 0)])
+    assert "share none with any gradient" in call([(at, 8, 0), (at + 64, 8, 0)], [(at, 8, 0), (at + 8, 8, 0)])
+
+
+TILES = """
+#include <cstdio>
+#include <vector>
+#include "tile_order.hpp"
+using namespace mops::amd;
+int main() {
+    for (int tiles : {0, 1, 7, 8, 9, 63, 64, 65, 901, 4000}) for (int rest : {0, 1, 5, 8, 77, 1328}) {
+        std::vector<int> made(tiles + rest, 0);
+        const long long workgroups = workgroups_for(tiles + rest);
+        for (long long b = 0; b < workgroups; b++) {
+            const int tile = tile_of(static_cast<unsigned>(b), tiles, rest);
+            if (tile >= tiles + rest) return 1;
+            if (tile >= 0) made[tile]++;
+        }
+        int once = 0, of_first = 0;
+        for (int x : made) once += x == 1;
+        for (long long b = 0; b < workgroups; b += 8) {
+            const int tile = tile_of(static_cast<unsigned>(b), tiles, rest);
+            of_first += tile >= 0 && tile < tiles;
+        }
+        printf("%d %d %d %d %lld\\n", tiles, rest, once, of_first, workgroups);
+    }
+}
+"""
+
+
+def test_every_tile_is_made_once(tmp_path):
+    """Over the kernels' own header: each tile by one workgroup of those there are, however many of the rows are in no group,
+    and no XCD has more than its share of the others' tiles."""
+    got = run_on_host(tmp_path, TILES)
+    tiles, rest, once, of_first, workgroups = got.T
+    assert len(got) == 60 and (once == tiles + rest).all()
+    assert (of_first <= -(-tiles // 8)).all() and (workgroups <= tiles + rest + 16).all()
 
 
 # ------------------------------------------------------ PyTorch operators ----
