@@ -599,9 +599,13 @@ template <typename T, Form FORM, typename Scale = AsTheyAre> struct StoreSums {
 
 /// WM x WN wavefronts; every one of them makes BM / WM x BN / WN numbers, in steps of DEEP pieces of k of which STAGES
 /// are in LDS or on their way there.
+constexpr int ROWS_AT_ONCE = 512;
 template <int BM, int BN, int DEEP, int STAGES> struct TileLds {
     char stages[STAGES * (BM + BN) * DEEP * 16] __attribute__((aligned(16)));
-    int32_t rows[BM];
+    union {
+        int32_t rows[BM];                // behind the tile's
+        int32_t summed[2][ROWS_AT_ONCE]; // GRAD_SUMS, ALIGNED: behind the places that are summed up next
+    };
 };
 template <typename T, Form FORM, int BM, int BN, int WM, int WN, int DEEP, int STAGES, bool ALIGNED, typename Finish>
 __device__ __forceinline__ void make_tile(
@@ -727,9 +731,27 @@ __device__ __forceinline__ void make_tile(
         // them then waits for no pieces that were asked for later)
         constexpr int ROW_SETS = ALIGNED ? 1 : SETS;
         [[maybe_unused]] int32_t row_of_piece[ROW_SETS][SUMS ? EACH : 1];
+        // GRAD_SUMS, pieces that go straight to LDS: the rows come there ROWS_AT_ONCE at a time, long before they are asked for. (A
+        // row that is loaded for each piece is waited for behind all pieces that were asked for before it: gradients of 20011 rows
+        // of 24 groups, 1280 x 1000, bfloat16: 148 us instead of 137; 8192 x 32768 by 8192 x 2048 and both gradients: 2290
+        // instead of 2060.)
+        [[maybe_unused]] auto fill_rows = [&](int32_t from) {
+            for (int i = threadIdx.x; i < ROWS_AT_ONCE; i += THREADS) {
+                const int32_t at = from + i;
+                lds.summed[from / ROWS_AT_ONCE % 2][i] = at < k_size ? g.groups.row_at(unit.begin + at) : -1;
+            }
+        };
+        constexpr bool FILLED = SUMS && ALIGNED;
+        static_assert(!FILLED || (ROWS_AT_ONCE % STEP == 0 && (STAGES + 1) * STEP <= ROWS_AT_ONCE), "");
         auto find_rows = [&](int set, int32_t k0) {
             if constexpr (SUMS) {
-                auto row_at = [&](int k) { return k0 + k < k_size ? g.groups.row_at(unit.begin + k0 + k) : -1; };
+                auto row_at = [&](int k) {
+                    if constexpr (FILLED) {
+                        return lds.summed[(k0 + k) / ROWS_AT_ONCE % 2][(k0 + k) % ROWS_AT_ONCE];
+                    } else {
+                        return k0 + k < k_size ? g.groups.row_at(unit.begin + k0 + k) : -1;
+                    }
+                };
 #pragma unroll
                 for (int j = 0; j < EACH; j++) {
                     row_of_piece[set][j] = j >= Q_EACH && QLoader::K_EACH == PLoader::K_EACH
@@ -852,6 +874,11 @@ __device__ __forceinline__ void make_tile(
             }
         };
         if constexpr (ALIGNED) {
+            if constexpr (FILLED) {
+                fill_rows(0);
+                fill_rows(ROWS_AT_ONCE);
+                meet<-1>();
+            }
 #pragma unroll
             for (int t = 0; t < STAGES; t++) {
                 find_rows(0, t * STEP);
@@ -860,6 +887,12 @@ __device__ __forceinline__ void make_tile(
             meet<(STAGES - 2) * EACH + EARLY>();
             read_first();
             for (int32_t k0 = 0; k0 < k_size; k0 += STEP) {
+                if constexpr (FILLED) {
+                    // (the places in front of this step have been summed up, those of the next steps are there)
+                    if (k0 > 0 && k0 % ROWS_AT_ONCE == 0 && k0 + ROWS_AT_ONCE < k_size) { // (uniform)
+                        fill_rows(k0 + ROWS_AT_ONCE);
+                    }
+                }
 #pragma unroll
                 for (int step = 0; step < STEPS - 1; step++) {
                     if (step == 0) {
