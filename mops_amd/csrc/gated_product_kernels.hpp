@@ -54,7 +54,7 @@ template <typename Wide> struct Sigmoid {
 /// gives to 1.0e-8 of itself (coefficients: least squares, weighted until the relative error is the same everywhere,
 /// 0 <= z <= 14; 1 + erf has lost its digits where x is far below zero). No branches: the error function of the mathematical
 /// library took a third of a tile's time (20011 rows of 24 groups, 1280 x 2 x 1000, bfloat16, projections with their
-/// gradients: 171 us, 138 like this).
+/// gradients: 171 us, 153 like this).
 template <typename Wide> struct Normal {
     Wide below, density;
 

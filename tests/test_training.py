@@ -307,6 +307,35 @@ def test_cross_entropy_in_pieces_of_the_classes(device, tag):
     assert not grad_A[(on_device[2] < 0) | (on_device[2] >= classes)].any()
 
 
+# every extent of tiles in each of the three products, on 16-byte boundaries and off them, copied and not; several pieces
+LARGE_LOSSES = [
+    (8200, 2056, 2056), (8200, 520, 33), (8200, 40, 515), (131100, 130, 65), (16500, 17000, 1032), (8200, 9000, 520),
+    (4100, 3000, 1027),
+]  # fmt: skip
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tag", list(DTYPES))
+@pytest.mark.parametrize("rows,classes,K", LARGE_LOSSES)
+def test_large_cross_entropy(device, rows, classes, K, tag):
+    """(The definition in 64 bits on the device.)"""
+    dtype = DTYPES[tag]
+    A, W, targets, grads = loss_case(rows, classes, K, "padded", dtype)
+    on_device = [t.to(device) for t in (A, W, targets)]
+    grads = [g.to(device) for g in grads]
+    results = loss_by_definition(*on_device, grads, dtype)
+    losses, log_sums = mops_amd.linear_cross_entropy(*on_device)
+    held_to(losses, *results[0], "losses")
+    held_to(log_sums, *results[1], "log_sums")
+    grad_A, grad_W = mops_amd.linear_cross_entropy_vjp(*grads, *on_device, log_sums)
+    held_to(grad_A, *results[2], "grad_A")
+    held_to(grad_W, *results[3], "grad_W")
+    again = mops_amd.linear_cross_entropy_vjp(*grads, *on_device, log_sums, compute_grad_A=False)
+    assert again[0] is None and torch.equal(again[1], grad_W)
+    again = mops_amd.linear_cross_entropy_vjp(*grads, *on_device, log_sums, compute_grad_W=False)
+    assert again[1] is None and torch.equal(again[0], grad_A)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("tag", list(DTYPES))
 @pytest.mark.parametrize("rows,classes,K", [(70, 40, 24), (600, 300, 40), (20, 33, 1600), (3000, 512, 64)])
