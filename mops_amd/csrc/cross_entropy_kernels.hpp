@@ -584,27 +584,28 @@ void forward(const Inputs<T>& inputs, wide_t<T>* losses, wide_t<T>* log_sums, hi
     call.run(losses, log_sums, workspace, stream);
 }
 
-/// Bytes of d that are in memory at a time, at most (but for the smallest piece).
-constexpr size_t MOST_BYTES = size_t(1) << 29;
+/// Bytes of d that are in memory at a time, at most (but for the smallest piece): fewer and larger pieces of the classes read
+/// grad_A's sums less often and have more rounds of tiles. Less where the device has not as much (gradients).
+constexpr size_t MOST_BYTES = size_t(1) << 29, LEAST_BYTES = size_t(1) << 23;
 constexpr size_t SMALLEST_PIECE = 256;
 
 template <typename T> class Backward : Call<T> {
 public:
     Backward(const Inputs<T>& inputs, T* grad_A, T* grad_W) : Call<T>(inputs), grad_A_(grad_A), grad_W_(grad_W) {
-        const size_t classes = inputs.classes, row_bytes = std::max<size_t>(inputs.rows, 1) * sizeof(T);
-        const size_t most = std::max(MOST_BYTES / row_bytes / SMALLEST_PIECE * SMALLEST_PIECE, SMALLEST_PIECE);
+        sums_.groups = last_sums_.groups = rows_.groups = this->logits_.groups;
+        sums_.n_size = last_sums_.n_size = rows_.n_size = inputs.k_size;
+        choose(worth_copying(this->A_, this->W_, 3 * this->operations()), MOST_BYTES);
+    }
+    void choose(bool copied, size_t most_bytes) {
+        const size_t classes = this->in_.classes, row_bytes = std::max<size_t>(this->in_.rows, 1) * sizeof(T);
+        const size_t most = std::max(most_bytes / row_bytes / SMALLEST_PIECE * SMALLEST_PIECE, SMALLEST_PIECE);
         // Tiles of grad_W in whole rounds of all compute units, where a piece has room for one (8192 rows, 100003 classes, K =
         // 2048, bfloat16: 10.3 ms; in four pieces of the same size, 3.06 rounds each, 11.2).
         constexpr size_t TILE = sizeof(T) == 2 ? 256 : 128;
         const size_t units = static_cast<size_t>(compute_units());
-        const size_t round = TILE * (units / std::gcd(units, std::max<size_t>(tiles(inputs.k_size, TILE), 1)));
+        const size_t round = TILE * (units / std::gcd(units, std::max<size_t>(tiles(this->in_.k_size, TILE), 1)));
         each_ = classes <= most ? classes : round <= most ? most / round * round : most;
         stride_ = static_cast<int32_t>(ceil_div(each_, PIECE<T>)) * PIECE<T>;
-        sums_.groups = last_sums_.groups = rows_.groups = this->logits_.groups;
-        sums_.n_size = last_sums_.n_size = rows_.n_size = inputs.k_size;
-        choose(worth_copying(this->A_, this->W_, 3 * this->operations()));
-    }
-    void choose(bool copied) {
         this->choose_logits(copied, static_cast<int32_t>(each_));
         sums_.in_place = last_sums_.in_place = copied || this->A_.in_place();
         rows_.in_place = copied || this->W_.in_place();
@@ -761,9 +762,13 @@ void gradients(
     T* grad_A, T* grad_W, hipStream_t stream
 ) {
     Backward<T> call(inputs, grad_A, grad_W);
-    char* workspace = call.copies() ? static_cast<char*>(scratch_or_null(call.bytes())) : nullptr;
+    // (as much as there is: smaller pieces of the classes do as well, and so do operands that are not copied)
+    char* workspace = static_cast<char*>(scratch_or_null(call.bytes()));
+    for (size_t most = MOST_BYTES; workspace == nullptr && most >= LEAST_BYTES; most /= 4) {
+        call.choose(false, most);
+        workspace = static_cast<char*>(scratch_or_null(call.bytes()));
+    }
     if (workspace == nullptr) {
-        call.choose(false);
         workspace = static_cast<char*>(scratch(call.bytes()));
     }
     call.run(grad_losses, grad_log_sums, log_sums, workspace, stream);

@@ -134,8 +134,9 @@ def linear_cross_entropy_vjp(
     (either may be None: zero) and the ``log_sums`` it returned.
 
     The logits are computed again, a piece of the classes at a time; their gradients are held in the thread's scratch
-    memory, about half a gigabyte, rounded to the type of the tensors. The order of summation depends on the shapes and
-    on which rows have a target only: the same call gives the same bits.
+    memory, about half a gigabyte (less where the device has not as much left), rounded to the type of the tensors. The
+    order of summation depends on the shapes, on which rows have a target and on that memory only: the same call gives
+    the same bits.
     """
     result = _native.linear_cross_entropy_vjp(
         grad_losses, grad_log_sums, A, W, targets, log_sums, compute_grad_A, compute_grad_W

@@ -876,6 +876,70 @@ def test_every_tile_is_made_once(tmp_path):
     assert (of_first <= -(-tiles // 8)).all() and (workgroups <= tiles + rest + 16).all()
 
 
+FULL_DEVICE = """
+import ctypes, os, sys
+sys.path.insert(0, os.getcwd())
+import torch
+import mops_amd
+from mops_amd._c_lib import device_library
+from tests import test_training as t
+os.environ["MOPS_AMD_TEST_SCRATCH_LIMIT"] = str(48 << 20)  # what a nearly full device has left for the block
+library = device_library().cdll
+library.mops_amd_scratch_capacity.restype = ctypes.c_int64
+device = torch.device("cuda:0")
+for rows, classes, K, dtype in [(4100, 9000, 72, torch.bfloat16), (2100, 9001, 65, torch.float32), (4100, 9000, 71, torch.float16)]:
+    A, W, targets, grads = [
+        [x.to(device) for x in y] if isinstance(y, list) else y.to(device)
+        for y in t.loss_case(rows, classes, K, "padded", dtype)
+    ]
+    results = t.loss_by_definition(A, W, targets, grads, dtype)
+    losses, log_sums = mops_amd.linear_cross_entropy(A, W, targets)
+    t.held_to(losses, *results[0], "losses")
+    grad_A, grad_W = mops_amd.linear_cross_entropy_vjp(*grads, A, W, targets, log_sums)
+    t.held_to(grad_A, *results[2], "grad_A")
+    t.held_to(grad_W, *results[3], "grad_W")
+    assert library.mops_amd_scratch_capacity() <= 48 << 20
+    print("ok", library.mops_amd_scratch_capacity(), flush=True)
+# gated products at odd addresses, without room for copies
+generator = torch.Generator().manual_seed(1)
+A, W, c = [t.random(generator, shape, torch.float16, scale).to(device)
+           for shape, scale in (((5000, 1031), 1.0), ((1, 1031, 2 * 1033), 0.03), ((5000, 1033), 1.0))]
+offsets = torch.tensor([0, 5000], dtype=torch.int32, device=device)
+index = torch.zeros(5000, dtype=torch.int32)
+output = mops_amd.gated_grouped_product(A, W, offsets)
+results = t.gated_by_definition(A.cpu(), W.cpu(), index, "silu", c.cpu(), torch.float16)
+t.held_to(output, *results[0], "output")
+grads = mops_amd.gated_grouped_product_vjp(c, A, W, offsets)
+t.held_to(grads[0], *results[1], "grad_A")
+t.held_to(grads[1], *results[2], "grad_W")
+assert library.mops_amd_scratch_capacity() <= 48 << 20
+# memory that a call cannot do without: an error, and no trace of it in the next call
+os.environ["MOPS_AMD_TEST_SCRATCH_LIMIT"] = str(1 << 20)
+try:
+    mops_amd.gated_grouped_product_vjp(c.repeat(4, 1), A.repeat(4, 1), W, offsets * 4)
+    raise SystemExit("no error")
+except mops_amd.MopsError:
+    pass
+del os.environ["MOPS_AMD_TEST_SCRATCH_LIMIT"]
+assert torch.equal(mops_amd.gated_grouped_product(A[:64], W, torch.tensor([0, 64], dtype=torch.int32, device=device)),
+                   mops_amd.gated_grouped_product(A[:64].clone(), W, torch.tensor([0, 64], dtype=torch.int32, device=device)))
+print("ok", flush=True)
+"""
+
+
+@pytest.mark.gpu
+def test_on_a_device_that_is_nearly_full(device):
+    """Copies of operands and large pieces of the classes are memory that a call can do without."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FULL_DEVICE], cwd=root, capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0, done.stdout + done.stderr[-3000:]
+    assert done.stdout.count("ok") == 4, done.stdout
+
+
 # ------------------------------------------------------ PyTorch operators ----
 def operators():
     import mops_amd.torch  # noqa: F401  (registers the operators)
