@@ -96,12 +96,12 @@ __global__ __launch_bounds__(CHUNK) void order_kernel(
 constexpr int SCALE_THREADS = 1024;
 __global__ __launch_bounds__(SCALE_THREADS) void find_scale_kernel(
     float* __restrict__ scale, const float* __restrict__ grad_losses, const float* __restrict__ grad_log_sums,
-    const int32_t* __restrict__ targets, int32_t rows, int32_t classes
+    const int32_t* __restrict__ targets, RowGroups groups, int32_t classes, bool of_powers
 ) {
     __shared__ float shared[SCALE_THREADS / WAVE];
     float most = 0;
 #pragma unroll 4
-    for (int32_t r = threadIdx.x; r < rows; r += SCALE_THREADS) {
+    for (int32_t r = threadIdx.x; of_powers && r < groups.n_rows; r += SCALE_THREADS) {
         const bool kept = targets[r] >= 0 && targets[r] < classes;
         const float g = grad_losses != nullptr ? grad_losses[r] : 0, h = grad_log_sums != nullptr ? grad_log_sums[r] : 0;
         const float weight = fmaxf(fabsf(g), fabsf(g + h));
@@ -117,24 +117,29 @@ __global__ __launch_bounds__(SCALE_THREADS) void find_scale_kernel(
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < SCALE_THREADS / WAVE; w++) {
+        for (int w = 1; w < static_cast<int>(blockDim.x / WAVE); w++) {
             most = fmaxf(most, shared[w]);
         }
         int exponent = 0;
-        frexpf(most, &exponent); // most < 2^exponent
-        exponent = most > 0 ? min(max(14 - exponent, -126), 126) : 0;
-        scale[0] = ldexpf(1.f, exponent);
-        scale[1] = ldexpf(1.f, -exponent);
+        const float first = grad_losses != nullptr && groups.n_rows > 0 ? fabsf(grad_losses[groups.row_at(0)]) : 0;
+        const bool has_digits = first > 0 && first <= std::numeric_limits<float>::max();
+        const float digits = has_digits ? 2 * frexpf(first, &exponent) : 1;
+        exponent = 0;
+        frexpf(most / digits, &exponent); // most / digits < 2^exponent
+        exponent = most > 0 ? min(max(14 - exponent, -125), 125) : 0;
+        scale[0] = ldexpf(1 / digits, exponent);
+        scale[1] = ldexpf(digits, -exponent);
     }
 }
 
 } // namespace
 
 void find_scale(
-    float* scale, const float* grad_losses, const float* grad_log_sums, const int32_t* targets, int32_t rows,
-    int32_t classes, hipStream_t stream
+    float* scale, const float* grad_losses, const float* grad_log_sums, const int32_t* targets, const RowGroups& groups,
+    int32_t classes, bool of_powers, hipStream_t stream
 ) {
-    find_scale_kernel<<<1, SCALE_THREADS, 0, stream>>>(scale, grad_losses, grad_log_sums, targets, rows, classes);
+    const int threads = of_powers ? SCALE_THREADS : WAVE;
+    find_scale_kernel<<<1, threads, 0, stream>>>(scale, grad_losses, grad_log_sums, targets, groups, classes, of_powers);
     MOPS_HIP_CHECK(hipGetLastError());
 }
 

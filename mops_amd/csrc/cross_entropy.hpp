@@ -8,6 +8,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include "group_units.hpp"
 #include "numbers.hpp"
 
 namespace mops::amd::cross_entropy {
@@ -36,10 +37,10 @@ void rows_with_targets(
     hipStream_t stream
 );
 
-/// scale = {a power of two, its inverse}: see Unscale.
+/// scale = {what d is multiplied by, its inverse}: the first kept row's weight, its digits only, or times a power of two.
 void find_scale(
-    float* scale, const float* grad_losses, const float* grad_log_sums, const int32_t* targets, int32_t rows,
-    int32_t classes, hipStream_t stream
+    float* scale, const float* grad_losses, const float* grad_log_sums, const int32_t* targets, const RowGroups& groups,
+    int32_t classes, bool of_powers, hipStream_t stream
 );
 
 } // namespace mops::amd::cross_entropy

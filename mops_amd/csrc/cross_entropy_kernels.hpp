@@ -12,7 +12,7 @@
 // row's logits in registers, and its finish makes of them the row's largest one
 // and the sum of the powers below it (two numbers per row and tile, joined
 // afterwards), or the numbers d, rounded to T (what the matrix instructions
-// take; 16-bit floats scaled, see Unscale). Of d, a piece of the classes is in
+// take; 16-bit types scaled, and in two parts for few rows: SCALED, IN_TWO_PARTS). Of d, a piece of the classes is in
 // memory at a time, and both products with it follow while the caches hold what
 // they can of it; grad_A is summed up over the pieces in 32 bits.
 //
@@ -23,6 +23,7 @@
 
 #include <limits>
 #include <numeric>
+#include <tuple>
 #include <type_traits>
 
 #include "cross_entropy.hpp"
@@ -246,23 +247,37 @@ __global__ __launch_bounds__(ROW_THREADS) void join_shared_sums_kernel(
 }
 
 // ---------------------------------------------------------------- gradients --
-/// 16-bit floats have five bits of exponent: d, most of whose numbers are a probability times a weight (of a mean: one in
-/// the number of rows), would lose most of its bits. It is stored times a power of two that brings the largest weight of
-/// the call to 2^13 .. 2^14 (twice that is the most d can be: below 65504), and the sums are divided by it again before they
-/// are rounded, which is exact. The other types have the exponents of `wide` or more than the weights need.
-template <typename T> constexpr bool SCALED = std::is_same_v<T, _Float16>;
+/// 16-bit types: d is stored relative to the weight of the first row with a target (its digits: a number in [1, 2)), and the
+/// sums are multiplied by it again, in 32 bits. The largest numbers of d are a weight times something just below one, and
+/// in the loss of a mean all weights are the same: rounded as they are, they would all be off by the same part, up to 2^-9
+/// of the gradients in bfloat16, and those would be off by it however many rows they sum up. 16-bit floats have five bits of
+/// exponent as well, and d, most of whose numbers are a probability times a weight (of a mean: one in the number of rows),
+/// would lose most of its bits: a power of two brings the largest weight of the call to 2^13 .. 2^14 (twice that is the
+/// most d can be: below 65504). The other types need neither.
+template <typename T> constexpr bool SCALED = sizeof(T) == 2;
+/// Up to so many rows the 16-bit types have d in two parts, what it is rounded to and what that leaves (as rows of their own,
+/// behind the others): a gradient of few rows consists of few numbers d, each times many numbers, and whether their errors
+/// are above or below the average is chance (3 rows of 38982 classes, K = 1127, bfloat16: errors of 2.8e-3 of the result,
+/// 1.7e-3 in two parts, which is what the result's own rounding makes). Rows cost little where the classes have to be
+/// read and their gradients written anyway.
+constexpr int32_t IN_TWO_PARTS = 256;
+/// Up to so many rows of d, grad_A takes as long as the classes take to be read, and two shares of them per compute unit have
+/// more on their way than one (rows of 50000 classes, K = 2048, bfloat16, one / two / three, us, all of the gradients: 3
+/// rows 249 / 214 / 209, 64 rows 307 / 288 / 261, 256 rows 592 / 510 / 527; of 32000, K = 512: 62 / 58 / 61, 73 / 75 / 75,
+/// 131 / 121 / 127; of 20000, K = 1127, float: 204 / 166 / 164, 500 rows 879 / 783 / 732).
+constexpr int32_t FEW_ROWS_OF_D = 512;
 template <typename T> struct Unscale {
-    const float* scale; // and its inverse (SCALED)
+    const float* scale; // and its inverse (SCALED; null: one)
 
     __device__ __forceinline__ wide_t<T> factor() const {
         if constexpr (SCALED<T>) {
-            return scale[0];
+            return scale != nullptr ? scale[0] : 1;
         }
         return 1;
     }
     __device__ __forceinline__ wide_t<T> operator()(wide_t<T> sum) const {
         if constexpr (SCALED<T>) {
-            return sum * scale[1];
+            return scale != nullptr ? sum * scale[1] : sum;
         }
         return sum;
     }
@@ -292,13 +307,20 @@ template <typename T> struct Weights {
     }
 };
 
-/// d[row, 0 .. stride - 1], whole pieces with zeros behind n_size.
+/// What the rounding to T leaves (nothing of what is infinite).
+template <typename T> __device__ __forceinline__ wide_t<T> rest_of(wide_t<T> x) {
+    const wide_t<T> rest = x - static_cast<wide_t<T>>(static_cast<T>(x));
+    return rest == rest ? rest : wide_t<T>(0);
+}
+
+/// d[row, 0 .. stride - 1], whole pieces with zeros behind n_size; what the rounding leaves of it in rows of their own.
 template <typename T> struct StoreGradients : Weights<T> {
     typedef wide_t<T> Wide;
     static constexpr bool PAIRS = false, RESTS = false;
     template <int BM, int BN> static constexpr bool ONCE = BM != BN; // (wide tiles: launch_logits)
     T* d;
     int32_t stride;
+    size_t rest_at; // numbers from a row to the row of what is left of it (0: nowhere)
 
     template <bool MAY_SPLIT, int LDS_BYTES, int BM, int BN, int WM, int WN>
     __device__ __forceinline__ void operator()(const Product<T>& g, const TileOf<T, BM, BN, WM, WN>& t) const {
@@ -339,13 +361,20 @@ template <typename T> struct StoreGradients : Weights<T> {
                 }
             });
         }
-        turn_over<T, Tile::NB, LDS_BYTES>(
-            t, [&](int i, int j, int e) { return t.sums[i][j][e]; },
-            [&](int row, int column, const typename Packed<T>::Numbers& numbers) {
-                T* const to = row < t.unit.count ? d + static_cast<size_t>(t.rows[row]) * stride : nullptr;
-                store_piece<false, T>(to, t.n0 + column, stride, numbers);
-            }
-        );
+        auto store = [&](T* rows) {
+            turn_over<T, Tile::NB, LDS_BYTES>(
+                t, [&](int i, int j, int e) { return t.sums[i][j][e]; },
+                [&](int row, int column, const typename Packed<T>::Numbers& numbers) {
+                    T* const to = row < t.unit.count ? rows + static_cast<size_t>(t.rows[row]) * stride : nullptr;
+                    store_piece<false, T>(to, t.n0 + column, stride, numbers);
+                }
+            );
+        };
+        store(d);
+        if (sizeof(T) == 2 && rest_at > 0) { // (uniform)
+            t.for_each([&](int i, int j, int e) { t.sums[i][j][e] = rest_of<T>(t.sums[i][j][e]); });
+            store(d + rest_at);
+        }
     }
 };
 
@@ -368,15 +397,53 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_shared_gradients_kernel(Pro
         x = finish.of_row(static_cast<int32_t>(row)).make(x, n);
     }
     finish.d[i] = static_cast<T>(x);
+    if (sizeof(T) == 2 && finish.rest_at > 0) {
+        finish.d[finish.rest_at + i] = static_cast<T>(rest_of<T>(x));
+    }
 }
 
-/// grad_A, summed up over the pieces of the classes in `sums` [row][n_size] (only where there are several).
+/// The rows and the plan of d in two parts: rows n_rows .. 2 n_rows - 1 of A are rows 0 .. n_rows - 1 again, in whole pieces
+/// with zeros behind them, and the places are those of the rows with a target, of what is left of them, and of the others.
+constexpr int TWICE_THREADS = 256;
+template <typename T>
+__global__ __launch_bounds__(TWICE_THREADS) void twice_kernel(
+    T* __restrict__ to, Operand<T> from, int32_t width, int32_t pieces, RowGroups groups, int32_t* __restrict__ order,
+    int32_t* __restrict__ offsets
+) {
+    constexpr int32_t COUNT = Matrix<T>::COUNT;
+    const int32_t rows = groups.n_rows;
+    const uint32_t i = blockIdx.x * TWICE_THREADS + threadIdx.x; // (of up to IN_TWO_PARTS rows: below 2^31)
+    if (i < static_cast<uint32_t>(rows) * pieces) {
+        const size_t row = i / pieces, piece = i % pieces;
+        const int32_t first = static_cast<int32_t>(piece) * COUNT;
+        const T* const at = from.data + row * from.stride + first;
+        const Numbers<T> numbers =
+            first + COUNT <= width ? load_numbers<T>(at) : load_some_numbers<T>(at, width - first);
+        *reinterpret_cast<Numbers<T>*>(to + (row * pieces + piece) * COUNT) = numbers;
+        *reinterpret_cast<Numbers<T>*>(to + ((row + rows) * pieces + piece) * COUNT) = numbers;
+    }
+    if (blockIdx.x == 0) {
+        const int32_t kept = groups.end_of(0, groups.begin_of(0));
+        for (int32_t place = threadIdx.x; place < rows; place += TWICE_THREADS) {
+            const int32_t row = groups.row_at(place), at = place < kept ? place : place + kept;
+            order[at] = row;
+            order[at + (place < kept ? kept : rows - kept)] = row + rows;
+        }
+        if (threadIdx.x == 0) {
+            offsets[0] = 0;
+            offsets[1] = 2 * kept;
+        }
+    }
+}
+
+/// grad_A, summed up over the pieces of the classes in `sums` [row][n_size] (only where there are several), or as partial
+/// results where d is in two parts.
 template <typename T> struct AddRows {
     typedef wide_t<T> Wide;
     static constexpr bool PAIRS = false, RESTS = true;
     template <int BM, int BN> static constexpr bool ONCE = false;
     Wide* sums;
-    bool first, last;
+    bool first, last, twice;
     Unscale<T> scale;
 
     template <bool MAY_SPLIT, int LDS_BYTES, int BM, int BN, int WM, int WN>
@@ -384,9 +451,22 @@ template <typename T> struct AddRows {
         typedef TileOf<T, BM, BN, WM, WN> Tile;
         const bool alone = first && last;
         const bool rest = t.unit.group == g.groups.n_groups;
-        if ((MAY_SPLIT && g.splits > 1) || alone) { // (uniform)
+        if ((MAY_SPLIT && g.splits > 1) || (alone && !twice)) { // (uniform)
             StoreSums<T, Form::FORWARD, Unscale<T>>{scale}.template operator()<MAY_SPLIT, LDS_BYTES>(g, t);
             return;
+        }
+        if constexpr (sizeof(T) == 2) {
+            if (twice) { // (uniform)
+                turn_over<Wide, Tile::NB, LDS_BYTES>(
+                    t, [&](int i, int j, int e) { return scale(t.sums[i][j][e]); },
+                    [&](int row, int column, const typename Packed<Wide>::Numbers& numbers) {
+                        Wide* const to =
+                            row < t.unit.count ? g.partial + static_cast<size_t>(t.rows[row]) * g.n_size : nullptr;
+                        store_piece<false, Wide>(to, t.n0 + column, g.n_size, numbers);
+                    }
+                );
+                return;
+            }
         }
         if (rest && !last) { // (uniform)
             return;
@@ -437,15 +517,23 @@ template <typename T> struct AddRows {
     }
 };
 
-/// The same from shares of k (which are scaled already): a thread per number.
+/// The same from shares of k and from both parts of d (which are scaled already): a thread per number.
 template <typename T> __global__ __launch_bounds__(JOIN_THREADS) void add_shares_kernel(Product<T> g, AddRows<T> finish) {
-    const size_t size = static_cast<size_t>(g.groups.n_rows) * g.n_size;
+    const size_t size = static_cast<size_t>(g.groups.n_rows) * g.n_size; // (of a share)
+    const size_t results = finish.twice ? size / 2 : size;
     const size_t i = blockIdx.x * static_cast<size_t>(JOIN_THREADS) + threadIdx.x;
-    if (i < size) {
+    if (i < results) {
         wide_t<T> sum = finish.first ? wide_t<T>(0) : finish.sums[i];
+        const int32_t splits = max(g.splits, 1);
 #pragma unroll 8
-        for (int32_t s = 0; s < g.splits; s++) {
+        for (int32_t s = 0; s < splits; s++) {
             sum += g.partial[s * size + i];
+        }
+        if (finish.twice) { // (uniform)
+#pragma unroll 8
+            for (int32_t s = 0; s < splits; s++) {
+                sum += g.partial[s * size + results + i];
+            }
         }
         if (finish.last) {
             g.out[i] = static_cast<T>(sum);
@@ -592,12 +680,13 @@ constexpr size_t SMALLEST_PIECE = 256;
 template <typename T> class Backward : Call<T> {
 public:
     Backward(const Inputs<T>& inputs, T* grad_A, T* grad_W) : Call<T>(inputs), grad_A_(grad_A), grad_W_(grad_W) {
-        sums_.groups = last_sums_.groups = rows_.groups = this->logits_.groups;
+        twice_ = sizeof(T) == 2 && inputs.rows <= IN_TWO_PARTS;
+        sums_.groups = last_sums_.groups = rows_.groups = RowGroups{nullptr, nullptr, 1, rows_of_d()};
         sums_.n_size = last_sums_.n_size = rows_.n_size = inputs.k_size;
         choose(worth_copying(this->A_, this->W_, 3 * this->operations()), MOST_BYTES);
     }
     void choose(bool copied, size_t most_bytes) {
-        const size_t classes = this->in_.classes, row_bytes = std::max<size_t>(this->in_.rows, 1) * sizeof(T);
+        const size_t classes = this->in_.classes, row_bytes = std::max<size_t>(rows_of_d(), 1) * sizeof(T);
         const size_t most = std::max(most_bytes / row_bytes / SMALLEST_PIECE * SMALLEST_PIECE, SMALLEST_PIECE);
         // Tiles of grad_W in whole rounds of all compute units, where a piece has room for one (8192 rows, 100003 classes, K =
         // 2048, bfloat16: 10.3 ms; in four pieces of the same size, 3.06 rounds each, 11.2).
@@ -607,7 +696,7 @@ public:
         each_ = classes <= most ? classes : round <= most ? most / round * round : most;
         stride_ = static_cast<int32_t>(ceil_div(each_, PIECE<T>)) * PIECE<T>;
         this->choose_logits(copied, static_cast<int32_t>(each_));
-        sums_.in_place = last_sums_.in_place = copied || this->A_.in_place();
+        sums_.in_place = last_sums_.in_place = copied || twice_ || this->A_.in_place();
         rows_.in_place = copied || this->W_.in_place();
         sums_.m_size = rows_.k_size = static_cast<int32_t>(each_);
         // (the last piece may be a small one, whose rows are shared out further)
@@ -615,11 +704,11 @@ public:
         of_sums_ = choose_sums(sums_);
         of_last_sums_ = choose_sums(last_sums_);
         of_rows_ = tile_of_rows(rows_);
-        share_k(rows_, of_rows_);
+        share_k(rows_, of_rows_, rows_.groups.n_rows <= FEW_ROWS_OF_D ? 2 : 1);
     }
     bool copies() const { return this->copied_bytes() > 0; }
     size_t bytes() const {
-        return Plan::bytes(this->in_.rows) + this->copied_bytes() + 256 + d_bytes() + total_bytes() +
+        return Plan::bytes(this->in_.rows) + this->copied_bytes() + 256 + twice_bytes() + d_bytes() + total_bytes() +
                std::max(split_bytes(this->logits_), row_bytes() + sum_bytes());
     }
     void run(
@@ -629,13 +718,25 @@ public:
         typedef wide_t<T> Wide;
         const Inputs<T>& in = this->in_;
         const RowGroups groups = this->begin(room, true, stream);
-        const Unscale<T> scale{reinterpret_cast<float*>(room)};
+        // (numbers in two parts are as good at any scale that their type holds)
+        const bool scaled = SCALED<T> && (std::is_same_v<T, _Float16> || !twice_);
+        const Unscale<T> scale{scaled ? reinterpret_cast<float*>(room) : nullptr};
         if constexpr (SCALED<T>) {
-            find_scale(
-                reinterpret_cast<float*>(room), grad_losses, grad_log_sums, in.targets, in.rows, in.classes, stream
-            );
+            if (scaled) {
+                find_scale(
+                    reinterpret_cast<float*>(room), grad_losses, grad_log_sums, in.targets, groups, in.classes,
+                    std::is_same_v<T, _Float16>, stream
+                );
+            }
         }
         room += 256;
+        RowGroups groups_of_d = groups;
+        Operand<T> A = this->of_A_;
+        if constexpr (sizeof(T) == 2) {
+            if (twice_) {
+                std::tie(groups_of_d, A) = twice(groups, room, stream);
+            }
+        }
         T* const d = reinterpret_cast<T*>(room);
         room += d_bytes();
         Wide* const totals = reinterpret_cast<Wide*>(room);
@@ -653,7 +754,8 @@ public:
             g.p = Operand<T>{this->of_W_.data + W_at, this->of_W_.stride};
             g.partial = reinterpret_cast<Wide*>(room);
             const StoreGradients<T> make{
-                {grad_losses, grad_log_sums, log_sums, in.targets, static_cast<int32_t>(first), scale}, d, stride_
+                {grad_losses, grad_log_sums, log_sums, in.targets, static_cast<int32_t>(first), scale}, d, stride_,
+                twice_ ? static_cast<size_t>(in.rows) * stride_ : 0
             };
             if (count > 0) {
                 this->launch_logits(g, stream, make);
@@ -664,27 +766,48 @@ public:
                 MOPS_HIP_CHECK(hipGetLastError());
             }
             Product<T> sums = last ? last_sums_ : sums_, rows = rows_;
-            sums.groups = rows.groups = groups;
+            sums.groups = rows.groups = groups_of_d;
             sums.out = grad_W_ != nullptr ? grad_W_ + first * in.k_size : nullptr;
             rows.k_size = count;
             sums.q = rows.q = Operand<T>{d, stride_};
-            sums.p = this->of_A_;
+            sums.p = A;
             rows.out = grad_A_;
             rows.p = g.p;
             rows.partial = reinterpret_cast<Wide*>(room);
             sums.partial = reinterpret_cast<Wide*>(room + row_bytes());
-            multiply(sums, last ? of_last_sums_ : of_sums_, rows, StoreSums<T, Form::GRAD_SUMS, Unscale<T>>{scale}, AddRows<T>{totals, first == 0, last, scale}, stream);
+            multiply(sums, last ? of_last_sums_ : of_sums_, rows, StoreSums<T, Form::GRAD_SUMS, Unscale<T>>{scale}, AddRows<T>{totals, first == 0, last, twice_, scale}, stream);
         }
     }
 
 private:
-    size_t d_bytes() const { return align256(static_cast<size_t>(this->in_.rows) * stride_ * sizeof(T)); }
+    int32_t rows_of_d() const { return this->in_.rows * (twice_ ? 2 : 1); }
+    size_t d_bytes() const { return align256(static_cast<size_t>(rows_of_d()) * stride_ * sizeof(T)); }
+    size_t plan_of_d_bytes() const { return 256 + align256(static_cast<size_t>(rows_of_d()) * 4); }
+    size_t twice_bytes() const {
+        return twice_ ? plan_of_d_bytes() + align256(static_cast<size_t>(rows_of_d()) * this->A_.pieces() * 16) : 0;
+    }
+    /// The rows of A twice and the plan of both parts of d.
+    std::tuple<RowGroups, Operand<T>> twice(const RowGroups& groups, char*& room, hipStream_t stream) const {
+        int32_t *const offsets = reinterpret_cast<int32_t*>(room), *const order = offsets + 64;
+        T* const to = reinterpret_cast<T*>(room + plan_of_d_bytes());
+        const int32_t pieces = this->A_.pieces();
+        const size_t blocks = std::max<size_t>(ceil_div(static_cast<size_t>(this->in_.rows) * pieces, TWICE_THREADS), 1);
+        twice_kernel<T><<<static_cast<unsigned>(blocks), TWICE_THREADS, 0, stream>>>(
+            to, this->of_A_, this->in_.k_size, pieces, groups, order, offsets
+        );
+        MOPS_HIP_CHECK(hipGetLastError());
+        room += twice_bytes();
+        return {RowGroups{offsets, order, 1, rows_of_d()}, Operand<T>{to, pieces * PIECE<T>}};
+    }
     size_t total_bytes() const { // (of grad_A over the pieces)
         return grad_A_ != nullptr && each_ < static_cast<size_t>(this->in_.classes)
                    ? align256(static_cast<size_t>(this->in_.rows) * this->in_.k_size * sizeof(wide_t<T>))
                    : 0;
     }
-    size_t row_bytes() const { return grad_A_ != nullptr ? split_bytes(rows_) : 0; }
+    size_t row_bytes() const {
+        const size_t of_share = align256(static_cast<size_t>(rows_of_d()) * rows_.n_size * sizeof(wide_t<T>));
+        return grad_A_ == nullptr ? 0 : twice_ && rows_.splits <= 1 ? of_share : split_bytes(rows_);
+    }
     size_t sum_bytes() const {
         auto of = [](const Product<T>& sums) {
             return sums.most_slots * partial_size(sums.m_size, sums.n_size) * sizeof(wide_t<T>);
@@ -737,8 +860,8 @@ private:
                 launch<T, Form::FORWARD>(rows, of_rows_, stream, finish_rows);
             }
         }
-        if (of_A && rows.splits > 1) {
-            const size_t blocks = ceil_div(static_cast<size_t>(rows.groups.n_rows) * rows.n_size, JOIN_THREADS);
+        if (of_A && (rows.splits > 1 || (twice_ && this->in_.rows > 0 && rows.n_size > 0))) {
+            const size_t blocks = ceil_div(static_cast<size_t>(this->in_.rows) * rows.n_size, JOIN_THREADS); // (of numbers of grad_A)
             add_shares_kernel<T><<<static_cast<unsigned>(blocks), JOIN_THREADS, 0, stream>>>(rows, finish_rows);
             MOPS_HIP_CHECK(hipGetLastError());
         }
@@ -750,6 +873,7 @@ private:
     }
 
     T *const grad_A_, *const grad_W_;
+    bool twice_; // d is in two parts
     size_t each_; // classes per piece
     int32_t stride_;
     Product<T> sums_{}, last_sums_{}, rows_{};

@@ -192,8 +192,8 @@ template <typename T> int tile_of_sums(Product<T>& g) {
 }
 
 /// FORWARD and GRAD_ROWS with few tiles and long sums: every compute unit gets a share of k (250 rows of 19 groups, K = 24,
-/// L = 1226 in float, gradients: 20 workgroups, one of 39 steps after the other, are 41 us). At least four steps each.
-template <typename T> void share_k(Product<T>& g, int tile) {
+/// L = 1226 in float, gradients: 20 workgroups, one of 39 steps after the other, are 41 us), or `per_unit` of them. At least four steps each.
+template <typename T> void share_k(Product<T>& g, int tile, size_t per_unit = 1) {
     g.splits = 1;
     g.k_each = g.k_size;
     if (tile != 64) {
@@ -202,7 +202,7 @@ template <typename T> void share_k(Product<T>& g, int tile) {
     const size_t step = 16 / sizeof(T) * DEEP, steps = ceil_div(static_cast<size_t>(g.k_size), step);
     const size_t rows = static_cast<size_t>(g.groups.n_rows), groups = static_cast<size_t>(g.groups.n_groups);
     const size_t workgroups = std::min(ceil_div(rows, 64) + groups, rows) * tiles(g.n_size, 64);
-    const size_t units = static_cast<size_t>(compute_units());
+    const size_t units = per_unit * static_cast<size_t>(compute_units());
     if (workgroups > 0 && workgroups < units && steps >= 8) {
         const size_t splits = std::min(ceil_div(units, workgroups), steps / 4), each = ceil_div(steps, splits);
         g.splits = static_cast<int32_t>(ceil_div(steps, each));

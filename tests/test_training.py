@@ -220,14 +220,14 @@ def loss_case(rows, classes, K, kind, dtype, spread=3.0):
     return A, W, targets, grads
 
 
-def loss_by_definition(A, W, targets, grads, dtype):
+def loss_by_definition(A, W, targets, grads, dtype, of_rounding=None):
     """Per result, exact and bound. The logits x are off by E = (K + 32) 2^-p X, X the sum of their terms' magnitudes.
     A power exp(x - m) is off by its argument's error and 2^-p (|x| + |m| + 8) of itself, so the sums' logarithm s by
     S = max(E) + 2^-p (2 max|x| + V + 64 + 4 |s|), a loss by S + E[target] + 4 2^-p (|s| + |loss|). d = a exp(x - s) - g 1
     is off by |a| exp(x - s) (E + S + 2^-p (|x| + |s| + 8)) + 4 2^-p (|a| p + g 1) and, rounded to the type, by 2^-q |d|
     (float16: by its smallest number's half, at the scale at which the largest weight is 2^13 at least: 2^-38 of that); the
-    products of d add (n + 16) 2^-p of their terms' magnitudes."""
-    p, q = unit(dtype), 2.0 ** -BITS[dtype]
+    products of d add (n + 16) 2^-p of their terms' magnitudes. `of_rounding`: another part of d than 2^-q."""
+    p, q = unit(dtype), 2.0 ** -BITS[dtype] if of_rounding is None else of_rounding
     A, W, (g, h) = A.double(), W.double(), [x.double() for x in grads]
     rows, K, V = A.shape[0], A.shape[1], W.shape[0]
     kept = (targets >= 0) & (targets < V)
@@ -286,6 +286,71 @@ def test_linear_cross_entropy(device, rows, classes, K, kind, tag):
             mops_amd.linear_cross_entropy_vjp(*one, A, W, targets, log_sums),
             mops_amd.linear_cross_entropy_vjp(*other, A, W, targets, log_sums),
         )
+
+
+HALVES = ["bf16", "f16"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tag", HALVES)
+@pytest.mark.parametrize(
+    "rows,classes,K,kind",
+    [
+        (1, 3, 8, "uniform"), (3, 4001, 127, "uniform"), (2, 33001, 64, "uniform"), (9, 95, 200, "padded"),
+        (64, 500, 64, "frequent"), (65, 130, 1030, "padded"), (200, 94, 128, "one"), (255, 700, 33, "padded"),
+        (256, 1500, 72, "uniform"), (40, 70, 2, "nowhere"), (7, 5, 2001, "padded"),
+    ],
+)  # fmt: skip
+def test_gradients_of_few_rows_are_rounded_once(device, rows, classes, K, kind, tag):
+    """d is held in two parts: what the second one's rounding leaves is 2^-q of 2^-q of d (and of a part that is infinite or
+    not a number nothing)."""
+    dtype = DTYPES[tag]
+    A, W, targets, grads = loss_case(rows, classes, K, kind, dtype)
+    results = loss_by_definition(A, W, targets, grads, dtype, 2.0 ** (-2 * BITS[dtype]))
+    A, W, targets, grads = A.to(device), W.to(device), targets.to(device), [g.to(device) for g in grads]
+    _, log_sums = mops_amd.linear_cross_entropy(A, W, targets)
+    grad_A, grad_W = mops_amd.linear_cross_entropy_vjp(*grads, A, W, targets, log_sums)
+    held_to(grad_A, *results[2], "grad_A")
+    held_to(grad_W, *results[3], "grad_W")
+    # what rows without a target hold reaches nothing, and an infinite weight everything
+    outside = (targets < 0) | (targets >= classes)
+    B = A.clone()
+    B[outside] = float("nan")
+    assert same(mops_amd.linear_cross_entropy_vjp(*grads, B, W, targets, log_sums), (grad_A, grad_W))
+    grads[0][0] = float("inf")
+    of_infinite = mops_amd.linear_cross_entropy_vjp(*grads, A, W, targets, log_sums)
+    assert outside[0] or (not of_infinite[0][0].isfinite().any() and not of_infinite[1].isfinite().any())
+    assert torch.equal(of_infinite[0][1:], grad_A[1:]) or tag == "f16"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [100, 600, 2000])
+@pytest.mark.parametrize("weight", [1 + 2.0**-8, 1 + 2.0**-11, 1.5 + 2.0**-8 + 2.0**-10])
+@pytest.mark.parametrize("tag", HALVES)
+def test_gradients_of_a_mean_are_not_off_by_its_weight(device, tag, weight, rows):
+    """Rows with one weight g each, of a number that the type rounds, and logits that are zero: the powers are 2^-12 each, d is
+    g 2^-12 (of the type, but for g) and g (2^-12 - 1) at the target, which is off by g 2^-12 at most where g is not rounded
+    itself (2^-8 g and 2^-11 g). Products add (n + 16) 2^-24 of their terms' magnitudes, powers 64 2^-24."""
+    dtype, classes, K = DTYPES[tag], 4096, 16
+    generator = generator_of(rows)
+    A, W = random(generator, (rows, K), dtype), random(generator, (classes, K), dtype)
+    A[:, K // 2 :], W[:, : K // 2] = 0, 0
+    targets = indices_of("uniform", rows, classes)
+    g = weight / 1024
+    d = torch.full((rows, classes), g / classes, dtype=torch.float64)
+    at = torch.arange(rows), targets.long()
+    d[at] -= g
+    off = 80 * 2.0**-24 * d.abs()
+    off[at] += g * 2.0**-12
+    a, w = A.double(), W.double()
+    bound_A = off @ w.abs() + (classes + 16) * 2.0**-24 * (d.abs() @ w.abs())
+    bound_W = off.t() @ a.abs() + (rows + 16) * 2.0**-24 * (d.abs().t() @ a.abs())
+    A, W, targets = A.to(device), W.to(device), targets.to(device)
+    _, log_sums = mops_amd.linear_cross_entropy(A, W, targets)
+    grads = torch.full((rows,), g, device=device)
+    grad_A, grad_W = mops_amd.linear_cross_entropy_vjp(grads, None, A, W, targets, log_sums)
+    held_to(grad_A, d @ w, bound_A, "grad_A")
+    held_to(grad_W, d.t() @ a, bound_W, "grad_W")
 
 
 @pytest.mark.gpu
@@ -887,12 +952,16 @@ os.environ["MOPS_AMD_TEST_SCRATCH_LIMIT"] = str(48 << 20)  # what a nearly full 
 library = device_library().cdll
 library.mops_amd_scratch_capacity.restype = ctypes.c_int64
 device = torch.device("cuda:0")
-for rows, classes, K, dtype in [(4100, 9000, 72, torch.bfloat16), (2100, 9001, 65, torch.float32), (4100, 9000, 71, torch.float16)]:
+cases = [
+    (4100, 9000, 72, torch.bfloat16), (2100, 9001, 65, torch.float32), (4100, 9000, 71, torch.float16),
+    (250, 90001, 72, torch.bfloat16), (250, 90001, 40, torch.float16),  # (in two parts, three pieces each)
+]
+for rows, classes, K, dtype in cases:
     A, W, targets, grads = [
         [x.to(device) for x in y] if isinstance(y, list) else y.to(device)
         for y in t.loss_case(rows, classes, K, "padded", dtype)
     ]
-    results = t.loss_by_definition(A, W, targets, grads, dtype)
+    results = t.loss_by_definition(A, W, targets, grads, dtype, 2.0 ** (-2 * t.BITS[dtype]) if rows == 250 else None)
     losses, log_sums = mops_amd.linear_cross_entropy(A, W, targets)
     t.held_to(losses, *results[0], "losses")
     grad_A, grad_W = mops_amd.linear_cross_entropy_vjp(*grads, A, W, targets, log_sums)
@@ -937,7 +1006,7 @@ def test_on_a_device_that_is_nearly_full(device):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     done = subprocess.run([sys.executable, "-c", FULL_DEVICE], cwd=root, capture_output=True, text=True, timeout=100)
     assert done.returncode == 0, done.stdout + done.stderr[-3000:]
-    assert done.stdout.count("ok") == 4, done.stdout
+    assert done.stdout.count("ok") == 6, done.stdout
 
 
 # ------------------------------------------------------ PyTorch operators ----
