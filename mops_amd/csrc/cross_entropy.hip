@@ -104,9 +104,7 @@ __global__ __launch_bounds__(SCALE_THREADS) void find_scale_kernel(
     for (int32_t r = threadIdx.x; of_powers && r < groups.n_rows; r += SCALE_THREADS) {
         const bool kept = targets[r] >= 0 && targets[r] < classes;
         const float g = grad_losses != nullptr ? grad_losses[r] : 0, h = grad_log_sums != nullptr ? grad_log_sums[r] : 0;
-        const float weight = fmaxf(fabsf(g), fabsf(g + h));
-        // (no scale makes numbers of what is none)
-        most = kept && weight <= std::numeric_limits<float>::max() ? fmaxf(most, weight) : most;
+        most = kept ? fmaxf(most, weight_of(g, h)) : most;
     }
 #pragma unroll
     for (int s = 1; s < WAVE; s *= 2) {
@@ -120,15 +118,7 @@ __global__ __launch_bounds__(SCALE_THREADS) void find_scale_kernel(
         for (int w = 1; w < static_cast<int>(blockDim.x / WAVE); w++) {
             most = fmaxf(most, shared[w]);
         }
-        int exponent = 0;
-        const float first = grad_losses != nullptr && groups.n_rows > 0 ? fabsf(grad_losses[groups.row_at(0)]) : 0;
-        const bool has_digits = first > 0 && first <= std::numeric_limits<float>::max();
-        const float digits = has_digits ? 2 * frexpf(first, &exponent) : 1;
-        exponent = 0;
-        frexpf(most / digits, &exponent); // most / digits < 2^exponent
-        exponent = most > 0 ? min(max(14 - exponent, -125), 125) : 0;
-        scale[0] = ldexpf(1 / digits, exponent);
-        scale[1] = ldexpf(digits, -exponent);
+        set_scale(scale, grad_losses != nullptr && groups.n_rows > 0 ? grad_losses[groups.row_at(0)] : 0, most);
     }
 }
 

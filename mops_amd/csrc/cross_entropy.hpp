@@ -5,6 +5,7 @@
 #define MOPS_AMD_CROSS_ENTROPY_HPP
 
 #include <cstdint>
+#include <limits>
 
 #include <hip/hip_runtime.h>
 
@@ -36,6 +37,24 @@ void rows_with_targets(
     int32_t* order, int32_t* offsets, int32_t* counts, const int32_t* targets, int32_t rows, int32_t classes,
     hipStream_t stream
 );
+
+/// The largest that d can be made of, but for a factor of two (0 where that is no number: no scale makes one of it).
+__device__ __forceinline__ float weight_of(float g, float h) {
+    const float weight = fmaxf(fabsf(g), fabsf(g + h));
+    return weight <= std::numeric_limits<float>::max() ? weight : 0;
+}
+/// The scale of d, from the first kept row's weight of the loss and the largest of all of them (0: no power of two).
+__device__ __forceinline__ void set_scale(float* scale, float first, float most) {
+    int exponent = 0;
+    first = fabsf(first);
+    const bool has_digits = first > 0 && first <= std::numeric_limits<float>::max();
+    const float digits = has_digits ? 2 * frexpf(first, &exponent) : 1;
+    exponent = 0;
+    frexpf(most / digits, &exponent); // most / digits < 2^exponent
+    exponent = most > 0 ? min(max(14 - exponent, -125), 125) : 0;
+    scale[0] = ldexpf(1 / digits, exponent);
+    scale[1] = ldexpf(digits, -exponent);
+}
 
 /// scale = {what d is multiplied by, its inverse}: the first kept row's weight, its digits only, or times a power of two.
 void find_scale(

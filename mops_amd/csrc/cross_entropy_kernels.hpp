@@ -267,7 +267,7 @@ constexpr int32_t IN_TWO_PARTS = 256;
 /// 131 / 121 / 127; of 20000, K = 1127, float: 204 / 166 / 164, 500 rows 879 / 783 / 732).
 constexpr int32_t FEW_ROWS_OF_D = 512;
 template <typename T> struct Unscale {
-    const float* scale; // and its inverse (SCALED; null: one)
+    float* scale; // and its inverse (SCALED; null: one)
 
     __device__ __forceinline__ wide_t<T> factor() const {
         if constexpr (SCALED<T>) {
@@ -402,16 +402,21 @@ __global__ __launch_bounds__(JOIN_THREADS) void join_shared_gradients_kernel(Pro
     }
 }
 
-/// The rows and the plan of d in two parts: rows n_rows .. 2 n_rows - 1 of A are rows 0 .. n_rows - 1 again, in whole pieces
-/// with zeros behind them, and the places are those of the rows with a target, of what is left of them, and of the others.
-constexpr int TWICE_THREADS = 256;
+/// The plans of few rows, of d in two parts and the scale of it, in one launch (50 rows of 63 classes, K = 4, float16, losses and
+/// gradients: 31.8 us; 37.1 in launches of their own). Rows n_rows .. 2 n_rows - 1 of A are rows 0 .. n_rows - 1 again, in whole pieces with zeros behind
+/// them; the places are those of the rows with a target, of what is left of them, and of the others.
+constexpr int TWICE_THREADS = IN_TWO_PARTS; // (a row each in the first workgroup)
+struct PlanOfTwice {
+    int32_t *order, *offsets;             // of the rows: as rows_with_targets
+    int32_t *twice_order, *twice_offsets; // of the rows of d
+    float* scale;                         // (null: none)
+};
 template <typename T>
 __global__ __launch_bounds__(TWICE_THREADS) void twice_kernel(
-    T* __restrict__ to, Operand<T> from, int32_t width, int32_t pieces, RowGroups groups, int32_t* __restrict__ order,
-    int32_t* __restrict__ offsets
+    T* __restrict__ to, Operand<T> from, int32_t width, int32_t pieces, PlanOfTwice plan, const int32_t* __restrict__ targets,
+    const float* __restrict__ grad_losses, const float* __restrict__ grad_log_sums, int32_t rows, int32_t classes
 ) {
     constexpr int32_t COUNT = Matrix<T>::COUNT;
-    const int32_t rows = groups.n_rows;
     const uint32_t i = blockIdx.x * TWICE_THREADS + threadIdx.x; // (of up to IN_TWO_PARTS rows: below 2^31)
     if (i < static_cast<uint32_t>(rows) * pieces) {
         const size_t row = i / pieces, piece = i % pieces;
@@ -422,17 +427,48 @@ __global__ __launch_bounds__(TWICE_THREADS) void twice_kernel(
         *reinterpret_cast<Numbers<T>*>(to + (row * pieces + piece) * COUNT) = numbers;
         *reinterpret_cast<Numbers<T>*>(to + ((row + rows) * pieces + piece) * COUNT) = numbers;
     }
-    if (blockIdx.x == 0) {
-        const int32_t kept = groups.end_of(0, groups.begin_of(0));
-        for (int32_t place = threadIdx.x; place < rows; place += TWICE_THREADS) {
-            const int32_t row = groups.row_at(place), at = place < kept ? place : place + kept;
-            order[at] = row;
-            order[at + (place < kept ? kept : rows - kept)] = row + rows;
-        }
-        if (threadIdx.x == 0) {
-            offsets[0] = 0;
-            offsets[1] = 2 * kept;
-        }
+    if (blockIdx.x > 0) { // (uniform)
+        return;
+    }
+    constexpr int WAVES = TWICE_THREADS / WAVE;
+    __shared__ int32_t counts[WAVES];
+    __shared__ float largest[WAVES];
+    const int32_t row = threadIdx.x;
+    const int lane = threadIdx.x % WAVE, wave = threadIdx.x / WAVE;
+    const bool kept = row < rows && in_bounds(targets[row], classes);
+    const float g = kept && grad_losses != nullptr ? grad_losses[row] : 0;
+    const float h = kept && grad_log_sums != nullptr ? grad_log_sums[row] : 0;
+    float most = weight_of(g, h);
+#pragma unroll
+    for (int s = 1; s < WAVE; s *= 2) {
+        most = fmaxf(most, __shfl_xor(most, s));
+    }
+    const uint64_t of_lanes = __ballot(kept);
+    if (lane == 0) {
+        counts[wave] = __popcll(of_lanes);
+        largest[wave] = most;
+    }
+    __syncthreads();
+    int32_t before = __popcll(of_lanes & ((uint64_t(1) << lane) - 1)), all = 0; // of the kept rows
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        before += w < wave ? counts[w] : 0;
+        all += counts[w];
+        most = fmaxf(most, largest[w]);
+    }
+    if (row < rows) {
+        const int32_t at = kept ? before : 2 * all + row - before;
+        plan.order[kept ? before : all + row - before] = row;
+        plan.twice_order[at] = row;
+        plan.twice_order[at + (kept ? all : rows - all)] = row + rows;
+    }
+    if (threadIdx.x == 0) {
+        plan.offsets[0] = plan.twice_offsets[0] = 0;
+        plan.offsets[1] = all;
+        plan.twice_offsets[1] = 2 * all;
+    }
+    if (plan.scale != nullptr && (kept ? before == 0 : all == 0 && threadIdx.x == 0)) {
+        set_scale(plan.scale, g, most);
     }
 }
 
@@ -553,9 +589,10 @@ constexpr int32_t FEW_ROWS = 256;
 
 /// The plan of a call's rows, in its workspace.
 struct Plan {
-    int32_t *order, *offsets, *counts;
+    int32_t *order = nullptr, *offsets = nullptr, *counts = nullptr;
 
     static size_t bytes(int32_t rows) { return align256(static_cast<size_t>(rows) * 4) + 256 + align256(row_chunks(rows) * 4); }
+    Plan() = default;
     Plan(char*& room, int32_t rows) {
         order = reinterpret_cast<int32_t*>(room);
         offsets = reinterpret_cast<int32_t*>(room + align256(static_cast<size_t>(rows) * 4));
@@ -597,20 +634,21 @@ protected:
     size_t copied_bytes() const { return copied_ ? A_.copied_bytes() + W_.copied_bytes() : 0; }
     /// The operands, the plan (if `planned`) and the groups of everything.
     RowGroups begin(char*& room, bool planned, hipStream_t stream) {
-        const Plan plan(room, in_.rows);
+        plan_ = Plan(room, in_.rows);
         if (planned) {
-            rows_with_targets(plan.order, plan.offsets, plan.counts, in_.targets, in_.rows, in_.classes, stream);
+            rows_with_targets(plan_.order, plan_.offsets, plan_.counts, in_.targets, in_.rows, in_.classes, stream);
         }
         char* none = nullptr;
         of_A_ = place(A_, copied_ ? room : none, stream);
         of_W_ = place(W_, copied_ ? room : none, stream);
-        return planned ? RowGroups{plan.offsets, plan.order, 1, in_.rows} : RowGroups{nullptr, nullptr, 1, in_.rows};
+        return planned ? RowGroups{plan_.offsets, plan_.order, 1, in_.rows} : RowGroups{nullptr, nullptr, 1, in_.rows};
     }
 
     const Inputs<T> in_;
     const Matrices<T> A_, W_;
     Operand<T> of_A_{}, of_W_{};
     Product<T> logits_{};
+    Plan plan_;
     int of_logits_ = 64; // columns of a tile of logits
     bool wide_ = false, copied_ = false;
 };
@@ -717,24 +755,20 @@ public:
     ) {
         typedef wide_t<T> Wide;
         const Inputs<T>& in = this->in_;
-        const RowGroups groups = this->begin(room, true, stream);
+        RowGroups groups = this->begin(room, !twice_, stream), groups_of_d = groups;
         // (numbers in two parts are as good at any scale that their type holds)
         const bool scaled = SCALED<T> && (std::is_same_v<T, _Float16> || !twice_);
         const Unscale<T> scale{scaled ? reinterpret_cast<float*>(room) : nullptr};
+        room += 256;
+        Operand<T> A = this->of_A_;
         if constexpr (SCALED<T>) {
-            if (scaled) {
+            if (twice_) {
+                std::tie(groups, groups_of_d, A) = twice(scale.scale, grad_losses, grad_log_sums, room, stream);
+            } else {
                 find_scale(
-                    reinterpret_cast<float*>(room), grad_losses, grad_log_sums, in.targets, groups, in.classes,
+                    scale.scale, grad_losses, grad_log_sums, in.targets, groups, in.classes,
                     std::is_same_v<T, _Float16>, stream
                 );
-            }
-        }
-        room += 256;
-        RowGroups groups_of_d = groups;
-        Operand<T> A = this->of_A_;
-        if constexpr (sizeof(T) == 2) {
-            if (twice_) {
-                std::tie(groups_of_d, A) = twice(groups, room, stream);
             }
         }
         T* const d = reinterpret_cast<T*>(room);
@@ -786,18 +820,25 @@ private:
     size_t twice_bytes() const {
         return twice_ ? plan_of_d_bytes() + align256(static_cast<size_t>(rows_of_d()) * this->A_.pieces() * 16) : 0;
     }
-    /// The rows of A twice and the plan of both parts of d.
-    std::tuple<RowGroups, Operand<T>> twice(const RowGroups& groups, char*& room, hipStream_t stream) const {
+    /// The plans of the rows and of both parts of d, and the rows of A twice.
+    std::tuple<RowGroups, RowGroups, Operand<T>> twice(
+        float* scale, const float* grad_losses, const float* grad_log_sums, char*& room, hipStream_t stream
+    ) const {
+        const Inputs<T>& in = this->in_;
         int32_t *const offsets = reinterpret_cast<int32_t*>(room), *const order = offsets + 64;
         T* const to = reinterpret_cast<T*>(room + plan_of_d_bytes());
         const int32_t pieces = this->A_.pieces();
-        const size_t blocks = std::max<size_t>(ceil_div(static_cast<size_t>(this->in_.rows) * pieces, TWICE_THREADS), 1);
+        const size_t blocks = std::max<size_t>(ceil_div(static_cast<size_t>(in.rows) * pieces, TWICE_THREADS), 1);
         twice_kernel<T><<<static_cast<unsigned>(blocks), TWICE_THREADS, 0, stream>>>(
-            to, this->of_A_, this->in_.k_size, pieces, groups, order, offsets
+            to, this->of_A_, in.k_size, pieces, PlanOfTwice{this->plan_.order, this->plan_.offsets, order, offsets, scale},
+            in.targets, grad_losses, grad_log_sums, in.rows, in.classes
         );
         MOPS_HIP_CHECK(hipGetLastError());
         room += twice_bytes();
-        return {RowGroups{offsets, order, 1, rows_of_d()}, Operand<T>{to, pieces * PIECE<T>}};
+        return {
+            RowGroups{this->plan_.offsets, this->plan_.order, 1, in.rows}, RowGroups{offsets, order, 1, rows_of_d()},
+            Operand<T>{to, pieces * PIECE<T>}
+        };
     }
     size_t total_bytes() const { // (of grad_A over the pieces)
         return grad_A_ != nullptr && each_ < static_cast<size_t>(this->in_.classes)
