@@ -10,6 +10,7 @@
 #include <Python.h>
 
 #include <array>
+#include <exception>
 #include <vector>
 
 #include <torch/csrc/autograd/python_variable.h>
@@ -656,7 +657,8 @@ bool gradients_of(PyObject* object, std::vector<at::Tensor>& gradients, bool in_
             return false;
         }
         const at::Tensor& t = THPVariable_Unpack(item);
-        if (!is_gradient(t) || (i > 0 && t.device() != gradients[0].device()) || (in_place && t.requires_grad())) {
+        if (!is_gradient(t) || (i > 0 && t.device() != gradients[0].device()) ||
+            (in_place && (t.requires_grad() || !is_writable(t)))) {
             return false;
         }
         gradients.push_back(t);
@@ -664,57 +666,84 @@ bool gradients_of(PyObject* object, std::vector<at::Tensor>& gradients, bool in_
     return n > 0;
 }
 
-PyObject* gradient_norm(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
-    std::vector<at::Tensor> gradients;
-    if (n != 1 || !gradients_of(arguments[0], gradients, false)) {
-        Py_RETURN_NONE;
+/// body(), and what it throws as a Python error (behind work that has been enqueued: None would have it done again).
+template <typename Body> PyObject* with_errors(Body&& body) {
+    try {
+        return body();
+    } catch (const std::exception& error) {
+        PyErr_SetString(PyExc_RuntimeError, error.what());
+        return nullptr;
     }
-    return run<OfIndices>(
-        gradients[0], [&] { return new_norm(gradients); },
-        [&](int32_t, at::Tensor& norm) { norm_of_gradients(norm, gradients); }
-    );
+}
+
+PyObject* gradient_norm(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
+    return with_errors([&]() -> PyObject* {
+        std::vector<at::Tensor> gradients;
+        if (n != 1 || !gradients_of(arguments[0], gradients, false)) {
+            Py_RETURN_NONE;
+        }
+        return run<OfIndices>(
+            gradients[0], [&] { return new_norm(gradients); },
+            [&](int32_t, at::Tensor& norm) { norm_of_gradients(norm, gradients); }
+        );
+    });
+}
+
+/// (the tensors in a list, the other object behind them; takes over `last`)
+PyObject* list_and(const std::vector<at::Tensor>& tensors, PyObject* last) {
+    PyObject* const both = PyTuple_New(2);
+    if (both == nullptr) {
+        Py_DECREF(last);
+        return nullptr;
+    }
+    PyTuple_SET_ITEM(both, 1, last);
+    PyTuple_SET_ITEM(both, 0, PyList_New(static_cast<Py_ssize_t>(tensors.size())));
+    PyObject* const list = PyTuple_GET_ITEM(both, 0);
+    try {
+        for (size_t i = 0; list != nullptr && i < tensors.size(); i++) {
+            PyObject* const tensor = wrap(tensors[i]);
+            if (tensor == nullptr) {
+                Py_DECREF(both);
+                return nullptr;
+            }
+            PyList_SET_ITEM(list, static_cast<Py_ssize_t>(i), tensor);
+        }
+    } catch (...) {
+        Py_DECREF(both);
+        throw;
+    }
+    if (list == nullptr) {
+        Py_DECREF(both);
+        return nullptr;
+    }
+    return both;
 }
 
 /// gradients, max_norm, whether in place: the norm, or the clipped gradients in front of it.
 PyObject* clip_gradients(PyObject*, PyObject* const* arguments, Py_ssize_t n) {
-    std::vector<at::Tensor> gradients, outputs;
-    double max_norm;
-    std::array<bool, 1> in_place;
-    if (n != 3 || !flags(arguments + 2, in_place) || !gradients_of(arguments[0], gradients, in_place[0]) ||
-        !number(arguments[1], max_norm)) {
-        Py_RETURN_NONE;
-    }
-    PyObject* const norm = run<OfIndices>(
-        gradients[0],
-        [&] {
-            outputs = in_place[0] ? gradients : new_gradients(gradients);
-            return new_norm(gradients);
-        },
-        [&](int32_t, at::Tensor& to) { clip_gradients_to(to, outputs, gradients, max_norm); }
-    );
-    if (norm == nullptr || norm == Py_None) {
-        return norm;
-    }
-    if (in_place[0]) {
-        for (const at::Tensor& gradient : gradients) {
-            gradient.unsafeGetTensorImpl()->bump_version();
+    return with_errors([&]() -> PyObject* {
+        std::vector<at::Tensor> gradients, outputs;
+        double max_norm;
+        std::array<bool, 1> in_place;
+        if (n != 3 || !flags(arguments + 2, in_place) || !gradients_of(arguments[0], gradients, in_place[0]) ||
+            !number(arguments[1], max_norm)) {
+            Py_RETURN_NONE;
         }
-        return norm;
-    }
-    PyObject* const list = PyList_New(static_cast<Py_ssize_t>(outputs.size()));
-    PyObject* const both = PyTuple_New(2);
-    if (list == nullptr || both == nullptr) {
-        Py_XDECREF(list);
-        Py_XDECREF(both);
-        Py_DECREF(norm);
-        return nullptr;
-    }
-    for (size_t i = 0; i < outputs.size(); i++) {
-        PyList_SET_ITEM(list, static_cast<Py_ssize_t>(i), wrap(outputs[i]));
-    }
-    PyTuple_SET_ITEM(both, 0, list);
-    PyTuple_SET_ITEM(both, 1, norm);
-    return both;
+        PyObject* const norm = run<OfIndices>(
+            gradients[0],
+            [&] {
+                outputs = in_place[0] ? gradients : new_gradients(gradients);
+                return new_norm(gradients);
+            },
+            [&](int32_t, at::Tensor& to) {
+                clip_gradients_to(to, outputs, gradients, max_norm);
+                if (in_place[0]) {
+                    mark_written(gradients);
+                }
+            }
+        );
+        return norm == nullptr || norm == Py_None || in_place[0] ? norm : list_and(outputs, norm);
+    });
 }
 
 #define MOPS_METHOD(NAME, FUNCTION)                                                                 \

@@ -1113,6 +1113,11 @@ std::vector<at::Tensor> gradients_of(at::TensorList tensors, const char* op, boo
                 std::string("mops::") + op + ": derivatives are not supported, and a gradient requires one"
             );
         }
+        if (in_place && !is_writable(tensor)) {
+            throw std::runtime_error(
+                std::string("mops::") + op + ": a gradient made in inference mode cannot be changed outside of it"
+            );
+        }
         if (is_gradient(tensor)) {
             gradients.push_back(tensor);
         } else if (in_place) {
@@ -1149,9 +1154,7 @@ at::Tensor clip_gradients_in_place(at::TensorList tensors, double max_norm) {
     OnTorchStream stream(gradients[0]);
     at::Tensor norm = new_norm(gradients);
     clip_gradients_to(norm, gradients, gradients, max_norm);
-    for (const at::Tensor& gradient : gradients) {
-        gradient.unsafeGetTensorImpl()->bump_version();
-    }
+    mark_written(gradients);
     return norm;
 }
 

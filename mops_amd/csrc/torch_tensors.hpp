@@ -11,6 +11,7 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/InferenceMode.h>
 #include <torch/types.h>
 
 #include "mops/amd.h"
@@ -102,6 +103,15 @@ inline at::Tensor new_sums(const at::Tensor& like) {
 inline bool is_gradient(const at::Tensor& t) {
     return t.is_cuda() && t.layout() == at::kStrided && t.has_storage() && !t.is_neg() &&
            is_layer_dtype(t.scalar_type()) && t.is_non_overlapping_and_dense();
+}
+/// Whether it may be written to here: a tensor that was made in inference mode has no version to count up outside of it, and
+/// counting throws (too late, behind the launches that write).
+inline bool is_writable(const at::Tensor& t) { return !t.is_inference() || c10::InferenceMode::is_enabled(); }
+/// Autograd is told (of tensors that are writable).
+inline void mark_written(const std::vector<at::Tensor>& gradients) {
+    for (const at::Tensor& gradient : gradients) {
+        gradient.unsafeGetTensorImpl()->bump_version();
+    }
 }
 /// Their likes, in the same order of dimensions. Up to SMALL_LIST bytes they share one piece of memory, which is asked for
 /// once (20 tensors of 2 MB: 23 us a call with memory for each, 14 like this); larger ones have their own, which

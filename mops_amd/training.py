@@ -262,7 +262,8 @@ def clip_gradients(gradients, max_norm):
 def clip_gradients_(gradients, max_norm):
     """``clip_gradients`` in place; returns the norm they had. Where it is at most ``max_norm``, nothing is written.
 
-    Every tensor must fill its memory (any order of dimensions), and none may share memory with another.
+    Every tensor must fill its memory (any order of dimensions), and none may share memory with another. One that was made
+    in inference mode can be changed there only.
     """
     result = _native.clip_gradients(gradients, max_norm, True)
     if result is not None:
@@ -277,6 +278,10 @@ def clip_gradients_(gradients, max_norm):
             raise ValueError(f"`gradients[{i}]` must fill its memory without gaps in {function}")
         if tensor.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"`gradients[{i}]` requires a gradient itself: it cannot be changed in place in {function}")
+        if tensor.is_inference() and not torch.is_inference_mode_enabled():
+            raise ValueError(
+                f"`gradients[{i}]` was made in inference mode and cannot be changed outside of it, in {function}"
+            )
     norm = _empty_norm(gradients)
     array = _array_of(gradients)
     _call_gradients("clip_gradients", norm, array, array, len(gradients), float(max_norm))

@@ -1118,6 +1118,41 @@ def test_operators_without_derivatives_say_so(device):
 
 
 @pytest.mark.gpu
+def test_operators_on_gradients_of_inference_mode(device, monkeypatch):
+    """Outside of inference mode they can be read, not changed: an error in front of the launches, on every path; inside they
+    can."""
+    from mops_amd import _c_lib
+
+    def in_place(gradients):
+        return mops_amd.clip_gradients_(gradients, 1.0)
+
+    def by_operator(gradients):
+        return operators().clip_gradients_(gradients, 1.0)
+
+    with torch.inference_mode():
+        made = torch.full((4,), 2.0, device=device)
+    ordinary = torch.full((9,), 3.0, device=device)
+    for path in ("native", "ctypes"):
+        if path == "ctypes":
+            monkeypatch.setattr(training, "_native", _c_lib._NoFunctions())
+        for call in (in_place, by_operator):
+            for gradients in ([made], [ordinary, made]):
+                with pytest.raises((RuntimeError, ValueError), match="made in inference mode"):
+                    call(gradients)
+            assert made.eq(2).all() and ordinary.eq(3).all() and ordinary._version == 0, path
+        clipped, norm = mops_amd.clip_gradients([made, ordinary], 1.0)
+        assert abs(norm.item() - math.sqrt(97)) < 1e-5 and abs(exact_norm(clipped) - 1) < 1e-5
+        with torch.inference_mode():
+            for call in (in_place, by_operator):
+                inside, ordinary_inside = made.clone(), ordinary.clone()
+                assert abs(call([inside, ordinary_inside]).item() - math.sqrt(97)) < 1e-5
+                assert torch.equal(inside, clipped[0]) and torch.equal(ordinary_inside, clipped[1])
+    versions = ordinary._version
+    in_place([ordinary])
+    assert ordinary._version > versions
+
+
+@pytest.mark.gpu
 def test_operators_registered_from_python():
     """The same tests with the operators of mops_amd/_torch_python_ops.py, in a process of their own."""
     import os
