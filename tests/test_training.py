@@ -607,6 +607,31 @@ def test_gradients_of_any_size(device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize(
+    "size,max_norm,dtypes",
+    [
+        (3e38, 1e-3, (torch.bfloat16, torch.float32)), (3e38, 1e-5, (torch.bfloat16,)), (3e38, 1e-30, (torch.bfloat16, torch.float32)),
+        (1e150, 1e-200, (torch.float64,)), (1e30, 1e-14, (torch.bfloat16, torch.float64)), (6e4, 1e-2, (torch.float16, torch.float32)),
+    ],
+)  # fmt: skip
+def test_factors_below_every_number_of_the_type(device, size, max_norm, dtypes):
+    """max_norm / norm is a number below the smallest one of 32 bits (or 64), a gradient times it is an ordinary number: off by its
+    rounding, the factor's digits and the norm's (2^-23 for 16 bits, (n + 8) 2^-53 for the others)."""
+    generator = torch.Generator().manual_seed(8)
+    gradients = [(torch.rand(shape, generator=generator) * 0.9 + 0.1).double().mul(size).to(dtype).to(device)
+                 for dtype in dtypes for shape in ((3001,), (20, 33))]  # fmt: skip
+    exact = exact_norm(gradients)
+    numbers = sum(g.numel() for g in gradients)
+    clipped, _ = mops_amd.clip_gradients(gradients, max_norm)
+    for actual, g in zip(clipped, gradients, strict=True):
+        expected = g.double().cpu() / exact * max_norm
+        off = (2.0**-23 if torch.finfo(g.dtype).bits == 16 else 0) + (numbers + 8) * 2.0**-53
+        held_to(actual, expected, off * expected.abs(), str(g.dtype))
+    mops_amd.clip_gradients_(gradients, max_norm)
+    assert same(tuple(gradients), tuple(clipped))
+
+
+@pytest.mark.gpu
 def test_layouts_of_gradients(device):
     """Any order of dimensions in place; gaps, expanded numbers and memory off every boundary where nothing is written."""
     generator = torch.Generator().manual_seed(5)
