@@ -67,16 +67,17 @@ typedef struct mops_amd_gradient_t {
 } mops_amd_gradient_t;
 
 /* norm[0] = sqrt(sum of the squares of all numbers of all gradients), added up
- * in 64 bits in an order that depends on the sizes only. The array is read
- * before the call returns. */
+ * in 64 bits in an order that depends on the sizes only; no square leaves their
+ * range, of 64-bit numbers either. The array is read before the call returns. */
 #define MOPS_GRADIENTS_DECLARE(W)                                                                  \
     MOPS_EXPORT int mops_amd_gradient_norm_##W(                                                    \
         mops_tensor_1d_##W##_t norm, const mops_amd_gradient_t* gradients, int64_t n_gradients     \
     );                                                                                             \
     /* And outputs[i] = gradients[i] * min(1, max_norm / norm), of the same size and type. An      \
      * output is its gradient's own memory (in place), or shares none with any gradient; outputs   \
-     * share none with each other. max_norm is not negative. A norm that is infinite or            \
-     * not-a-number makes of the gradients what the formula does. */                               \
+     * share none with each other. max_norm is not negative. The norm is not rounded to the type of \
+     * `norm` in between, nor the factor to that of a gradient. Infinities and not-a-number among   \
+     * the gradients make of them what the formula does. */                               \
     MOPS_EXPORT int mops_amd_clip_gradients_##W(                                                   \
         mops_tensor_1d_##W##_t norm, const mops_amd_gradient_t* outputs,                           \
         const mops_amd_gradient_t* gradients, int64_t n_gradients, double max_norm                 \

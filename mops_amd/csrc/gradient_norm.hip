@@ -9,7 +9,9 @@
 // captured launch keeps its own), and their numbers are cut into chunks that the
 // workgroups take in turn. Squares are added up in 64 bits, where neither those
 // of the largest 32-bit or bfloat16 number nor a sum of billions of them lose
-// anything that matters; the order depends on the sizes only. Every workgroup of
+// anything that matters; 64-bit numbers whose squares would leave the range have
+// sums of their own, of squares at another scale (Squares). The order depends on
+// the sizes only. Every workgroup of
 // the second launch adds up the partial sums for itself, and goes through the
 // chunks from the last one back: the caches still hold those.
 //
@@ -133,6 +135,38 @@ template <bool BACK, typename Body> __device__ __forceinline__ void for_parts(co
     }
 }
 
+/// Sums of squares. Of 64-bit numbers, those above LARGE and below SMALL have sums of their own, of the numbers times
+/// 2^-SCALE and 2^SCALE: the squares of all others, 2^60 of them, and those of the scaled ones are ordinary numbers (three
+/// sums by size: J. L. Blue, ACM Trans. Math. Software 4, 1978). Infinities are large, what is not a number is ordinary.
+struct Squares {
+    static constexpr double LARGE = 0x1p480, SMALL = 0x1p-480;
+    static constexpr int SCALE = 600;
+    double ordinary, large, small;
+
+    __device__ __forceinline__ void add(double x) {
+        const bool is_large = fabs(x) > LARGE, is_small = fabs(x) < SMALL;
+        const double scaled = x * (is_large ? 0x1p-600 : is_small ? 0x1p600 : 1.0), square = scaled * scaled;
+        large += is_large ? square : 0;
+        small += is_small ? square : 0;
+        ordinary += is_large || is_small ? 0 : square;
+    }
+};
+/// A norm: `number` times a power of two.
+struct Norm {
+    double number;
+    int exponent;
+
+    /// (infinite beyond the range)
+    __device__ __forceinline__ double rounded() const { return ldexp(number, exponent); }
+    static __device__ __forceinline__ Norm of(const Squares& squares) {
+        if (squares.large != 0) {
+            return Norm{sqrt(squares.large + ldexp(squares.ordinary, -2 * Squares::SCALE)), Squares::SCALE};
+        }
+        return squares.ordinary != 0 ? Norm{sqrt(squares.ordinary + ldexp(squares.small, -2 * Squares::SCALE)), 0}
+                                     : Norm{sqrt(squares.small), -Squares::SCALE};
+    }
+};
+
 __device__ __forceinline__ double sum_of_wave(double sum) {
 #pragma unroll
     for (int s = 1; s < WAVE; s *= 2) {
@@ -144,6 +178,7 @@ __device__ __forceinline__ double sum_of_wave(double sum) {
 __device__ __forceinline__ double sum_of_workgroup(double sum) {
     __shared__ double of_wave[THREADS / WAVE];
     sum = sum_of_wave(sum);
+    __syncthreads(); // (of another sum in front)
     if (threadIdx.x % WAVE == 0) {
         of_wave[threadIdx.x / WAVE] = sum;
     }
@@ -156,21 +191,44 @@ __device__ __forceinline__ double sum_of_workgroup(double sum) {
     return sum;
 }
 
+/// The partial sums of all workgroups in memory: [count] ordinary ones, and with 64-bit numbers among the gradients [count]
+/// large and [count] small ones behind them.
+struct Parts {
+    int32_t count;
+    bool of_doubles;
+
+    size_t bytes() const { return align256(std::max<size_t>((of_doubles ? 3 : 1) * static_cast<size_t>(count), 1) * sizeof(double)); }
+    __device__ __forceinline__ void store(double* partial, int32_t i, const Squares& squares) const {
+        partial[i] = squares.ordinary;
+        if (of_doubles) { // (uniform)
+            partial[count + i] = squares.large;
+            partial[2 * count + i] = squares.small;
+        }
+    }
+};
+
 /// KEPT: the gradients are read again, and the caches should have what they can (616 million bfloat16 numbers, squares and
 /// scaling: 205 + 430 us; streamed past the caches 179 + 478). For the norm alone they stream past (260 million: 77 us, 6.8
 /// TB/s).
 template <bool KEPT>
-__global__ __launch_bounds__(THREADS) void squares_kernel(double* __restrict__ partial, const Table table) {
+__global__ __launch_bounds__(THREADS) void squares_kernel(double* __restrict__ partial, Parts parts, int32_t first, const Table table) {
     double sums[2] = {0, 0};
+    Squares of_double{0, 0, 0};
     for_parts<false>(table, [&](auto zero, int32_t tensor, const auto& part) {
         typedef decltype(zero) T;
         typedef typename Part<T>::Numbers Numbers;
         const T* const from = static_cast<const T*>(table.from[tensor]);
+        auto add_one = [&](double x, int e) {
+            if constexpr (std::is_same_v<T, double>) {
+                of_double.add(x);
+            } else {
+                sums[e % 2] += x * x;
+            }
+        };
         auto add = [&](const Numbers& numbers) {
 #pragma unroll
             for (int e = 0; e < PIECE<T>; e++) {
-                const double x = static_cast<double>(numbers.get(e));
-                sums[e % 2] += x * x;
+                add_one(static_cast<double>(numbers.get(e)), e);
             }
         };
         part.template go<false>(
@@ -188,33 +246,42 @@ __global__ __launch_bounds__(THREADS) void squares_kernel(double* __restrict__ p
                     add(numbers[i]);
                 }
             },
-            [&](int64_t at) {
-                const double x = static_cast<double>(from[at]);
-                sums[0] += x * x;
-            }
+            [&](int64_t at) { add_one(static_cast<double>(from[at]), 0); }
         );
     });
-    const double sum = sum_of_workgroup(sums[0] + sums[1]);
+    const Squares all{
+        sum_of_workgroup(sums[0] + sums[1] + of_double.ordinary), parts.of_doubles ? sum_of_workgroup(of_double.large) : 0,
+        parts.of_doubles ? sum_of_workgroup(of_double.small) : 0
+    };
     if (threadIdx.x == 0) {
-        partial[blockIdx.x] = sum;
+        parts.store(partial, first + static_cast<int32_t>(blockIdx.x), all);
     }
 }
 
 /// The norm, from the partial sums of all workgroups, in all threads.
-__device__ __forceinline__ double norm_of(const double* partial, int32_t parts) {
-    double sum = 0;
+__device__ __forceinline__ Norm norm_of(const double* partial, const Parts& parts) {
+    Squares sums{0, 0, 0};
 #pragma unroll 4
-    for (int32_t i = threadIdx.x; i < parts; i += THREADS) {
-        sum += partial[i];
+    for (int32_t i = threadIdx.x; i < parts.count; i += THREADS) {
+        sums.ordinary += partial[i];
     }
-    return sqrt(sum_of_workgroup(sum));
+    sums.ordinary = sum_of_workgroup(sums.ordinary);
+    if (parts.of_doubles) { // (uniform)
+        for (int32_t i = threadIdx.x; i < parts.count; i += THREADS) {
+            sums.large += partial[parts.count + i];
+            sums.small += partial[2 * parts.count + i];
+        }
+        sums.large = sum_of_workgroup(sums.large);
+        sums.small = sum_of_workgroup(sums.small);
+    }
+    return Norm::of(sums);
 }
 
 template <typename Sum>
-__global__ __launch_bounds__(THREADS) void norm_kernel(Sum* __restrict__ norm, const double* __restrict__ partial, int32_t parts) {
-    const double all = norm_of(partial, parts);
+__global__ __launch_bounds__(THREADS) void norm_kernel(Sum* __restrict__ norm, const double* __restrict__ partial, Parts parts) {
+    const Norm all = norm_of(partial, parts);
     if (threadIdx.x == 0) {
-        *norm = static_cast<Sum>(all);
+        *norm = static_cast<Sum>(all.rounded());
     }
 }
 
@@ -225,14 +292,14 @@ struct Factor {
     int exponent;
 };
 /// (a norm that is none, or infinite, makes of the gradients what the formula does)
-__device__ __forceinline__ Factor factor_of(double norm, double max_norm) {
-    if (norm <= max_norm) {
+__device__ __forceinline__ Factor factor_of(const Norm& norm, double max_norm) {
+    if (norm.rounded() <= max_norm) {
         return Factor{1, 0};
     }
     int of_max = 0, of_norm = 0;
-    const double ratio = frexp(max_norm, &of_max) / frexp(norm, &of_norm); // (0.5 to 2)
+    const double ratio = frexp(max_norm, &of_max) / frexp(norm.number, &of_norm); // (0.5 to 2)
     const int more = ratio > 1 ? 1 : 0;
-    return Factor{more > 0 ? 0.5 * ratio : ratio, of_max - of_norm + more};
+    return Factor{more > 0 ? 0.5 * ratio : ratio, of_max - of_norm - norm.exponent + more};
 }
 /// A number times the factor, rounded once. 16 bits: a factor of 32 bits is exact enough, 2^-24 beside the result's 2^-9. SMALL:
 /// a factor that is no ordinary number of its type (an instruction more for each number: 616 million in bfloat16, 643 us
@@ -262,13 +329,13 @@ template <typename T, typename Body> __device__ __forceinline__ void with_scalin
 /// norm: null in all launches but one.
 template <typename Sum>
 __global__ __launch_bounds__(THREADS) void scale_kernel(
-    Sum* __restrict__ norm, const double* __restrict__ partial, int32_t parts, double max_norm, bool in_place, const Table table
+    Sum* __restrict__ norm, const double* __restrict__ partial, Parts parts, double max_norm, bool in_place, const Table table
 ) {
-    const double all = norm_of(partial, parts);
+    const Norm all = norm_of(partial, parts);
     if (norm != nullptr && blockIdx.x == 0 && threadIdx.x == 0) {
-        *norm = static_cast<Sum>(all);
+        *norm = static_cast<Sum>(all.rounded());
     }
-    if (in_place && all <= max_norm) {
+    if (in_place && all.rounded() <= max_norm) {
         return; // (uniform)
     }
     const Factor factor = factor_of(all, max_norm);
@@ -333,18 +400,19 @@ unsigned workgroups_of(const Table& table) {
     return static_cast<unsigned>(std::min<int64_t>(table.end[table.count - 1], WORKGROUPS_PER_UNIT * compute_units()));
 }
 
-/// The partial sums, in the thread's scratch memory; how many there are.
-template <bool KEPT> double* sum_squares(const std::vector<Table>& tables, int32_t& parts, hipStream_t stream) {
-    size_t all = 0;
+/// The partial sums, in the thread's scratch memory, and what there is of them.
+template <bool KEPT> double* sum_squares(const std::vector<Table>& tables, Parts& parts, hipStream_t stream) {
+    parts = Parts{0, false};
     for (const Table& table : tables) {
-        all += workgroups_of(table);
+        parts.count += static_cast<int32_t>(workgroups_of(table));
+        parts.of_doubles = parts.of_doubles || std::find(table.type, table.type + table.count, GradientType::F64) != table.type + table.count;
     }
-    double* const partial = static_cast<double*>(scratch(align256(std::max<size_t>(all, 1) * sizeof(double))));
-    parts = 0;
+    double* const partial = static_cast<double*>(scratch(parts.bytes()));
+    int32_t first = 0;
     for (const Table& table : tables) {
-        squares_kernel<KEPT><<<workgroups_of(table), THREADS, 0, stream>>>(partial + parts, table);
+        squares_kernel<KEPT><<<workgroups_of(table), THREADS, 0, stream>>>(partial, parts, first, table);
         MOPS_HIP_CHECK(hipGetLastError());
-        parts += static_cast<int32_t>(workgroups_of(table));
+        first += static_cast<int32_t>(workgroups_of(table));
     }
     return partial;
 }
@@ -423,7 +491,7 @@ void gradient_norm(Tensor<sum_t, 1> norm, const Gradient* gradients, size_t n_gr
     own::check(gradients, n_gradients, "gradients", "gradient_norm");
     const auto tables = own::tables_of(nullptr, gradients, n_gradients);
     const hipStream_t stream = current_stream();
-    int32_t parts = 0;
+    own::Parts parts{};
     const double* const partial = own::sum_squares<false>(tables, parts, stream);
     own::norm_kernel<sum_t><<<1, own::THREADS, 0, stream>>>(to, partial, parts);
     finish_call("gradient_norm");
@@ -450,7 +518,7 @@ void clip_gradients(
     own::check_memory(outputs, gradients, n_gradients);
     const auto tables = own::tables_of(outputs, gradients, n_gradients);
     const hipStream_t stream = current_stream();
-    int32_t parts = 0;
+    own::Parts parts{};
     const double* const partial = own::sum_squares<true>(tables, parts, stream);
     if (tables.empty()) {
         own::norm_kernel<sum_t><<<1, own::THREADS, 0, stream>>>(to, partial, parts);

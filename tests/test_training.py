@@ -632,6 +632,39 @@ def test_factors_below_every_number_of_the_type(device, size, max_norm, dtypes):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize(
+    "sizes", [(1e200,), (1.7e308,), (1e-200,), (1e-308,), (5e-324 * 2.0**20,), (1e150, 1e-160), (1e-150, 1e170), (1e250, 1e-250, 1.0)],
+)  # fmt: skip
+def test_double_gradients_whose_squares_leave_the_range(device, sizes):
+    """Norm and clipped gradients against the same numbers divided by the largest of the sizes (products of numbers of 64 bits
+    are off by 2^-53 each, sums of n squares by n 2^-53; beside it smaller sizes are nothing, or as exact)."""
+    generator = torch.Generator().manual_seed(9)
+    unit_numbers = [torch.rand(shape, generator=generator, dtype=torch.float64) * 0.9 + 0.1 for shape in ((3,), (5001,), (33, 7))]
+    largest = max(sizes)
+    gradients = [g * size for size in sizes for g in unit_numbers]
+    exact = math.sqrt(sum(((g / largest) ** 2).sum().item() for g in gradients))  # times `largest`
+    gradients = [g.to(device) for g in gradients] + [torch.full((40,), 1e-38, device=device, dtype=torch.bfloat16)]
+    if largest < 1e-38:
+        gradients.pop()
+    numbers = sum(g.numel() for g in gradients)
+    norm = mops_amd.gradient_norm(gradients)
+    representable = exact * (largest * 0.001) < 1.7e305
+    if representable:
+        assert abs(norm.item() / largest - exact) <= (numbers + 8) * 2.0**-53 * exact + 5e-324 / largest
+    else:
+        assert norm.item() == math.inf
+    for max_norm in (0.25 * largest, 1e-3 if largest > 1 else 1e-3 * largest):
+        clipped, again = mops_amd.clip_gradients(gradients, max_norm)
+        assert torch.equal(again, norm)
+        for actual, g in zip(clipped, gradients, strict=True):
+            expected = g.double().cpu() / exact * (max_norm / largest)
+            off = (2.0**-23 if g.dtype == torch.bfloat16 else 0) + (numbers + 8) * 2.0**-53
+            held_to(actual, expected, off * expected.abs(), str(g.dtype))
+    unchanged, _ = mops_amd.clip_gradients(gradients, math.inf)
+    assert same(tuple(unchanged), tuple(gradients))
+
+
+@pytest.mark.gpu
 def test_layouts_of_gradients(device):
     """Any order of dimensions in place; gaps, expanded numbers and memory off every boundary where nothing is written."""
     generator = torch.Generator().manual_seed(5)
