@@ -75,8 +75,8 @@ typedef struct mops_amd_gradient_t {
     );                                                                                             \
     /* And outputs[i] = gradients[i] * min(1, max_norm / norm), of the same size and type. An      \
      * output is its gradient's own memory (in place), or shares none with any gradient; outputs   \
-     * share none with each other. max_norm is not negative. The norm is not rounded to the type of \
-     * `norm` in between, nor the factor to that of a gradient. Infinities and not-a-number among   \
+     * share none with each other, and `norm` with none of them. max_norm is not negative. The norm \
+     * is not rounded to the type of `norm` in between, nor the factor to that of a gradient. Infinities and not-a-number among   \
      * the gradients make of them what the formula does. */                               \
     MOPS_EXPORT int mops_amd_clip_gradients_##W(                                                   \
         mops_tensor_1d_##W##_t norm, const mops_amd_gradient_t* outputs,                           \

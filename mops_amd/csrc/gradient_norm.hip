@@ -433,8 +433,9 @@ void check(const Gradient* gradients, size_t n, const char* what, const char* op
     }
 }
 
-/// Every output is its own gradient's memory, or shares none with anything else.
-void check_memory(const Gradient* outputs, const Gradient* gradients, size_t n) {
+/// Every output is its own gradient's memory, or shares none with anything else; the norm shares none with anything (it is
+/// written while gradients are read).
+template <typename Sum> void check_memory(const Sum* norm, const Gradient* outputs, const Gradient* gradients, size_t n) {
     struct Span {
         const char *begin, *end;
     };
@@ -468,11 +469,22 @@ void check_memory(const Gradient* outputs, const Gradient* gradients, size_t n) 
             );
         }
     }
+    const Span of_norm{reinterpret_cast<const char*>(norm), reinterpret_cast<const char*>(norm + 1)};
+    for (size_t i = 0; i < n; i++) {
+        for (const Span& other : {span(gradients[i]), span(outputs[i])}) {
+            if (other.begin != other.end && other.begin < of_norm.end && of_norm.begin < other.end) {
+                throw std::runtime_error("norm must not share memory with a gradient or an output in clip_gradients");
+            }
+        }
+    }
 }
 
 template <typename Sum, typename Norm> Sum* check_norm(const Norm& norm, const char* operation) {
     if (norm.shape[0] != 1) {
         throw std::runtime_error(std::string("norm must have one element in ") + operation);
+    }
+    if (norm.data == nullptr) {
+        throw std::runtime_error(std::string("norm has no memory in ") + operation);
     }
     return norm.data;
 }
@@ -515,7 +527,7 @@ void clip_gradients(
             );
         }
     }
-    own::check_memory(outputs, gradients, n_gradients);
+    own::check_memory(to, outputs, gradients, n_gradients);
     const auto tables = own::tables_of(outputs, gradients, n_gradients);
     const hipStream_t stream = current_stream();
     own::Parts parts{};

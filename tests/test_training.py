@@ -964,6 +964,41 @@ def test_refusals_of_lists(tmp_path):
     assert "share none with any gradient" in call([(at, 8, 0), (at + 64, 8, 0)], [(at, 8, 0), (at + 8, 8, 0)])
 
 
+def test_refusals_of_the_memory_of_a_norm():
+    """Likewise: a norm without memory, and one that lies in a gradient or an output."""
+    from mops_amd._c_lib import device_library
+
+    library = device_library()
+    gradient = training._Gradient
+    memory = (ctypes.c_double * 64)()
+    at = ctypes.addressof(memory)
+    for tag, size in (("f32", 4), ("f64", 8)):
+        view = training._STRUCTS[(1, tag)]
+
+        def call(name, address, *lists, tag=tag, view=view):
+            norm = view()
+            norm.data = ctypes.cast(ctypes.c_void_p(address), type(norm.data))
+            norm.shape[0] = 1
+            entry = getattr(library.cdll, f"mops_amd_{name}_{tag}")
+            entry.restype = ctypes.c_int
+            entry.argtypes = [view, *[ctypes.POINTER(gradient)] * len(lists), ctypes.c_int64]
+            arrays = [(gradient * len(x))(*[gradient(*y) for y in x]) for x in lists]
+            arguments = [norm, *arrays, len(lists[0])]
+            if name == "clip_gradients":
+                entry.argtypes = [*entry.argtypes, ctypes.c_double]
+                arguments.append(1.0)
+            assert entry(*arguments) == 1
+            return library.last_error()
+
+        gradients, outputs = [(at, 8, 0), (at + 64, 8, 0)], [(at + 128, 8, 0), (at + 192, 8, 0)]
+        assert "norm has no memory in gradient_norm" in call("gradient_norm", None, gradients)
+        assert "norm has no memory in clip_gradients" in call("clip_gradients", None, outputs, gradients)
+        inside = [at, at + 96 - size, at + 128, at + 216]
+        for address in inside:
+            assert "norm must not share memory" in call("clip_gradients", address, outputs, gradients)
+        assert "norm must not share memory" in call("clip_gradients", at + 32 - size, gradients, gradients)
+
+
 TILES = """
 #include <cstdio>
 #include <vector>
