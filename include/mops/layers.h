@@ -139,8 +139,10 @@ MOPS_GRADIENTS_DECLARE(f64)
     /* With x[r, v] = A[r, :] . W[v, :] for all classes v (rows of W):                             \
      *   log_sums[r] = log(sum over v of exp(x[r, v]))                                             \
      *   losses[r] = log_sums[r] - x[r, targets[r]]                                                \
-     * Both zero for a row whose target is negative or too large: padding, of which nothing is     \
-     * read but the target. The logits x are not rounded, and not held in memory. */               \
+     * Both zero for a row whose target is negative or too large: padding, and what it holds does  \
+     * not matter. The logits x are not rounded, and not held in memory; two numbers per row and   \
+     * tile of classes are, in scratch memory, for a piece of the classes at a time (half a        \
+     * gigabyte at most, less where the device has not as much). */                                \
     MOPS_EXPORT int mops_amd_linear_cross_entropy_##S(                                             \
         mops_tensor_1d_##R##_t losses, mops_tensor_1d_##R##_t log_sums, mops_tensor_2d_##S##_t A,  \
         mops_tensor_2d_##S##_t W, mops_tensor_1d_i32_t targets                                     \

@@ -11,7 +11,8 @@
 // The logits x never reach memory. A tile of grouped_tiles.hpp ends with a
 // row's logits in registers, and its finish makes of them the row's largest one
 // and the sum of the powers below it (two numbers per row and tile, joined
-// afterwards), or the numbers d, rounded to T (what the matrix instructions
+// afterwards, a piece of the classes at a time where those of all would take too
+// much memory), or the numbers d, rounded to T (what the matrix instructions
 // take; 16-bit types scaled, and in two parts for few rows: SCALED, IN_TWO_PARTS). Of d, a piece of the classes is in
 // memory at a time, and both products with it follow while the caches hold what
 // they can of it; grad_A is summed up over the pieces in 32 bits.
@@ -73,7 +74,8 @@ template <typename Wide> struct Sum {
 };
 
 // ----------------------------------------------------------- sums by tiles --
-/// partial[tile of classes][place]; target_logits[row], where the tile has the row's target.
+/// partial[tile of classes][place]; target_logits[row], where the tile has the row's target. The classes are those from
+/// `first_class` on.
 template <typename T> struct StorePartialSums {
     typedef wide_t<T> Wide;
     static constexpr bool PAIRS = false, RESTS = false;
@@ -81,6 +83,7 @@ template <typename T> struct StorePartialSums {
     Sum<Wide>* partial;
     Wide* target_logits;
     const int32_t* targets;
+    int32_t first_class;
 
     template <bool MAY_SPLIT, int LDS_BYTES, int BM, int BN, int WM, int WN>
     __device__ __forceinline__ void operator()(const Product<T>& g, const TileOf<T, BM, BN, WM, WN>& t) const {
@@ -105,7 +108,8 @@ template <typename T> struct StorePartialSums {
 #pragma unroll
         for (int i = 0; i < Tile::MB; i++) {
             const int32_t row = t.rows[min(t.row(i), t.unit.count - 1)];
-            const int32_t target = targets[row] - first;
+            // (any target: the difference wraps around, but never to one of the columns)
+            const int32_t target = static_cast<int32_t>(static_cast<uint32_t>(targets[row]) - (first_class + first));
             // (few wavefronts have a target of their rows among their columns; one lane of all tiles has its logit)
             if (__any(target >= 0 && target < COLUMNS)) {
 #pragma unroll
@@ -162,13 +166,14 @@ template <typename T> struct StorePartialSums {
 };
 
 /// losses and log_sums of ROWS places per workgroup, as many threads each as there are for them, from the sums of `parts`
-/// tiles; zeros for the rows without a target.
+/// tiles; zeros for the rows without a target. running[place]: the sums of the pieces of classes in front (not in the first
+/// one) and up to this one (not in the last).
 constexpr int JOIN_SUM_THREADS = 256;
 template <typename T, int ROWS>
 __global__ __launch_bounds__(JOIN_SUM_THREADS) void join_sums_kernel(
     wide_t<T>* __restrict__ losses, wide_t<T>* __restrict__ log_sums, const Sum<wide_t<T>>* __restrict__ partial,
-    const wide_t<T>* __restrict__ target_logits, const int32_t* __restrict__ targets, RowGroups groups, int32_t parts,
-    int32_t classes
+    Sum<wide_t<T>>* __restrict__ running, const wide_t<T>* __restrict__ target_logits, const int32_t* __restrict__ targets,
+    RowGroups groups, int32_t parts, int32_t classes, bool first, bool last
 ) {
     typedef wide_t<T> Wide;
     constexpr int LANES = JOIN_SUM_THREADS / ROWS;
@@ -177,6 +182,9 @@ __global__ __launch_bounds__(JOIN_SUM_THREADS) void join_sums_kernel(
     const int32_t place = blockIdx.x * ROWS + in_block, kept = groups.end_of(0, groups.begin_of(0));
     Sum<Wide> all{Sum<Wide>::lowest(), 0};
     if (place < kept) {
+        if (!first && lane == 0) {
+            all = running[place];
+        }
 #pragma unroll 4
         for (int32_t p = lane; p < parts; p += LANES) {
             all.join(partial[static_cast<size_t>(p) * groups.n_rows + place]);
@@ -191,7 +199,11 @@ __global__ __launch_bounds__(JOIN_SUM_THREADS) void join_sums_kernel(
             shared[lane][in_block] = all;
         }
     }
-    if (lane == 0 && place < groups.n_rows) {
+    if (!last) { // (uniform)
+        if (lane == 0 && place < kept) {
+            running[place] = all;
+        }
+    } else if (lane == 0 && place < groups.n_rows) {
         const int32_t row = groups.row_at(place);
         const bool has_target = place < kept && in_bounds(targets[row], classes);
         losses[row] = has_target ? all.logarithm_above(target_logits[row]) : Wide(0);
@@ -656,58 +668,89 @@ protected:
     bool wide_ = false, copied_ = false;
 };
 
+/// Bytes of partial sums that are in memory at a time, at most (but for those of one tile of classes): two numbers per row and
+/// tile, 25 MB for 8192 rows and 100003 classes. Less where the device has not as much (forward).
+constexpr size_t MOST_SUMS = size_t(1) << 29, LEAST_SUMS = size_t(1) << 17;
+
 template <typename T> class Forward : Call<T> {
 public:
-    explicit Forward(const Inputs<T>& inputs) : Call<T>(inputs) { choose(worth_copying(this->A_, this->W_, this->operations())); }
-    void choose(bool copied) { this->choose_logits(copied, this->in_.classes); }
-    bool copies() const { return this->copied_bytes() > 0; }
-    size_t bytes() const { return Plan::bytes(this->in_.rows) + this->copied_bytes() + target_bytes() + partial_bytes(); }
+    explicit Forward(const Inputs<T>& inputs) : Call<T>(inputs) {
+        choose(worth_copying(this->A_, this->W_, this->operations()), MOST_SUMS);
+    }
+    void choose(bool copied, size_t most_bytes) {
+        this->choose_logits(copied, this->in_.classes);
+        const size_t most = std::max<size_t>(most_bytes / (std::max(this->in_.rows, 1) * sizeof(Sum<wide_t<T>>)), 1);
+        // (where k is shared, there are few rows and few classes, and logits instead)
+        each_ = this->logits_.splits > 1 || parts(this->in_.classes) <= most ? this->in_.classes
+                                                                             : static_cast<int32_t>(most * this->of_logits_);
+    }
+    size_t bytes() const {
+        return Plan::bytes(this->in_.rows) + this->copied_bytes() + target_bytes() + running_bytes() + partial_bytes();
+    }
     void run(wide_t<T>* losses, wide_t<T>* log_sums, char* room, hipStream_t stream) {
         typedef wide_t<T> Wide;
         Product<T> g = this->logits_;
         g.groups = this->begin(room, this->in_.rows > FEW_ROWS, stream);
         g.q = this->of_A_;
-        g.p = this->of_W_;
         Wide* const target_logits = reinterpret_cast<Wide*>(room);
         room += target_bytes();
+        Sum<Wide>* const running = reinterpret_cast<Sum<Wide>*>(room);
+        room += running_bytes();
         Sum<Wide>* const partial = reinterpret_cast<Sum<Wide>*>(room);
         g.partial = reinterpret_cast<Wide*>(room);
-        if (g.n_size > 0) {
-            this->launch_logits(g, stream, StorePartialSums<T>{partial, target_logits, this->in_.targets});
-        }
         const unsigned rows = static_cast<unsigned>(this->in_.rows);
-        auto join = [&](auto each) {
-            constexpr int ROWS = decltype(each)::value;
-            join_sums_kernel<T, ROWS><<<static_cast<unsigned>(ceil_div(rows, ROWS)), JOIN_SUM_THREADS, 0, stream>>>(
-                losses, log_sums, partial, target_logits, this->in_.targets, g.groups, static_cast<int32_t>(parts()),
-                this->in_.classes
-            );
-        };
-        if (g.splits > 1) {
-            join_shared_sums_kernel<T><<<rows, ROW_THREADS, 0, stream>>>(losses, log_sums, this->in_.targets, g);
-        } else if (rows <= FEW_JOINED) {
-            join(std::integral_constant<int, 2>{});
-        } else {
-            join(std::integral_constant<int, 16>{});
+        // (without classes: one piece of none, for the zeros)
+        bool last = false;
+        for (int64_t at = 0; !last; at += each_) {
+            const int32_t first = static_cast<int32_t>(at);
+            last = this->in_.classes - first <= each_;
+            g.n_size = last ? this->in_.classes - first : each_;
+            g.p = Operand<T>{this->of_W_.data + static_cast<size_t>(first) * this->of_W_.stride, this->of_W_.stride};
+            if (g.n_size > 0) {
+                this->launch_logits(g, stream, StorePartialSums<T>{partial, target_logits, this->in_.targets, first});
+            }
+            auto join = [&](auto each) {
+                constexpr int ROWS = decltype(each)::value;
+                join_sums_kernel<T, ROWS><<<static_cast<unsigned>(ceil_div(rows, ROWS)), JOIN_SUM_THREADS, 0, stream>>>(
+                    losses, log_sums, partial, running, target_logits, this->in_.targets, g.groups,
+                    static_cast<int32_t>(parts(g.n_size)), this->in_.classes, first == 0, last
+                );
+            };
+            if (g.splits > 1) {
+                join_shared_sums_kernel<T><<<rows, ROW_THREADS, 0, stream>>>(losses, log_sums, this->in_.targets, g);
+            } else if (rows <= FEW_JOINED) {
+                join(std::integral_constant<int, 2>{});
+            } else {
+                join(std::integral_constant<int, 16>{});
+            }
+            MOPS_HIP_CHECK(hipGetLastError());
         }
-        MOPS_HIP_CHECK(hipGetLastError());
     }
 
 private:
     size_t target_bytes() const { return align256(static_cast<size_t>(this->in_.rows) * sizeof(wide_t<T>)); }
-    size_t parts() const { return tiles(this->in_.classes, this->of_logits_); }
+    size_t parts(int32_t classes) const { return tiles(classes, this->of_logits_); }
+    size_t running_bytes() const {
+        return each_ < this->in_.classes ? align256(static_cast<size_t>(this->in_.rows) * sizeof(Sum<wide_t<T>>)) : 0;
+    }
     size_t partial_bytes() const {
         return this->logits_.splits > 1 ? split_bytes(this->logits_)
-                                        : align256(parts() * this->in_.rows * sizeof(Sum<wide_t<T>>));
+                                        : align256(parts(each_) * this->in_.rows * sizeof(Sum<wide_t<T>>));
     }
+
+    int32_t each_ = 0; // classes per piece
 };
 
 template <typename T>
 void forward(const Inputs<T>& inputs, wide_t<T>* losses, wide_t<T>* log_sums, hipStream_t stream) {
     Forward<T> call(inputs);
-    char* workspace = call.copies() ? static_cast<char*>(scratch_or_null(call.bytes())) : nullptr;
+    char* workspace = static_cast<char*>(scratch_or_null(call.bytes()));
+    // (as much as there is: smaller pieces of the classes do as well, and so do operands that are not copied)
+    for (size_t most = MOST_SUMS; workspace == nullptr && most >= LEAST_SUMS; most /= 4) {
+        call.choose(false, most);
+        workspace = static_cast<char*>(scratch_or_null(call.bytes()));
+    }
     if (workspace == nullptr) {
-        call.choose(false);
         workspace = static_cast<char*>(scratch(call.bytes()));
     }
     call.run(losses, log_sums, workspace, stream);

@@ -112,8 +112,9 @@ def linear_cross_entropy(A, W, targets):
         losses[r] = log_sums[r] - logits[r, targets[r]]
 
     Both are ``float32`` (``float64`` for ``float64``) and zero for a row whose target is outside of the classes
-    (negative: padding), of which nothing else is read. ``W`` lies like the table of ``scaled_embedding`` and can be it.
-    The logits are not rounded and not held in memory.
+    (negative: padding); what such a row holds does not matter. ``W`` lies like the table of ``scaled_embedding`` and can be
+    it. The logits are not rounded and not held in memory. The thread's scratch memory has two numbers per row and tile of
+    classes, half a gigabyte at most (then, and where the device has not as much, a piece of the classes at a time).
     """
     result = _native.linear_cross_entropy(A, W, targets)
     if result is not None:

@@ -1102,6 +1102,68 @@ def test_on_a_device_that_is_nearly_full(device):
     assert done.stdout.count("ok") == 6, done.stdout
 
 
+LOSSES_ON_A_FULL_DEVICE = """
+import ctypes, os, sys
+sys.path.insert(0, os.getcwd())
+import torch
+import mops_amd
+from mops_amd._c_lib import device_library
+from tests import test_training as t
+os.environ["MOPS_AMD_TEST_SCRATCH_LIMIT"] = str(3 << 20)
+library = device_library().cdll
+library.mops_amd_scratch_capacity.restype = ctypes.c_int64
+cases = [
+    (20000, 9000, 72, torch.bfloat16), (20000, 9000, 71, torch.float16), (20000, 4001, 40, torch.float32),
+    (9000, 2003, 33, torch.float64), (20000, 300, 16, torch.bfloat16),
+]
+for rows, classes, K, dtype in cases:
+    A, W, targets, _ = t.loss_case(rows, classes, K, "padded", dtype)
+    A, W, targets = [x.cuda() for x in (A, W, targets)]
+    none = torch.zeros(rows, dtype=torch.float64, device="cuda")
+    results = t.loss_by_definition(A, W, targets, [none, none], dtype)
+    losses, log_sums = mops_amd.linear_cross_entropy(A, W, targets)
+    t.held_to(losses, *results[0], "losses")
+    t.held_to(log_sums, *results[1], "log_sums")
+    again = mops_amd.linear_cross_entropy(A, W, targets)
+    assert torch.equal(losses, again[0]) and torch.equal(log_sums, again[1])
+    outside = (targets < 0) | (targets >= classes)
+    assert outside.any() and not losses[outside].any() and not log_sums[outside].any()
+    assert library.mops_amd_scratch_capacity() <= 3 << 20
+    print("ok", library.mops_amd_scratch_capacity(), flush=True)
+"""
+
+
+@pytest.mark.gpu
+def test_losses_on_a_device_that_is_nearly_full(device):
+    """The partial sums of all classes at once are memory that a call can do without."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    program = [sys.executable, "-c", LOSSES_ON_A_FULL_DEVICE]
+    done = subprocess.run(program, cwd=root, capture_output=True, text=True, timeout=100)
+    assert done.returncode == 0, done.stdout + done.stderr[-3000:]
+    assert done.stdout.count("ok") == 5, done.stdout
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif("not torch.cuda.is_available() or torch.cuda.mem_get_info()[0] < 60e9")
+def test_losses_in_pieces_of_the_classes(device):
+    """More partial sums than are held at a time (some rows against the definition in 64 bits)."""
+    rows, classes, K = 140000, 128301, 8
+    A, W, targets, _ = loss_case(rows, classes, K, "padded", torch.bfloat16)
+    some = torch.arange(0, rows, 611)
+    none = torch.zeros(len(some), dtype=torch.float64, device=device)
+    A, W, targets = A.to(device), W.to(device), targets.to(device)
+    results = loss_by_definition(A[some], W, targets[some], [none, none], torch.bfloat16)
+    losses, log_sums = mops_amd.linear_cross_entropy(A, W, targets)
+    held_to(losses[some], *results[0], "losses")
+    held_to(log_sums[some], *results[1], "log_sums")
+    outside = (targets < 0) | (targets >= classes)
+    assert outside.any() and not losses[outside].any() and not log_sums[outside].any()
+
+
 # ------------------------------------------------------ PyTorch operators ----
 def operators():
     import mops_amd.torch  # noqa: F401  (registers the operators)
