@@ -446,6 +446,49 @@ def test_logits_of_any_size(device, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("tag", list(DTYPES))
+@pytest.mark.parametrize("base", [60.0, 1000.0, -768.0])
+@pytest.mark.parametrize("classes,K", [(12, 2), (700, 2), (40, 2048), (9000, 8)])
+def test_classes_that_are_all_but_certain(device, classes, K, base, tag):
+    """Logits base + t that are exact (the products and sums are), t = 0 for the likeliest class, ten others near it, all further
+    ones far away (their powers are 0 in 32 bits, and nothing beside 1 in 64). A power e^(t - ..) is off by (2 |t| + 8) 2^-p of
+    itself, which is (2 |t| + 8) e^t <= 8 2^-p of their sum; so a loss, from differences of logits and the logarithm of a sum of 11
+    powers, by (11 * 8 + 16 + 4 |loss|) 2^-p, however large the logits. log_sums has its own rounding besides. d = a e^(x - s) - g
+    with the s that is handed in: (a p (2 |x - s| + 8) + 4 (a p + g)) 2^-p and the rounding to the type."""
+    dtype = DTYPES[tag]
+    p = unit(dtype)
+    t = torch.cat([torch.tensor([0.0, -11, -13, -14.5, -12, -20, -9.5, -30, -16, -13.25, -11.75], dtype=torch.float64),
+                   torch.full((classes - 11,), -2048.0, dtype=torch.float64)])  # fmt: skip
+    t = t[torch.randperm(classes, generator=generator_of(classes, K))]
+    W = torch.zeros(classes, K, dtype=dtype)
+    W[:, 0], W[:, 1] = base, t.to(dtype)
+    targets = torch.cat([t.argmax()[None], (t == -13.25).nonzero()[0], (t == -9.5).nonzero()[0]]).int()
+    A = torch.zeros(3, K, dtype=dtype)
+    A[:, :2] = 1
+    x = base + t
+    s = torch.logsumexp(t, 0)
+    losses, log_sums = mops_amd.linear_cross_entropy(A.to(device), W.to(device), targets.to(device))
+    exact = s - t[targets.long()]
+    assert ((losses.double().cpu() - exact).abs() <= (11 * 8 + 16 + 4 * exact) * p).all(), losses
+    assert ((log_sums.double().cpu() - (base + s)).abs() <= (11 * 8 + 16 + 2 * abs(base)) * p).all(), log_sums
+    wide = losses.dtype
+    handed = (base + s).to(wide)[None]
+    g, h = 0.75, 0.5
+    power = torch.exp(x - handed.double())
+    for i in range(3):
+        row = [A[i : i + 1].to(device), W.to(device), targets[i : i + 1].to(device)]
+        for weights in ((g, h), (g, 0.0)):
+            grads = [torch.tensor([w], dtype=wide, device=device) for w in weights]
+            grad_W = mops_amd.linear_cross_entropy_vjp(*grads, *row, handed.to(device), compute_grad_A=False)[1]
+            one = torch.zeros(classes, dtype=torch.float64)
+            one[targets[i].item()] = weights[0]
+            d = sum(weights) * power - one
+            bound = (sum(weights) * power * (2 * (x - handed.double()).abs() + 8) + 4 * (sum(weights) * power + one)) * p
+            bound = bound + 2.0 ** (-2 * BITS[dtype]) * d.abs()  # (16 bits: what two parts leave)
+            held_to(grad_W[:, 0], d, bound, f"row {i}")
+
+
+@pytest.mark.gpu
 def test_scale_of_float16_gradients(device):
     """Weights of any size, far below the smallest float16 and far apart from row to row: grad_A of a row, divided by its
     weight, is what it is with the weight one (d is rounded to 2^-11 of itself at the scale of the largest weight, and to
