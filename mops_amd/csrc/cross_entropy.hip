@@ -118,7 +118,11 @@ __global__ __launch_bounds__(SCALE_THREADS) void find_scale_kernel(
         for (int w = 1; w < static_cast<int>(blockDim.x / WAVE); w++) {
             most = fmaxf(most, shared[w]);
         }
-        set_scale(scale, grad_losses != nullptr && groups.n_rows > 0 ? grad_losses[groups.row_at(0)] : 0, most);
+        const int32_t row = groups.n_rows > 0 ? groups.row_at(0) : -1;
+        set_scale(
+            scale, row >= 0 && grad_losses != nullptr ? grad_losses[row] : 0,
+            row >= 0 && grad_log_sums != nullptr ? grad_log_sums[row] : 0, most
+        );
     }
 }
 

@@ -43,10 +43,11 @@ __device__ __forceinline__ float weight_of(float g, float h) {
     const float weight = fmaxf(fabsf(g), fabsf(g + h));
     return weight <= std::numeric_limits<float>::max() ? weight : 0;
 }
-/// The scale of d, from the first kept row's weight of the loss and the largest of all of them (0: no power of two).
-__device__ __forceinline__ void set_scale(float* scale, float first, float most) {
+/// The scale of d, from the weights of the first kept row (of its loss, or of its log_sum where that has none) and the largest
+/// of all of them (0: no power of two).
+__device__ __forceinline__ void set_scale(float* scale, float g, float h, float most) {
     int exponent = 0;
-    first = fabsf(first);
+    const float first = fabsf(g != 0 ? g : h);
     const bool has_digits = first > 0 && first <= std::numeric_limits<float>::max();
     const float digits = has_digits ? 2 * frexpf(first, &exponent) : 1;
     exponent = 0;

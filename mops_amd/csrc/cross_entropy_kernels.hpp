@@ -487,7 +487,7 @@ __global__ __launch_bounds__(TWICE_THREADS) void twice_kernel(
         plan.twice_offsets[1] = 2 * all;
     }
     if (plan.scale != nullptr && (kept ? before == 0 : all == 0 && threadIdx.x == 0)) {
-        set_scale(plan.scale, g, most);
+        set_scale(plan.scale, g, h, most);
     }
 }
 

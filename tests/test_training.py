@@ -354,6 +354,38 @@ def test_gradients_of_a_mean_are_not_off_by_its_weight(device, tag, weight, rows
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("rows", [100, 600, 2000])
+@pytest.mark.parametrize("weight", [1 + 2.0**-8, 1 + 2.0**-11, 1.5 + 2.0**-8 + 2.0**-10])
+@pytest.mark.parametrize("tag", HALVES)
+def test_gradients_of_log_sums_are_not_off_by_their_weight(device, tag, weight, rows):
+    """Likewise for rows whose log_sums have one weight h, with a class each that is certain: logits of 32 and 0, the power of the
+    one is 1 - 8e-13 and those of the 63 others 1.3e-14, d is h and h 1.3e-14, off by 80 2^-24 of itself (what h d is held in is
+    not rounded: 1; the others are below 2^-38 of the largest in float16)."""
+    dtype, classes, extra = DTYPES[tag], 64, 16
+    generator = generator_of(rows, 3)
+    certain = indices_of("uniform", rows, classes).long()
+    A, W = torch.zeros(rows, classes + extra, dtype=dtype), torch.zeros(classes, classes + extra, dtype=dtype)
+    A[torch.arange(rows), certain] = 32
+    A[:, classes:] = random(generator, (rows, extra), dtype)
+    W[torch.arange(classes), torch.arange(classes)] = 1
+    h = weight / 1024
+    x = A.double() @ W.double().t()
+    d = h * torch.softmax(x, 1)
+    off = 80 * 2.0**-24 * d + 2.0**-38 * h
+    a, w = A.double(), W.double()
+    bound_A = off @ w.abs() + (classes + 16) * 2.0**-24 * (d @ w.abs())
+    bound_W = off.t() @ a.abs() + (rows + 16) * 2.0**-24 * (d.t() @ a.abs())
+    A, W, targets = A.to(device), W.to(device), indices_of("frequent", rows, classes).to(device)
+    _, log_sums = mops_amd.linear_cross_entropy(A, W, targets)
+    grads = torch.full((rows,), h, device=device)
+    grad_A, grad_W = mops_amd.linear_cross_entropy_vjp(None, grads, A, W, targets, log_sums)
+    held_to(grad_A, d @ w, bound_A, "grad_A")
+    held_to(grad_W, d.t() @ a, bound_W, "grad_W")
+    without = mops_amd.linear_cross_entropy_vjp(0 * grads, grads, A, W, targets, log_sums)
+    assert same((grad_A, grad_W), without)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("tag", list(DTYPES))
 def test_cross_entropy_in_pieces_of_the_classes(device, tag):
     """More gradients of logits than are held at a time: grad_A is added up over several pieces. (The definition in 64 bits
