@@ -169,6 +169,52 @@ def test_activations_far_from_zero(device, activation, tag):
         held_to(grad_A[0, 0], terms[0] + terms[1], bound, f"derivative at {x[i]}")
 
 
+def activated_far_from_zero(name, x):
+    """act(x), act'(x), the magnitudes of the latter's terms and how many units (16 + 2 |x| or 2 x^2) each is held to: the normal
+    distribution's integral from an argument in more than 64 bits."""
+    import numpy as np
+
+    if name == "gelu":
+        exact = np.asarray(x, dtype=np.longdouble) * -np.sqrt(np.longdouble(0.5))
+        z = torch.from_numpy(exact.astype(np.float64))
+        rest = torch.from_numpy((exact - exact.astype(np.float64)).astype(np.float64))
+        below = torch.special.erfc(z) / 2 - torch.exp(-z * z) * rest / math.sqrt(math.pi)
+        density = torch.exp(-x * x / 2) / math.sqrt(2 * math.pi)
+        return x * below, below + x * density, below + x.abs() * density, 16 + 2 * x * x
+    s, rest = torch.sigmoid(x), torch.sigmoid(-x)
+    if name == "sigmoid":
+        return s, s * rest, s * rest, 16 + 2 * x.abs()
+    return x * s, s + x * s * rest, s + x.abs() * s * rest, 16 + 2 * x.abs()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tag", list(DTYPES))
+@pytest.mark.parametrize("activation", ACTIVATIONS)
+def test_activations_point_by_point(device, activation, tag):
+    """The activation and its derivative at arguments that are exact (one product and a one each), every point to the share that
+    the rounding of its own exponent has: (16 + 2 |x|) 2^-p, for GELU (16 + 2 x^2) 2^-p, of the terms, and the result's rounding.
+    (Powers below the smallest number of 32 bits are zero.) float64: the oracle's own exponentials are off as much again."""
+    dtype = DTYPES[tag]
+    x = torch.cat([torch.linspace(-13, 13, 209), torch.tensor([-0.75179, -1.2784, -1e-3, 1e-3, -5.5, 1e-6])])
+    if activation != "gelu":
+        x = torch.cat([x, torch.linspace(-87, 87, 117), torch.tensor([-88.5, 88.5])])
+    x = x.to(dtype)
+    n = len(x)
+    A = torch.stack([x, torch.ones_like(x)], 1)
+    W = torch.eye(2, dtype=dtype).repeat(n, 1, 1)  # gate = x, up = 1, a group for every row
+    offsets = torch.arange(n + 1, dtype=torch.int32)
+    arguments = [A.to(device), W.to(device), offsets.to(device), None, activation]
+    x = x.double()
+    value, slope, terms, units = activated_far_from_zero(activation, x)
+    share = units * unit(dtype) * (2 if dtype == torch.float64 else 1)
+    smallest = torch.finfo(torch.float64 if dtype == torch.float64 else torch.float32).tiny * (x.abs() + 1)
+    held_to(mops_amd.gated_grouped_product(*arguments)[:, 0], value, share * value.abs() + smallest, "value")
+    _, grad_W = mops_amd.gated_grouped_product_vjp(torch.ones(n, 1, dtype=dtype, device=device), *arguments)
+    # (of 16-bit types the projections' gradients are rounded, and a sum of one of them is not rounded again)
+    held_to(grad_W[:, 1, 0], slope, share * terms + smallest, "slope")
+    held_to(grad_W[:, 1, 1], value, share * value.abs() + smallest, "value in the gradient")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("tag", list(DTYPES))
 @pytest.mark.parametrize("rows,K,L", [(70, 40, 72), (9, 1600, 30), (300, 33, 20), (3000, 64, 520)])
@@ -321,6 +367,30 @@ def test_gradients_of_few_rows_are_rounded_once(device, rows, classes, K, kind, 
     of_infinite = mops_amd.linear_cross_entropy_vjp(*grads, A, W, targets, log_sums)
     assert outside[0] or (not of_infinite[0][0].isfinite().any() and not of_infinite[1].isfinite().any())
     assert torch.equal(of_infinite[0][1:], grad_A[1:]) or tag == "f16"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tag", list(DTYPES))
+@pytest.mark.parametrize("rows,classes,K", [(9, 95, 200), (64, 500, 64), (256, 700, 33), (600, 300, 40), (3000, 94, 128)])
+def test_rows_beside_one_of_infinite_weight(device, rows, classes, K, tag):
+    """grad_A of all rows but the one whose weight is infinite (or not a number): what it is without that one, to its own bound."""
+    dtype = DTYPES[tag]
+    A, W, targets, grads = loss_case(rows, classes, K, "padded", dtype)
+    on_device = [t.to(device) for t in (A, W, targets)]
+    log_sums = mops_amd.linear_cross_entropy(*on_device)[1]
+    kept = ((targets >= 0) & (targets < classes)).nonzero().squeeze(1)
+    for row in (kept[0].item(), kept[len(kept) // 2].item()):
+        without = [g.clone() for g in grads]
+        for g in without:
+            g[row] = 0
+        exact, bound = loss_by_definition(A, W, targets, without, dtype)[2]
+        others = torch.arange(rows) != row
+        for poison, which in ((math.inf, 0), (-math.inf, 1), (math.nan, 0)):
+            bad = [g.clone() for g in grads]
+            bad[which][row] = poison
+            grad_A, _ = mops_amd.linear_cross_entropy_vjp(*[g.to(device) for g in bad], *on_device, log_sums)
+            held_to(grad_A[others.to(device)], exact[others], bound[others], f"beside {poison}")
+            assert not grad_A[row].isfinite().any()
 
 
 @pytest.mark.gpu
