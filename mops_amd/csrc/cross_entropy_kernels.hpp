@@ -276,8 +276,10 @@ template <typename T> constexpr bool SCALED = sizeof(T) == 2;
 /// are above or below the average is chance (3 rows of 38982 classes, K = 1127, bfloat16: errors of 2.8e-3 of the result,
 /// 1.7e-3 in two parts, which is what the result's own rounding makes). Rows cost little where the classes have to be
 /// read and their gradients written anyway: 256 rows of 50000 classes, K = 2048, are 505 us (257 in one part
-/// 437), of 38982, K = 1127, 351 (301), of 32000, K = 512, 118 (113). 512 rows would be 928 (776), 632 (424) and 204 (161),
-/// and chance has evened out.
+/// 437), of 38982, K = 1127, 351 (301), of 32000, K = 512, 118 (113). 512 rows would be 928 (776), 632 (424) and 204 (161).
+/// The error, against a single rounding of the results, is 1.00 in two parts and 1.3 to 1.5 in one, at 257 rows as at 1024 (50000 x
+/// 2048, 13112 x 50, 94 x 128, 4000 x 512, bfloat16 and float16; up to 1.6 where a few frequent classes have most of the
+/// rows): the border is where the second part begins to cost, the error is the same behind it.
 constexpr int32_t IN_TWO_PARTS = 256;
 /// Up to so many rows of d, grad_A takes as long as the classes take to be read, and two shares of them per compute unit have
 /// more on their way than one (rows of 50000 classes, K = 2048, bfloat16, one / two / three, us, all of the gradients: 3
