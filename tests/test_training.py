@@ -1260,6 +1260,7 @@ library.mops_amd_scratch_capacity.restype = ctypes.c_int64
 cases = [
     (20000, 9000, 72, torch.bfloat16), (20000, 9000, 71, torch.float16), (20000, 4001, 40, torch.float32),
     (9000, 2003, 33, torch.float64), (20000, 300, 16, torch.bfloat16),
+    (200, 500001, 8, torch.float32), (60, 1000003, 8, torch.bfloat16),  # (without a plan; wide tiles)
 ]
 for rows, classes, K, dtype in cases:
     A, W, targets, _ = t.loss_case(rows, classes, K, "padded", dtype)
@@ -1275,6 +1276,23 @@ for rows, classes, K, dtype in cases:
     assert outside.any() and not losses[outside].any() and not log_sums[outside].any()
     assert library.mops_amd_scratch_capacity() <= 3 << 20
     print("ok", library.mops_amd_scratch_capacity(), flush=True)
+    # captured, in what the block has room for
+    stream, graph, fixed = torch.cuda.Stream(), torch.cuda.CUDAGraph(), A.clone()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        captured = mops_amd.linear_cross_entropy(fixed, W, targets)
+    for repeat in range(3):
+        fixed.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        same = torch.where(outside, 0.0, torch.full_like(losses, classes).log())
+        assert (captured[1] - same).abs().max() <= 1e-5
+        fixed.copy_(A)
+        graph.replay()
+        torch.cuda.synchronize()
+        t.held_to(captured[0], *results[0], "losses")
+        t.held_to(captured[1], *results[1], "log_sums")
+        assert torch.equal(mops_amd.linear_cross_entropy(A, W, targets)[0], losses)
 """
 
 
@@ -1289,7 +1307,7 @@ def test_losses_on_a_device_that_is_nearly_full(device):
     program = [sys.executable, "-c", LOSSES_ON_A_FULL_DEVICE]
     done = subprocess.run(program, cwd=root, capture_output=True, text=True, timeout=100)
     assert done.returncode == 0, done.stdout + done.stderr[-3000:]
-    assert done.stdout.count("ok") == 5, done.stdout
+    assert done.stdout.count("ok") == 7, done.stdout
 
 
 @pytest.mark.gpu
